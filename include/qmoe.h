@@ -49,6 +49,9 @@ enum {
 /* Weighted-sum rounding modes: titan/kernels/moe_weighted_sum.py:44-49. */
 enum { QMOE_WSUM_FAST = 0, QMOE_WSUM_OPS = 1, QMOE_WSUM_CLONE = 2 };
 
+/* Element types of the entry points that take more than one. */
+enum { QMOE_BF16 = 0, QMOE_FP16 = 1, QMOE_FP32 = 2 };
+
 int qmoe_abi_version(void);
 /* Thread-local message of the last failing call on this thread. */
 const char* qmoe_last_error(void);
@@ -460,6 +463,90 @@ int qmoe_router_logits(const uint16_t* x, int64_t T, int64_t K,
 int qmoe_router_logits_dense(const uint16_t* x, int64_t T, int64_t K,
                              const uint16_t* w, int64_t E, float* logits,
                              void* stream);
+
+/* ----------------------------------------------------------------- mxfp4 --
+ * Microscaled 4-bit floating point (OCP Microscaling Formats v1.0), the
+ * mode="mxfp4" of mx.quantize, mx.dequantize, mx.quantized_matmul,
+ * mx.gather_qmm and mx.qqmm: blocks of 32 elements along the packed axis
+ * share a scale 2^(byte - 127) (byte 255: every element reads as NaN), an
+ * element is a sign over one of 0, 0.5, 1, 1.5, 2, 3, 4, 6, eight codes to a
+ * word, low bits first.  Codes are uint32 [.., K/8], scales uint8 [.., K/32],
+ * K a multiple of 32; there are no biases.
+ *
+ * Quantise: the scale of a block with largest magnitude m is 2^e, e =
+ * floor(log2 m) - 2 clamped to [-127, 127]; an element is x / 2^e rounded to
+ * the nearest value, ties to the even code, at most 6 in magnitude.  A block
+ * with a NaN or an infinity gets byte 255.  x has QMOE_BF16, _FP16 or _FP32
+ * elements, as has what dequantise writes. */
+int qmoe_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t K,
+                        uint32_t* w, uint8_t* scales, void* stream);
+int qmoe_mxfp4_dequantize(const uint32_t* w, const uint8_t* scales,
+                          int64_t rows, int64_t K, int dtype, void* out,
+                          void* stream);
+
+/* Few rows: out[r] = x[xr] W[experts[r]]^T (transpose: x [n_x, >= K], out
+ * [n_rows, N]) or x[xr] W[experts[r]] (x [n_x, >= N], out [n_rows, K]), with
+ * W [num_experts, N, K]; xr = x_rows[r], or r / x_div where x_rows is NULL;
+ * experts NULL: expert 0 for all rows.  x is bf16, its rows ldx elements
+ * apart (transpose: a multiple of 8); products and sums in fp32, out bf16 or
+ * fp32 (out_dtype).  Indices are clamped into range.  n_rows <= 65535. */
+int qmoe_mxfp4_gather_qmv(const uint16_t* x, int64_t n_x, int64_t ldx,
+                          const int32_t* x_rows, int32_t x_div,
+                          const int32_t* experts, int64_t n_rows,
+                          const uint32_t* w, const uint8_t* scales,
+                          int32_t num_experts, int64_t N, int64_t K,
+                          int transpose, int out_dtype, void* out,
+                          void* stream);
+
+/* Many rows: the same products for rows sorted by expert, as described by a
+ * tile table (qmoe_route / qmoe_build_tiles with qmoe_gemm_tile_rows() rows
+ * per tile), or, with the four tables NULL, for rows of one expert
+ * (num_experts = 1).  x_rows NULL: row r reads x[r].  ldx is a multiple of 8;
+ * without transpose the elements of a row of x from N up to the next multiple
+ * of 8, where ldx reaches there, must be zero. */
+int qmoe_mxfp4_gather_qmm(const uint16_t* x, int64_t n_x, int64_t ldx,
+                          const int32_t* x_rows, int64_t n_rows,
+                          const uint32_t* w, const uint8_t* scales,
+                          int32_t num_experts, int64_t N, int64_t K,
+                          int transpose, const int32_t* offsets,
+                          const int32_t* tile_row, const int32_t* tile_exp,
+                          const int32_t* ntiles, int64_t max_tiles,
+                          int out_dtype, void* out, void* stream);
+
+/* Both operands in mxfp4: out [n_rows, N] (bf16) = deq(xq)[xr] W[e]^T, xq
+ * [n_x, K/8] and xs [n_x, K/32] from qmoe_mxfp4_quantize, rows as above. */
+int qmoe_mxfp4_gather_qqmm(const uint32_t* xq, const uint8_t* xs, int64_t n_x,
+                           const int32_t* x_rows, int64_t n_rows,
+                           const uint32_t* w, const uint8_t* scales,
+                           int32_t num_experts, int64_t N, int64_t K,
+                           const int32_t* offsets, const int32_t* tile_row,
+                           const int32_t* tile_exp, const int32_t* ntiles,
+                           int64_t max_tiles, void* out, void* stream);
+
+/* ------------------------------------------- tokens to experts, gradients --
+ * The row movement of switch_layers.py:13-25 and moe_weighted_sum.py:44-98
+ * with gradients, for QMOE_BF16, _FP16 and _FP32 rows of any length.  Pair
+ * p = t * top_k + j is slot j of token t; order [n] and inv [n] are inverse
+ * permutations of the n = T * top_k pairs (qmoe_route).  Sums are fp32, in
+ * slot order, rounded once.
+ *   qmoe_sort_rows    out[i] = x[order[i] / top_k]
+ *   qmoe_unsort_sum   y[t] = sum_j s[p] xs[inv[p]]; scores NULL: s = 1; inv
+ *                     NULL: the identity.  first [T + 1]: the pairs of y[t]
+ *                     are first[t] .. first[t + 1] - 1 instead (top_k unused,
+ *                     scores by pair).  fp32 rows may have a bf16 sum.
+ *   qmoe_unsort_grad  dxs[inv[p]] = s[p] dy[t]; dscores[p] = <dy[t], xs[inv[p]]>;
+ *                     either may be NULL: not wanted. */
+int qmoe_sort_rows(const void* x, int64_t T, const int32_t* order,
+                   int64_t top_k, int64_t D, int dtype, void* out,
+                   void* stream);
+int qmoe_unsort_sum(const void* xs, int64_t n, int dtype, const int32_t* inv,
+                    const float* scores, const int32_t* first, int64_t T,
+                    int64_t top_k, int64_t D, int out_dtype, void* y,
+                    void* stream);
+int qmoe_unsort_grad(const void* dy, const void* xs, int64_t n, int dtype,
+                     const int32_t* inv, const float* scores, int64_t T,
+                     int64_t top_k, int64_t D, void* dxs, float* dscores,
+                     void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,154 @@
+// Quantisation to and from mxfp4 (the format is in mxfp4.h).
+//
+// For a block of 32 with largest magnitude m, the scale is 2^e with
+// e = floor(log2 m) - 2, clamped to [-127, 127] (OCP MX v1.0, 6.3: the largest
+// power of two in m over the largest one in an element, 4 = 2^2); every
+// element is x / 2^e rounded to the nearest e2m1 value, ties to the even code,
+// magnitudes past 6 to 6 (v_cvt_scalef32_pk_fp4_*, which divides by the power
+// of two exactly).  A block that holds a NaN or an infinity gets the scale
+// byte 255, so all of it reads back as NaN.  An all-zero block keeps its signs
+// under byte 0.
+//
+// Both directions are bound by HBM: 2 or 4 bytes an element on one side,
+// 17/32 on the other.
+#include "mxfp4.h"
+
+namespace {
+
+using namespace qmoe_mx;
+
+typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2_t;
+
+// Largest of v over each aligned group of four lanes (quad permutes).
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
+  return v;
+}
+
+// Eight consecutive elements as fp32 (exact for the 16-bit types).
+template <int DT>
+__device__ __forceinline__ void load8(const void* x, int64_t u, float (&f)[8]) {
+  if constexpr (DT == QMOE_FP32) {
+    const f32x4_t a = __builtin_nontemporal_load(static_cast<const f32x4_t*>(x) + 2 * u);
+    const f32x4_t b = __builtin_nontemporal_load(static_cast<const f32x4_t*>(x) + 2 * u + 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
+  } else {
+    const i32x4_t a = __builtin_nontemporal_load(static_cast<const i32x4_t*>(x) + u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t p = (uint32_t)a[i];  // a copy: a bit cast of a[i] itself reads a[0]
+      if constexpr (DT == QMOE_BF16) {
+        f[2 * i] = bf16lo(p);
+        f[2 * i + 1] = bf16hi(p);
+      } else {
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, p);
+        f[2 * i] = (float)h[0];
+        f[2 * i + 1] = (float)h[1];
+      }
+    }
+  }
+}
+
+// One thread per word of codes, four neighbouring lanes per block.
+template <int DT>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict__ x, int64_t words,
+                                                          uint32_t* __restrict__ w, uint8_t* __restrict__ s) {
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= words) return;  // whole quads: words is a multiple of four
+  float f[8];
+  load8<DT>(x, u, f);
+  // magnitudes compare as integers; an infinity or a NaN is past all finite ones
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+  m = quad_max(m);
+  // the exponent field of a normal m is floor(log2 m) + 127; a subnormal one
+  // (field 0) and fields up to 2 clamp to byte 0, a non-finite one is 255
+  const int field = (int)(m >> 23);
+  const uint32_t byte = field == 255 ? 255u : (uint32_t)max(field - 2, 0);
+  const float sc = scale_of(byte);
+  uint32_t q = 0;
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[0], f[1], sc, 0);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2], f[3], sc, 1);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4], f[5], sc, 2);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6], f[7], sc, 3);
+  w[u] = byte == 255u ? 0u : q;
+  if ((threadIdx.x & 3) == 0) s[u >> 2] = (uint8_t)byte;
+}
+
+// One thread per word of codes.
+template <int DT>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __restrict__ w,
+                                                            const uint8_t* __restrict__ s, int64_t words,
+                                                            void* __restrict__ out) {
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= words) return;
+  const uint32_t q = __builtin_nontemporal_load(w + u);
+  const float sc = scale_of(s[u >> 2]);
+  if constexpr (DT == QMOE_BF16) {
+    uint32_t o[4];
+    unpack8(q, sc, o);
+    const i32x4_t v = {(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
+    __builtin_nontemporal_store(v, static_cast<i32x4_t*>(out) + u);
+  } else {
+    const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, sc, 0);
+    const auto p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, sc, 1);
+    const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, sc, 2);
+    const auto p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, sc, 3);
+    if constexpr (DT == QMOE_FP32) {
+      const f32x4_t a = {p0[0], p0[1], p1[0], p1[1]}, b = {p2[0], p2[1], p3[0], p3[1]};
+      __builtin_nontemporal_store(a, static_cast<f32x4_t*>(out) + 2 * u);
+      __builtin_nontemporal_store(b, static_cast<f32x4_t*>(out) + 2 * u + 1);
+    } else {
+      const f16x2_t h[4] = {{(_Float16)p0[0], (_Float16)p0[1]}, {(_Float16)p1[0], (_Float16)p1[1]},
+                            {(_Float16)p2[0], (_Float16)p2[1]}, {(_Float16)p3[0], (_Float16)p3[1]}};
+      i32x4_t v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(int, h[i]);
+      __builtin_nontemporal_store(v, static_cast<i32x4_t*>(out) + u);
+    }
+  }
+}
+
+int check(const void* x, const void* w, const void* s, int dtype, int64_t rows, int64_t K) {
+  if (dtype != QMOE_BF16 && dtype != QMOE_FP16 && dtype != QMOE_FP32)
+    return qmoe::fail(QMOE_ERR_UNSUPPORTED, "dtype=%d", dtype);
+  if (rows < 0 || K < 0) return qmoe::fail(QMOE_ERR_INVALID, "bad sizes rows=%lld K=%lld", (long long)rows, (long long)K);
+  if (K % kBlock) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "K=%lld: must be a multiple of 32", (long long)K);
+  if (rows == 0 || K == 0) return QMOE_OK;
+  if (!x || !w || !s) return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
+  if (!qmoe::aligned16(x) || !qmoe::aligned4(w))
+    return qmoe::fail(QMOE_ERR_UNSUPPORTED, "the values must be 16-byte aligned, the codes 4-byte aligned");
+  if (rows > (int64_t)0x7FFFFFFF * 256 / (K / 8)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "too many elements");
+  return QMOE_OK;
+}
+
+}  // namespace
+
+extern "C" int qmoe_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t K, uint32_t* w, uint8_t* scales,
+                                   void* stream) {
+  const int rc = check(x, w, scales, dtype, rows, K);
+  if (rc != QMOE_OK || rows == 0 || K == 0) return rc;
+  const int64_t words = rows * (K / 8);
+  const dim3 grid((unsigned)((words + 255) / 256)), block(256);
+  hipStream_t st = qmoe::as_stream(stream);
+  if (dtype == QMOE_BF16) mx_quantize_kernel<QMOE_BF16><<<grid, block, 0, st>>>(x, words, w, scales);
+  else if (dtype == QMOE_FP16) mx_quantize_kernel<QMOE_FP16><<<grid, block, 0, st>>>(x, words, w, scales);
+  else mx_quantize_kernel<QMOE_FP32><<<grid, block, 0, st>>>(x, words, w, scales);
+  return qmoe::launch_status("mx_quantize_kernel");
+}
+
+extern "C" int qmoe_mxfp4_dequantize(const uint32_t* w, const uint8_t* scales, int64_t rows, int64_t K, int dtype,
+                                     void* out, void* stream) {
+  const int rc = check(out, w, scales, dtype, rows, K);
+  if (rc != QMOE_OK || rows == 0 || K == 0) return rc;
+  const int64_t words = rows * (K / 8);
+  const dim3 grid((unsigned)((words + 255) / 256)), block(256);
+  hipStream_t st = qmoe::as_stream(stream);
+  if (dtype == QMOE_BF16) mx_dequantize_kernel<QMOE_BF16><<<grid, block, 0, st>>>(w, scales, words, out);
+  else if (dtype == QMOE_FP16) mx_dequantize_kernel<QMOE_FP16><<<grid, block, 0, st>>>(w, scales, words, out);
+  else mx_dequantize_kernel<QMOE_FP32><<<grid, block, 0, st>>>(w, scales, words, out);
+  return qmoe::launch_status("mx_dequantize_kernel");
+}

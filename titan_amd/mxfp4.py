@@ -1,0 +1,344 @@
+"""Microscaled 4-bit floating point: the ``mode="mxfp4"`` of the quantized
+matmuls (mx.quantize, mx.dequantize, mx.quantized_matmul, mx.gather_qmm,
+mx.qqmm; reached through :mod:`titan_amd.ops`).
+
+Weights are codes [.., N, K/8] (int32 or uint32 words, eight e2m1 codes each,
+low bits first) and scales uint8 [.., N, K/32], 2^(byte - 127) per block of 32
+along K (OCP Microscaling Formats v1.0); there are no biases.  Activations are
+bf16, products and sums fp32, results bf16.
+
+The products are differentiable in x: with ``transpose`` (x W^T) dx = dy W, and
+without (x W) dx = dy W^T, by the same kernels over the same codes.  The codes
+and scales are constants of the graph.  ``qqmm`` and ``gather_qqmm`` quantise x
+as well and have no gradient.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib, ops, token_sort
+from ._lib import QmoeUnsupported
+
+__all__ = ["BLOCK", "quantize", "dequantize", "quantized_matmul", "gather_qmm", "qqmm", "gather_qqmm"]
+
+BLOCK = 32
+# rows of one expert up to which the matrix-vector kernels run (above: the GEMM)
+QMV_MAX_ROWS = 4
+# gathered rows from which unsorted calls are sorted for the grouped GEMM, as sorted ones take it
+SORTED_MIN_ROWS = 64
+
+
+def _format(group_size: int | None, bits: int, biases=None) -> None:
+    if group_size not in (None, BLOCK) or bits != 4:
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mxfp4 has group_size 32 and 4 bits, got {group_size} and {bits}")
+    if biases is not None:
+        raise ValueError("mxfp4 weights have no biases")
+
+
+def _scales(t: torch.Tensor, device) -> torch.Tensor:
+    ops._dev(t, "scales")
+    ops._same_device(device, scales=t)
+    if t.dtype != torch.uint8:
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mxfp4 scales must be uint8, got {t.dtype}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _weights(w: torch.Tensor, scales: torch.Tensor, device, dims: int):
+    """Checked codes and scales, and their [(E,) N, K]."""
+    w = ops._words(w, "w")
+    ops._same_device(device, w=w)
+    scales = _scales(scales, device)
+    if w.dim() != dims:
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"w must have {dims} dimensions, got {tuple(w.shape)}")
+    K = w.shape[-1] * 8
+    if K % BLOCK or tuple(scales.shape) != (*w.shape[:-1], K // BLOCK):
+        raise ValueError(f"codes {tuple(w.shape)} and scales {tuple(scales.shape)} disagree")
+    return w, scales, w.shape[-2], K
+
+
+# ------------------------------------------------------------ quantisation
+
+
+def quantize(w: torch.Tensor, group_size: int | None = None, bits: int = 4, mode: str = "mxfp4"):
+    """(codes int32 [.., K/8], scales uint8 [.., K/32]) of bf16, fp16 or fp32
+    values [.., K], K a multiple of 32: scale 2^(floor(log2 max|w|) - 2) per
+    block, elements to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to the
+    even code, larger ones to 6); a block with a NaN or an infinity reads back
+    as NaN."""
+    if mode != "mxfp4":
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}: quantize makes mxfp4")
+    _format(group_size, bits)
+    ops._dev(w, "w")
+    if w.dtype not in ops._DTYPES:
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"w must be bfloat16, float16 or float32, got {w.dtype}")
+    if w.dim() < 1 or w.shape[-1] % BLOCK:
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"the last dimension must be a multiple of 32, got {tuple(w.shape)}")
+    w = ops._ready(w)
+    K = w.shape[-1]
+    q = torch.empty(*w.shape[:-1], K // 8, dtype=torch.int32, device=w.device)
+    s = torch.empty(*w.shape[:-1], K // BLOCK, dtype=torch.uint8, device=w.device)
+    ops._launch("qmoe_mxfp4_quantize", w, w.data_ptr(), ops._DTYPES[w.dtype], w.numel() // K if K else 0, K, q.data_ptr(),
+            s.data_ptr())
+    return q, s
+
+
+def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size: int | None = None, bits: int = 4,
+               dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [.., K] of codes [.., K/8], exact in bf16 and fp32 (but for
+    magnitudes past the type's range, which become infinite), rounded in fp16."""
+    _format(group_size, bits, biases)
+    if dtype not in ops._DTYPES:
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"dtype={dtype}: bfloat16, float16 or float32")
+    w = ops._words(w, "w")
+    scales = _scales(scales, w.device)
+    K = w.shape[-1] * 8 if w.dim() else 0
+    if w.dim() < 1 or K % BLOCK or tuple(scales.shape) != (*w.shape[:-1], K // BLOCK):
+        raise ValueError(f"codes {tuple(w.shape)} and scales {tuple(scales.shape)} disagree")
+    out = torch.empty(*w.shape[:-1], K, dtype=dtype, device=w.device)
+    ops._launch("qmoe_mxfp4_dequantize", w, w.data_ptr(), scales.data_ptr(), w.numel() // w.shape[-1] if K else 0, K,
+            ops._DTYPES[dtype], out.data_ptr())
+    return out
+
+
+# --------------------------------------------------------------- products
+
+
+class _Rows:
+    """Which activation row and which expert each output row takes: ``x_rows``
+    (or row i // div), ``experts`` (None: one expert for all), and the tile
+    table of sorted rows (None: not sorted, or one expert)."""
+
+    __slots__ = ("n", "x_rows", "div", "experts", "tiles")
+
+    def __init__(self, n, x_rows=None, div=1, experts=None, tiles=None):
+        self.n, self.x_rows, self.div, self.experts, self.tiles = n, x_rows, div, experts, tiles
+
+
+def _pad8(x: torch.Tensor) -> torch.Tensor:
+    """Rows of a multiple of eight elements, zeros behind the given ones."""
+    extra = -x.shape[1] % 8
+    return torch.nn.functional.pad(x, (0, extra)) if extra else x
+
+
+def _product(x, w, scales, E, N, K, transpose, rows: _Rows, dtype=torch.bfloat16):
+    """out[r] = x[row of r] W[expert of r]^T (transpose) or W, rows as ``rows`` says."""
+    out = torch.empty(rows.n, N if transpose else K, dtype=dtype, device=x.device)
+    if rows.n == 0 or out.shape[1] == 0:
+        return out
+    if x.shape[1] == 0:
+        return out.zero_()
+    if (rows.experts is not None and rows.tiles is None) or rows.n <= QMV_MAX_ROWS:
+        ops._launch("qmoe_mxfp4_gather_qmv", x, x.data_ptr(), x.shape[0], x.shape[1], ops._ptr(rows.x_rows), rows.div,
+                ops._ptr(rows.experts), rows.n, w.data_ptr(), scales.data_ptr(), E, N, K, int(transpose), ops._DTYPES[dtype],
+                out.data_ptr())
+        return out
+    x = _pad8(x)
+    t = rows.tiles
+    table = (None, None, None, None, 0) if t is None else (t.offsets.data_ptr(), t.tile_row.data_ptr(),
+                                                           t.tile_exp.data_ptr(), t.ntiles.data_ptr(), t.maxt)
+    ops._launch("qmoe_mxfp4_gather_qmm", x, x.data_ptr(), x.shape[0], x.shape[1], ops._ptr(_x_rows(rows, x.device)), rows.n,
+            w.data_ptr(), scales.data_ptr(), E, N, K, int(transpose), *table, ops._DTYPES[dtype], out.data_ptr())
+    return out
+
+
+def _x_rows(rows: _Rows, device):
+    """The activation row of each row for the GEMMs, None for row r itself."""
+    if rows.x_rows is not None or rows.div == 1:
+        return rows.x_rows
+    return torch.div(torch.arange(rows.n, device=device, dtype=torch.int32), rows.div,
+                     rounding_mode="floor").to(torch.int32)
+
+
+class _Product(torch.autograd.Function):
+    """_product with its gradient in x."""
+
+    @staticmethod
+    def forward(ctx, x, w, scales, E, N, K, transpose, rows):
+        ctx.save_for_backward(w, scales)
+        ctx.args = x.shape[0], E, N, K, transpose, rows
+        return _product(x, w, scales, E, N, K, transpose, rows)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        w, scales = ctx.saved_tensors
+        n_x, E, N, K, transpose, rows = ctx.args
+        own = _Rows(rows.n, None, 1, rows.experts, rows.tiles)  # row r of dy for row r
+        dy = ops._ready(dy)
+        if rows.x_rows is None and rows.div == 1:
+            dx = _product(dy, w, scales, E, N, K, not transpose, own)
+        else:  # several rows share an activation row: their gradients are added in fp32, rounded once
+            dr = _product(dy, w, scales, E, N, K, not transpose, own, torch.float32)
+            if rows.x_rows is None:
+                dx = token_sort.unsort_sum(dr, None, None, n_x, rows.div, dtype=torch.bfloat16)
+            else:
+                at, order = torch.sort(rows.x_rows.clamp(0, max(n_x - 1, 0)), stable=True)
+                first = torch.searchsorted(at, torch.arange(n_x + 1, device=dy.device, dtype=torch.int32),
+                                           out_int32=True)
+                dx = token_sort.unsort_sum(dr, order.to(torch.int32), None, n_x, 0, first, torch.bfloat16)
+        return dx, None, None, None, None, None, None, None
+
+
+def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=None, transpose: bool = True,
+                     group_size: int | None = None, bits: int = 4) -> torch.Tensor:
+    """x [.., K] W^T (transpose) or x [.., N] W for codes w [N, K/8]."""
+    _format(group_size, bits, biases)
+    x = ops._bf16(x, "x")
+    w, scales, N, K = _weights(w, scales, x.device, 2)
+    if x.dim() < 1 or x.shape[-1] != (K if transpose else N):
+        raise ValueError(f"x {tuple(x.shape)} does not fit w [{N}, {K}] with transpose={transpose}")
+    x2 = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(math.prod(x.shape[:-1]), x.shape[-1])
+    y = _Product.apply(x2, w, scales, 1, N, K, bool(transpose), _Rows(x2.shape[0]))
+    return y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
+    """(batch, rows, order): the broadcast batch of a gather call over x
+    [.., M, C], its output rows in the order they are computed in, and that
+    order with its inverse (None: the batch's own).  ``min_rows`` rows or more
+    are sorted and get a tile table."""
+    dev = x.device
+    M, xb = x.shape[-2], tuple(x.shape[:-2])
+    if rhs is None:
+        rhs = torch.arange(E, device=dev, dtype=torch.int32)
+    else:
+        ops._dev(rhs, "rhs_indices")
+        ops._same_device(dev, rhs_indices=rhs)
+    x_rows, div = None, 1
+    if lhs is None:
+        batch = torch.broadcast_shapes(xb, tuple(rhs.shape))
+        nb, nx = math.prod(batch), math.prod(xb)
+        # batch index i reads x's batch index i // (nb / nx) where only x's last dimensions are broadcast
+        lead = (1,) * (len(batch) - len(xb)) + xb
+        cut = next((d for d in range(len(batch) + 1) if math.prod(lead[d:]) == 1), len(batch))
+        if lead[:cut] == tuple(batch[:cut]):
+            div = nb // nx if nx else 1
+        else:
+            x_rows = torch.arange(nx, device=dev, dtype=torch.int32).reshape(lead).expand(batch).reshape(-1)
+    else:
+        ops._dev(lhs, "lhs_indices")
+        ops._same_device(dev, lhs_indices=lhs)
+        batch = torch.broadcast_shapes(tuple(lhs.shape), tuple(rhs.shape))
+        nb = math.prod(batch)
+        x_rows = ops._i32(lhs.expand(batch).reshape(-1), "lhs_indices", dev)
+    experts = ops._i32(rhs.expand(batch).reshape(-1), "rhs_indices", dev)
+    if M != 1 and nb:  # rows of one batch index: M activation rows, one expert
+        ar = torch.arange(M, device=dev, dtype=torch.int32)
+        base = x_rows if x_rows is not None else None if div == 1 else _x_rows(_Rows(nb, None, div), dev)
+        x_rows = None if base is None else (base[:, None] * M + ar).reshape(-1)
+        div = 1
+        experts = experts.repeat_interleave(M)
+    n, order = nb * M, None
+    if n and (E == 0 or math.prod(x.shape[:-1]) == 0):
+        raise ValueError("rows are asked for, but there are no experts or no activation rows")
+    if n >= min_rows:
+        if sorted_indices:
+            if tiles is None or tiles.rows != n:
+                tiles = ops.build_tiles(experts, E)
+            elif tiles.num_experts != E or tiles.tile_rows != ops.tile_rows():
+                raise ValueError("tile table does not match this call")
+        else:
+            r = ops.route(experts, E)
+            order, inv, tiles = r.order, r.inv_order, r.tiles
+            experts = r.sorted_ids
+            x_rows = _x_rows(_Rows(n, x_rows, div), dev)
+            x_rows = order if x_rows is None else x_rows[order.long()]
+            order = order, inv
+            div = 1
+    else:
+        tiles = None
+    return batch, _Rows(n, x_rows, div, experts, tiles), order
+
+
+def _check_gather(x, w, scales, transpose, lhs, rhs):
+    w, scales, N, K = _weights(w, scales, x.device, 3)
+    if x.dim() < 2:
+        raise ValueError("x must be at least 2-D ([..., M, K])")
+    if x.shape[-1] != (K if transpose else N):
+        raise ValueError(f"x {tuple(x.shape)} does not fit w [{w.shape[0]}, {N}, {K}] with transpose={transpose}")
+    for name, t in (("lhs_indices", lhs), ("rhs_indices", rhs)):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.is_floating_point() or t.dtype == torch.bool):
+            raise TypeError(f"{name} must be an integer tensor")
+    return w, scales, w.shape[0], N, K
+
+
+def _rows_of(x):
+    return x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(math.prod(x.shape[:-1]), x.shape[-1])
+
+
+def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=None, lhs_indices=None,
+               rhs_indices=None, transpose: bool = True, group_size: int | None = None, bits: int = 4,
+               sorted_indices: bool = False, tiles=None) -> torch.Tensor:
+    """:func:`titan_amd.ops.gather_qmm` for codes w [E, N, K/8]: x [.., M, K]
+    times W^T, or x [.., M, N] times W without ``transpose``.  From 64 rows on
+    the rows run through the grouped GEMM: as they are with ``sorted_indices``
+    (ascending ``rhs_indices``), else sorted by expert first."""
+    _format(group_size, bits, biases)
+    x = ops._bf16(x, "x")
+    w, scales, E, N, K = _check_gather(x, w, scales, transpose, lhs_indices, rhs_indices)
+    batch, rows, order = _gathered(x, E, lhs_indices, rhs_indices, sorted_indices, tiles, SORTED_MIN_ROWS)
+    x2 = _rows_of(x)
+    y = _Product.apply(x2, w, scales, E, N, K, bool(transpose), rows)
+    if order is not None:
+        y = token_sort._Sort.apply(y, order[1], order[0])
+    return y.reshape(*batch, x.shape[-2], y.shape[-1])
+
+
+def _no_grad(x: torch.Tensor) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, "the products of quantised activations have no gradient: "
+                                                    "detach x, or use quantized_matmul / gather_qmm")
+
+
+def _qq_product(x2, w, scales, E, N, K, rows: _Rows):
+    xq, xs = quantize(x2)
+    out = torch.empty(rows.n, N, dtype=torch.bfloat16, device=x2.device)
+    if rows.n == 0 or N == 0:
+        return out
+    if K == 0:
+        return out.zero_()
+    t = rows.tiles
+    table = (None, None, None, None, 0) if t is None else (t.offsets.data_ptr(), t.tile_row.data_ptr(),
+                                                           t.tile_exp.data_ptr(), t.ntiles.data_ptr(), t.maxt)
+    ops._launch("qmoe_mxfp4_gather_qqmm", x2, xq.data_ptr(), xs.data_ptr(), x2.shape[0], ops._ptr(_x_rows(rows, x2.device)),
+            rows.n, w.data_ptr(), scales.data_ptr(), E, N, K, *table, out.data_ptr())
+    return out
+
+
+def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, group_size: int | None = None, bits: int = 4,
+         mode: str = "mxfp4") -> torch.Tensor:
+    """x [.., K], quantised to mxfp4 as :func:`quantize` does, times W^T for
+    codes w [N, K/8], both operands on the 4-bit matrix instructions (mx.qqmm)."""
+    if mode != "mxfp4":
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}: only mxfp4")
+    _format(group_size, bits)
+    x = ops._bf16(x, "x")
+    _no_grad(x)
+    w, scales, N, K = _weights(w, scales, x.device, 2)
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"x {tuple(x.shape)} does not fit w [{N}, {K}]")
+    x2 = _rows_of(x)
+    return _qq_product(x2, w, scales, 1, N, K, _Rows(x2.shape[0])).reshape(*x.shape[:-1], N)
+
+
+def gather_qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, lhs_indices=None, rhs_indices=None,
+                group_size: int | None = None, bits: int = 4, mode: str = "mxfp4", sorted_indices: bool = False,
+                tiles=None) -> torch.Tensor:
+    """:func:`gather_qmm` (transpose) with x quantised as in :func:`qqmm`, each
+    activation row once however many experts take it.  Takes the grouped
+    kernel's rows at any count: unsorted calls are sorted first."""
+    if mode != "mxfp4":
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}: only mxfp4")
+    _format(group_size, bits)
+    x = ops._bf16(x, "x")
+    _no_grad(x)
+    w, scales, E, N, K = _check_gather(x, w, scales, True, lhs_indices, rhs_indices)
+    batch, rows, order = _gathered(x, E, lhs_indices, rhs_indices, sorted_indices, tiles, 1)
+    x2 = _rows_of(x)
+    y = _qq_product(x2, w, scales, E, N, K, rows)
+    if order is not None:
+        y = token_sort._Sort.apply(y, order[1], order[0])
+    return y.reshape(*batch, x.shape[-2], N)

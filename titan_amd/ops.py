@@ -19,6 +19,12 @@ Call-surface parity with the reference (paths relative to its root):
   engine/patches/decode-fusion/fused_kernels.py:194-231
 * :func:`quantize_act_int8` / :func:`gather_qmm_int8`
   titan/kernels/moe_gather_int8.py:168-182, 393-425
+* :func:`quantize`, :func:`qqmm`, :func:`gather_qqmm` and ``mode="mxfp4"`` of
+  :func:`dequantize`, :func:`quantized_matmul` and :func:`gather_qmm`: the same
+  mx functions' microscaled mode (:mod:`titan_amd.mxfp4`)
+* :func:`sort_tokens` / :func:`unsort_tokens`   _gather_sort, _scatter_unsort
+  (switch_layers.py:13-25) and the weighted sum, with gradients
+  (:mod:`titan_amd.token_sort`)
 """
 
 from __future__ import annotations
@@ -36,6 +42,10 @@ BITS = 4
 # SwitchGLU sorts when indices.size >= 64 (switch_layers.py:218); the grouped
 # GEMM takes sorted calls from that size up.
 SORTED_MIN_ROWS = 64
+
+
+# QMOE_BF16, QMOE_FP16, QMOE_FP32
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def tile_rows() -> int:
@@ -99,7 +109,28 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _same_device(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
+
+
+def _launch(name: str, t: torch.Tensor, *args) -> None:
+    """Entry point ``name`` on the device of ``t`` and that device's current
+    stream (every entry point's last argument), whichever device is current."""
+    if t.device.index in (None, torch.cuda.current_device()):
+        _lib.call(name, *args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, _stream(t))
+
+
 # ------------------------------------------------------------------ layout
+
+
+def quantize(w: torch.Tensor, group_size: int | None = None, bits: int = BITS, mode: str = "mxfp4"):
+    """mx.quantize into mxfp4 (:func:`titan_amd.mxfp4.quantize`): (codes, scales)."""
+    return mxfp4.quantize(w, group_size, bits, mode)
 
 
 def unpack(w: torch.Tensor, bits: int = BITS) -> torch.Tensor:
@@ -111,9 +142,16 @@ def unpack(w: torch.Tensor, bits: int = BITS) -> torch.Tensor:
     return out
 
 
-def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, group_size: int = GROUP,
-               bits: int = BITS) -> torch.Tensor:
-    """bf16_rne(fmaf(q, s, b)) for every element (mx.dequantize)."""
+def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor | None = None,
+               group_size: int | None = None, bits: int = BITS, mode: str = "affine",
+               dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """bf16_rne(fmaf(q, s, b)) for every element (mx.dequantize); mode "mxfp4":
+    :func:`titan_amd.mxfp4.dequantize`, into bf16, fp16 or fp32."""
+    if mode == "mxfp4":
+        return mxfp4.dequantize(w, scales, biases, group_size, bits, dtype=dtype)
+    group_size = _affine(mode, biases, group_size)
+    if dtype != torch.bfloat16:
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"dtype={dtype}: affine weights dequantise to bfloat16")
     w, scales, biases = _words(w, "w"), _bf16(scales, "scales"), _bf16(biases, "biases")
     K = w.shape[-1] * 32 // bits
     rows = w.numel() // w.shape[-1]
@@ -248,6 +286,15 @@ def swiglu(gate_up: torch.Tensor) -> torch.Tensor:
 
 
 # ------------------------------------------------------------- gather_qmm
+
+
+def _affine(mode: str, biases, group_size: int | None) -> int:
+    """The group size of a call with affine weights; refuses other modes."""
+    if mode != "affine":
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}: 'affine' or 'mxfp4'")
+    if biases is None:
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, "affine weights need biases")
+    return GROUP if group_size is None else group_size
 
 
 def _check_quant(w, scales, group_size, bits, K):
@@ -509,9 +556,10 @@ def gemm_supported(K: int, N: int, group_size: int, bits: int) -> bool:
 
 def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor | None = None,
                lhs_indices: torch.Tensor | None = None, rhs_indices: torch.Tensor | None = None,
-               transpose: bool = True, group_size: int = GROUP, bits: int = BITS, mode: str = "affine",
+               transpose: bool = True, group_size: int | None = None, bits: int = BITS, mode: str = "affine",
                sorted_indices: bool = False, *, tiles: TileTable | None = None) -> torch.Tensor:
-    """mx.gather_qmm for transpose=True affine weights.
+    """mx.gather_qmm for transpose=True affine weights, and for mxfp4 weights
+    either way round, with a gradient (:func:`titan_amd.mxfp4.gather_qmm`).
 
     ``x`` is [..., M, K] and ``w`` [E, N, K*bits/32].  The batch is the
     broadcast of ``lhs_indices`` (default: x's own batch) with ``rhs_indices``
@@ -519,12 +567,12 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
     out[i, m] = x[lhs[i], m] @ deq(W[rhs[i]])^T.  ``sorted_indices`` promises
     ascending ``rhs_indices`` and selects the grouped GEMM for 64 rows or more.
     """
-    if mode != "affine":
-        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}: only affine quantization")
+    if mode == "mxfp4":
+        return mxfp4.gather_qmm(x, w, scales, biases, lhs_indices, rhs_indices, transpose, group_size, bits,
+                                sorted_indices, tiles)
+    group_size = _affine(mode, biases, group_size)
     if not transpose:
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, "transpose=False")
-    if biases is None:
-        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, "affine weights need biases")
     if w.dim() != 3:
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"w must be [E, N, K*bits/32], got {tuple(w.shape)}")
     x = _bf16(x, "x")
@@ -566,12 +614,29 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
     return out.reshape(*batch, M, N)
 
 
-def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
-                     transpose: bool = True, group_size: int = GROUP, bits: int = BITS,
+def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, group_size: int | None = None, bits: int = BITS,
+         mode: str = "mxfp4") -> torch.Tensor:
+    """mx.qqmm: both operands in mxfp4 (:func:`titan_amd.mxfp4.qqmm`)."""
+    return mxfp4.qqmm(x, w, scales, group_size, bits, mode)
+
+
+def gather_qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, lhs_indices: torch.Tensor | None = None,
+                rhs_indices: torch.Tensor | None = None, group_size: int | None = None, bits: int = BITS,
+                mode: str = "mxfp4", sorted_indices: bool = False, *, tiles: TileTable | None = None) -> torch.Tensor:
+    """:func:`gather_qmm` with the activations quantised to mxfp4 too
+    (:func:`titan_amd.mxfp4.gather_qqmm`)."""
+    return mxfp4.gather_qqmm(x, w, scales, lhs_indices, rhs_indices, group_size, bits, mode, sorted_indices, tiles)
+
+
+def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor | None = None,
+                     transpose: bool = True, group_size: int | None = None, bits: int = BITS,
                      mode: str = "affine") -> torch.Tensor:
-    """mx.quantized_matmul for transpose=True affine weights: x[..., K] @ deq(W)^T."""
-    if mode != "affine":
-        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}")
+    """mx.quantized_matmul for transpose=True affine weights: x[..., K] @ deq(W)^T;
+    mode "mxfp4": :func:`titan_amd.mxfp4.quantized_matmul`, either way round,
+    with a gradient."""
+    if mode == "mxfp4":
+        return mxfp4.quantized_matmul(x, w, scales, biases, transpose, group_size, bits)
+    group_size = _affine(mode, biases, group_size)
     if not transpose:
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, "transpose=False")
     x = _bf16(x, "x")
@@ -676,6 +741,19 @@ def moe_weighted_sum(xs: torch.Tensor, inv_order: torch.Tensor | None, scores: t
     _lib.call("qmoe_weighted_sum", xs2.data_ptr(), _ptr(inv), sc.data_ptr(), rows, k, dim,
               _lib.WSUM_MODES[mode], out.data_ptr(), _stream(xs))
     return out
+
+
+def sort_tokens(x: torch.Tensor, order: torch.Tensor, inv_order: torch.Tensor) -> torch.Tensor:
+    """Each pair's token row in expert order, with its gradient
+    (:func:`titan_amd.token_sort.sort_tokens`)."""
+    return token_sort.sort_tokens(x, order, inv_order)
+
+
+def unsort_tokens(xs: torch.Tensor, order: torch.Tensor, inv_order: torch.Tensor,
+                  scores: torch.Tensor | None = None) -> torch.Tensor:
+    """Sorted rows back to their tokens, summed with their scores, with gradients
+    (:func:`titan_amd.token_sort.unsort_tokens`)."""
+    return token_sort.unsort_tokens(xs, order, inv_order, scores)
 
 
 # -------------------------------------------------------------------- int8
@@ -877,6 +955,9 @@ def router_logits(x: torch.Tensor, router, group_size: int = GROUP, bits: int = 
     return out
 
 
+# at the end: both are written over the functions above
+from . import mxfp4, token_sort  # noqa: E402
+
 __all__ = [
     "GROUP", "BITS", "QmoeError", "QmoeUnsupported", "TileTable", "TileWeights", "Routing", "build_tiles", "route",
     "repack_tiles", "gather_qmm_sorted_tiles", "gather_qmm_int8_sorted_tiles", "router_topk", "router_logits", "gather_qmm_swiglu_sorted_tiles", "swiglu_pair_order", "gather_qmv_tiles", "gate_up_silu_tiles",
@@ -884,5 +965,5 @@ __all__ = [
     "route_block", "gather_qmm_sorted_tiles_shared", "moe_weighted_sum_shared", "router_topk_shared",
     "gate_up_silu_topk", "gate_up_topk_supported", "gather_rows", "swiglu", "shared_combine", "max_tiles", "tile_rows", "unpack", "dequantize", "gather_qmv", "gather_qmm_sorted", "gather_qmm",
     "gemm_supported", "quantized_matmul", "gate_up_silu", "down_wsum", "moe_weighted_sum",
-    "quantize_act_int8", "gather_qmm_int8_sorted",
+    "quantize_act_int8", "gather_qmm_int8_sorted", "quantize", "qqmm", "gather_qqmm", "sort_tokens", "unsort_tokens",
 ]
