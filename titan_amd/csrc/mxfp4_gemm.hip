@@ -41,90 +41,775 @@ __device__ __forceinline__ qmoe_gemm::TileRows tile_of(const GemmArgs& a, int64_
   return t;
 }
 
-constexpr int kStep = 32, kOut = 64, kPitch = kStep + 8;
+// Layout of the work.  A unit is a tile of up to 128 rows of one expert times
+// 256 outputs.  Four waves share it two by two: wave (wm, wn) takes half the
+// tile's rows and 128 of the outputs, so weights are converted twice per tile
+// and activations read twice from LDS (one by four would halve the first and
+// double the second, and LDS reads are the scarcer: at 128 B a clock and CU
+// they take 55% of the matrix cores' time as it is).  Blocks are persistent,
+// two per CU, and take the units heavy-first (gemm_common.h).  Tiles of at
+// most 64 rows run with half the row subtiles.
+//
+// Operands reach LDS by asynchronous copies into a ring of NS stages and are
+// read from there as matrix fragments; the fragments of a step are prepared
+// during the step before.  The barrier that hands over a stage stands before
+// a group's last step, whose operands are in registers by then: past it the
+// next group's first fragments are read, and the stage just emptied takes the
+// copies of NS groups ahead.
+constexpr int kRowsHalf = kTileRows / 2;
+constexpr int kCols = 256;
+__device__ __attribute__((aligned(16))) uint32_t zero_page[4];  // what copies past the contraction's end read
 
-template <int MODE>
-__global__ __launch_bounds__(256) void mx_gemm_kernel(GemmArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t xa[kTileRows][kPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t wb[kOut][kPitch];
-  const qmoe_gemm::TileRows t = tile_of(a, blockIdx.x);
-  if (t.valid <= 0) return;
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-  const int64_t C = MODE == kT ? a.N : a.K, O = MODE == kT ? a.K : a.N;
-  const int64_t o0 = (int64_t)blockIdx.y * kOut;
-  const int64_t units = a.K / kBlock;
-  f32x4_t acc[2][4] = {};
-  for (int64_t c0 = 0; c0 < C; c0 += kStep) {
-    __syncthreads();
-    for (int i = tid; i < kTileRows * 4; i += 256) {
-      const int m = i / 4, u = i % 4;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (m < t.valid && c0 + 8 * u < C) {
-        const int64_t r = t.row0 + m;
-        const int64_t xr = min(max(a.x_rows ? (int64_t)a.x_rows[r] : r, (int64_t)0), a.n_x - 1);
-        if constexpr (MODE == kQQ) {
-          uint32_t p[4];
-          unpack8(a.xq[xr * 4 * units + c0 / 8 + u], scale_of(a.xs[xr * units + c0 / kBlock]), p);
-          v = make_uint4(p[0], p[1], p[2], p[3]);
-        } else {
-          v = *reinterpret_cast<const uint4*>(a.x + xr * a.ldx + c0 + 8 * u);
-        }
-      }
-      *reinterpret_cast<uint4*>(&xa[m][8 * u]) = v;
-    }
-    {
-      uint32_t p[4] = {0, 0, 0, 0};
-      if constexpr (MODE == kT) {
-        const int n = tid / 8, j = tid % 8;  // weight row of the step, word of its 64 outputs
-        if (c0 + n < C && o0 + 8 * j < O) {
-          const int64_t row = (int64_t)t.e * a.N + c0 + n;
-          unpack8(a.w[row * 4 * units + o0 / 8 + j], scale_of(a.s[row * units + (o0 + 8 * j) / kBlock]), p);
-        }
+__device__ __forceinline__ void dma1s(const void* sbase, uint32_t voff, uint32_t lds_base) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_ubyte %1, %2"
+      :
+      : "s"(lds_base), "v"(voff), "s"(sbase)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void dma1(const void* g, uint32_t lds_base) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_ubyte %1, off"
+      :
+      : "s"(lds_base), "v"(g)
+      : "memory", "m0");
+}
+
+// The thread's index through an empty asm, so that what is computed from it is
+// computed here and not kept in registers across the unit loop.
+__device__ __forceinline__ int fresh_tid() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
+
+struct Unit {
+  int e, valid, nblk;
+  int64_t row0;
+};
+
+// Swizzle of the eight 16-byte units of a 128-byte activation row in LDS, of
+// the four of a 64-byte row: conflict-free 16-byte reads of one unit by
+// sixteen consecutive rows.
+__device__ __forceinline__ int swz8(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+__device__ __forceinline__ int swz4(int row) { return (row >> 2) & 3; }
+
+// Sources of the copies of the tile's activation rows: copy d of a wave fills
+// 1 KiB, 64 / UNITS rows of UNITS 16-byte units.  Rows past the tile's end are
+// its last row again (nothing of them is stored).
+template <int COPIES, int UNITS>
+struct RowSrc {
+  const char* p[COPIES];
+  int unit[COPIES];
+};
+template <int COPIES, int UNITS>
+__device__ __forceinline__ RowSrc<COPIES, UNITS> row_sources(const GemmArgs& a, const Unit& u, const void* base,
+                                                             int64_t pitch, int wave, int lane) {
+  RowSrc<COPIES, UNITS> r;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) wb[8 * j + i][n] = (uint16_t)(p[i / 2] >> (16 * (i & 1)));
-      } else {
-        const int n = tid / 4, j = tid % 4;
-        if (o0 + n < O) {
-          const int64_t row = (int64_t)t.e * a.N + o0 + n;
-          unpack8(a.w[row * 4 * units + c0 / 8 + j], scale_of(a.s[row * units + c0 / kBlock]), p);
-        }
-        *reinterpret_cast<uint4*>(&wb[n][8 * j]) = make_uint4(p[0], p[1], p[2], p[3]);
-      }
-    }
-    __syncthreads();
-    bf16x8_t fa[2], fb[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      fa[i] = *reinterpret_cast<const bf16x8_t*>(&xa[32 * wave + 16 * i + lane % 16][8 * (lane / 16)]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) fb[j] = *reinterpret_cast<const bf16x8_t*>(&wb[16 * j + lane % 16][8 * (lane / 16)]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+  for (int d = 0; d < COPIES; ++d) {
+    const int row = (d * 4 + wave) * (64 / UNITS) + lane / UNITS;
+    r.unit[d] = (lane % UNITS) ^ (UNITS == 8 ? swz8(row) : swz4(row));
+    const int64_t i = u.row0 + min(row, u.valid - 1);
+    const int64_t x = min(max(a.x_rows ? (int64_t)a.x_rows[i] : i, (int64_t)0), a.n_x - 1);
+    r.p[d] = static_cast<const char*>(base) + x * pitch + r.unit[d] * 16;
   }
+  return r;
+}
+
+// Writes a unit's results.  put(i, j, ...) pieces are staged through LDS, 64
+// rows a pass, so that a row's 256 results leave as 512 contiguous bytes.
+__device__ __forceinline__ void store_rows(const GemmArgs& a, const char* ep, const Unit& u, int64_t O, int half,
+                                           int pass) {
+  const int64_t o0 = (int64_t)u.nblk * kCols;
+  uint16_t* out = static_cast<uint16_t*>(a.out);
+  const int tid = fresh_tid();
+  if (O % 8 == 0) {
+    for (int i = tid; i < 64 * 32; i += 256) {
+      const int lr = i / 32, unit = i % 32;
+      const int row = half * (lr / 32) + 32 * pass + lr % 32;
+      if (row < u.valid && o0 + 8 * unit < O)
+        *reinterpret_cast<uint4*>(out + (u.row0 + row) * O + o0 + 8 * unit) =
+            *reinterpret_cast<const uint4*>(ep + lr * 512 + ((2 * unit) ^ (2 * (lr % 32))) * 8);
+    }
+  } else {
+    for (int i = tid; i < 64 * kCols; i += 256) {
+      const int lr = i / kCols, c = i % kCols;
+      const int row = half * (lr / 32) + 32 * pass + lr % 32;
+      if (row < u.valid && o0 + c < O)
+        out[(u.row0 + row) * O + o0 + c] =
+            *reinterpret_cast<const uint16_t*>(ep + lr * 512 + ((c / 4) ^ (2 * (lr % 32))) * 8 + (c % 4) * 2);
+    }
+  }
+}
+
+// ----------------------------------------------------------- x W^T, bf16 x
+//
+// Contraction in groups of 64, weights in pairs of groups, so that a weight
+// row is copied 64 bytes at a time.  Per group a wave reads each of its four
+// 32-column subtiles' codes once (16 bytes, one block, per lane) and converts
+// a word of each per step: lane half h supplies elements 32h + 8kk .. + 7 of
+// the group at step kk, from word kk of its block.
+template <bool S4, int MSUB>  // S4: scales copied four blocks at a time (K % 128 == 0, aligned)
+struct Fwd {
+  static constexpr int kA = 64 * MSUB * 128, kB = kCols * 64, kS = kCols * (S4 ? 4 : 16);
+  static constexpr int kBOff = 2 * kA, kSOff = kBOff + 2 * kB;
+  static constexpr int kLds = kSOff + 2 * kS;
+  static constexpr int kACopies = 2 * MSUB;
+
+  struct Ctx {
+    RowSrc<kACopies, 8> x;
+    const char *w, *s;  // the column block's codes and scales
+    uint32_t woff[4];   // copy d's column and unit; the unit
+    uint32_t soff;
+    int wunit[4];
+    uint32_t lds;
+    int wave, lane, units, G;
+    int64_t C;
+  };
+
+  static __device__ __forceinline__ void copy_x(const Ctx& c, int g) {
+    const uint32_t dst = c.lds + (g & 1) * kA + c.wave * 1024;
+    const bool whole = (int64_t)(g + 1) * 64 <= c.C;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int d = 0; d < kACopies; ++d) {
+      const char* p = c.x.p[d] + (size_t)g * 128;
+      if (!whole && (int64_t)g * 64 + c.x.unit[d] * 8 >= c.C) p = reinterpret_cast<const char*>(zero_page);
+      qmoe_gemm::dma16(p, dst + d * 4096);
+    }
+  }
+  static __device__ __forceinline__ void copy_w(const Ctx& c, int p) {
+    const uint32_t dst = c.lds + kBOff + (p & 1) * kB + c.wave * 1024;
+    const uint32_t sdst = c.lds + kSOff + (p & 1) * kS + c.wave * 256;
+    const bool whole = 4 * (p + 1) <= c.units;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      if (whole) {
+        qmoe_gemm::dma16s(c.w + (size_t)p * 64, c.woff[d], dst + d * 4096);
+      } else {
+        const char* q = c.w + (size_t)p * 64 + c.woff[d];
+        if (4 * p + c.wunit[d] >= c.units) q = reinterpret_cast<const char*>(zero_page);
+        qmoe_gemm::dma16(q, dst + d * 4096);
+      }
+    }
+    if constexpr (S4) {
+      qmoe_gemm::dma4s(c.s + (size_t)p * 4, c.soff, sdst);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (4 * p + b < c.units) dma1s(c.s + (size_t)p * 4 + b, c.soff, sdst + b * 1024);
+        else dma1(zero_page, sdst + b * 1024);
+      }
+    }
+  }
+
+  struct Frag {
+    i32x4_t a[MSUB], b[4];
+  };
+  struct Codes {
+    i32x4_t w[4];
+    float s[4];
+  };
+  static __device__ __forceinline__ void read_x(const Ctx& c, const char* smem, int g, int kk, int row0, Frag& f) {
+    const int l32 = c.lane % 32, h = c.lane / 32;
+    const char* st = smem + (g & 1) * kA + row0 * 128;
+#pragma unroll
+    for (int i = 0; i < MSUB; ++i)  // swz8(row0 + 32 i + l32) == swz8(l32)
+      f.a[i] = *reinterpret_cast<const i32x4_t*>(st + (32 * i + l32) * 128 + ((4 * h + kk) ^ swz8(l32)) * 16);
+  }
+  static __device__ __forceinline__ Codes read_codes(const Ctx& c, const char* smem, int g, int col0) {
+    const int l32 = c.lane % 32, unit = 2 * (g & 1) + c.lane / 32;
+    const char* st = smem + kBOff + ((g >> 1) & 1) * kB;
+    const char* ss = smem + kSOff + ((g >> 1) & 1) * kS;
+    Codes r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = col0 + 32 * j + l32;
+      r.w[j] = *reinterpret_cast<const i32x4_t*>(st + col * 64 + (unit ^ swz4(col)) * 16);
+      if constexpr (S4) r.s[j] = scale_of((*reinterpret_cast<const uint32_t*>(ss + col * 4) >> (8 * unit)) & 255u);
+      else r.s[j] = scale_of(*reinterpret_cast<const uint32_t*>(ss + (unit * kCols + col) * 4));
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void convert(const Codes& q, int kk, int j, Frag& f) {
+    uint32_t o[4];
+    unpack8((uint32_t)q.w[j][kk], q.s[j], o);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) f.b[j][d] = (int)o[d];
+  }
+  // One step's products, the next step's conversions between them.
+  template <bool NEXT>
+  static __device__ __forceinline__ void step(const Frag& cur, Frag& nxt, const Codes& q, int kkn,
+                                              f32x16_t (&acc)[MSUB][4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i < MSUB; ++i) {
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, cur.b[j]),
+                                                            __builtin_bit_cast(bf16x8_t, cur.a[i]), acc[i][j], 0, 0, 0);
+        if constexpr (NEXT) {
+          if (i == 0) convert(q, kkn, j, nxt);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  static __device__ void run(const GemmArgs& a, const Unit& u, char* smem) {
+    Ctx c;
+    const int tid = fresh_tid();
+    c.lane = tid % 64;
+    c.wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wm = c.wave / 2, wn = c.wave % 2;
+    c.units = (int)(a.K / kBlock);
+    c.C = a.K;
+    c.G = (int)((a.K + 63) / 64);
+    c.lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)smem);
+    c.x = row_sources<kACopies, 8>(a, u, a.x, a.ldx * 2, c.wave, c.lane);
+    const int64_t row = (int64_t)u.e * a.N + (int64_t)u.nblk * kCols;
+    const int cols = (int)min((int64_t)kCols, a.N - (int64_t)u.nblk * kCols);
+    c.w = reinterpret_cast<const char*>(a.w) + qmoe_gemm::uniform64(row * c.units * 16);
+    c.s = reinterpret_cast<const char*>(a.s) + qmoe_gemm::uniform64(row * c.units);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const int col = (d * 4 + c.wave) * 16 + c.lane / 4;
+      c.wunit[d] = (c.lane % 4) ^ swz4(col);
+      c.woff[d] = (uint32_t)(min(col, cols - 1) * c.units * 16 + c.wunit[d] * 16);
+    }
+    c.soff = (uint32_t)(min(c.wave * 64 + c.lane, cols - 1) * c.units);
+    const int G = c.G, P = (G + 1) / 2;
+    const int row0 = 32 * MSUB * wm, col0 = 128 * wn;
+
+    f32x16_t acc[MSUB][4] = {};
+    copy_x(c, 0);
+    copy_w(c, 0);
+    if (G > 1) copy_x(c, 1);
+    if (P > 1) copy_w(c, 1);
+    qmoe_gemm::wait_vmem<0>();
+    __builtin_amdgcn_s_barrier();
+    Frag fa, fb;
+    Codes q = read_codes(c, smem, 0, col0);
+    read_x(c, smem, 0, 0, row0, fa);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) convert(q, 0, j, fa);
+    for (int g = 0; g < G - 1; ++g) {
+      read_x(c, smem, g, 1, row0, fb);
+      step<true>(fa, fb, q, 1, acc);
+      read_x(c, smem, g, 2, row0, fa);
+      step<true>(fb, fa, q, 2, acc);
+      read_x(c, smem, g, 3, row0, fb);
+      step<true>(fa, fb, q, 3, acc);
+      qmoe_gemm::wait_vmem<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      if (g + 2 < G) copy_x(c, g + 2);
+      if ((g & 1) && (g >> 1) + 2 < P) copy_w(c, (g >> 1) + 2);
+      q = read_codes(c, smem, g + 1, col0);
+      read_x(c, smem, g + 1, 0, row0, fa);
+      step<true>(fb, fa, q, 0, acc);
+    }
+    read_x(c, smem, G - 1, 1, row0, fb);
+    step<true>(fa, fb, q, 1, acc);
+    read_x(c, smem, G - 1, 2, row0, fa);
+    step<true>(fb, fa, q, 2, acc);
+    read_x(c, smem, G - 1, 3, row0, fb);
+    step<true>(fa, fb, q, 3, acc);
+    step<false>(fb, fa, q, 0, acc);
+    const int lane = fresh_tid() % 64, l32 = lane % 32, h = lane / 32;
+    if (a.out_f32) {
+#pragma unroll
+      for (int i = 0; i < MSUB; ++i) {
+        const int r = row0 + 32 * i + l32;
+        if (r >= u.valid) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int64_t o = (int64_t)u.nblk * kCols + col0 + 32 * j + 8 * (v / 4) + 4 * h + v % 4;
+            if (o < a.N) static_cast<float*>(a.out)[(u.row0 + r) * a.N + o] = acc[i][j][v];
+          }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < MSUB; ++i) {
+      __syncthreads();
+      const int lr = 32 * wm + l32;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+          const int gi = (col0 + 32 * j + 2 * v + 4 * h) / 4;
+          *reinterpret_cast<uint2*>(smem + lr * 512 + (gi ^ (2 * l32)) * 8) =
+              make_uint2(qmoe_gemm::cvt_pk_bf16(acc[i][j][v], acc[i][j][v + 1]),
+                         qmoe_gemm::cvt_pk_bf16(acc[i][j][v + 2], acc[i][j][v + 3]));
+        }
+      __syncthreads();
+      store_rows(a, smem, u, a.N, 32 * MSUB, i);
+    }
+  }
+};
+
+// ------------------------------------------------------------- x W, bf16 x
+//
+// The contraction runs over the weights' rows n, in groups of 64; the outputs
+// lie along the packed axis.  A lane takes one word of codes (eight outputs)
+// of eight consecutive rows n: four conversions a word give pairs of outputs
+// of one n, and a byte permute of two n's words gives the pairs of n of one
+// output that the matrix instruction wants.  With v_mfma_f32_16x16x32 the
+// sixteen words of a wave's 128 outputs are the sixteen lanes of a quarter
+// wave and the four quarters the four octets of n, so no value crosses lanes:
+// the sixteen outputs of subtile j are 8c + j, c = 0 .. 15.
+template <bool S4, int MSUB>  // MSUB: 16-row subtiles per wave
+struct Trn {
+  static constexpr int kA = 32 * MSUB * 128, kB = 64 * 128, kS = 64 * (S4 ? 8 : 32);
+  static constexpr int kStage = kA + kB + kS;
+  static constexpr int NS = 3;
+  static constexpr int kLds = NS * kStage;
+  static constexpr int kACopies = MSUB;
+  static constexpr int kCopies = kACopies + 2 + (S4 ? 1 : 2);  // per wave and group
+
+  struct Ctx {
+    RowSrc<kACopies, 8> x;
+    const char *w, *s;  // of the expert's first row, at the column block
+    int64_t wpitch, spitch;
+    int wunit, wrow, sblk[2];
+    uint32_t lds;
+    int wave, lane, G;
+    int64_t C;
+  };
+
+  static __device__ __forceinline__ void copy(const Ctx& c, int g) {
+    const uint32_t st = c.lds + (g % NS) * kStage;
+    const int64_t left = c.C - (int64_t)g * 64;  // rows n of this group and after
+#pragma unroll
+    for (int d = 0; d < kACopies; ++d) {
+      const char* p = c.x.p[d] + (size_t)g * 128;
+      if (c.x.unit[d] * 8 >= left) p = reinterpret_cast<const char*>(zero_page);
+      qmoe_gemm::dma16(p, st + (d * 4 + c.wave) * 1024);
+    }
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const int n = c.wrow + 32 * d;
+      const char* p = c.w + ((int64_t)g * 64 + n) * c.wpitch;
+      if (n >= left) p = reinterpret_cast<const char*>(zero_page);
+      qmoe_gemm::dma16(p, st + kA + (d * 4 + c.wave) * 1024);
+    }
+    const char* s = c.s + ((int64_t)g * 64 + c.lane) * c.spitch;
+    if constexpr (S4) {
+      s += c.sblk[0];
+      if (c.lane >= left) s = reinterpret_cast<const char*>(zero_page);
+      qmoe_gemm::dma4(s, st + kA + kB + (c.wave & 1) * 256);
+    } else {
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const char* p = s + c.sblk[d];
+        if (c.lane >= left) p = reinterpret_cast<const char*>(zero_page);
+        dma1(p, st + kA + kB + (2 * c.wave + d) * 256);
+      }
+    }
+  }
+
+  struct Words {
+    uint32_t w[8];
+    float s[8];
+  };
+  static __device__ __forceinline__ Words read_words(const Ctx& c, const char* smem, int g, int s, int wn) {
+    const int co = c.lane % 16, q = c.lane / 16;
+    const char* st = smem + (g % NS) * kStage + kA;
+    const int unit = (4 * wn + co / 4) ^ (4 * (q >> 1));
+    Words r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int pos = (32 * s + 8 * q + i) ^ (q & 1);
+      r.w[i] = *reinterpret_cast<const uint32_t*>(st + pos * 128 + unit * 16 + (co % 4) * 4);
+    }
+    const int blk = 4 * wn + co / 4;
+    const char* ss = st + kB + (S4 ? wn : blk) * 256 + (32 * s + 8 * q) * 4;
+    const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(ss), hi = *reinterpret_cast<const i32x4_t*>(ss + 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t v = (uint32_t)(i < 4 ? lo[i & 3] : hi[i & 3]);
+      r.s[i] = scale_of(S4 ? (v >> (8 * (co / 4))) & 255u : v);
+    }
+    return r;
+  }
+  // Fragments of outputs 8c + 2T and 8c + 2T + 1.
+  template <int T>
+  static __device__ __forceinline__ void pair(const Words& q, i32x4_t (&b)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = pair_of<T>(q.w[2 * i], q.s[2 * i]), hi = pair_of<T>(q.w[2 * i + 1], q.s[2 * i + 1]);
+      b[0][i] = (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u);
+      b[1][i] = (int)__builtin_amdgcn_perm(hi, lo, 0x07060302u);
+    }
+  }
+  static __device__ __forceinline__ void read_x(const Ctx& c, const char* smem, int g, int s, int row0,
+                                                i32x4_t (&f)[MSUB]) {
+    const int l16 = c.lane % 16, q = c.lane / 16;
+    const char* st = smem + (g % NS) * kStage + row0 * 128;
+#pragma unroll
+    for (int i = 0; i < MSUB; ++i)
+      f[i] = *reinterpret_cast<const i32x4_t*>(st + (16 * i + l16) * 128 + ((4 * s + q) ^ swz8(l16)) * 16);
+  }
+  static __device__ __forceinline__ void products(const i32x4_t (&x)[MSUB], const i32x4_t (&b)[2],
+                                                  f32x4_t (&acc)[MSUB][8], int t) {
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int i = 0; i < MSUB; ++i)
+        acc[i][2 * t + v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b[v]),
+                                                                    __builtin_bit_cast(bf16x8_t, x[i]),
+                                                                    acc[i][2 * t + v], 0, 0, 0);
+  }
+  // One step: the pairs of outputs in turn, each prepared during the one before.
+  static __device__ __forceinline__ void step(const i32x4_t (&x)[MSUB], const Words& cur, const Words& nxt,
+                                              i32x4_t (&b0)[2], i32x4_t (&b1)[2], f32x4_t (&acc)[MSUB][8]) {
+    pair<1>(cur, b1);
+    products(x, b0, acc, 0);
+    pair<2>(cur, b0);
+    products(x, b1, acc, 1);
+    pair<3>(cur, b1);
+    products(x, b0, acc, 2);
+    pair<0>(nxt, b0);
+    products(x, b1, acc, 3);
+  }
+
+  static __device__ void run(const GemmArgs& a, const Unit& u, char* smem) {
+    Ctx c;
+    const int tid = fresh_tid();
+    c.lane = tid % 64;
+    c.wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wm = c.wave / 2, wn = c.wave % 2;
+    const int64_t units = a.K / kBlock;
+    c.C = a.N;
+    c.G = (int)((a.N + 63) / 64);
+    c.lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)smem);
+    c.x = row_sources<kACopies, 8>(a, u, a.x, a.ldx * 2, c.wave, c.lane);
+    const int64_t row = (int64_t)u.e * a.N, u0 = (int64_t)u.nblk * (kCols / kBlock);
+    const int last = (int)min((int64_t)(kCols / kBlock), units - u0) - 1;  // columns past the end: the last again
+    c.wpitch = units * 16;
+    c.spitch = units;
+    // copy d's row slot 32d + 8 wave + lane / 8 holds row n = slot ^ (slot / 8 & 1), its unit slot the unit
+    // ^ 4 (slot / 16 & 1): the eight words a lane reads then fall on all 64 banks
+    const int pos = 8 * c.wave + c.lane / 8;
+    c.wrow = pos ^ ((pos >> 3) & 1);
+    c.wunit = (c.lane % 8) ^ (4 * ((pos >> 4) & 1));
+    c.w = reinterpret_cast<const char*>(a.w) + (row * units + u0 + min(c.wunit, last)) * 16;
+    c.s = reinterpret_cast<const char*>(a.s) + row * units + u0;
+    if constexpr (S4) c.sblk[0] = 4 * (c.wave & 1) <= last ? 4 * (c.wave & 1) : 0;
+    else
+#pragma unroll
+      for (int d = 0; d < 2; ++d) c.sblk[d] = min(2 * c.wave + d, last);
+    const int G = c.G;
+    const int row0 = 16 * MSUB * wm;
+
+    f32x4_t acc[MSUB][8] = {};
+#pragma unroll
+    for (int i = 0; i < NS; ++i) copy(c, min(i, G - 1));
+    qmoe_gemm::wait_vmem<(NS - 1) * kCopies>();
+    __builtin_amdgcn_s_barrier();
+    i32x4_t xa[MSUB], xb[MSUB], b0[2], b1[2];
+    Words wa = read_words(c, smem, 0, 0, wn), wb;
+    read_x(c, smem, 0, 0, row0, xa);
+    pair<0>(wa, b0);
+    for (int g = 0; g < G - 1; ++g) {
+      wb = read_words(c, smem, g, 1, wn);
+      read_x(c, smem, g, 1, row0, xb);
+      step(xa, wa, wb, b0, b1, acc);
+      // group g + 1 landed (copies of NS - 2 groups after it may be in flight); all reads of stage g are done
+      qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      copy(c, min(g + NS, G - 1));  // past the end: the last group again, the same bytes to where they are
+      wa = read_words(c, smem, g + 1, 0, wn);
+      read_x(c, smem, g + 1, 0, row0, xa);
+      step(xb, wb, wa, b0, b1, acc);
+    }
+    wb = read_words(c, smem, G - 1, 1, wn);
+    read_x(c, smem, G - 1, 1, row0, xb);
+    step(xa, wa, wb, b0, b1, acc);
+    step(xb, wb, wb, b0, b1, acc);
+    qmoe_gemm::wait_vmem<0>();
+    const int lane = fresh_tid() % 64, l16 = lane % 16, q = lane / 16;
+    if (a.out_f32) {
+#pragma unroll
+      for (int i = 0; i < MSUB; ++i) {
+        const int r = row0 + 16 * i + l16;
+        if (r >= u.valid) continue;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int64_t o = (int64_t)u.nblk * kCols + 128 * wn + 8 * (4 * q + t);
+          if (o >= a.K) continue;
+          f32x4_t* out = reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + (u.row0 + r) * a.K + o);
+          out[0] = f32x4_t{acc[i][0][t], acc[i][1][t], acc[i][2][t], acc[i][3][t]};
+          out[1] = f32x4_t{acc[i][4][t], acc[i][5][t], acc[i][6][t], acc[i][7][t]};
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int p = 0; p < MSUB / 2; ++p) {
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int i = 2 * p + v, lr = 32 * wm + 16 * v + l16;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int gi = 2 * (16 * wn + 4 * q + t);
+          uint4 o;
+          o.x = qmoe_gemm::cvt_pk_bf16(acc[i][0][t], acc[i][1][t]);
+          o.y = qmoe_gemm::cvt_pk_bf16(acc[i][2][t], acc[i][3][t]);
+          o.z = qmoe_gemm::cvt_pk_bf16(acc[i][4][t], acc[i][5][t]);
+          o.w = qmoe_gemm::cvt_pk_bf16(acc[i][6][t], acc[i][7][t]);
+          *reinterpret_cast<uint4*>(smem + lr * 512 + (gi ^ (2 * (lr % 32))) * 8) = o;
+        }
+      }
+      __syncthreads();
+      store_rows(a, smem, u, a.K, 16 * MSUB, p);
+    }
+  }
+};
+
+// ------------------------------------------------------- x W^T, both mxfp4
+//
+// v_mfma_scale_f32_32x32x64_f8f6f4 takes both operands as codes, 16 bytes of
+// one block per lane, and a scale byte for each; nothing is converted.
+// Contraction in groups of 128.  A lane's scale byte at step kk is block 2kk +
+// h of its row: the row's four bytes shifted by h, byte 2kk picked by the
+// instruction.
+template <bool S4, int MSUB>
+struct QQ {
+  static constexpr int kRows = 64 * MSUB;
+  static constexpr int kA = kRows * 64, kB = kCols * 64;
+  static constexpr int kSA = kTileRows * (S4 ? 4 : 16), kSB = kCols * (S4 ? 4 : 16);
+  static constexpr int kBOff = kA, kSAOff = kBOff + kB, kSBOff = kSAOff + kSA, kStage = kSBOff + kSB;
+  static constexpr int NS = S4 ? 3 : 2;
+  static constexpr int kLds = NS * kStage;
+  static constexpr int kACopies = MSUB;
+  static constexpr int kCopies = kACopies + 4 + (S4 ? 2 : 8);
+
+  struct Ctx {
+    RowSrc<kACopies, 4> x;
+    const char *w, *s, *xs;
+    uint32_t woff[4], soff;
+    int wunit[4];
+    uint32_t lds;
+    int wave, lane, units, G;
+  };
+
+  static __device__ __forceinline__ void copy(const Ctx& c, int g) {
+    const uint32_t st = c.lds + (g % NS) * kStage;
+    const bool whole = 4 * (g + 1) <= c.units;
+#pragma unroll
+    for (int d = 0; d < kACopies; ++d) {
+      const char* p = c.x.p[d] + (size_t)g * 64;
+      if (!whole && 4 * g + c.x.unit[d] >= c.units) p = reinterpret_cast<const char*>(zero_page);
+      qmoe_gemm::dma16(p, st + (d * 4 + c.wave) * 1024);
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      if (whole) {
+        qmoe_gemm::dma16s(c.w + (size_t)g * 64, c.woff[d], st + kBOff + (d * 4 + c.wave) * 1024);
+      } else {
+        const char* q = c.w + (size_t)g * 64 + c.woff[d];
+        if (4 * g + c.wunit[d] >= c.units) q = reinterpret_cast<const char*>(zero_page);
+        qmoe_gemm::dma16(q, st + kBOff + (d * 4 + c.wave) * 1024);
+      }
+    }
+    if constexpr (S4) {
+      qmoe_gemm::dma4(c.xs + (size_t)g * 4, st + kSAOff + (c.wave & 1) * 256);
+      qmoe_gemm::dma4s(c.s + (size_t)g * 4, c.soff, st + kSBOff + c.wave * 256);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const bool in = 4 * g + b < c.units;
+        dma1(in ? c.xs + (size_t)g * 4 + b : reinterpret_cast<const char*>(zero_page),
+             st + kSAOff + b * 512 + (c.wave & 1) * 256);
+        if (in) dma1s(c.s + (size_t)g * 4 + b, c.soff, st + kSBOff + b * 1024 + c.wave * 256);
+        else dma1(zero_page, st + kSBOff + b * 1024 + c.wave * 256);
+      }
+    }
+  }
+
+  // A row's four scale bytes in group g, those of lane half h at bytes 0 and 2.
+  static __device__ __forceinline__ int scales(const char* st, int rows, int row, int h) {
+    if constexpr (S4) {
+      return (int)(*reinterpret_cast<const uint32_t*>(st + row * 4) >> (8 * h));
+    } else {
+      const uint32_t lo = *reinterpret_cast<const uint32_t*>(st + (h * rows + row) * 4);
+      const uint32_t hi = *reinterpret_cast<const uint32_t*>(st + ((2 + h) * rows + row) * 4);
+      return (int)(lo | (hi << 16));
+    }
+  }
+  struct Frag {
+    i32x4_t a[MSUB], b[4];
+  };
+  static __device__ __forceinline__ void read(const Ctx& c, const char* st, int kk, int row0, int col0, Frag& f) {
+    const int l32 = c.lane % 32, unit = (2 * kk + c.lane / 32) ^ swz4(l32);  // swz4 repeats every 16 rows
+#pragma unroll
+    for (int i = 0; i < MSUB; ++i)
+      f.a[i] = *reinterpret_cast<const i32x4_t*>(st + (row0 + 32 * i + l32) * 64 + unit * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      f.b[j] = *reinterpret_cast<const i32x4_t*>(st + kBOff + (col0 + 32 * j + l32) * 64 + unit * 16);
+  }
+  typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8_t;
+  static __device__ __forceinline__ i32x8_t wide(const i32x4_t& v) {
+    return i32x8_t{v[0], v[1], v[2], v[3], 0, 0, 0, 0};  // the fp4 form reads the first four registers
+  }
+  template <int KK>
+  static __device__ __forceinline__ void products(const Frag& f, const int (&sa)[MSUB], const int (&sb)[4],
+                                                  f32x16_t (&acc)[MSUB][4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int m = 32 * wave + 16 * i + lane % 16;
-        const int64_t o = o0 + 16 * j + 4 * (lane / 16) + q;
-        if (m >= t.valid || o >= O) continue;
-        const int64_t at = (t.row0 + m) * O + o;
-        if (a.out_f32) static_cast<float*>(a.out)[at] = acc[i][j][q];
-        else static_cast<uint16_t*>(a.out)[at] = (uint16_t)f32_to_bf16(acc[i][j][q]);
+      for (int i = 0; i < MSUB; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f.b[j]), wide(f.a[i]), acc[i][j], 4, 4,
+                                                                    2 * KK, sb[j], 2 * KK, sa[i]);
+  }
+
+  static __device__ void run(const GemmArgs& a, const Unit& u, char* smem) {
+    Ctx c;
+    const int tid = fresh_tid();
+    c.lane = tid % 64;
+    c.wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wm = c.wave / 2, wn = c.wave % 2;
+    c.units = (int)(a.K / kBlock);
+    c.G = (c.units + 3) / 4;
+    c.lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)smem);
+    c.x = row_sources<kACopies, 4>(a, u, a.xq, (int64_t)c.units * 16, c.wave, c.lane);
+    {
+      const int64_t i = u.row0 + min((c.wave & 1) * 64 + c.lane, u.valid - 1);
+      const int64_t x = min(max(a.x_rows ? (int64_t)a.x_rows[i] : i, (int64_t)0), a.n_x - 1);
+      c.xs = reinterpret_cast<const char*>(a.xs) + x * c.units;
+    }
+    const int64_t row = (int64_t)u.e * a.N + (int64_t)u.nblk * kCols;
+    const int cols = (int)min((int64_t)kCols, a.N - (int64_t)u.nblk * kCols);
+    c.w = reinterpret_cast<const char*>(a.w) + qmoe_gemm::uniform64(row * c.units * 16);
+    c.s = reinterpret_cast<const char*>(a.s) + qmoe_gemm::uniform64(row * c.units);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const int col = (d * 4 + c.wave) * 16 + c.lane / 4;
+      c.wunit[d] = (c.lane % 4) ^ swz4(col);
+      c.woff[d] = (uint32_t)(min(col, cols - 1) * c.units * 16 + c.wunit[d] * 16);
+    }
+    c.soff = (uint32_t)(min(c.wave * 64 + c.lane, cols - 1) * c.units);
+    const int G = c.G;
+    const int row0 = 32 * MSUB * wm, col0 = 128 * wn;
+    const int l32 = c.lane % 32, h = c.lane / 32;
+
+    f32x16_t acc[MSUB][4] = {};
+#pragma unroll
+    for (int i = 0; i < NS; ++i) copy(c, min(i, G - 1));
+    qmoe_gemm::wait_vmem<(NS - 1) * kCopies>();
+    __builtin_amdgcn_s_barrier();
+    Frag fa, fb;
+    int sa[MSUB], sb[4];
+    read(c, smem, 0, row0, col0, fa);
+    for (int g = 0; g < G; ++g) {
+      const char* st = smem + (g % NS) * kStage;
+#pragma unroll
+      for (int i = 0; i < MSUB; ++i) sa[i] = scales(st + kSAOff, kTileRows, row0 + 32 * i + l32, h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sb[j] = scales(st + kSBOff, kCols, col0 + 32 * j + l32, h);
+      read(c, st, 1, row0, col0, fb);
+      products<0>(fa, sa, sb, acc);
+      if (g + 1 < G) {
+        qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        copy(c, min(g + NS, G - 1));
+        read(c, smem + ((g + 1) % NS) * kStage, 0, row0, col0, fa);
       }
+      products<1>(fb, sa, sb, acc);
+    }
+    qmoe_gemm::wait_vmem<0>();
+    const int el = fresh_tid() % 64, e32 = el % 32, eh = el / 32;
+#pragma unroll
+    for (int i = 0; i < MSUB; ++i) {
+      __syncthreads();
+      const int lr = 32 * wm + e32;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+          const int gi = (col0 + 32 * j + 2 * v + 4 * eh) / 4;
+          *reinterpret_cast<uint2*>(smem + lr * 512 + (gi ^ (2 * e32)) * 8) =
+              make_uint2(qmoe_gemm::cvt_pk_bf16(acc[i][j][v], acc[i][j][v + 1]),
+                         qmoe_gemm::cvt_pk_bf16(acc[i][j][v + 2], acc[i][j][v + 3]));
+        }
+      __syncthreads();
+      store_rows(a, smem, u, a.N, 32 * MSUB, i);
+    }
+  }
+};
+
+template <int MODE, bool S4>
+struct Kernel;
+template <bool S4>
+struct Kernel<kFwd, S4> {
+  typedef Fwd<S4, 2> Full;
+  typedef Fwd<S4, 1> Half;
+};
+template <bool S4>
+struct Kernel<kT, S4> {
+  typedef Trn<S4, 4> Full;
+  typedef Trn<S4, 2> Half;
+};
+template <bool S4>
+struct Kernel<kQQ, S4> {
+  typedef QQ<S4, 2> Full;
+  typedef QQ<S4, 1> Half;
+};
+
+template <int MODE, bool S4>
+__global__ __launch_bounds__(256, 2) void mx_gemm_kernel(GemmArgs a, int64_t dense_tiles, int NB) {
+  typedef Kernel<MODE, S4> K;
+  constexpr int kRing = K::Full::kLds > K::Half::kLds ? K::Full::kLds : K::Half::kLds;
+  static_assert(kRing >= 64 * 512, "the epilogue's 64 rows");
+  static_assert(kRing >= 4 * qmoe_gemm::kMaxOrder, "the ranking's scratch");
+  static_assert(2 * (kRing + 4 * qmoe_gemm::kMaxOrder) <= 160 * 1024, "two blocks per CU");
+  __shared__ __attribute__((aligned(16))) char smem[kRing];
+  __shared__ int order[qmoe_gemm::kMaxOrder];
+  const int64_t tiles = a.offsets ? (int64_t)max(a.ntiles[0], 0) : dense_tiles;
+  const bool ranked = a.offsets && tiles <= qmoe_gemm::kMaxOrder;
+  if (ranked) {
+    const qmoe_gemm::Tiles table{a.offsets, a.tile_row, a.tile_exp, a.ntiles, a.n_rows, a.num_experts};
+    qmoe_gemm::rank_tiles(table, (int)tiles, order, reinterpret_cast<int*>(smem));
+  }
+  const qmoe_gemm::Snake snake(tiles * NB);
+  for (int64_t k = 0;; ++k) {
+    const int64_t at = snake.unit(k);
+    if (at < 0) break;
+    int64_t tile = at / NB;
+    if (ranked) tile = order[tile];
+    const qmoe_gemm::TileRows t = tile_of(a, tile);
+    if (t.valid <= 0) continue;
+    Unit u;
+    u.e = __builtin_amdgcn_readfirstlane(t.e);
+    u.valid = __builtin_amdgcn_readfirstlane(t.valid);
+    u.nblk = __builtin_amdgcn_readfirstlane((int)(at % NB));
+    u.row0 = qmoe_gemm::uniform64(t.row0);
+    if (u.valid > kRowsHalf) K::Full::run(a, u, smem);
+    else K::Half::run(a, u, smem);
+    __syncthreads();  // the ring is free for the next unit
+  }
 }
 
 template <int MODE>
 int launch(GemmArgs a, int64_t max_tiles, hipStream_t st) {
   const int64_t O = MODE == kT ? a.K : a.N;
-  const int64_t tiles = a.offsets ? max_tiles : (a.n_rows + kTileRows - 1) / kTileRows;
-  const int64_t cols = (O + kOut - 1) / kOut;
-  if (tiles > 0x7FFFFFFF || cols > 65535) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
-  mx_gemm_kernel<MODE><<<dim3((unsigned)tiles, (unsigned)cols), dim3(256), 0, st>>>(a);
+  const int64_t dense = (a.n_rows + kTileRows - 1) / kTileRows;
+  const int64_t NB = (O + kCols - 1) / kCols;
+  const dim3 grid((unsigned)qmoe_gemm::grid_blocks((a.offsets ? max_tiles : dense) * NB)), block(256);
+  const auto even = [](const void* p) { return qmoe::aligned4(p); };
+  if (a.K % 128 == 0 && even(a.s) && (MODE != kQQ || even(a.xs))) mx_gemm_kernel<MODE, true><<<grid, block, 0, st>>>(a, dense, (int)NB);
+  else mx_gemm_kernel<MODE, false><<<grid, block, 0, st>>>(a, dense, (int)NB);
   return qmoe::launch_status("mx_gemm_kernel");
 }
 
@@ -146,7 +831,8 @@ int check(const GemmArgs& a, int mode, int64_t max_tiles, int out_dtype, bool* r
   if (!any && a.num_experts != 1) return qmoe::fail(QMOE_ERR_INVALID, "several experts need a tile table");
   if (!any && !a.x_rows && a.n_x < a.n_rows) return qmoe::fail(QMOE_ERR_INVALID, "fewer activation rows than rows");
   if (any && max_tiles == 0) return qmoe::fail(QMOE_ERR_INVALID, "an empty tile table");
-  if (a.N > 0x7FFFFFFF || a.K > 0x7FFFFFFF || a.n_rows > 0x7FFFFFFF || a.n_x > 0x7FFFFFFF || max_tiles > 0x7FFFFFFF)
+  // a block of 256 weight rows is addressed by 32-bit byte offsets
+  if (a.N > 0x7FFFFFFF || a.K > (1 << 23) || a.n_rows > 0x7FFFFFFF || a.n_x > 0x7FFFFFFF || max_tiles > 0x7FFFFFFF)
     return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
   if (!qmoe::aligned16(a.w) || !qmoe::aligned16(a.out)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "codes and out must be 16-byte aligned");
   if (mode == kQQ ? !qmoe::aligned16(a.xq) : (!qmoe::aligned16(a.x) || a.ldx % 8 || a.ldx < C))
