@@ -176,3 +176,13 @@ def test_graph_replays(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_second_derivatives_are_refused(dev):
+    """The gradients are not differentiable themselves, and say so instead of being constants."""
+    g, ids, order, inv, x, ys, scores = _setup(dev, 4, 2, 4, 16, torch.float32)
+    xd = x.to(dev).requires_grad_(True)
+    (dx,) = torch.autograd.grad(ops.sort_tokens(xd, order.to(dev), inv.to(dev)).square().sum(), xd, create_graph=True)
+    assert torch.equal(dx.cpu(), 2 * 2 * x)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()

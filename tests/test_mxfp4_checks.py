@@ -122,7 +122,7 @@ def test_gather(op):
             op(x, w, s, rhs_indices=bad, **kw)
         with pytest.raises(TypeError, match="lhs_indices"):
             op(x, w, s, lhs_indices=bad, rhs_indices=ids, **kw)
-    with pytest.raises(RuntimeError):  # batches that do not broadcast
+    with pytest.raises(ValueError, match="broadcast"):
         op(x, w, s, rhs_indices=ids[:2], **kw)
     with pytest.raises(ValueError, match="no activation rows"):
         op(x[:0], w, s, lhs_indices=ids, rhs_indices=ids, **kw)

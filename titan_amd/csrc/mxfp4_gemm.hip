@@ -2,6 +2,8 @@
 // activations either way round (x W^T over the packed axis, x W over the
 // rows), and activations in mxfp4 too (format in mxfp4.h).  Rows are those of
 // a tile table (sorted by expert), or of one expert without a table.
+#include <algorithm>
+
 #include "gemm_common.h"
 #include "mxfp4.h"
 
@@ -56,8 +58,14 @@ __device__ __forceinline__ qmoe_gemm::TileRows tile_of(const GemmArgs& a, int64_
 // a group's last step, whose operands are in registers by then: past it the
 // next group's first fragments are read, and the stage just emptied takes the
 // copies of NS groups ahead.
+//
+// Where the units are too few for that to fill the chip (SPLIT), a unit is 64
+// (32) rows times 128 outputs, every wave computes all of it over a quarter of
+// the contraction, in a ring of its own without barriers, and the four partial
+// sums are added through LDS in wave order: an eighth of the work per unit.
 constexpr int kRowsHalf = kTileRows / 2;
-constexpr int kCols = 256;
+constexpr int kWideCols = 256, kSplitCols = 128;
+constexpr int kLdsCU = 160 * 1024;
 __device__ __attribute__((aligned(16))) uint32_t zero_page[4];  // what copies past the contraction's end read
 
 __device__ __forceinline__ void dma1s(const void* sbase, uint32_t voff, uint32_t lds_base) {
@@ -88,8 +96,31 @@ __device__ __forceinline__ int fresh_tid() {
 }
 
 struct Unit {
-  int e, valid, nblk;
-  int64_t row0;
+  int e, valid;
+  int64_t row0, o0;  // first row; first output
+};
+
+// What differs between the two ways: outputs per unit, the waves that fill one
+// ring, and the wave's part of the groups (in steps of UNIT groups).
+template <bool SPLIT>
+struct Geo {
+  static constexpr int kCols = SPLIT ? kSplitCols : kWideCols;
+  static constexpr int kWaves = SPLIT ? 1 : 4;  // per ring
+  static constexpr int kRings = SPLIT ? 4 : 1;
+  static __device__ __forceinline__ void barrier() {
+    if constexpr (!SPLIT) __builtin_amdgcn_s_barrier();
+  }
+  template <int UNIT>
+  static __device__ __forceinline__ void part(int groups, int wave, int* first, int* end) {
+    if constexpr (SPLIT) {
+      const int per = ((groups + UNIT - 1) / UNIT + 3) / 4 * UNIT;
+      *first = min(wave * per, groups);
+      *end = min(*first + per, groups);
+    } else {
+      *first = 0;
+      *end = groups;
+    }
+  }
 };
 
 // Swizzle of the eight 16-byte units of a 128-byte activation row in LDS, of
@@ -101,48 +132,88 @@ __device__ __forceinline__ int swz4(int row) { return (row >> 2) & 3; }
 // Sources of the copies of the tile's activation rows: copy d of a wave fills
 // 1 KiB, 64 / UNITS rows of UNITS 16-byte units.  Rows past the tile's end are
 // its last row again (nothing of them is stored).
-template <int COPIES, int UNITS>
+template <int COPIES, int UNITS, int WAVES>
 struct RowSrc {
   const char* p[COPIES];
-  int unit[COPIES];
+  int unit0;
+  // source unit of copy d: the row's swizzle differs between copies only where a lone wave makes all of them
+  __device__ __forceinline__ int unit(int d) const { return UNITS == 8 && WAVES == 1 ? unit0 ^ (d & 1) : unit0; }
 };
-template <int COPIES, int UNITS>
-__device__ __forceinline__ RowSrc<COPIES, UNITS> row_sources(const GemmArgs& a, const Unit& u, const void* base,
+template <int COPIES, int UNITS, int WAVES>
+__device__ __forceinline__ RowSrc<COPIES, UNITS, WAVES> row_sources(const GemmArgs& a, const Unit& u, const void* base,
                                                              int64_t pitch, int wave, int lane) {
-  RowSrc<COPIES, UNITS> r;
+  RowSrc<COPIES, UNITS, WAVES> r;
+  r.unit0 = (lane % UNITS) ^ (UNITS == 8 ? swz8(wave * 8 + lane / UNITS) : swz4(lane / UNITS));
 #pragma unroll
   for (int d = 0; d < COPIES; ++d) {
-    const int row = (d * 4 + wave) * (64 / UNITS) + lane / UNITS;
-    r.unit[d] = (lane % UNITS) ^ (UNITS == 8 ? swz8(row) : swz4(row));
+    const int row = (d * WAVES + wave) * (64 / UNITS) + lane / UNITS;
     const int64_t i = u.row0 + min(row, u.valid - 1);
     const int64_t x = min(max(a.x_rows ? (int64_t)a.x_rows[i] : i, (int64_t)0), a.n_x - 1);
-    r.p[d] = static_cast<const char*>(base) + x * pitch + r.unit[d] * 16;
+    r.p[d] = static_cast<const char*>(base) + x * pitch + r.unit(d) * 16;
   }
   return r;
 }
 
-// Writes a unit's results.  put(i, j, ...) pieces are staged through LDS, 64
-// rows a pass, so that a row's 256 results leave as 512 contiguous bytes.
-__device__ __forceinline__ void store_rows(const GemmArgs& a, const char* ep, const Unit& u, int64_t O, int half,
-                                           int pass) {
-  const int64_t o0 = (int64_t)u.nblk * kCols;
+// One pass of a unit's results, staged in LDS as 64 rows of 256 bf16, so that a
+// row leaves as 512 contiguous bytes.  HALF rows per wave: with two waves along
+// the rows (WM) a pass takes 32 of each one's, else 64 of the one's.
+template <int WM, int HALF>
+__device__ __forceinline__ void store_rows(const GemmArgs& a, const char* ep, const Unit& u, int64_t O, int pass) {
   uint16_t* out = static_cast<uint16_t*>(a.out);
   const int tid = fresh_tid();
+  const auto row_of = [&](int lr) {  // past the tile's end: not stored
+    if constexpr (WM == 1) return 64 * pass + lr;
+    const int r = 32 * pass + lr % 32;
+    return r < HALF ? HALF * (lr / 32) + r : kTileRows;
+  };
   if (O % 8 == 0) {
     for (int i = tid; i < 64 * 32; i += 256) {
       const int lr = i / 32, unit = i % 32;
-      const int row = half * (lr / 32) + 32 * pass + lr % 32;
-      if (row < u.valid && o0 + 8 * unit < O)
-        *reinterpret_cast<uint4*>(out + (u.row0 + row) * O + o0 + 8 * unit) =
+      const int row = row_of(lr);
+      if (row < u.valid && u.o0 + 8 * unit < O)
+        *reinterpret_cast<uint4*>(out + (u.row0 + row) * O + u.o0 + 8 * unit) =
             *reinterpret_cast<const uint4*>(ep + lr * 512 + ((2 * unit) ^ (2 * (lr % 32))) * 8);
     }
   } else {
-    for (int i = tid; i < 64 * kCols; i += 256) {
-      const int lr = i / kCols, c = i % kCols;
-      const int row = half * (lr / 32) + 32 * pass + lr % 32;
-      if (row < u.valid && o0 + c < O)
-        out[(u.row0 + row) * O + o0 + c] =
+    for (int i = tid; i < 64 * 256; i += 256) {
+      const int lr = i / 256, c = i % 256;
+      const int row = row_of(lr);
+      if (row < u.valid && u.o0 + c < O)
+        out[(u.row0 + row) * O + u.o0 + c] =
             *reinterpret_cast<const uint16_t*>(ep + lr * 512 + ((c / 4) ^ (2 * (lr % 32))) * 8 + (c % 4) * 2);
+    }
+  }
+}
+
+// A split unit's results: the waves' partial sums, staged as ROWS x 128 floats
+// each, 16-byte units of a row swizzled by row, added in wave order.
+__device__ __forceinline__ int part_at(int row, int col4) { return (row * 32 + (col4 ^ (row & 31))) * 16; }
+template <int ROWS>
+__device__ __forceinline__ void store_parts(const GemmArgs& a, const char* ep, const Unit& u, int64_t O) {
+  const int tid = fresh_tid();
+  for (int i = tid; i < ROWS * 32; i += 256) {
+    const int row = i / 32, c = i % 32;
+    if (row >= u.valid) continue;
+    f32x4_t v = *reinterpret_cast<const f32x4_t*>(ep + part_at(row, c));
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const f32x4_t p = *reinterpret_cast<const f32x4_t*>(ep + w * ROWS * 512 + part_at(row, c));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] += p[k];
+    }
+    const int64_t o = u.o0 + 4 * c, at = (u.row0 + row) * O + o;
+    if (o >= O) continue;
+    if (a.out_f32) {
+      float* out = static_cast<float*>(a.out) + at;
+      if (O % 4 == 0) *reinterpret_cast<f32x4_t*>(out) = v;
+      else
+        for (int k = 0; k < 4 && o + k < O; ++k) out[k] = v[k];
+    } else {
+      uint16_t* out = static_cast<uint16_t*>(a.out) + at;
+      const uint2 b = make_uint2(qmoe_gemm::cvt_pk_bf16(v[0], v[1]), qmoe_gemm::cvt_pk_bf16(v[2], v[3]));
+      if (O % 4 == 0) *reinterpret_cast<uint2*>(out) = b;
+      else
+        for (int k = 0; k < 4 && o + k < O; ++k) out[k] = (uint16_t)((k < 2 ? b.x : b.y) >> (16 * (k & 1)));
     }
   }
 }
@@ -154,21 +225,26 @@ __device__ __forceinline__ void store_rows(const GemmArgs& a, const char* ep, co
 // 32-column subtiles' codes once (16 bytes, one block, per lane) and converts
 // a word of each per step: lane half h supplies elements 32h + 8kk .. + 7 of
 // the group at step kk, from word kk of its block.
-template <bool S4, int MSUB>  // S4: scales copied four blocks at a time (K % 128 == 0, aligned)
+// WM: waves along the rows, of four.  S4: scales copied four blocks at a time (K % 128 == 0, aligned)
+template <bool S4, int WM, int MSUB, bool SPLIT>
 struct Fwd {
-  static constexpr int kA = 64 * MSUB * 128, kB = kCols * 64, kS = kCols * (S4 ? 4 : 16);
+  typedef Geo<SPLIT> Way;
+  static constexpr int kCols = Way::kCols, kRows = 32 * WM * MSUB;
+  static constexpr int NSUB = SPLIT ? 4 : 2 * WM;  // 32-column subtiles per wave
+  static constexpr int kA = kRows * 128, kB = kCols * 64, kS = kCols * (S4 ? 4 : 16);
   static constexpr int kBOff = 2 * kA, kSOff = kBOff + 2 * kB;
-  static constexpr int kLds = kSOff + 2 * kS;
-  static constexpr int kACopies = 2 * MSUB;
+  static constexpr int kRing = kSOff + 2 * kS;
+  static constexpr int kACopies = kRows / 8 / Way::kWaves, kBCopies = kCols / 16 / Way::kWaves;
+  static constexpr int kSCopies = kCols / 64 / Way::kWaves;
 
   struct Ctx {
-    RowSrc<kACopies, 8> x;
+    RowSrc<kACopies, 8, Way::kWaves> x;
     const char *w, *s;  // the column block's codes and scales
-    uint32_t woff[4];   // copy d's column and unit; the unit
-    uint32_t soff;
-    int wunit[4];
+    uint32_t woff[kBCopies];  // copy d's column and unit; the unit
+    uint32_t soff[kSCopies];
+    int wunit;
     uint32_t lds;
-    int wave, lane, units, G;
+    int wave, lane, units;  // wave: of those that fill the ring
     int64_t C;
   };
 
@@ -178,8 +254,8 @@ struct Fwd {
 #pragma unroll
     for (int d = 0; d < kACopies; ++d) {
       const char* p = c.x.p[d] + (size_t)g * 128;
-      if (!whole && (int64_t)g * 64 + c.x.unit[d] * 8 >= c.C) p = reinterpret_cast<const char*>(zero_page);
-      qmoe_gemm::dma16(p, dst + d * 4096);
+      if (!whole && (int64_t)g * 64 + c.x.unit(d) * 8 >= c.C) p = reinterpret_cast<const char*>(zero_page);
+      qmoe_gemm::dma16(p, dst + d * Way::kWaves * 1024);
     }
   }
   static __device__ __forceinline__ void copy_w(const Ctx& c, int p) {
@@ -187,32 +263,35 @@ struct Fwd {
     const uint32_t sdst = c.lds + kSOff + (p & 1) * kS + c.wave * 256;
     const bool whole = 4 * (p + 1) <= c.units;
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
+    for (int d = 0; d < kBCopies; ++d) {
       if (whole) {
-        qmoe_gemm::dma16s(c.w + (size_t)p * 64, c.woff[d], dst + d * 4096);
+        qmoe_gemm::dma16s(c.w + (size_t)p * 64, c.woff[d], dst + d * Way::kWaves * 1024);
       } else {
         const char* q = c.w + (size_t)p * 64 + c.woff[d];
-        if (4 * p + c.wunit[d] >= c.units) q = reinterpret_cast<const char*>(zero_page);
-        qmoe_gemm::dma16(q, dst + d * 4096);
+        if (4 * p + c.wunit >= c.units) q = reinterpret_cast<const char*>(zero_page);
+        qmoe_gemm::dma16(q, dst + d * Way::kWaves * 1024);
       }
     }
-    if constexpr (S4) {
-      qmoe_gemm::dma4s(c.s + (size_t)p * 4, c.soff, sdst);
-    } else {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        if (4 * p + b < c.units) dma1s(c.s + (size_t)p * 4 + b, c.soff, sdst + b * 1024);
-        else dma1(zero_page, sdst + b * 1024);
+    for (int d = 0; d < kSCopies; ++d) {
+      if constexpr (S4) {
+        qmoe_gemm::dma4s(c.s + (size_t)p * 4, c.soff[d], sdst + d * 256);
+      } else {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if (4 * p + b < c.units) dma1s(c.s + (size_t)p * 4 + b, c.soff[d], sdst + b * kCols * 4 + d * 256);
+          else dma1(zero_page, sdst + b * kCols * 4 + d * 256);
+        }
       }
     }
   }
 
   struct Frag {
-    i32x4_t a[MSUB], b[4];
+    i32x4_t a[MSUB], b[NSUB];
   };
   struct Codes {
-    i32x4_t w[4];
-    float s[4];
+    i32x4_t w[NSUB];
+    float s[NSUB];
   };
   static __device__ __forceinline__ void read_x(const Ctx& c, const char* smem, int g, int kk, int row0, Frag& f) {
     const int l32 = c.lane % 32, h = c.lane / 32;
@@ -227,7 +306,7 @@ struct Fwd {
     const char* ss = smem + kSOff + ((g >> 1) & 1) * kS;
     Codes r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NSUB; ++j) {
       const int col = col0 + 32 * j + l32;
       r.w[j] = *reinterpret_cast<const i32x4_t*>(st + col * 64 + (unit ^ swz4(col)) * 16);
       if constexpr (S4) r.s[j] = scale_of((*reinterpret_cast<const uint32_t*>(ss + col * 4) >> (8 * unit)) & 255u);
@@ -244,9 +323,9 @@ struct Fwd {
   // One step's products, the next step's conversions between them.
   template <bool NEXT>
   static __device__ __forceinline__ void step(const Frag& cur, Frag& nxt, const Codes& q, int kkn,
-                                              f32x16_t (&acc)[MSUB][4]) {
+                                              f32x16_t (&acc)[MSUB][NSUB]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NSUB; ++j) {
 #pragma unroll
       for (int i = 0; i < MSUB; ++i) {
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, cur.b[j]),
@@ -259,44 +338,63 @@ struct Fwd {
     }
   }
 
-  static __device__ void run(const GemmArgs& a, const Unit& u, char* smem) {
+  // A split wave's partial sums into LDS (part_at's layout), once no wave reads its ring any more.
+  static __device__ __forceinline__ void put_parts(char* ep, int l32, int h, const f32x16_t (&acc)[MSUB][NSUB]) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MSUB; ++i)
+#pragma unroll
+      for (int j = 0; j < NSUB; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4)
+          *reinterpret_cast<f32x4_t*>(ep + part_at(32 * i + l32, (32 * j + 2 * v + 4 * h) / 4)) =
+              f32x4_t{acc[i][j][v], acc[i][j][v + 1], acc[i][j][v + 2], acc[i][j][v + 3]};
+  }
+
+  static __device__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
     Ctx c;
     const int tid = fresh_tid();
     c.lane = tid % 64;
-    c.wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const int wm = c.wave / 2, wn = c.wave % 2;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wm = SPLIT || WM == 1 ? 0 : wave / 2, wn = SPLIT ? 0 : WM == 1 ? wave : wave % 2;
+    char* smem = block_smem + (SPLIT ? wave * kRing : 0);
+    c.wave = SPLIT ? 0 : wave;
     c.units = (int)(a.K / kBlock);
     c.C = a.K;
-    c.G = (int)((a.K + 63) / 64);
     c.lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)smem);
-    c.x = row_sources<kACopies, 8>(a, u, a.x, a.ldx * 2, c.wave, c.lane);
-    const int64_t row = (int64_t)u.e * a.N + (int64_t)u.nblk * kCols;
-    const int cols = (int)min((int64_t)kCols, a.N - (int64_t)u.nblk * kCols);
+    c.x = row_sources<kACopies, 8, Way::kWaves>(a, u, a.x, a.ldx * 2, c.wave, c.lane);
+    const int64_t row = (int64_t)u.e * a.N + u.o0;
+    const int cols = (int)min((int64_t)kCols, a.N - u.o0);
     c.w = reinterpret_cast<const char*>(a.w) + qmoe_gemm::uniform64(row * c.units * 16);
     c.s = reinterpret_cast<const char*>(a.s) + qmoe_gemm::uniform64(row * c.units);
+    c.wunit = (c.lane % 4) ^ swz4(c.lane / 4);  // swz4 repeats every 16 columns
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const int col = (d * 4 + c.wave) * 16 + c.lane / 4;
-      c.wunit[d] = (c.lane % 4) ^ swz4(col);
-      c.woff[d] = (uint32_t)(min(col, cols - 1) * c.units * 16 + c.wunit[d] * 16);
+    for (int d = 0; d < kBCopies; ++d) {
+      const int col = (d * Way::kWaves + c.wave) * 16 + c.lane / 4;
+      c.woff[d] = (uint32_t)(min(col, cols - 1) * c.units * 16 + c.wunit * 16);
     }
-    c.soff = (uint32_t)(min(c.wave * 64 + c.lane, cols - 1) * c.units);
-    const int G = c.G, P = (G + 1) / 2;
-    const int row0 = 32 * MSUB * wm, col0 = 128 * wn;
-
-    f32x16_t acc[MSUB][4] = {};
-    copy_x(c, 0);
-    copy_w(c, 0);
-    if (G > 1) copy_x(c, 1);
-    if (P > 1) copy_w(c, 1);
-    qmoe_gemm::wait_vmem<0>();
-    __builtin_amdgcn_s_barrier();
-    Frag fa, fb;
-    Codes q = read_codes(c, smem, 0, col0);
-    read_x(c, smem, 0, 0, row0, fa);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) convert(q, 0, j, fa);
-    for (int g = 0; g < G - 1; ++g) {
+    for (int d = 0; d < kSCopies; ++d)
+      c.soff[d] = (uint32_t)(min((d * Way::kWaves + c.wave) * 64 + c.lane, cols - 1) * c.units);
+    int g0, G;  // this wave's groups, whole pairs
+    Way::template part<2>((int)((a.K + 63) / 64), wave, &g0, &G);
+    const int P = (G + 1) / 2;
+    const int row0 = 32 * MSUB * wm, col0 = 32 * NSUB * wn;
+
+    f32x16_t acc[MSUB][NSUB] = {};
+    if (!SPLIT || g0 < G) {
+    copy_x(c, g0);
+    copy_w(c, g0 / 2);
+    if (g0 + 1 < G) copy_x(c, g0 + 1);
+    if (g0 / 2 + 1 < P) copy_w(c, g0 / 2 + 1);
+    qmoe_gemm::wait_vmem<0>();
+    Way::barrier();
+    Frag fa, fb;
+    Codes q = read_codes(c, smem, g0, col0);
+    read_x(c, smem, g0, 0, row0, fa);
+#pragma unroll
+    for (int j = 0; j < NSUB; ++j) convert(q, 0, j, fa);
+    for (int g = g0; g < G - 1; ++g) {
       read_x(c, smem, g, 1, row0, fb);
       step<true>(fa, fb, q, 1, acc);
       read_x(c, smem, g, 2, row0, fa);
@@ -305,7 +403,7 @@ struct Fwd {
       step<true>(fa, fb, q, 3, acc);
       qmoe_gemm::wait_vmem<0>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
+      Way::barrier();
       if (g + 2 < G) copy_x(c, g + 2);
       if ((g & 1) && (g >> 1) + 2 < P) copy_w(c, (g >> 1) + 2);
       q = read_codes(c, smem, g + 1, col0);
@@ -319,28 +417,36 @@ struct Fwd {
     read_x(c, smem, G - 1, 3, row0, fb);
     step<true>(fa, fb, q, 3, acc);
     step<false>(fb, fa, q, 0, acc);
+    }
     const int lane = fresh_tid() % 64, l32 = lane % 32, h = lane / 32;
+    if constexpr (SPLIT) {
+      put_parts(block_smem + wave * kRows * 512, l32, h, acc);
+      __syncthreads();
+      store_parts<kRows>(a, block_smem, u, a.N);
+      return;
+    }
     if (a.out_f32) {
 #pragma unroll
       for (int i = 0; i < MSUB; ++i) {
         const int r = row0 + 32 * i + l32;
         if (r >= u.valid) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NSUB; ++j)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const int64_t o = (int64_t)u.nblk * kCols + col0 + 32 * j + 8 * (v / 4) + 4 * h + v % 4;
+            const int64_t o = u.o0 + col0 + 32 * j + 8 * (v / 4) + 4 * h + v % 4;
             if (o < a.N) static_cast<float*>(a.out)[(u.row0 + r) * a.N + o] = acc[i][j][v];
           }
       }
       return;
     }
+    constexpr int kPer = WM == 1 ? 2 : 1;  // row subtiles per pass
 #pragma unroll
     for (int i = 0; i < MSUB; ++i) {
-      __syncthreads();
-      const int lr = 32 * wm + l32;
+      if (i % kPer == 0) __syncthreads();
+      const int lr = 32 * (WM == 1 ? i % 2 : wm) + l32;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < NSUB; ++j)
 #pragma unroll
         for (int v = 0; v < 16; v += 4) {
           const int gi = (col0 + 32 * j + 2 * v + 4 * h) / 4;
@@ -348,8 +454,10 @@ struct Fwd {
               make_uint2(qmoe_gemm::cvt_pk_bf16(acc[i][j][v], acc[i][j][v + 1]),
                          qmoe_gemm::cvt_pk_bf16(acc[i][j][v + 2], acc[i][j][v + 3]));
         }
-      __syncthreads();
-      store_rows(a, smem, u, a.N, 32 * MSUB, i);
+      if (i % kPer == kPer - 1 || i == MSUB - 1) {
+        __syncthreads();
+        store_rows<WM, 32 * MSUB>(a, smem, u, a.N, i / kPer);
+      }
     }
   }
 };
@@ -364,22 +472,27 @@ struct Fwd {
 // sixteen words of a wave's 128 outputs are the sixteen lanes of a quarter
 // wave and the four quarters the four octets of n, so no value crosses lanes:
 // the sixteen outputs of subtile j are 8c + j, c = 0 .. 15.
-template <bool S4, int MSUB>  // MSUB: 16-row subtiles per wave
+template <bool S4, int MSUB, bool SPLIT>  // MSUB: 16-row subtiles per wave
 struct Trn {
-  static constexpr int kA = 32 * MSUB * 128, kB = 64 * 128, kS = 64 * (S4 ? 8 : 32);
+  typedef Geo<SPLIT> Way;
+  static constexpr int kCols = Way::kCols, kRows = (SPLIT ? 16 : 32) * MSUB;
+  static constexpr int kUnits = kCols / kBlock;  // 16-byte units of codes per row n
+  static constexpr int kA = kRows * 128, kB = 64 * kUnits * 16, kS = 64 * kUnits * (S4 ? 1 : 4);
   static constexpr int kStage = kA + kB + kS;
   static constexpr int NS = 3;
-  static constexpr int kLds = NS * kStage;
-  static constexpr int kACopies = MSUB;
-  static constexpr int kCopies = kACopies + 2 + (S4 ? 1 : 2);  // per wave and group
+  static constexpr int kRing = NS * kStage;
+  static constexpr int kACopies = kRows / 8 / Way::kWaves;
+  static constexpr int kBCopies = SPLIT ? 4 : 2;
+  static constexpr int kSCopies = S4 ? 1 : SPLIT ? 4 : 2;
+  static constexpr int kCopies = kACopies + kBCopies + kSCopies;  // per wave and group
 
   struct Ctx {
-    RowSrc<kACopies, 8> x;
+    RowSrc<kACopies, 8, Way::kWaves> x;
     const char *w, *s;  // of the expert's first row, at the column block
     int64_t wpitch, spitch;
-    int wunit, wrow, sblk[2];
+    int wunit, wrow, sblk[kSCopies];
     uint32_t lds;
-    int wave, lane, G;
+    int wave, lane;  // wave: of those that fill the ring
     int64_t C;
   };
 
@@ -389,15 +502,15 @@ struct Trn {
 #pragma unroll
     for (int d = 0; d < kACopies; ++d) {
       const char* p = c.x.p[d] + (size_t)g * 128;
-      if (c.x.unit[d] * 8 >= left) p = reinterpret_cast<const char*>(zero_page);
-      qmoe_gemm::dma16(p, st + (d * 4 + c.wave) * 1024);
+      if (c.x.unit(d) * 8 >= left) p = reinterpret_cast<const char*>(zero_page);
+      qmoe_gemm::dma16(p, st + (d * Way::kWaves + c.wave) * 1024);
     }
 #pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      const int n = c.wrow + 32 * d;
+    for (int d = 0; d < kBCopies; ++d) {
+      const int n = SPLIT ? w_row(16 * d + c.wrow) : c.wrow + 32 * d;  // w_row(pos + 32) == w_row(pos) + 32
       const char* p = c.w + ((int64_t)g * 64 + n) * c.wpitch;
       if (n >= left) p = reinterpret_cast<const char*>(zero_page);
-      qmoe_gemm::dma16(p, st + kA + (d * 4 + c.wave) * 1024);
+      qmoe_gemm::dma16(p, st + kA + (d * Way::kWaves + c.wave) * 1024);
     }
     const char* s = c.s + ((int64_t)g * 64 + c.lane) * c.spitch;
     if constexpr (S4) {
@@ -406,13 +519,19 @@ struct Trn {
       qmoe_gemm::dma4(s, st + kA + kB + (c.wave & 1) * 256);
     } else {
 #pragma unroll
-      for (int d = 0; d < 2; ++d) {
+      for (int d = 0; d < kSCopies; ++d) {
         const char* p = s + c.sblk[d];
         if (c.lane >= left) p = reinterpret_cast<const char*>(zero_page);
-        dma1(p, st + kA + kB + (2 * c.wave + d) * 256);
+        dma1(p, st + kA + kB + (kSCopies * c.wave + d) * 256);
       }
     }
   }
+  // Row n of the group in the codes' row slot `pos` (its own inverse), and the unit in a unit slot: chosen so that
+  // the words that a wave reads at once, those of rows n + 8 q, fall on all 64 banks.
+  static __device__ __forceinline__ int w_row(int pos) {
+    return SPLIT ? pos ^ ((pos >> 3) & 3) : pos ^ ((pos >> 3) & 1);
+  }
+  static __device__ __forceinline__ int w_unit(int slot, int pos) { return SPLIT ? slot : slot ^ (4 * ((pos >> 4) & 1)); }
 
   struct Words {
     uint32_t w[8];
@@ -421,13 +540,16 @@ struct Trn {
   static __device__ __forceinline__ Words read_words(const Ctx& c, const char* smem, int g, int s, int wn) {
     const int co = c.lane % 16, q = c.lane / 16;
     const char* st = smem + (g % NS) * kStage + kA;
-    const int unit = (4 * wn + co / 4) ^ (4 * (q >> 1));
+    const int unit = w_unit(4 * wn + co / 4, 8 * q);
     Words r;
+    // w_row(8 q + i) = 8 q + (i & ~m) + w_row of the low bits: few bases, the rest in the offsets
+    constexpr int m = SPLIT ? 3 : 1, kPitch = kUnits * 16;
+    const char* base[m + 1];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int pos = (32 * s + 8 * q + i) ^ (q & 1);
-      r.w[i] = *reinterpret_cast<const uint32_t*>(st + pos * 128 + unit * 16 + (co % 4) * 4);
-    }
+    for (int i = 0; i <= m; ++i) base[i] = st + w_row(8 * q + i) * kPitch + unit * 16 + (co % 4) * 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      r.w[i] = *reinterpret_cast<const uint32_t*>(base[i & m] + (32 * s + (i & ~m)) * kPitch);
     const int blk = 4 * wn + co / 4;
     const char* ss = st + kB + (S4 ? wn : blk) * 256 + (32 * s + 8 * q) * 4;
     const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(ss), hi = *reinterpret_cast<const i32x4_t*>(ss + 16);
@@ -466,76 +588,101 @@ struct Trn {
                                                                     __builtin_bit_cast(bf16x8_t, x[i]),
                                                                     acc[i][2 * t + v], 0, 0, 0);
   }
-  // One step: the pairs of outputs in turn, each prepared during the one before.
-  static __device__ __forceinline__ void step(const i32x4_t (&x)[MSUB], const Words& cur, const Words& nxt,
-                                              i32x4_t (&b0)[2], i32x4_t (&b1)[2], f32x4_t (&acc)[MSUB][8]) {
-    pair<1>(cur, b1);
+  // One step: the pairs of outputs in turn, each prepared during the one before.  next() reads the next step's
+  // words and activations, late, when the current words are used up: 128 accumulators leave few registers.
+  template <class Next>
+  static __device__ __forceinline__ void step(const i32x4_t (&x)[MSUB], Words& w, i32x4_t (&b0)[2], i32x4_t (&b1)[2],
+                                              f32x4_t (&acc)[MSUB][8], Next next) {
+    pair<1>(w, b1);
     products(x, b0, acc, 0);
-    pair<2>(cur, b0);
+    pair<2>(w, b0);
     products(x, b1, acc, 1);
-    pair<3>(cur, b1);
+    pair<3>(w, b1);
+    __builtin_amdgcn_sched_barrier(0);
+    next();
     products(x, b0, acc, 2);
-    pair<0>(nxt, b0);
+    pair<0>(w, b0);
     products(x, b1, acc, 3);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
-  static __device__ void run(const GemmArgs& a, const Unit& u, char* smem) {
+  static __device__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
     Ctx c;
     const int tid = fresh_tid();
     c.lane = tid % 64;
-    c.wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const int wm = c.wave / 2, wn = c.wave % 2;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wm = SPLIT ? 0 : wave / 2, wn = SPLIT ? 0 : wave % 2;
+    char* smem = block_smem + (SPLIT ? wave * kRing : 0);
+    c.wave = SPLIT ? 0 : wave;
     const int64_t units = a.K / kBlock;
     c.C = a.N;
-    c.G = (int)((a.N + 63) / 64);
     c.lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)smem);
-    c.x = row_sources<kACopies, 8>(a, u, a.x, a.ldx * 2, c.wave, c.lane);
-    const int64_t row = (int64_t)u.e * a.N, u0 = (int64_t)u.nblk * (kCols / kBlock);
-    const int last = (int)min((int64_t)(kCols / kBlock), units - u0) - 1;  // columns past the end: the last again
+    c.x = row_sources<kACopies, 8, Way::kWaves>(a, u, a.x, a.ldx * 2, c.wave, c.lane);
+    const int64_t row = (int64_t)u.e * a.N, u0 = u.o0 / kBlock;
+    const int last = (int)min((int64_t)kUnits, units - u0) - 1;  // columns past the end: the last again
     c.wpitch = units * 16;
     c.spitch = units;
-    // copy d's row slot 32d + 8 wave + lane / 8 holds row n = slot ^ (slot / 8 & 1), its unit slot the unit
-    // ^ 4 (slot / 16 & 1): the eight words a lane reads then fall on all 64 banks
-    const int pos = 8 * c.wave + c.lane / 8;
-    c.wrow = pos ^ ((pos >> 3) & 1);
-    c.wunit = (c.lane % 8) ^ (4 * ((pos >> 4) & 1));
+    const int pos = c.wave * 8 + c.lane / kUnits;  // row slot of copy 0
+    c.wrow = SPLIT ? pos : w_row(pos);
+    c.wunit = w_unit(c.lane % kUnits, pos);
     c.w = reinterpret_cast<const char*>(a.w) + (row * units + u0 + min(c.wunit, last)) * 16;
     c.s = reinterpret_cast<const char*>(a.s) + row * units + u0;
-    if constexpr (S4) c.sblk[0] = 4 * (c.wave & 1) <= last ? 4 * (c.wave & 1) : 0;
+    if constexpr (S4) c.sblk[0] = !SPLIT && 4 * (c.wave & 1) <= last ? 4 * (c.wave & 1) : 0;
     else
 #pragma unroll
-      for (int d = 0; d < 2; ++d) c.sblk[d] = min(2 * c.wave + d, last);
-    const int G = c.G;
+      for (int d = 0; d < kSCopies; ++d) c.sblk[d] = min(kSCopies * c.wave + d, last);
+    int g0, G;  // this wave's groups
+    Way::template part<1>((int)((a.N + 63) / 64), wave, &g0, &G);
     const int row0 = 16 * MSUB * wm;
 
     f32x4_t acc[MSUB][8] = {};
+    if (!SPLIT || g0 < G) {
 #pragma unroll
-    for (int i = 0; i < NS; ++i) copy(c, min(i, G - 1));
+    for (int i = 0; i < NS; ++i) copy(c, min(g0 + i, G - 1));
     qmoe_gemm::wait_vmem<(NS - 1) * kCopies>();
-    __builtin_amdgcn_s_barrier();
+    Way::barrier();
     i32x4_t xa[MSUB], xb[MSUB], b0[2], b1[2];
-    Words wa = read_words(c, smem, 0, 0, wn), wb;
-    read_x(c, smem, 0, 0, row0, xa);
-    pair<0>(wa, b0);
-    for (int g = 0; g < G - 1; ++g) {
-      wb = read_words(c, smem, g, 1, wn);
-      read_x(c, smem, g, 1, row0, xb);
-      step(xa, wa, wb, b0, b1, acc);
-      // group g + 1 landed (copies of NS - 2 groups after it may be in flight); all reads of stage g are done
-      qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      copy(c, min(g + NS, G - 1));  // past the end: the last group again, the same bytes to where they are
-      wa = read_words(c, smem, g + 1, 0, wn);
-      read_x(c, smem, g + 1, 0, row0, xa);
-      step(xb, wb, wa, b0, b1, acc);
+    Words w = read_words(c, smem, g0, 0, wn);
+    read_x(c, smem, g0, 0, row0, xa);
+    pair<0>(w, b0);
+    for (int g = g0; g < G - 1; ++g) {
+      step(xa, w, b0, b1, acc, [&] {
+        w = read_words(c, smem, g, 1, wn);
+        read_x(c, smem, g, 1, row0, xb);
+      });
+      step(xb, w, b0, b1, acc, [&] {
+        // group g + 1 landed (copies of NS - 2 groups after it may be in flight); all reads of stage g are done
+        qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        Way::barrier();
+        copy(c, min(g + NS, G - 1));  // past the end: the last group again, the same bytes to where they are
+        w = read_words(c, smem, g + 1, 0, wn);
+        read_x(c, smem, g + 1, 0, row0, xa);
+      });
     }
-    wb = read_words(c, smem, G - 1, 1, wn);
-    read_x(c, smem, G - 1, 1, row0, xb);
-    step(xa, wa, wb, b0, b1, acc);
-    step(xb, wb, wb, b0, b1, acc);
+    step(xa, w, b0, b1, acc, [&] {
+      w = read_words(c, smem, G - 1, 1, wn);
+      read_x(c, smem, G - 1, 1, row0, xb);
+    });
+    step(xb, w, b0, b1, acc, [] {});
+    }
     qmoe_gemm::wait_vmem<0>();
     const int lane = fresh_tid() % 64, l16 = lane % 16, q = lane / 16;
+    if constexpr (SPLIT) {
+      __syncthreads();  // no wave reads its ring any more
+      char* ep = block_smem + wave * kRows * 512;
+#pragma unroll
+      for (int i = 0; i < MSUB; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+            *reinterpret_cast<f32x4_t*>(ep + part_at(16 * i + l16, 2 * (4 * q + t) + v)) =
+                f32x4_t{acc[i][4 * v][t], acc[i][4 * v + 1][t], acc[i][4 * v + 2][t], acc[i][4 * v + 3][t]};
+      __syncthreads();
+      store_parts<kRows>(a, block_smem, u, a.K);
+      return;
+    }
     if (a.out_f32) {
 #pragma unroll
       for (int i = 0; i < MSUB; ++i) {
@@ -543,7 +690,7 @@ struct Trn {
         if (r >= u.valid) continue;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const int64_t o = (int64_t)u.nblk * kCols + 128 * wn + 8 * (4 * q + t);
+          const int64_t o = u.o0 + 128 * wn + 8 * (4 * q + t);
           if (o >= a.K) continue;
           f32x4_t* out = reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + (u.row0 + r) * a.K + o);
           out[0] = f32x4_t{acc[i][0][t], acc[i][1][t], acc[i][2][t], acc[i][3][t]};
@@ -553,11 +700,12 @@ struct Trn {
       return;
     }
 #pragma unroll
-    for (int p = 0; p < MSUB / 2; ++p) {
+    for (int p = 0; p < (MSUB + 1) / 2; ++p) {
       __syncthreads();
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
         const int i = 2 * p + v, lr = 32 * wm + 16 * v + l16;
+        if (i >= MSUB) break;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const int gi = 2 * (16 * wn + 4 * q + t);
@@ -570,7 +718,7 @@ struct Trn {
         }
       }
       __syncthreads();
-      store_rows(a, smem, u, a.K, 16 * MSUB, p);
+      store_rows<2, 16 * MSUB>(a, smem, u, a.K, p);
     }
   }
 };
@@ -582,24 +730,27 @@ struct Trn {
 // Contraction in groups of 128.  A lane's scale byte at step kk is block 2kk +
 // h of its row: the row's four bytes shifted by h, byte 2kk picked by the
 // instruction.
-template <bool S4, int MSUB>
+template <bool S4, int MSUB, bool SPLIT>
 struct QQ {
-  static constexpr int kRows = 64 * MSUB;
+  typedef Geo<SPLIT> Way;
+  static constexpr int kCols = Way::kCols, kRows = (SPLIT ? 32 : 64) * MSUB;
+  static constexpr int kScaleRows = SPLIT ? 64 : kTileRows;  // rows whose scales are copied: whole waves' worth
   static constexpr int kA = kRows * 64, kB = kCols * 64;
-  static constexpr int kSA = kTileRows * (S4 ? 4 : 16), kSB = kCols * (S4 ? 4 : 16);
+  static constexpr int kSA = kScaleRows * (S4 ? 4 : 16), kSB = kCols * (S4 ? 4 : 16);
   static constexpr int kBOff = kA, kSAOff = kBOff + kB, kSBOff = kSAOff + kSA, kStage = kSBOff + kSB;
   static constexpr int NS = S4 ? 3 : 2;
-  static constexpr int kLds = NS * kStage;
-  static constexpr int kACopies = MSUB;
-  static constexpr int kCopies = kACopies + 4 + (S4 ? 2 : 8);
+  static constexpr int kRing = NS * kStage;
+  static constexpr int kACopies = kRows / 16 / Way::kWaves, kBCopies = kCols / 16 / Way::kWaves;
+  static constexpr int kSCopies = kCols / 64 / Way::kWaves;
+  static constexpr int kCopies = kACopies + kBCopies + (1 + kSCopies) * (S4 ? 1 : 4);
 
   struct Ctx {
-    RowSrc<kACopies, 4> x;
+    RowSrc<kACopies, 4, Way::kWaves> x;
     const char *w, *s, *xs;
-    uint32_t woff[4], soff;
-    int wunit[4];
+    uint32_t woff[kBCopies], soff[kSCopies];
+    int wunit;
     uint32_t lds;
-    int wave, lane, units, G;
+    int wave, lane, units;  // wave: of those that fill the ring
   };
 
   static __device__ __forceinline__ void copy(const Ctx& c, int g) {
@@ -608,30 +759,35 @@ struct QQ {
 #pragma unroll
     for (int d = 0; d < kACopies; ++d) {
       const char* p = c.x.p[d] + (size_t)g * 64;
-      if (!whole && 4 * g + c.x.unit[d] >= c.units) p = reinterpret_cast<const char*>(zero_page);
-      qmoe_gemm::dma16(p, st + (d * 4 + c.wave) * 1024);
+      if (!whole && 4 * g + c.x.unit(d) >= c.units) p = reinterpret_cast<const char*>(zero_page);
+      qmoe_gemm::dma16(p, st + (d * Way::kWaves + c.wave) * 1024);
     }
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
+    for (int d = 0; d < kBCopies; ++d) {
+      const uint32_t dst = st + kBOff + (d * Way::kWaves + c.wave) * 1024;
       if (whole) {
-        qmoe_gemm::dma16s(c.w + (size_t)g * 64, c.woff[d], st + kBOff + (d * 4 + c.wave) * 1024);
+        qmoe_gemm::dma16s(c.w + (size_t)g * 64, c.woff[d], dst);
       } else {
         const char* q = c.w + (size_t)g * 64 + c.woff[d];
-        if (4 * g + c.wunit[d] >= c.units) q = reinterpret_cast<const char*>(zero_page);
-        qmoe_gemm::dma16(q, st + kBOff + (d * 4 + c.wave) * 1024);
+        if (4 * g + c.wunit >= c.units) q = reinterpret_cast<const char*>(zero_page);
+        qmoe_gemm::dma16(q, dst);
       }
     }
+    const uint32_t sa = st + kSAOff + (c.wave & 1) * 256, sb = st + kSBOff + c.wave * 256;
     if constexpr (S4) {
-      qmoe_gemm::dma4(c.xs + (size_t)g * 4, st + kSAOff + (c.wave & 1) * 256);
-      qmoe_gemm::dma4s(c.s + (size_t)g * 4, c.soff, st + kSBOff + c.wave * 256);
+      qmoe_gemm::dma4(c.xs + (size_t)g * 4, sa);
+#pragma unroll
+      for (int d = 0; d < kSCopies; ++d) qmoe_gemm::dma4s(c.s + (size_t)g * 4, c.soff[d], sb + d * 256);
     } else {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const bool in = 4 * g + b < c.units;
-        dma1(in ? c.xs + (size_t)g * 4 + b : reinterpret_cast<const char*>(zero_page),
-             st + kSAOff + b * 512 + (c.wave & 1) * 256);
-        if (in) dma1s(c.s + (size_t)g * 4 + b, c.soff, st + kSBOff + b * 1024 + c.wave * 256);
-        else dma1(zero_page, st + kSBOff + b * 1024 + c.wave * 256);
+        dma1(in ? c.xs + (size_t)g * 4 + b : reinterpret_cast<const char*>(zero_page), sa + b * kScaleRows * 4);
+#pragma unroll
+        for (int d = 0; d < kSCopies; ++d) {
+          if (in) dma1s(c.s + (size_t)g * 4 + b, c.soff[d], sb + b * kCols * 4 + d * 256);
+          else dma1(zero_page, sb + b * kCols * 4 + d * 256);
+        }
       }
     }
   }
@@ -673,48 +829,53 @@ struct QQ {
                                                                     2 * KK, sb[j], 2 * KK, sa[i]);
   }
 
-  static __device__ void run(const GemmArgs& a, const Unit& u, char* smem) {
+  static __device__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
     Ctx c;
     const int tid = fresh_tid();
     c.lane = tid % 64;
-    c.wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const int wm = c.wave / 2, wn = c.wave % 2;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wm = SPLIT ? 0 : wave / 2, wn = SPLIT ? 0 : wave % 2;
+    char* smem = block_smem + (SPLIT ? wave * kRing : 0);
+    c.wave = SPLIT ? 0 : wave;
     c.units = (int)(a.K / kBlock);
-    c.G = (c.units + 3) / 4;
     c.lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)smem);
-    c.x = row_sources<kACopies, 4>(a, u, a.xq, (int64_t)c.units * 16, c.wave, c.lane);
+    c.x = row_sources<kACopies, 4, Way::kWaves>(a, u, a.xq, (int64_t)c.units * 16, c.wave, c.lane);
     {
       const int64_t i = u.row0 + min((c.wave & 1) * 64 + c.lane, u.valid - 1);
       const int64_t x = min(max(a.x_rows ? (int64_t)a.x_rows[i] : i, (int64_t)0), a.n_x - 1);
       c.xs = reinterpret_cast<const char*>(a.xs) + x * c.units;
     }
-    const int64_t row = (int64_t)u.e * a.N + (int64_t)u.nblk * kCols;
-    const int cols = (int)min((int64_t)kCols, a.N - (int64_t)u.nblk * kCols);
+    const int64_t row = (int64_t)u.e * a.N + u.o0;
+    const int cols = (int)min((int64_t)kCols, a.N - u.o0);
     c.w = reinterpret_cast<const char*>(a.w) + qmoe_gemm::uniform64(row * c.units * 16);
     c.s = reinterpret_cast<const char*>(a.s) + qmoe_gemm::uniform64(row * c.units);
+    c.wunit = (c.lane % 4) ^ swz4(c.lane / 4);  // swz4 repeats every 16 columns
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const int col = (d * 4 + c.wave) * 16 + c.lane / 4;
-      c.wunit[d] = (c.lane % 4) ^ swz4(col);
-      c.woff[d] = (uint32_t)(min(col, cols - 1) * c.units * 16 + c.wunit[d] * 16);
+    for (int d = 0; d < kBCopies; ++d) {
+      const int col = (d * Way::kWaves + c.wave) * 16 + c.lane / 4;
+      c.woff[d] = (uint32_t)(min(col, cols - 1) * c.units * 16 + c.wunit * 16);
     }
-    c.soff = (uint32_t)(min(c.wave * 64 + c.lane, cols - 1) * c.units);
-    const int G = c.G;
+#pragma unroll
+    for (int d = 0; d < kSCopies; ++d)
+      c.soff[d] = (uint32_t)(min((d * Way::kWaves + c.wave) * 64 + c.lane, cols - 1) * c.units);
+    int g0, G;  // this wave's groups
+    Way::template part<1>((c.units + 3) / 4, wave, &g0, &G);
     const int row0 = 32 * MSUB * wm, col0 = 128 * wn;
     const int l32 = c.lane % 32, h = c.lane / 32;
 
     f32x16_t acc[MSUB][4] = {};
+    if (!SPLIT || g0 < G) {
 #pragma unroll
-    for (int i = 0; i < NS; ++i) copy(c, min(i, G - 1));
+    for (int i = 0; i < NS; ++i) copy(c, min(g0 + i, G - 1));
     qmoe_gemm::wait_vmem<(NS - 1) * kCopies>();
-    __builtin_amdgcn_s_barrier();
+    Way::barrier();
     Frag fa, fb;
     int sa[MSUB], sb[4];
-    read(c, smem, 0, row0, col0, fa);
-    for (int g = 0; g < G; ++g) {
+    read(c, smem + (g0 % NS) * kStage, 0, row0, col0, fa);
+    for (int g = g0; g < G; ++g) {
       const char* st = smem + (g % NS) * kStage;
 #pragma unroll
-      for (int i = 0; i < MSUB; ++i) sa[i] = scales(st + kSAOff, kTileRows, row0 + 32 * i + l32, h);
+      for (int i = 0; i < MSUB; ++i) sa[i] = scales(st + kSAOff, kScaleRows, row0 + 32 * i + l32, h);
 #pragma unroll
       for (int j = 0; j < 4; ++j) sb[j] = scales(st + kSBOff, kCols, col0 + 32 * j + l32, h);
       read(c, st, 1, row0, col0, fb);
@@ -722,14 +883,21 @@ struct QQ {
       if (g + 1 < G) {
         qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
+        Way::barrier();
         copy(c, min(g + NS, G - 1));
         read(c, smem + ((g + 1) % NS) * kStage, 0, row0, col0, fa);
       }
       products<1>(fb, sa, sb, acc);
     }
+    }
     qmoe_gemm::wait_vmem<0>();
     const int el = fresh_tid() % 64, e32 = el % 32, eh = el / 32;
+    if constexpr (SPLIT) {
+      Fwd<S4, 1, MSUB, true>::put_parts(block_smem + wave * kRows * 512, e32, eh, acc);
+      __syncthreads();
+      store_parts<kRows>(a, block_smem, u, a.N);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < MSUB; ++i) {
       __syncthreads();
@@ -744,36 +912,59 @@ struct QQ {
                          qmoe_gemm::cvt_pk_bf16(acc[i][j][v + 2], acc[i][j][v + 3]));
         }
       __syncthreads();
-      store_rows(a, smem, u, a.N, 32 * MSUB, i);
+      store_rows<2, 32 * MSUB>(a, smem, u, a.N, i);
     }
   }
 };
 
-template <int MODE, bool S4>
+// The forms of a unit by its rows, widest first, each for units of more rows than the next takes.
+template <class... Forms>
+struct Pick;
+template <class F>
+struct Pick<F> {
+  static constexpr int kRing = F::kRing;
+  static __device__ __forceinline__ void run(const GemmArgs& a, const Unit& u, char* smem) { F::run(a, u, smem); }
+};
+template <class F, class G, class... Rest>
+struct Pick<F, G, Rest...> {
+  typedef Pick<G, Rest...> Next;
+  static constexpr int kRing = F::kRing > Next::kRing ? F::kRing : Next::kRing;
+  static __device__ __forceinline__ void run(const GemmArgs& a, const Unit& u, char* smem) {
+    if (u.valid > G::kRows) F::run(a, u, smem);
+    else Next::run(a, u, smem);
+  }
+};
+template <int MODE, bool S4, bool SPLIT>
 struct Kernel;
 template <bool S4>
-struct Kernel<kFwd, S4> {
-  typedef Fwd<S4, 2> Full;
-  typedef Fwd<S4, 1> Half;
+struct Kernel<kFwd, S4, false> {
+  typedef Pick<Fwd<S4, 2, 2, false>, Fwd<S4, 1, 3, false>, Fwd<S4, 1, 2, false>, Fwd<S4, 1, 1, false>> Forms;
 };
 template <bool S4>
-struct Kernel<kT, S4> {
-  typedef Trn<S4, 4> Full;
-  typedef Trn<S4, 2> Half;
+struct Kernel<kFwd, S4, true> {
+  typedef Pick<Fwd<S4, 1, 2, true>, Fwd<S4, 1, 1, true>> Forms;
 };
 template <bool S4>
-struct Kernel<kQQ, S4> {
-  typedef QQ<S4, 2> Full;
-  typedef QQ<S4, 1> Half;
+struct Kernel<kT, S4, false> {
+  typedef Pick<Trn<S4, 4, false>, Trn<S4, 3, false>, Trn<S4, 2, false>, Trn<S4, 1, false>> Forms;
+};
+template <bool S4>
+struct Kernel<kT, S4, true> {
+  typedef Pick<Trn<S4, 4, true>, Trn<S4, 2, true>, Trn<S4, 1, true>> Forms;
+};
+template <bool S4, bool SPLIT>
+struct Kernel<kQQ, S4, SPLIT> {
+  typedef Pick<QQ<S4, 2, SPLIT>, QQ<S4, 1, SPLIT>> Forms;
 };
 
-template <int MODE, bool S4>
-__global__ __launch_bounds__(256, 2) void mx_gemm_kernel(GemmArgs a, int64_t dense_tiles, int NB) {
-  typedef Kernel<MODE, S4> K;
-  constexpr int kRing = K::Full::kLds > K::Half::kLds ? K::Full::kLds : K::Half::kLds;
-  static_assert(kRing >= 64 * 512, "the epilogue's 64 rows");
+template <int MODE, bool S4, bool SPLIT>
+__global__ __launch_bounds__(256, SPLIT ? 1 : 2) void mx_gemm_kernel(GemmArgs a, int64_t dense_tiles, int NB) {
+  typedef typename Kernel<MODE, S4, SPLIT>::Forms Forms;
+  typedef Geo<SPLIT> Way;
+  constexpr int kEnd = SPLIT ? 4 * 64 * 512 : 64 * 512;  // the epilogue's rows
+  constexpr int kRing = Way::kRings * Forms::kRing > kEnd ? Way::kRings * Forms::kRing : kEnd;
   static_assert(kRing >= 4 * qmoe_gemm::kMaxOrder, "the ranking's scratch");
-  static_assert(2 * (kRing + 4 * qmoe_gemm::kMaxOrder) <= 160 * 1024, "two blocks per CU");
+  static_assert((SPLIT ? 1 : 2) * (kRing + 4 * qmoe_gemm::kMaxOrder) <= kLdsCU, "LDS per CU");
   __shared__ __attribute__((aligned(16))) char smem[kRing];
   __shared__ int order[qmoe_gemm::kMaxOrder];
   const int64_t tiles = a.offsets ? (int64_t)max(a.ntiles[0], 0) : dense_tiles;
@@ -782,34 +973,58 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(GemmArgs a, int64_t den
     const qmoe_gemm::Tiles table{a.offsets, a.tile_row, a.tile_exp, a.ntiles, a.n_rows, a.num_experts};
     qmoe_gemm::rank_tiles(table, (int)tiles, order, reinterpret_cast<int*>(smem));
   }
-  const qmoe_gemm::Snake snake(tiles * NB);
+  // a split unit is half a tile
+  const int per = SPLIT ? 2 * NB : NB;
+  const qmoe_gemm::Snake snake(tiles * per);
   for (int64_t k = 0;; ++k) {
     const int64_t at = snake.unit(k);
     if (at < 0) break;
-    int64_t tile = at / NB;
+    int64_t tile = at / per;
+    const int sub = (int)(at % per);
     if (ranked) tile = order[tile];
-    const qmoe_gemm::TileRows t = tile_of(a, tile);
+    qmoe_gemm::TileRows t = tile_of(a, tile);
+    if constexpr (SPLIT) {
+      if (sub >= NB) t.row0 += kRowsHalf, t.valid -= kRowsHalf;
+      t.valid = min(t.valid, kRowsHalf);
+    }
     if (t.valid <= 0) continue;
     Unit u;
     u.e = __builtin_amdgcn_readfirstlane(t.e);
     u.valid = __builtin_amdgcn_readfirstlane(t.valid);
-    u.nblk = __builtin_amdgcn_readfirstlane((int)(at % NB));
     u.row0 = qmoe_gemm::uniform64(t.row0);
-    if (u.valid > kRowsHalf) K::Full::run(a, u, smem);
-    else K::Half::run(a, u, smem);
+    u.o0 = (int64_t)__builtin_amdgcn_readfirstlane(SPLIT ? sub % NB : sub) * Way::kCols;
+    Forms::run(a, u, smem);
     __syncthreads();  // the ring is free for the next unit
   }
 }
 
-template <int MODE>
-int launch(GemmArgs a, int64_t max_tiles, hipStream_t st) {
+template <int MODE, bool SPLIT>
+void launch_way(const GemmArgs& a, int64_t max_tiles, hipStream_t st) {
   const int64_t O = MODE == kT ? a.K : a.N;
   const int64_t dense = (a.n_rows + kTileRows - 1) / kTileRows;
-  const int64_t NB = (O + kCols - 1) / kCols;
-  const dim3 grid((unsigned)qmoe_gemm::grid_blocks((a.offsets ? max_tiles : dense) * NB)), block(256);
-  const auto even = [](const void* p) { return qmoe::aligned4(p); };
-  if (a.K % 128 == 0 && even(a.s) && (MODE != kQQ || even(a.xs))) mx_gemm_kernel<MODE, true><<<grid, block, 0, st>>>(a, dense, (int)NB);
-  else mx_gemm_kernel<MODE, false><<<grid, block, 0, st>>>(a, dense, (int)NB);
+  const int64_t NB = (O + Geo<SPLIT>::kCols - 1) / Geo<SPLIT>::kCols;
+  const int64_t units = (a.offsets ? max_tiles : dense) * NB * (SPLIT ? 2 : 1);
+  const dim3 grid((unsigned)qmoe_gemm::grid_blocks(units, SPLIT ? 1 : 2)), block(256);
+  const bool s4 = a.K % 128 == 0 && qmoe::aligned4(a.s) && (MODE != kQQ || qmoe::aligned4(a.xs));
+  if (s4) mx_gemm_kernel<MODE, true, SPLIT><<<grid, block, 0, st>>>(a, dense, (int)NB);
+  else mx_gemm_kernel<MODE, false, SPLIT><<<grid, block, 0, st>>>(a, dense, (int)NB);
+}
+
+// Wide units from this many on: below, split ones are faster.  At 64, 128 and
+// 256 wide units (us, wide / split; 512 to 4096 rows of 4096 x 2048 and 1024 x
+// 2048 weights): forward 35.6 / 20.3, 37.5 / 36.9, 41.6 / 68.0; transposed
+// 74.8 / 28.2, 75.6 / 54.8, 83.0 / 102.9; both mxfp4 18.6 / 15.9, 19.9 / 27.3,
+// 22.3 / 46.9.
+constexpr int64_t kWideUnits = 160, kWideUnitsQQ = 96;
+
+template <int MODE>
+int launch(const GemmArgs& a, int64_t max_tiles, hipStream_t st) {
+  const int64_t O = MODE == kT ? a.K : a.N;
+  const int64_t tiles = a.offsets ? std::min(max_tiles, a.n_rows) : (a.n_rows + kTileRows - 1) / kTileRows;
+  if (tiles * ((O + kWideCols - 1) / kWideCols) < (MODE == kQQ ? kWideUnitsQQ : kWideUnits))
+    launch_way<MODE, true>(a, max_tiles, st);
+  else
+    launch_way<MODE, false>(a, max_tiles, st);
   return qmoe::launch_status("mx_gemm_kernel");
 }
 

@@ -40,7 +40,7 @@ def _format(group_size: int | None, bits: int, biases=None) -> None:
 
 def _scales(t: torch.Tensor, device) -> torch.Tensor:
     ops._dev(t, "scales")
-    ops._same_device(device, scales=t)
+    ops._same_device(t, "scales", device)
     if t.dtype != torch.uint8:
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mxfp4 scales must be uint8, got {t.dtype}")
     return t if t.is_contiguous() else t.contiguous()
@@ -49,7 +49,7 @@ def _scales(t: torch.Tensor, device) -> torch.Tensor:
 def _weights(w: torch.Tensor, scales: torch.Tensor, device, dims: int):
     """Checked codes and scales, and their [(E,) N, K]."""
     w = ops._words(w, "w")
-    ops._same_device(device, w=w)
+    ops._same_device(w, "w", device)
     scales = _scales(scales, device)
     if w.dim() != dims:
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"w must have {dims} dimensions, got {tuple(w.shape)}")
@@ -162,7 +162,7 @@ class _Product(torch.autograd.Function):
         return _product(x, w, scales, E, N, K, transpose, rows)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops._first_order
     def backward(ctx, dy):
         w, scales = ctx.saved_tensors
         n_x, E, N, K, transpose, rows = ctx.args
@@ -182,6 +182,11 @@ class _Product(torch.autograd.Function):
         return dx, None, None, None, None, None, None, None
 
 
+def _run(x, w, scales, E, N, K, transpose, rows):
+    """_product, recorded where a gradient of x may be asked for."""
+    return (_Product.apply if ops._records(x) else _product)(x, w, scales, E, N, K, transpose, rows)
+
+
 def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=None, transpose: bool = True,
                      group_size: int | None = None, bits: int = 4) -> torch.Tensor:
     """x [.., K] W^T (transpose) or x [.., N] W for codes w [N, K/8]."""
@@ -190,9 +195,27 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, bia
     w, scales, N, K = _weights(w, scales, x.device, 2)
     if x.dim() < 1 or x.shape[-1] != (K if transpose else N):
         raise ValueError(f"x {tuple(x.shape)} does not fit w [{N}, {K}] with transpose={transpose}")
-    x2 = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(math.prod(x.shape[:-1]), x.shape[-1])
-    y = _Product.apply(x2, w, scales, 1, N, K, bool(transpose), _Rows(x2.shape[0]))
-    return y.reshape(*x.shape[:-1], y.shape[-1])
+    x2 = _rows_of(x)
+    y = _run(x2, w, scales, 1, N, K, bool(transpose), _Rows(x2.shape[0]))
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+def _broadcast(a, b) -> tuple:
+    """torch.broadcast_shapes of two shapes, without its overhead."""
+    a, b = tuple(a), tuple(b)
+    a, b = (1,) * (len(b) - len(a)) + a, (1,) * (len(a) - len(b)) + b
+    if any(i != j and i != 1 and j != 1 for i, j in zip(a, b)):
+        raise ValueError(f"batches {a} and {b} do not broadcast")
+    return tuple(j if i == 1 else i for i, j in zip(a, b))
+
+
+def _flat(t, batch):
+    """Indices over the batch as a contiguous int32 vector."""
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    if t.shape != batch:
+        t = t.expand(batch)
+    return ops._ready(t if t.dim() == 1 else t.reshape(-1))
 
 
 def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
@@ -201,30 +224,34 @@ def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
     order with its inverse (None: the batch's own).  ``min_rows`` rows or more
     are sorted and get a tile table."""
     dev = x.device
-    M, xb = x.shape[-2], tuple(x.shape[:-2])
+    M, xb = x.shape[-2], x.shape[:-2]
     if rhs is None:
         rhs = torch.arange(E, device=dev, dtype=torch.int32)
     else:
         ops._dev(rhs, "rhs_indices")
-        ops._same_device(dev, rhs_indices=rhs)
+        ops._same_device(rhs, "rhs_indices", dev)
     x_rows, div = None, 1
     if lhs is None:
-        batch = torch.broadcast_shapes(xb, tuple(rhs.shape))
-        nb, nx = math.prod(batch), math.prod(xb)
-        # batch index i reads x's batch index i // (nb / nx) where only x's last dimensions are broadcast
-        lead = (1,) * (len(batch) - len(xb)) + xb
-        cut = next((d for d in range(len(batch) + 1) if math.prod(lead[d:]) == 1), len(batch))
-        if lead[:cut] == tuple(batch[:cut]):
-            div = nb // nx if nx else 1
-        else:
-            x_rows = torch.arange(nx, device=dev, dtype=torch.int32).reshape(lead).expand(batch).reshape(-1)
+        batch = rhs.shape if xb == rhs.shape else torch.Size(_broadcast(xb, rhs.shape))
+        nb = math.prod(batch)
+        if xb != batch:
+            nx = math.prod(xb)
+            # batch index i reads x's batch index i // (nb / nx) where only x's last dimensions are broadcast
+            lead = (1,) * (len(batch) - len(xb)) + tuple(xb)
+            cut = len(batch)
+            while cut and lead[cut - 1] == 1:
+                cut -= 1
+            if lead[:cut] == tuple(batch[:cut]):
+                div = nb // nx if nx else 1
+            else:
+                x_rows = torch.arange(nx, device=dev, dtype=torch.int32).reshape(lead).expand(batch).reshape(-1)
     else:
         ops._dev(lhs, "lhs_indices")
-        ops._same_device(dev, lhs_indices=lhs)
-        batch = torch.broadcast_shapes(tuple(lhs.shape), tuple(rhs.shape))
+        ops._same_device(lhs, "lhs_indices", dev)
+        batch = lhs.shape if lhs.shape == rhs.shape else torch.Size(_broadcast(lhs.shape, rhs.shape))
         nb = math.prod(batch)
-        x_rows = ops._i32(lhs.expand(batch).reshape(-1), "lhs_indices", dev)
-    experts = ops._i32(rhs.expand(batch).reshape(-1), "rhs_indices", dev)
+        x_rows = _flat(lhs, batch)
+    experts = _flat(rhs, batch)
     if M != 1 and nb:  # rows of one batch index: M activation rows, one expert
         ar = torch.arange(M, device=dev, dtype=torch.int32)
         base = x_rows if x_rows is not None else None if div == 1 else _x_rows(_Rows(nb, None, div), dev)
@@ -266,7 +293,8 @@ def _check_gather(x, w, scales, transpose, lhs, rhs):
 
 
 def _rows_of(x):
-    return x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(math.prod(x.shape[:-1]), x.shape[-1])
+    """x as [rows, C]."""
+    return x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
 
 
 def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=None, lhs_indices=None,
@@ -281,14 +309,14 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=No
     w, scales, E, N, K = _check_gather(x, w, scales, transpose, lhs_indices, rhs_indices)
     batch, rows, order = _gathered(x, E, lhs_indices, rhs_indices, sorted_indices, tiles, SORTED_MIN_ROWS)
     x2 = _rows_of(x)
-    y = _Product.apply(x2, w, scales, E, N, K, bool(transpose), rows)
+    y = _run(x2, w, scales, E, N, K, bool(transpose), rows)
     if order is not None:
-        y = token_sort._Sort.apply(y, order[1], order[0])
-    return y.reshape(*batch, x.shape[-2], y.shape[-1])
+        y = token_sort._sort(y, order[1], order[0])
+    return y.reshape(batch + (x.shape[-2], y.shape[-1]))
 
 
 def _no_grad(x: torch.Tensor) -> None:
-    if x.requires_grad and torch.is_grad_enabled():
+    if ops._records(x):
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, "the products of quantised activations have no gradient: "
                                                     "detach x, or use quantized_matmul / gather_qmm")
 
@@ -340,5 +368,5 @@ def gather_qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, lhs_indi
     x2 = _rows_of(x)
     y = _qq_product(x2, w, scales, E, N, K, rows)
     if order is not None:
-        y = token_sort._Sort.apply(y, order[1], order[0])
-    return y.reshape(*batch, x.shape[-2], N)
+        y = token_sort._sort(y, order[1], order[0])
+    return y.reshape(batch + (x.shape[-2], N))

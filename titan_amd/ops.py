@@ -109,20 +109,36 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _same_device(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
+def _same_device(t: torch.Tensor, name: str, device) -> None:
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
 
 
 def _launch(name: str, t: torch.Tensor, *args) -> None:
     """Entry point ``name`` on the device of ``t`` and that device's current
     stream (every entry point's last argument), whichever device is current."""
-    if t.device.index in (None, torch.cuda.current_device()):
-        _lib.call(name, *args, _stream(t))
+    index = t.get_device()
+    if index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(t.device):
-            _lib.call(name, *args, _stream(t))
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _first_order(backward):
+    """once_differentiable, whose wrapper runs only where a graph of the gradient
+    is asked for (it costs several us a call, of a backward pass of 15)."""
+    once = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (once if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
+def _records(t: torch.Tensor) -> bool:
+    """Must a call with ``t`` go through autograd?"""
+    return t.requires_grad and torch.is_grad_enabled()
 
 
 # ------------------------------------------------------------------ layout

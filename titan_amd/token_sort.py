@@ -30,12 +30,13 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
 
 def _pairs(t: torch.Tensor, name: str, device, n: int | None = None) -> torch.Tensor:
     ops._dev(t, name)
-    ops._same_device(device, **{name: t})
+    ops._same_device(t, name, device)
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
     if n is not None and t.numel() != n:
         raise ValueError(f"{name} holds {t.numel()} pairs, not {n}")
-    return ops._ready(t.reshape(-1).to(torch.int32))
+    t = t if t.dtype == torch.int32 else t.to(torch.int32)
+    return ops._ready(t if t.dim() == 1 else t.reshape(-1))
 
 
 def unsort_sum(rows: torch.Tensor, inv: torch.Tensor | None, scores: torch.Tensor | None, T: int, k: int,
@@ -48,22 +49,30 @@ def unsort_sum(rows: torch.Tensor, inv: torch.Tensor | None, scores: torch.Tenso
     return y
 
 
+def _sort_rows(x, order):
+    n, (T, D) = order.numel(), x.shape
+    xs = torch.empty(n, D, dtype=x.dtype, device=x.device)
+    ops._launch("qmoe_sort_rows", x, x.data_ptr(), T, order.data_ptr(), n // T if T else 0, D, ops._DTYPES[x.dtype],
+                xs.data_ptr())
+    return xs
+
+
 class _Sort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order, inv):
-        n, (T, D) = order.numel(), x.shape
-        k = n // T if T else 0
         ctx.save_for_backward(inv)
-        ctx.T, ctx.k = T, k
-        xs = torch.empty(n, D, dtype=x.dtype, device=x.device)
-        ops._launch("qmoe_sort_rows", x, x.data_ptr(), T, order.data_ptr(), k, D, ops._DTYPES[x.dtype], xs.data_ptr())
-        return xs
+        ctx.T = x.shape[0]
+        return _sort_rows(x, order)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops._first_order
     def backward(ctx, dxs):
-        (inv,) = ctx.saved_tensors
-        return unsort_sum(ops._ready(dxs), inv, None, ctx.T, ctx.k), None, None
+        (inv,), T = ctx.saved_tensors, ctx.T
+        return unsort_sum(ops._ready(dxs), inv, None, T, dxs.shape[0] // T if T else 0), None, None
+
+
+def _sort(x, order, inv):
+    return _Sort.apply(x, order, inv) if ops._records(x) else _sort_rows(x, order)
 
 
 class _Unsort(torch.autograd.Function):
@@ -75,7 +84,7 @@ class _Unsort(torch.autograd.Function):
         return unsort_sum(xs, inv, scores, T, k)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops._first_order
     def backward(ctx, dy):
         xs, inv, scores = ctx.saved_tensors
         (n, D), dtype = ctx.like
@@ -96,7 +105,7 @@ def sort_tokens(x: torch.Tensor, order: torch.Tensor, inv_order: torch.Tensor) -
     n, T = order.numel(), x.shape[0]
     if n % T if T else n:
         raise ValueError(f"order holds {n} pairs, not a multiple of x's {T} rows")
-    return _Sort.apply(x, order, _pairs(inv_order, "inv_order", x.device, n))
+    return _sort(x, order, _pairs(inv_order, "inv_order", x.device, n))
 
 
 def unsort_tokens(xs: torch.Tensor, order: torch.Tensor, inv_order: torch.Tensor,
@@ -110,9 +119,12 @@ def unsort_tokens(xs: torch.Tensor, order: torch.Tensor, inv_order: torch.Tensor
     inv = _pairs(inv_order, "inv_order", xs.device, n)
     order = _pairs(order, "order", xs.device, n)
     if scores is None:
-        return _Sort.apply(xs, inv, order)
+        return _sort(xs, inv, order)
     ops._dev(scores, "scores")
-    ops._same_device(xs.device, scores=scores)
+    ops._same_device(scores, "scores", xs.device)
     if scores.dim() != 2 or scores.numel() != n:
         raise ValueError(f"scores must be [T, k] with T * k = {n}, got {tuple(scores.shape)}")
-    return _Unsort.apply(xs, inv, ops._ready(scores.to(torch.float32)))
+    scores = ops._ready(scores if scores.dtype == torch.float32 else scores.to(torch.float32))
+    if ops._records(xs) or ops._records(scores):
+        return _Unsort.apply(xs, inv, scores)
+    return unsort_sum(xs, inv, scores, *scores.shape)
