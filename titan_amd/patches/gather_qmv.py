@@ -3,7 +3,10 @@
 
 The reference leaves these shapes on MLX's own gather_qmv
 (titan/adapters/mlx/compiled.py:490-518, 209-218); this overlay is their
-drop-in.  Routed when: ``sorted_indices`` false, affine ``transpose=True``
+drop-in.  It also takes every call of both with ``mode="mxfp4"`` and bf16
+activations on the GPU, sorted or not, either way round and with gradients
+(:mod:`titan_amd.mxfp4`): the prefill overlays above it take affine weights
+alone.  Affine calls are routed when: ``sorted_indices`` false, affine ``transpose=True``
 weights with biases, bf16 activations on the GPU.  Shapes the kernels do not
 take (bits other than 4 and 8, group sizes other than 32/64/128, K outside the
 kernels' range: 8-bit codes up to K = 4096) raise
@@ -27,13 +30,19 @@ def _gpu_bf16(x) -> bool:
 
 
 def _route_gather_ok(ov, x, w, args, kwargs) -> bool:
-    if not ov.enabled() or kwargs.get("sorted_indices") or not _gpu_bf16(x):
+    if not ov.enabled() or not _gpu_bf16(x):
+        return False
+    if arg(args, kwargs, 7, "mode", "affine") == "mxfp4":
+        return True
+    if kwargs.get("sorted_indices"):
         return False
     return (arg(args, kwargs, 7, "mode", "affine") == "affine" and bool(arg(args, kwargs, 4, "transpose", True))
             and arg(args, kwargs, 1, "biases") is not None)
 
 
 def _route_gather(x, w, args, kwargs):
+    if arg(args, kwargs, 7, "mode", "affine") == "mxfp4":
+        return ops.gather_qmm(x, w, *args, **kwargs)
     return ops.gather_qmm(x, w, arg(args, kwargs, 0, "scales"), arg(args, kwargs, 1, "biases"),
                           lhs_indices=arg(args, kwargs, 2, "lhs_indices"),
                           rhs_indices=arg(args, kwargs, 3, "rhs_indices"), transpose=True,
@@ -43,11 +52,15 @@ def _route_gather(x, w, args, kwargs):
 def _route_qmm_ok(ov, x, w, args, kwargs) -> bool:
     if not ov.enabled() or not _gpu_bf16(x):
         return False
+    if arg(args, kwargs, 5, "mode", "affine") == "mxfp4":
+        return True
     return (arg(args, kwargs, 5, "mode", "affine") == "affine" and bool(arg(args, kwargs, 2, "transpose", True))
             and arg(args, kwargs, 1, "biases") is not None)
 
 
 def _route_qmm(x, w, args, kwargs):
+    if arg(args, kwargs, 5, "mode", "affine") == "mxfp4":
+        return ops.quantized_matmul(x, w, *args, **kwargs)
     return ops.quantized_matmul(x, w, arg(args, kwargs, 0, "scales"), arg(args, kwargs, 1, "biases"),
                                 group_size=arg(args, kwargs, 3, "group_size", 64), bits=arg(args, kwargs, 4, "bits", 4))
 
@@ -55,9 +68,10 @@ def _route_qmm(x, w, args, kwargs):
 def _self_check(found) -> bool:
     if not torch.cuda.is_available():
         return True
-    from ._selfcheck import decode_gather_matches
+    from ._selfcheck import decode_gather_matches, mxfp4_gather_matches
 
-    return decode_gather_matches(found["gather_qmm"], ops.gather_qmm)
+    return (decode_gather_matches(found["gather_qmm"], ops.gather_qmm)
+            and mxfp4_gather_matches(found["gather_qmm"], ops.gather_qmm))
 
 
 _OV = Overlay("moe decode gather-qmv", MARKER, "TITAN_AMD_MOE_DECODE", True,

@@ -65,10 +65,18 @@ def _plain(t: torch.Tensor, width: int) -> bool:
             and t.is_contiguous() and width % 8 == 0 and t.data_ptr() % 16 == 0)
 
 
-def _gather_sort(x: torch.Tensor, indices: torch.Tensor, num_experts: int):
+def _learns(t: torch.Tensor) -> bool:
+    """May the token sort's kernels move the rows of ``t`` and their gradient?"""
+    return (type(t) is torch.Tensor and t.is_cuda and t.dtype in ops._DTYPES and ops._records(t)
+            and not torch._C._functorch.is_functorch_wrapped_tensor(t) and forward_ad._current_level < 0
+            and not torch.jit.is_tracing() and not torch.compiler.is_compiling())
+
+
+def _gather_sort(x: torch.Tensor, indices: torch.Tensor, num_experts: int, learns: bool = False):
     """Stable sort of the flattened pairs by expert (switch_layers.py:13-18):
     rows of x in sorted order, sorted ids, inverse permutation, tile table
-    (None off the GPU)."""
+    (None off the GPU).  With ``learns`` the permutation comes with its inverse
+    and the rows are ones whose gradient the token sort's kernels form."""
     M = indices.shape[-1]
     flat = indices.reshape(-1)
     rows = math.prod(x.shape[:-2])
@@ -77,6 +85,9 @@ def _gather_sort(x: torch.Tensor, indices: torch.Tensor, num_experts: int):
     if flat.is_cuda:
         r = ops.route(flat, num_experts)
         order, inv, ids, tiles = r.order, r.inv_order, r.sorted_ids, r.tiles
+        if learns:
+            return ops.sort_tokens(x.reshape(-1, x.shape[-1])[:flat.numel() // M], order, inv).unsqueeze(1), ids, \
+                (inv, order), tiles
         if x.numel() and _plain(x, x.shape[-1]) and x.shape[-2] == 1:
             xs = ops.gather_rows(x.reshape(-1, x.shape[-1]), order, M)
             return xs.unsqueeze(1), ids, inv, tiles
@@ -90,7 +101,9 @@ def _gather_sort(x: torch.Tensor, indices: torch.Tensor, num_experts: int):
 
 def _scatter_unsort(x: torch.Tensor, inv_order: torch.Tensor, shape=None) -> torch.Tensor:
     """switch_layers.py:21-25."""
-    if x.dim() == 3 and x.shape[1] == 1 and inv_order.dtype == torch.int32 and _plain(x, x.shape[-1]):
+    if isinstance(inv_order, tuple):
+        x = ops.unsort_tokens(x.squeeze(1), inv_order[1], inv_order[0]).unsqueeze(1)
+    elif x.dim() == 3 and x.shape[1] == 1 and inv_order.dtype == torch.int32 and _plain(x, x.shape[-1]):
         x = ops.gather_rows(x.reshape(-1, x.shape[-1]), inv_order).unsqueeze(1)
     else:
         x = x[inv_order.long()]
@@ -101,10 +114,13 @@ def _scatter_unsort(x: torch.Tensor, inv_order: torch.Tensor, shape=None) -> tor
 
 class QuantizedSwitchLinear:
     """Per-expert quantized linear layer: weight [E, N, K*bits/32] packed
-    words, scales/biases [E, N, K/group_size] bf16, optional bias [E, N]."""
+    words, scales/biases [E, N, K/group_size] bf16, optional bias [E, N].
+    ``mode="mxfp4"``: 4-bit codes, scales uint8 [E, N, K/32], biases None."""
 
-    def __init__(self, weight, scales, biases, group_size: int = 64, bits: int = 4, mode: str = "affine",
+    def __init__(self, weight, scales, biases=None, group_size: int | None = None, bits: int = 4, mode: str = "affine",
                  bias: torch.Tensor | None = None):
+        if group_size is None:
+            group_size = 32 if mode == "mxfp4" else 64
         self.weight, self.scales, self.biases = weight, scales, biases
         self.group_size, self.bits, self.mode = group_size, bits, mode
         self.bias = bias
@@ -178,7 +194,9 @@ class SwitchGLU:
         do_sort = indices.numel() >= 64
         idx, inv_order, tiles = indices, None, None
         if do_sort:
-            x, idx, inv_order, tiles = _gather_sort(x, indices, self.num_experts)
+            # through mxfp4 experts a layer can be trained: rows and gradients by the token sort's kernels
+            learns = self.down_proj.mode == "mxfp4" and _learns(x)
+            x, idx, inv_order, tiles = _gather_sort(x, indices, self.num_experts, learns)
         if self.gate_up_proj is not None:
             gu = self.gate_up_proj(x, idx, sorted_indices=do_sort, tiles=tiles)
             if _default(self.activation) and gu.shape[-1] % 2 == 0 and _plain(gu, gu.shape[-1] // 2):
