@@ -21,6 +21,11 @@ namespace qmoe_mx {
 constexpr int kBlock = 32;  // elements per scale
 
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+// Byte b of four scale bytes as the conversions' operand, in one rotation: they
+// use the exponent field alone, whatever the sign and the mantissa bits are.
+__device__ __forceinline__ float scale_of(uint32_t four, int b) {
+  return __uint_as_float(__builtin_amdgcn_alignbit(four, four, (8 * b + 9) & 31));
+}
 
 // Codes 2*SEL and 2*SEL + 1 of a word as a bf16 pair, low half first.
 template <int SEL>

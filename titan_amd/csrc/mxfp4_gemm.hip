@@ -3,6 +3,7 @@
 // rows), and activations in mxfp4 too (format in mxfp4.h).  Rows are those of
 // a tile table (sorted by expert), or of one expert without a table.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_common.h"
 #include "mxfp4.h"
@@ -171,8 +172,9 @@ __device__ __forceinline__ void store_rows(const GemmArgs& a, const char* ep, co
       const int lr = i / 32, unit = i % 32;
       const int row = row_of(lr);
       if (row < u.valid && u.o0 + 8 * unit < O)
-        *reinterpret_cast<uint4*>(out + (u.row0 + row) * O + u.o0 + 8 * unit) =
-            *reinterpret_cast<const uint4*>(ep + lr * 512 + ((2 * unit) ^ (2 * (lr % 32))) * 8);
+        __builtin_nontemporal_store(
+            *reinterpret_cast<const i32x4_t*>(ep + lr * 512 + ((2 * unit) ^ (2 * (lr % 32))) * 8),
+            reinterpret_cast<i32x4_t*>(out + (u.row0 + row) * O + u.o0 + 8 * unit));
     }
   } else {
     for (int i = tid; i < 64 * 256; i += 256) {
@@ -248,19 +250,24 @@ struct Fwd {
     int64_t C;
   };
 
-  static __device__ __forceinline__ void copy_x(const Ctx& c, int g) {
-    const uint32_t dst = c.lds + (g & 1) * kA + c.wave * 1024;
+  static __device__ __forceinline__ void copy_x(const Ctx& c, int g, int stage) {
+    const uint32_t dst = c.lds + stage * kA + c.wave * 1024;
     const bool whole = (int64_t)(g + 1) * 64 <= c.C;
+    if (whole) {
 #pragma unroll
-    for (int d = 0; d < kACopies; ++d) {
-      const char* p = c.x.p[d] + (size_t)g * 128;
-      if (!whole && (int64_t)g * 64 + c.x.unit(d) * 8 >= c.C) p = reinterpret_cast<const char*>(zero_page);
-      qmoe_gemm::dma16(p, dst + d * Way::kWaves * 1024);
+      for (int d = 0; d < kACopies; ++d) qmoe_gemm::dma16(c.x.p[d] + (size_t)g * 128, dst + d * Way::kWaves * 1024);
+    } else {
+#pragma unroll
+      for (int d = 0; d < kACopies; ++d) {
+        const bool in = (int64_t)g * 64 + c.x.unit(d) * 8 < c.C;
+        qmoe_gemm::dma16(in ? c.x.p[d] + (size_t)g * 128 : reinterpret_cast<const char*>(zero_page),
+                         dst + d * Way::kWaves * 1024);
+      }
     }
   }
-  static __device__ __forceinline__ void copy_w(const Ctx& c, int p) {
-    const uint32_t dst = c.lds + kBOff + (p & 1) * kB + c.wave * 1024;
-    const uint32_t sdst = c.lds + kSOff + (p & 1) * kS + c.wave * 256;
+  static __device__ __forceinline__ void copy_w(const Ctx& c, int p, int stage) {
+    const uint32_t dst = c.lds + kBOff + stage * kB + c.wave * 1024;
+    const uint32_t sdst = c.lds + kSOff + stage * kS + c.wave * 256;
     const bool whole = 4 * (p + 1) <= c.units;
 #pragma unroll
     for (int d = 0; d < kBCopies; ++d) {
@@ -293,24 +300,25 @@ struct Fwd {
     i32x4_t w[NSUB];
     float s[NSUB];
   };
-  static __device__ __forceinline__ void read_x(const Ctx& c, const char* smem, int g, int kk, int row0, Frag& f) {
+  // Group `at` of the wave's part (its stages, and the half of its pair): a constant in the main loop.
+  static __device__ __forceinline__ void read_x(const Ctx& c, const char* smem, int at, int kk, int row0, Frag& f) {
     const int l32 = c.lane % 32, h = c.lane / 32;
-    const char* st = smem + (g & 1) * kA + row0 * 128;
+    const char* st = smem + row0 * 128 + l32 * 128 + ((4 * h + kk) ^ swz8(l32)) * 16 + (at & 1) * kA;
 #pragma unroll
     for (int i = 0; i < MSUB; ++i)  // swz8(row0 + 32 i + l32) == swz8(l32)
-      f.a[i] = *reinterpret_cast<const i32x4_t*>(st + (32 * i + l32) * 128 + ((4 * h + kk) ^ swz8(l32)) * 16);
+      f.a[i] = *reinterpret_cast<const i32x4_t*>(st + i * 4096);
   }
-  static __device__ __forceinline__ Codes read_codes(const Ctx& c, const char* smem, int g, int col0) {
-    const int l32 = c.lane % 32, unit = 2 * (g & 1) + c.lane / 32;
-    const char* st = smem + kBOff + ((g >> 1) & 1) * kB;
-    const char* ss = smem + kSOff + ((g >> 1) & 1) * kS;
+  static __device__ __forceinline__ Codes read_codes(const Ctx& c, const char* smem, int at, int col0) {
+    const int l32 = c.lane % 32, h = c.lane / 32, half = at & 1, stage = (at >> 1) & 1;
+    // the lane's unit 2 half + h, swizzled: swz4(col) == swz4(l32)
+    const char* st = smem + kBOff + (col0 + l32) * 64 + ((h ^ swz4(l32)) ^ (2 * half)) * 16 + stage * kB;
+    const char* ss = smem + kSOff + (col0 + l32 + (S4 ? 0 : h * kCols)) * 4 + stage * kS + (S4 ? 0 : half * 2 * kCols * 4);
     Codes r;
 #pragma unroll
     for (int j = 0; j < NSUB; ++j) {
-      const int col = col0 + 32 * j + l32;
-      r.w[j] = *reinterpret_cast<const i32x4_t*>(st + col * 64 + (unit ^ swz4(col)) * 16);
-      if constexpr (S4) r.s[j] = scale_of((*reinterpret_cast<const uint32_t*>(ss + col * 4) >> (8 * unit)) & 255u);
-      else r.s[j] = scale_of(*reinterpret_cast<const uint32_t*>(ss + (unit * kCols + col) * 4));
+      r.w[j] = *reinterpret_cast<const i32x4_t*>(st + j * 2048);
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(ss + j * 128);
+      r.s[j] = S4 ? scale_of(v, 2 * half + h) : scale_of(v);
     }
     return r;
   }
@@ -351,7 +359,7 @@ struct Fwd {
               f32x4_t{acc[i][j][v], acc[i][j][v + 1], acc[i][j][v + 2], acc[i][j][v + 3]};
   }
 
-  static __device__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
+  static __device__ __forceinline__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
     Ctx c;
     const int tid = fresh_tid();
     c.lane = tid % 64;
@@ -383,40 +391,57 @@ struct Fwd {
 
     f32x16_t acc[MSUB][NSUB] = {};
     if (!SPLIT || g0 < G) {
-    copy_x(c, g0);
-    copy_w(c, g0 / 2);
-    if (g0 + 1 < G) copy_x(c, g0 + 1);
-    if (g0 / 2 + 1 < P) copy_w(c, g0 / 2 + 1);
-    qmoe_gemm::wait_vmem<0>();
-    Way::barrier();
-    Frag fa, fb;
-    Codes q = read_codes(c, smem, g0, col0);
-    read_x(c, smem, g0, 0, row0, fa);
-#pragma unroll
-    for (int j = 0; j < NSUB; ++j) convert(q, 0, j, fa);
-    for (int g = g0; g < G - 1; ++g) {
-      read_x(c, smem, g, 1, row0, fb);
-      step<true>(fa, fb, q, 1, acc);
-      read_x(c, smem, g, 2, row0, fa);
-      step<true>(fb, fa, q, 2, acc);
-      read_x(c, smem, g, 3, row0, fb);
-      step<true>(fa, fb, q, 3, acc);
-      qmoe_gemm::wait_vmem<0>();
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      constexpr int kPairCopies = kBCopies + kSCopies * (S4 ? 1 : 4);
+      const int p0 = g0 / 2;
+      copy_x(c, g0, 0);
+      copy_w(c, p0, 0);
+      if (g0 + 1 < G) copy_x(c, g0 + 1, 1);
+      if (p0 + 1 < P) copy_w(c, p0 + 1, 1);
+      if (p0 + 1 < P) qmoe_gemm::wait_vmem<kACopies + kPairCopies>();
+      else qmoe_gemm::wait_vmem<0>();
       Way::barrier();
-      if (g + 2 < G) copy_x(c, g + 2);
-      if ((g & 1) && (g >> 1) + 2 < P) copy_w(c, (g >> 1) + 2);
-      q = read_codes(c, smem, g + 1, col0);
-      read_x(c, smem, g + 1, 0, row0, fa);
-      step<true>(fb, fa, q, 0, acc);
-    }
-    read_x(c, smem, G - 1, 1, row0, fb);
-    step<true>(fa, fb, q, 1, acc);
-    read_x(c, smem, G - 1, 2, row0, fa);
-    step<true>(fb, fa, q, 2, acc);
-    read_x(c, smem, G - 1, 3, row0, fb);
-    step<true>(fa, fb, q, 3, acc);
-    step<false>(fb, fa, q, 0, acc);
+      Frag fa, fb;
+      Codes q = read_codes(c, smem, 0, col0);
+      read_x(c, smem, 0, 0, row0, fa);
+#pragma unroll
+      for (int j = 0; j < NSUB; ++j) convert(q, 0, j, fa);
+      int g = g0;
+      // a group but the last, `at` of the part (mod 4: a constant where four of them are run in turn)
+      const auto group = [&](auto at_) {
+        const int at = at_ & 3;
+        read_x(c, smem, at, 1, row0, fb);
+        step<true>(fa, fb, q, 1, acc);
+        read_x(c, smem, at, 2, row0, fa);
+        step<true>(fb, fa, q, 2, acc);
+        read_x(c, smem, at, 3, row0, fb);
+        step<true>(fa, fb, q, 3, acc);
+        // the next group landed, a pair of weights behind it may be in flight; this one's stages are read
+        if (at % 2 == 0 && g / 2 + 1 < P) qmoe_gemm::wait_vmem<kPairCopies>();
+        else qmoe_gemm::wait_vmem<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        Way::barrier();
+        if (g + 2 < G) copy_x(c, g + 2, at % 2);
+        if (at % 2 && g / 2 + 2 < P) copy_w(c, g / 2 + 2, at / 2);
+        q = read_codes(c, smem, (at + 1) % 4, col0);
+        read_x(c, smem, (at + 1) % 4, 0, row0, fa);
+        step<true>(fb, fa, q, 0, acc);
+        ++g;
+      };
+      while (g + 4 < G) {
+        group(std::integral_constant<int, 0>{});
+        group(std::integral_constant<int, 1>{});
+        group(std::integral_constant<int, 2>{});
+        group(std::integral_constant<int, 3>{});
+      }
+      while (g + 1 < G) group(g - g0);
+      const int at = (G - 1 - g0) & 3;
+      read_x(c, smem, at, 1, row0, fb);
+      step<true>(fa, fb, q, 1, acc);
+      read_x(c, smem, at, 2, row0, fa);
+      step<true>(fb, fa, q, 2, acc);
+      read_x(c, smem, at, 3, row0, fb);
+      step<true>(fa, fb, q, 3, acc);
+      step<false>(fb, fa, q, 0, acc);
     }
     const int lane = fresh_tid() % 64, l32 = lane % 32, h = lane / 32;
     if constexpr (SPLIT) {
@@ -490,48 +515,52 @@ struct Trn {
     RowSrc<kACopies, 8, Way::kWaves> x;
     const char *w, *s;  // of the expert's first row, at the column block
     int64_t wpitch, spitch;
-    int wunit, wrow, sblk[kSCopies];
+    uint32_t woff[kBCopies], soff[kSCopies];  // the lane's bytes from there
+    int pos;                                  // row slot of copy 0
     uint32_t lds;
     int wave, lane;  // wave: of those that fill the ring
     int64_t C;
+    __device__ __forceinline__ int row(int d) const { return w_row(pos + (SPLIT ? 16 : 32) * d); }
   };
 
   static __device__ __forceinline__ void copy(const Ctx& c, int g) {
     const uint32_t st = c.lds + (g % NS) * kStage;
+    const uint32_t xd = st + c.wave * 1024, wd = st + kA + c.wave * 1024, sd = st + kA + kB;
     const int64_t left = c.C - (int64_t)g * 64;  // rows n of this group and after
+    const char* w = c.w + (int64_t)g * 64 * c.wpitch;
+    const char* s = c.s + (int64_t)g * 64 * c.spitch;
+    if (left >= 64) {
 #pragma unroll
-    for (int d = 0; d < kACopies; ++d) {
-      const char* p = c.x.p[d] + (size_t)g * 128;
-      if (c.x.unit(d) * 8 >= left) p = reinterpret_cast<const char*>(zero_page);
-      qmoe_gemm::dma16(p, st + (d * Way::kWaves + c.wave) * 1024);
-    }
+      for (int d = 0; d < kACopies; ++d) qmoe_gemm::dma16(c.x.p[d] + (size_t)g * 128, xd + d * Way::kWaves * 1024);
 #pragma unroll
-    for (int d = 0; d < kBCopies; ++d) {
-      const int n = SPLIT ? w_row(16 * d + c.wrow) : c.wrow + 32 * d;  // w_row(pos + 32) == w_row(pos) + 32
-      const char* p = c.w + ((int64_t)g * 64 + n) * c.wpitch;
-      if (n >= left) p = reinterpret_cast<const char*>(zero_page);
-      qmoe_gemm::dma16(p, st + kA + (d * Way::kWaves + c.wave) * 1024);
-    }
-    const char* s = c.s + ((int64_t)g * 64 + c.lane) * c.spitch;
-    if constexpr (S4) {
-      s += c.sblk[0];
-      if (c.lane >= left) s = reinterpret_cast<const char*>(zero_page);
-      qmoe_gemm::dma4(s, st + kA + kB + (c.wave & 1) * 256);
-    } else {
+      for (int d = 0; d < kBCopies; ++d) qmoe_gemm::dma16s(w, c.woff[d], wd + d * Way::kWaves * 1024);
 #pragma unroll
       for (int d = 0; d < kSCopies; ++d) {
-        const char* p = s + c.sblk[d];
-        if (c.lane >= left) p = reinterpret_cast<const char*>(zero_page);
-        dma1(p, st + kA + kB + (kSCopies * c.wave + d) * 256);
+        if constexpr (S4) qmoe_gemm::dma4s(s, c.soff[d], sd + (c.wave & 1) * 256);
+        else dma1s(s, c.soff[d], sd + (kSCopies * c.wave + d) * 256);
+      }
+    } else {  // the last group of a contraction that is no multiple of 64
+      const char* zero = reinterpret_cast<const char*>(zero_page);
+#pragma unroll
+      for (int d = 0; d < kACopies; ++d)
+        qmoe_gemm::dma16(c.x.unit(d) * 8 < left ? c.x.p[d] + (size_t)g * 128 : zero, xd + d * Way::kWaves * 1024);
+#pragma unroll
+      for (int d = 0; d < kBCopies; ++d)
+        qmoe_gemm::dma16(c.row(d) < left ? w + c.woff[d] : zero, wd + d * Way::kWaves * 1024);
+#pragma unroll
+      for (int d = 0; d < kSCopies; ++d) {
+        const char* p = c.lane < left ? s + c.soff[d] : zero;
+        if constexpr (S4) qmoe_gemm::dma4(p, sd + (c.wave & 1) * 256);
+        else dma1(p, sd + (kSCopies * c.wave + d) * 256);
       }
     }
   }
   // Row n of the group in the codes' row slot `pos` (its own inverse), and the unit in a unit slot: chosen so that
-  // the words that a wave reads at once, those of rows n + 8 q, fall on all 64 banks.
+  // the words that a wave reads at once, those of rows n + 8 q, fall on all banks, and those of half a wave on half.
   static __device__ __forceinline__ int w_row(int pos) {
-    return SPLIT ? pos ^ ((pos >> 3) & 3) : pos ^ ((pos >> 3) & 1);
+    return SPLIT ? pos ^ ((pos >> 3) & 3) : pos ^ ((pos >> 4) & 1);
   }
-  static __device__ __forceinline__ int w_unit(int slot, int pos) { return SPLIT ? slot : slot ^ (4 * ((pos >> 4) & 1)); }
+  static __device__ __forceinline__ int w_unit(int slot, int pos) { return SPLIT ? slot : slot ^ (4 * ((pos >> 3) & 1)); }
 
   struct Words {
     uint32_t w[8];
@@ -556,7 +585,7 @@ struct Trn {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t v = (uint32_t)(i < 4 ? lo[i & 3] : hi[i & 3]);
-      r.s[i] = scale_of(S4 ? (v >> (8 * (co / 4))) & 255u : v);
+      r.s[i] = S4 ? scale_of(v, co / 4) : scale_of(v);
     }
     return r;
   }
@@ -606,7 +635,7 @@ struct Trn {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  static __device__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
+  static __device__ __forceinline__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
     Ctx c;
     const int tid = fresh_tid();
     c.lane = tid % 64;
@@ -622,15 +651,17 @@ struct Trn {
     const int last = (int)min((int64_t)kUnits, units - u0) - 1;  // columns past the end: the last again
     c.wpitch = units * 16;
     c.spitch = units;
-    const int pos = c.wave * 8 + c.lane / kUnits;  // row slot of copy 0
-    c.wrow = SPLIT ? pos : w_row(pos);
-    c.wunit = w_unit(c.lane % kUnits, pos);
-    c.w = reinterpret_cast<const char*>(a.w) + (row * units + u0 + min(c.wunit, last)) * 16;
-    c.s = reinterpret_cast<const char*>(a.s) + row * units + u0;
-    if constexpr (S4) c.sblk[0] = !SPLIT && 4 * (c.wave & 1) <= last ? 4 * (c.wave & 1) : 0;
-    else
+    c.pos = c.wave * 8 + c.lane / kUnits;
+    c.w = reinterpret_cast<const char*>(a.w) + qmoe_gemm::uniform64((row * units + u0) * 16);
+    c.s = reinterpret_cast<const char*>(a.s) + qmoe_gemm::uniform64(row * units + u0);
+    const int unit = min(w_unit(c.lane % kUnits, c.pos), last);
 #pragma unroll
-      for (int d = 0; d < kSCopies; ++d) c.sblk[d] = min(kSCopies * c.wave + d, last);
+    for (int d = 0; d < kBCopies; ++d) c.woff[d] = (uint32_t)(c.row(d) * (int)c.wpitch + unit * 16);
+#pragma unroll
+    for (int d = 0; d < kSCopies; ++d) {
+      const int blk = S4 ? (SPLIT ? 0 : 4 * (c.wave & 1)) : kSCopies * c.wave + d;
+      c.soff[d] = (uint32_t)(c.lane * (int)c.spitch + (blk <= last ? blk : S4 ? 0 : last));
+    }
     int g0, G;  // this wave's groups
     Way::template part<1>((int)((a.N + 63) / 64), wave, &g0, &G);
     const int row0 = 16 * MSUB * wm;
@@ -829,7 +860,7 @@ struct QQ {
                                                                     2 * KK, sb[j], 2 * KK, sa[i]);
   }
 
-  static __device__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
+  static __device__ __forceinline__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
     Ctx c;
     const int tid = fresh_tid();
     c.lane = tid % 64;
