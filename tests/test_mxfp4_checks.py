@@ -8,6 +8,19 @@ from titan_amd import _lib, mxfp4, ops
 from titan_amd.ops import QmoeUnsupported
 
 BF = torch.bfloat16
+_lib_binding = _lib.binding
+
+
+class Binding:
+    """Declines every call that may be declined, and counts the others as launches."""
+
+    def __getattr__(self, name):
+        def call(*args):
+            if args[-1] is False and name != "rows_product" or name == "gather":
+                return None
+            raise AssertionError(f"{name} launched")
+
+        return call
 
 
 @pytest.fixture(autouse=True)
@@ -17,9 +30,9 @@ def no_launch(monkeypatch):
 
     monkeypatch.setattr(ops, "_dev", lambda t, name: None)
     monkeypatch.setattr(ops, "_stream", lambda t: 0)
-    monkeypatch.setattr(ops, "_launch", launch)
     monkeypatch.setattr(ops, "tile_rows", lambda: 128)
     monkeypatch.setattr(_lib, "call", launch)
+    monkeypatch.setattr(_lib, "binding", lambda: Binding())
 
 
 def _w(*shape):
@@ -209,5 +222,20 @@ def test_bad_arguments_at_the_entry_points():
     assert L.qmoe_unsort_grad(one, one, 6, 0, one, None, 3, 2, 8, one, one, None) == INV
 
 
-def test_widths_where_the_kernels_change():
-    assert mxfp4.QMV_MAX_ROWS >= 1 and mxfp4.SORTED_MIN_ROWS == ops.SORTED_MIN_ROWS
+def test_the_binding_declines_what_is_not_on_the_gpu():
+    """Without a GPU tensor every function answers None, and says so where it must not."""
+    B = _lib_binding()
+    x, od, (w, s) = torch.zeros(4, 64, dtype=BF), torch.arange(4, dtype=torch.int32), _w(5, 64)
+    for call in (lambda m: B.quantize(x, m), lambda m: B.dequantize(w, s, 0, m), lambda m: B.sort_tokens(x, od, od, m),
+                 lambda m: B.unsort_tokens(x, od, od, torch.ones(4, 1), m), lambda m: B.matmul(x, w, s, True, False, m),
+                 lambda m: B.quantize(None, m), lambda m: B.matmul("x", w, s, True, True, m)):
+        assert call(False) is None
+        with pytest.raises(RuntimeError, match="not what the kernels read"):
+            call(True)
+    assert B.gather(x, w, s, None, od, True, True, False) is None
+    with pytest.raises(RuntimeError, match="not what the kernels read"):
+        B.rows_product(x, w[None], s[None], None, 1, None, None, 4, True, False)
+
+
+def test_one_width_of_sorting():
+    assert mxfp4.SORTED_MIN_ROWS == ops.SORTED_MIN_ROWS == 64

@@ -8,10 +8,12 @@ switch to something else.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libqmoe.so"
+BINDING_PATH = LIB_PATH.with_name("_binding.so")
 
 OK = 0
 ERR_INVALID = 1
@@ -98,6 +100,7 @@ SIGNATURES: dict[str, tuple] = {
 
 _lock = threading.Lock()
 _lib = None
+_binding = None
 
 
 def load() -> ctypes.CDLL:
@@ -118,6 +121,25 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+def binding():
+    """The torch binding of the mxfp4 and token-sort operators
+    (csrc/torch/binding.cpp), which carries their autograd nodes."""
+    global _binding
+    if _binding is None:
+        load()
+        with _lock:
+            if _binding is None:
+                if not BINDING_PATH.exists():
+                    raise QmoeLibraryMissing(f"{BINDING_PATH} is not built; run `python -m titan_amd.build`")
+                import torch  # noqa: F401 - its libraries are the binding's
+
+                spec = importlib.util.spec_from_file_location("titan_amd.lib._binding", BINDING_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _binding = module
+    return _binding
 
 
 def available() -> bool:

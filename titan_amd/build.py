@@ -7,7 +7,10 @@ measured-ceiling probes, include/qmoe_peaks.h) becomes
 libqmoe.so with the decode GEMV's per-phase timestamps and the bf16 grouped
 GEMM's per-unit timestamps compiled in (QMOE_QMV_STAMPS, QMOE_GEMM_STAMPS,
 read by ``bench.py --decode-phases`` and ``--gemm-units``), a measurement
-build that nothing else loads.  The libraries land in-tree so that they travel with
+build that nothing else loads.  ``csrc/torch/binding.cpp`` becomes
+``titan_amd/lib/_binding.so``, the torch binding of the operators with
+gradients (host code over libqmoe.so; the one part that needs torch).  The
+libraries land in-tree so that they travel with
 the source tree; nothing is installed anywhere else.
 
     python -m titan_amd.build            # build (always recompiles)
@@ -32,6 +35,8 @@ LIB = LIB_DIR / "libqmoe.so"
 PEAKS_SRC = CSRC / "peaks" / "peaks.hip"
 PEAKS_LIB = LIB_DIR / "libqmoe_peaks.so"
 STAMPS_LIB = LIB_DIR / "libqmoe_stamps.so"
+BINDING_SRC = CSRC / "torch" / "binding.cpp"
+BINDING_LIB = LIB_DIR / "_binding.so"
 ARCH = os.environ.get("QMOE_OFFLOAD_ARCH", "gfx950")
 
 # -packed-fp32-ops: hipcc must not form v_pk_{add,mul,fma}_f32 on its own.
@@ -73,23 +78,56 @@ def _link(objs, lib: Path) -> None:
     os.replace(tmp, lib)
 
 
+def _compile_binding() -> Path:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    obj = BUILD / "binding.o"
+    includes = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"], str(INCLUDE)]
+    cmd = [hipcc(), "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-Wall", "-Wno-unused-function",
+           *(f"-I{p}" for p in includes), "-c", str(BINDING_SRC), "-o", str(obj)]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"hipcc failed on {BINDING_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    return obj
+
+
+def _link_binding(obj: Path) -> None:
+    from torch.utils import cpp_extension
+
+    tmp = BINDING_LIB.with_suffix(".so.tmp")
+    cmd = [hipcc(), "-shared", "-fPIC", str(obj), "-o", str(tmp), f"-L{LIB_DIR}", "-lqmoe",
+           *(f"-L{p}" for p in cpp_extension.library_paths("cuda")), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+           "-ltorch_hip", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING_LIB)
+
+
 def build(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.hip"))
-    jobs = min(len(sources) + 1, max(1, min(8, os.cpu_count() or 1)))
+    jobs = min(len(sources) + 2, max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(jobs) as ex:
+        fut_binding = ex.submit(_compile_binding)
         fut_peaks = ex.submit(_compile, PEAKS_SRC)
         stamped = {"qmv": ex.submit(_compile, CSRC / "qmv.hip", "_stamps", ("QMOE_QMV_STAMPS",)),
                    "gemm_bf16": ex.submit(_compile, CSRC / "gemm_bf16.hip", "_stamps", ("QMOE_GEMM_STAMPS",))}
         objs = list(ex.map(_compile, sources))
         peaks_obj = fut_peaks.result()
+        binding_obj = fut_binding.result()
         stamped = {k: f.result() for k, f in stamped.items()}
     _link(objs, LIB)
     _link([peaks_obj], PEAKS_LIB)
     _link([stamped.get(o.stem, o) for o in objs], STAMPS_LIB)
+    _link_binding(binding_obj)
     if verbose:
-        print(f"built {LIB} from {len(sources)} sources, {PEAKS_LIB} and {STAMPS_LIB}")
+        print(f"built {LIB} from {len(sources)} sources, {PEAKS_LIB}, {STAMPS_LIB} and {BINDING_LIB}")
     return LIB
 
 

@@ -11,6 +11,10 @@ The products are differentiable in x: with ``transpose`` (x W^T) dx = dy W, and
 without (x W) dx = dy W^T, by the same kernels over the same codes.  The codes
 and scales are constants of the graph.  ``qqmm`` and ``gather_qqmm`` quantise x
 as well and have no gradient.
+
+The calls and their autograd nodes are csrc/torch/binding.cpp's.  It takes what
+the kernels can read as it is; the functions here check, convert, arrange or
+refuse the rest.
 """
 
 from __future__ import annotations
@@ -19,15 +23,13 @@ import math
 
 import torch
 
-from . import _lib, ops, token_sort
+from . import _lib, ops
 from ._lib import QmoeUnsupported
 
 __all__ = ["BLOCK", "quantize", "dequantize", "quantized_matmul", "gather_qmm", "qqmm", "gather_qqmm"]
 
 BLOCK = 32
-# rows of one expert up to which the matrix-vector kernels run (above: the GEMM)
-QMV_MAX_ROWS = 4
-# gathered rows from which unsorted calls are sorted for the grouped GEMM, as sorted ones take it
+# gathered rows from which the grouped GEMM runs, unsorted calls sorted for it (the binding has the same)
 SORTED_MIN_ROWS = 64
 
 
@@ -71,18 +73,15 @@ def quantize(w: torch.Tensor, group_size: int | None = None, bits: int = 4, mode
     if mode != "mxfp4":
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}: quantize makes mxfp4")
     _format(group_size, bits)
+    q = _lib.binding().quantize(w, False)
+    if q is not None:
+        return q
     ops._dev(w, "w")
     if w.dtype not in ops._DTYPES:
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"w must be bfloat16, float16 or float32, got {w.dtype}")
     if w.dim() < 1 or w.shape[-1] % BLOCK:
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"the last dimension must be a multiple of 32, got {tuple(w.shape)}")
-    w = ops._ready(w)
-    K = w.shape[-1]
-    q = torch.empty(*w.shape[:-1], K // 8, dtype=torch.int32, device=w.device)
-    s = torch.empty(*w.shape[:-1], K // BLOCK, dtype=torch.uint8, device=w.device)
-    ops._launch("qmoe_mxfp4_quantize", w, w.data_ptr(), ops._DTYPES[w.dtype], w.numel() // K if K else 0, K, q.data_ptr(),
-            s.data_ptr())
-    return q, s
+    return _lib.binding().quantize(ops._ready(w), True)
 
 
 def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size: int | None = None, bits: int = 4,
@@ -92,15 +91,15 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size: i
     _format(group_size, bits, biases)
     if dtype not in ops._DTYPES:
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"dtype={dtype}: bfloat16, float16 or float32")
+    out = _lib.binding().dequantize(w, scales, ops._DTYPES[dtype], False)
+    if out is not None:
+        return out
     w = ops._words(w, "w")
     scales = _scales(scales, w.device)
     K = w.shape[-1] * 8 if w.dim() else 0
     if w.dim() < 1 or K % BLOCK or tuple(scales.shape) != (*w.shape[:-1], K // BLOCK):
         raise ValueError(f"codes {tuple(w.shape)} and scales {tuple(scales.shape)} disagree")
-    out = torch.empty(*w.shape[:-1], K, dtype=dtype, device=w.device)
-    ops._launch("qmoe_mxfp4_dequantize", w, w.data_ptr(), scales.data_ptr(), w.numel() // w.shape[-1] if K else 0, K,
-            ops._DTYPES[dtype], out.data_ptr())
-    return out
+    return _lib.binding().dequantize(w, scales, ops._DTYPES[dtype], True)
 
 
 # --------------------------------------------------------------- products
@@ -108,8 +107,8 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size: i
 
 class _Rows:
     """Which activation row and which expert each output row takes: ``x_rows``
-    (or row i // div), ``experts`` (None: one expert for all), and the tile
-    table of sorted rows (None: not sorted, or one expert)."""
+    (or row i // div), ``experts``, and the tile table of sorted rows (None: not
+    sorted)."""
 
     __slots__ = ("n", "x_rows", "div", "experts", "tiles")
 
@@ -117,87 +116,34 @@ class _Rows:
         self.n, self.x_rows, self.div, self.experts, self.tiles = n, x_rows, div, experts, tiles
 
 
-def _pad8(x: torch.Tensor) -> torch.Tensor:
-    """Rows of a multiple of eight elements, zeros behind the given ones."""
-    extra = -x.shape[1] % 8
-    return torch.nn.functional.pad(x, (0, extra)) if extra else x
-
-
-def _product(x, w, scales, E, N, K, transpose, rows: _Rows, dtype=torch.bfloat16):
-    """out[r] = x[row of r] W[expert of r]^T (transpose) or W, rows as ``rows`` says."""
-    out = torch.empty(rows.n, N if transpose else K, dtype=dtype, device=x.device)
-    if rows.n == 0 or out.shape[1] == 0:
-        return out
-    if x.shape[1] == 0:
-        return out.zero_()
-    if (rows.experts is not None and rows.tiles is None) or rows.n <= QMV_MAX_ROWS:
-        ops._launch("qmoe_mxfp4_gather_qmv", x, x.data_ptr(), x.shape[0], x.shape[1], ops._ptr(rows.x_rows), rows.div,
-                ops._ptr(rows.experts), rows.n, w.data_ptr(), scales.data_ptr(), E, N, K, int(transpose), ops._DTYPES[dtype],
-                out.data_ptr())
-        return out
-    x = _pad8(x)
+def _product(x, w, scales, transpose, rows: _Rows, qq: bool = False):
+    """out[r] = x[row of r] W[expert of r]^T (transpose) or W, rows as ``rows``
+    says, recorded where a gradient of x may be asked for; ``qq``: x in mxfp4."""
     t = rows.tiles
-    table = (None, None, None, None, 0) if t is None else (t.offsets.data_ptr(), t.tile_row.data_ptr(),
-                                                           t.tile_exp.data_ptr(), t.ntiles.data_ptr(), t.maxt)
-    ops._launch("qmoe_mxfp4_gather_qmm", x, x.data_ptr(), x.shape[0], x.shape[1], ops._ptr(_x_rows(rows, x.device)), rows.n,
-            w.data_ptr(), scales.data_ptr(), E, N, K, int(transpose), *table, ops._DTYPES[dtype], out.data_ptr())
-    return out
+    table = None if t is None else (t.offsets, t.tile_row, t.tile_exp, t.ntiles, t.maxt)
+    return _lib.binding().rows_product(x, w, scales, rows.x_rows, rows.div, rows.experts, table, rows.n, bool(transpose), qq)
 
 
 def _x_rows(rows: _Rows, device):
-    """The activation row of each row for the GEMMs, None for row r itself."""
+    """The activation row of each row, None for row r itself."""
     if rows.x_rows is not None or rows.div == 1:
         return rows.x_rows
     return torch.div(torch.arange(rows.n, device=device, dtype=torch.int32), rows.div,
                      rounding_mode="floor").to(torch.int32)
 
 
-class _Product(torch.autograd.Function):
-    """_product with its gradient in x."""
-
-    @staticmethod
-    def forward(ctx, x, w, scales, E, N, K, transpose, rows):
-        ctx.save_for_backward(w, scales)
-        ctx.args = x.shape[0], E, N, K, transpose, rows
-        return _product(x, w, scales, E, N, K, transpose, rows)
-
-    @staticmethod
-    @ops._first_order
-    def backward(ctx, dy):
-        w, scales = ctx.saved_tensors
-        n_x, E, N, K, transpose, rows = ctx.args
-        own = _Rows(rows.n, None, 1, rows.experts, rows.tiles)  # row r of dy for row r
-        dy = ops._ready(dy)
-        if rows.x_rows is None and rows.div == 1:
-            dx = _product(dy, w, scales, E, N, K, not transpose, own)
-        else:  # several rows share an activation row: their gradients are added in fp32, rounded once
-            dr = _product(dy, w, scales, E, N, K, not transpose, own, torch.float32)
-            if rows.x_rows is None:
-                dx = token_sort.unsort_sum(dr, None, None, n_x, rows.div, dtype=torch.bfloat16)
-            else:
-                at, order = torch.sort(rows.x_rows.clamp(0, max(n_x - 1, 0)), stable=True)
-                first = torch.searchsorted(at, torch.arange(n_x + 1, device=dy.device, dtype=torch.int32),
-                                           out_int32=True)
-                dx = token_sort.unsort_sum(dr, order.to(torch.int32), None, n_x, 0, first, torch.bfloat16)
-        return dx, None, None, None, None, None, None, None
-
-
-def _run(x, w, scales, E, N, K, transpose, rows):
-    """_product, recorded where a gradient of x may be asked for."""
-    return (_Product.apply if ops._records(x) else _product)(x, w, scales, E, N, K, transpose, rows)
-
-
 def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=None, transpose: bool = True,
                      group_size: int | None = None, bits: int = 4) -> torch.Tensor:
     """x [.., K] W^T (transpose) or x [.., N] W for codes w [N, K/8]."""
     _format(group_size, bits, biases)
+    y = _lib.binding().matmul(x, w, scales, bool(transpose), False, False)
+    if y is not None:
+        return y
     x = ops._bf16(x, "x")
     w, scales, N, K = _weights(w, scales, x.device, 2)
     if x.dim() < 1 or x.shape[-1] != (K if transpose else N):
         raise ValueError(f"x {tuple(x.shape)} does not fit w [{N}, {K}] with transpose={transpose}")
-    x2 = _rows_of(x)
-    y = _run(x2, w, scales, 1, N, K, bool(transpose), _Rows(x2.shape[0]))
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
+    return _lib.binding().matmul(x, w, scales, bool(transpose), False, True)
 
 
 def _broadcast(a, b) -> tuple:
@@ -305,35 +251,23 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=No
     the rows run through the grouped GEMM: as they are with ``sorted_indices``
     (ascending ``rhs_indices``), else sorted by expert first."""
     _format(group_size, bits, biases)
+    if tiles is None:
+        y = _lib.binding().gather(x, w, scales, lhs_indices, rhs_indices, bool(transpose), bool(sorted_indices), False)
+        if y is not None:
+            return y
     x = ops._bf16(x, "x")
     w, scales, E, N, K = _check_gather(x, w, scales, transpose, lhs_indices, rhs_indices)
     batch, rows, order = _gathered(x, E, lhs_indices, rhs_indices, sorted_indices, tiles, SORTED_MIN_ROWS)
-    x2 = _rows_of(x)
-    y = _run(x2, w, scales, E, N, K, bool(transpose), rows)
+    y = _product(_rows_of(x), w, scales, transpose, rows)
     if order is not None:
-        y = token_sort._sort(y, order[1], order[0])
+        y = ops.sort_tokens(y, order[1], order[0])
     return y.reshape(batch + (x.shape[-2], y.shape[-1]))
 
 
 def _no_grad(x: torch.Tensor) -> None:
-    if ops._records(x):
+    if x.requires_grad and torch.is_grad_enabled():
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, "the products of quantised activations have no gradient: "
                                                     "detach x, or use quantized_matmul / gather_qmm")
-
-
-def _qq_product(x2, w, scales, E, N, K, rows: _Rows):
-    xq, xs = quantize(x2)
-    out = torch.empty(rows.n, N, dtype=torch.bfloat16, device=x2.device)
-    if rows.n == 0 or N == 0:
-        return out
-    if K == 0:
-        return out.zero_()
-    t = rows.tiles
-    table = (None, None, None, None, 0) if t is None else (t.offsets.data_ptr(), t.tile_row.data_ptr(),
-                                                           t.tile_exp.data_ptr(), t.ntiles.data_ptr(), t.maxt)
-    ops._launch("qmoe_mxfp4_gather_qqmm", x2, xq.data_ptr(), xs.data_ptr(), x2.shape[0], ops._ptr(_x_rows(rows, x2.device)),
-            rows.n, w.data_ptr(), scales.data_ptr(), E, N, K, *table, out.data_ptr())
-    return out
 
 
 def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, group_size: int | None = None, bits: int = 4,
@@ -343,13 +277,15 @@ def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, group_size: int
     if mode != "mxfp4":
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}: only mxfp4")
     _format(group_size, bits)
+    y = _lib.binding().matmul(x, w, scales, True, True, False)
+    if y is not None:
+        return y
     x = ops._bf16(x, "x")
     _no_grad(x)
     w, scales, N, K = _weights(w, scales, x.device, 2)
     if x.dim() < 1 or x.shape[-1] != K:
         raise ValueError(f"x {tuple(x.shape)} does not fit w [{N}, {K}]")
-    x2 = _rows_of(x)
-    return _qq_product(x2, w, scales, 1, N, K, _Rows(x2.shape[0])).reshape(*x.shape[:-1], N)
+    return _lib.binding().matmul(x, w, scales, True, True, True)
 
 
 def gather_qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, lhs_indices=None, rhs_indices=None,
@@ -361,12 +297,15 @@ def gather_qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, lhs_indi
     if mode != "mxfp4":
         raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"mode={mode!r}: only mxfp4")
     _format(group_size, bits)
+    if tiles is None:
+        y = _lib.binding().gather(x, w, scales, lhs_indices, rhs_indices, True, bool(sorted_indices), True)
+        if y is not None:
+            return y
     x = ops._bf16(x, "x")
     _no_grad(x)
     w, scales, E, N, K = _check_gather(x, w, scales, True, lhs_indices, rhs_indices)
     batch, rows, order = _gathered(x, E, lhs_indices, rhs_indices, sorted_indices, tiles, 1)
-    x2 = _rows_of(x)
-    y = _qq_product(x2, w, scales, E, N, K, rows)
+    y = _product(_rows_of(x), w, scales, True, rows, qq=True)
     if order is not None:
-        y = token_sort._sort(y, order[1], order[0])
+        y = ops.sort_tokens(y, order[1], order[0])
     return y.reshape(batch + (x.shape[-2], N))

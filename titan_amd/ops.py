@@ -44,7 +44,7 @@ BITS = 4
 SORTED_MIN_ROWS = 64
 
 
-# QMOE_BF16, QMOE_FP16, QMOE_FP32
+# the entry points' element types (QMOE_BF16, QMOE_FP16, QMOE_FP32)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -112,33 +112,6 @@ def _ptr(t):
 def _same_device(t: torch.Tensor, name: str, device) -> None:
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
-
-
-def _launch(name: str, t: torch.Tensor, *args) -> None:
-    """Entry point ``name`` on the device of ``t`` and that device's current
-    stream (every entry point's last argument), whichever device is current."""
-    index = t.get_device()
-    if index == torch._C._cuda_getDevice():
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-
-
-def _first_order(backward):
-    """once_differentiable, whose wrapper runs only where a graph of the gradient
-    is asked for (it costs several us a call, of a backward pass of 15)."""
-    once = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return (once if torch.is_grad_enabled() else backward)(ctx, *grads)
-
-    return run
-
-
-def _records(t: torch.Tensor) -> bool:
-    """Must a call with ``t`` go through autograd?"""
-    return t.requires_grad and torch.is_grad_enabled()
 
 
 # ------------------------------------------------------------------ layout

@@ -67,7 +67,8 @@ def _plain(t: torch.Tensor, width: int) -> bool:
 
 def _learns(t: torch.Tensor) -> bool:
     """May the token sort's kernels move the rows of ``t`` and their gradient?"""
-    return (type(t) is torch.Tensor and t.is_cuda and t.dtype in ops._DTYPES and ops._records(t)
+    return (type(t) is torch.Tensor and t.is_cuda and t.dtype in ops._DTYPES
+            and t.requires_grad and torch.is_grad_enabled()
             and not torch._C._functorch.is_functorch_wrapped_tensor(t) and forward_ad._current_level < 0
             and not torch.jit.is_tracing() and not torch.compiler.is_compiling())
 
