@@ -7,6 +7,7 @@
 
 #include "gemm_common.h"
 #include "mxfp4.h"
+#include "mxfp4_rows.h"
 
 namespace {
 
@@ -1059,6 +1060,10 @@ int launch(const GemmArgs& a, int64_t max_tiles, hipStream_t st) {
   return qmoe::launch_status("mx_gemm_kernel");
 }
 
+RowsArgs rows_of(const GemmArgs& a) {
+  return {a.x, a.xq, a.xs, a.x_rows, a.n_rows, a.n_x, a.ldx, a.w, a.s, a.N, a.K, a.out, a.out_f32};
+}
+
 // Argument checks shared by the entry points; QMOE_OK with *run = false: nothing to do.
 int check(const GemmArgs& a, int mode, int64_t max_tiles, int out_dtype, bool* run) {
   *run = false;
@@ -1100,6 +1105,7 @@ extern "C" int qmoe_mxfp4_gather_qmm(const uint16_t* x, int64_t n_x, int64_t ldx
   const int rc = check(a, transpose ? kFwd : kT, max_tiles, out_dtype, &run);
   if (rc != QMOE_OK || !run) return rc;
   hipStream_t st = qmoe::as_stream(stream);
+  if (transpose && !offsets && n_rows <= kFewRows) return rows_product(rows_of(a), false, st);
   return transpose ? launch<kFwd>(a, max_tiles, st) : launch<kT>(a, max_tiles, st);
 }
 
@@ -1113,5 +1119,6 @@ extern "C" int qmoe_mxfp4_gather_qqmm(const uint32_t* xq, const uint8_t* xs, int
   bool run;
   const int rc = check(a, kQQ, max_tiles, QMOE_BF16, &run);
   if (rc != QMOE_OK || !run) return rc;
+  if (!offsets && n_rows <= kFewRows) return rows_product(rows_of(a), true, qmoe::as_stream(stream));
   return launch<kQQ>(a, max_tiles, qmoe::as_stream(stream));
 }
