@@ -6,11 +6,13 @@
 // side by side cover one weight row.  Codes become bf16 pairs by the scaled
 // conversion (exact) and go through v_dot2_f32_bf16 with the activation's
 // pairs: 32 instructions per 32 codes.  Bound by the latency of one dependent
-// HBM round trip at one token, by HBM at more.
+// HBM round trip at one token (4096 x 2048: 4.0 us for 4.5 MB; top-10 of 1024 x
+// 2048: 5.7 us for 11 MB), by the caches and HBM at more (six tokens 16.2 us).
 //
 // Transposed, out[r, k] = sum_n x[r, n] W[e_r, n, k]: a lane owns the 32
-// outputs of one block column and walks n; sixteen waves share the n of one
-// block of 512 outputs and add up their sums through LDS in a fixed order.
+// outputs of one block column and walks n, four rows' loads ahead; sixteen
+// lanes and sixteen waves share the n of one block of 128 outputs and add up
+// their sums, through LDS and in a fixed order.
 #include "mxfp4.h"
 
 namespace {
@@ -100,63 +102,70 @@ __global__ __launch_bounds__(64 * kWaves) void mx_qmv_kernel(QmvArgs a) {
 }
 
 constexpr int kTWaves = 16;
-constexpr int kTUnits = 16;              // block columns (of 32 outputs) per workgroup
+constexpr int kTUnits = 4;               // block columns (of 32 outputs) per workgroup
 constexpr int kTOut = kTUnits * kBlock;  // outputs per workgroup
+constexpr int kTRows = 64 / kTUnits;     // rows n a wave takes at once
+constexpr int kTAhead = 4;               // of which so many batches are in flight
 
 __global__ __launch_bounds__(64 * kTWaves) void mx_qmv_t_kernel(QmvArgs a) {
   __shared__ float part[kTWaves][kTOut];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int c = lane % kTUnits, sub = lane / kTUnits;  // block column, one of four rows n
+  const int c = lane / kTRows, sub = lane % kTRows;  // block column, row n
   const int64_t r = blockIdx.y;
   const int64_t e = expert_of(a, r);
   const uint16_t* x = a.x + x_row_of(a, r) * a.ldx;
   const int units = (int)(a.K / kBlock);
-  const int64_t u = (int64_t)blockIdx.x * kTUnits + c;
-  const bool in = u < units;
-  const uint4* w = reinterpret_cast<const uint4*>(a.w) + e * a.N * units + (in ? u : 0);
-  const uint8_t* s = a.s + e * a.N * units + (in ? u : 0);
+  const int64_t u = min((int64_t)blockIdx.x * kTUnits + c, (int64_t)units - 1);  // past the end: not stored
+  const uint4* w = reinterpret_cast<const uint4*>(a.w) + e * a.N * units + u;
+  const uint8_t* s = a.s + e * a.N * units + u;
   float acc[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-  for (int64_t n = wave * 4 + sub; n < a.N; n += 4 * kTWaves) {
-    const uint4 q = w[n * units];
-    const float sc = scale_of(s[n * units]);
-    const float xv = bf16_to_f32(x[n]);
-    const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+  constexpr int kStep = kTWaves * kTRows;
+  for (int64_t n0 = wave * kTRows + sub; n0 < a.N; n0 += kTAhead * kStep) {
+    uint4 q[kTAhead];
+    float sc[kTAhead], xv[kTAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t p[4];
-      unpack8(qw[j], sc, p);
+    for (int i = 0; i < kTAhead; ++i) {
+      const int64_t n = n0 + i * kStep;
+      const bool in = n < a.N;
+      const int64_t at = in ? n * units : 0;
+      q[i] = w[at];
+      sc[i] = scale_of(in ? s[at] : 0u);  // past the end: 0 times what is there, which is finite
+      xv[i] = in ? bf16_to_f32(x[n]) : 0.f;
+    }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        acc[8 * j + 2 * t] = __builtin_fmaf(xv, bf16lo(p[t]), acc[8 * j + 2 * t]);
-        acc[8 * j + 2 * t + 1] = __builtin_fmaf(xv, bf16hi(p[t]), acc[8 * j + 2 * t + 1]);
+    for (int i = 0; i < kTAhead; ++i) {
+      const uint32_t qw[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t p[4];
+        unpack8(qw[j], sc[i], p);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          acc[8 * j + 2 * t] = __builtin_fmaf(xv[i], bf16lo(p[t]), acc[8 * j + 2 * t]);
+          acc[8 * j + 2 * t + 1] = __builtin_fmaf(xv[i], bf16hi(p[t]), acc[8 * j + 2 * t + 1]);
+        }
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
-    acc[i] += __shfl_xor(acc[i], 16);
-    acc[i] += __shfl_xor(acc[i], 32);
-  }
-  if (sub == 0) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) part[wave][i * kTUnits + c] = acc[i];  // [element][column]: consecutive lanes, banks
+    const float v = group_sum<kTRows>(acc[i]);
+    if (sub == 0) part[wave][c * kBlock + i] = v;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kTOut; i += blockDim.x) {
-    const int col = i / kBlock, el = i % kBlock;
-    const int64_t k = (int64_t)blockIdx.x * kTOut + i;
+  if (threadIdx.x < kTOut) {
+    const int64_t k = (int64_t)blockIdx.x * kTOut + threadIdx.x;
     float v = 0.f;
 #pragma unroll
-    for (int j = 0; j < kTWaves; ++j) v += part[j][el * kTUnits + col];
+    for (int j = 0; j < kTWaves; ++j) v += part[j][threadIdx.x];
     if (k < a.K) put(a, r * a.K + k, v);
   }
 }
 
-template <int LPR>
+template <int LPR, int NR>
 void launch_fwd(const QmvArgs& a, hipStream_t st) {
-  constexpr int NR = 2;
   constexpr int kRows = (64 / LPR) * NR * kWaves;
   const dim3 grid((unsigned)((a.N + kRows - 1) / kRows), (unsigned)a.n_rows);
   mx_qmv_kernel<LPR, NR><<<grid, dim3(64 * kWaves), 0, st>>>(a);
@@ -190,13 +199,16 @@ extern "C" int qmoe_mxfp4_gather_qmv(const uint16_t* x, int64_t n_x, int64_t ldx
     return qmoe::launch_status("mx_qmv_t_kernel");
   }
   const int64_t units = K / kBlock;
-  const auto slots = [&](int lpr) { return (units + lpr - 1) / lpr * lpr; };
-  // lanes per weight row: as many as there are units, fewer where that wastes less of the last pass
-  int lpr = 64;
-  if (slots(32) < slots(lpr)) lpr = 32;
-  if (slots(16) < slots(lpr)) lpr = 16;
-  if (lpr == 64) launch_fwd<64>(a, st);
-  else if (lpr == 32) launch_fwd<32>(a, st);
-  else launch_fwd<16>(a, st);
+  // Lanes per weight row: as many as give the fewest dependent passes (against
+  // the fewest idle lanes, 16 or 32, one row of N = 4096: K = 2080 4.4 / 5.3 us, 1056 3.3 /
+  // 3.4, 1536 3.4 / 4.1, 3200 4.8 / 7.1).
+  const int lpr = units > 32 ? 64 : units > 16 ? 32 : 16;
+  // Weight rows per wave: two, so that a row or a few fill the chip; four where
+  // the pairs do (one token x top-10 of 1024 x 2048 5.7 / 6.1 us, two 8.9 / 8.2,
+  // six 18.9 / 16.2).
+  const bool many = n_rows >= 16;
+  if (lpr == 64) many ? launch_fwd<64, 4>(a, st) : launch_fwd<64, 2>(a, st);
+  else if (lpr == 32) many ? launch_fwd<32, 4>(a, st) : launch_fwd<32, 2>(a, st);
+  else many ? launch_fwd<16, 4>(a, st) : launch_fwd<16, 2>(a, st);
   return qmoe::launch_status("mx_qmv_kernel");
 }

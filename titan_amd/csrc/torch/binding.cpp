@@ -31,7 +31,12 @@ using torch::autograd::variable_list;
 namespace {
 
 constexpr int64_t kSortedMinRows = 64;  // gathered rows from which the grouped GEMM takes sorted calls
-constexpr int64_t kQmvMaxRows = 4;      // rows of one expert up to which the matrix-vector kernels run
+// Rows of one matrix that the matrix-vector kernel takes: it reads the weights
+// once per row, mostly from the caches after the first, the kernel for few rows
+// once in all but with a longer start.  Two rows of 4096 x 2048 take 4.7 us
+// either way, four 6.4 and 4.7, four of 1024 x 2048 3.4 and 4.0.  Transposed
+// products take the GEMM from one row on (4096 x 2048: 20 and 14.6 us).
+constexpr int64_t kQmvMaxRows = 4, kQmvMaxWork = int64_t(1) << 24;
 
 struct Failure : std::runtime_error {
   int code;
@@ -255,7 +260,8 @@ Tensor product_run(const Tensor& x_, const Weights& g, const Rows& r, bool trans
   if (out.numel() == 0) return out;
   if (x.size(1) == 0) return out.zero_();
   const int t = type_of(out);
-  if ((r.experts.defined() && !r.offsets.defined()) || r.n <= kQmvMaxRows) {
+  const bool few = transpose && (r.n == 1 || (r.n <= kQmvMaxRows && r.n * g.N * g.K <= kQmvMaxWork));
+  if (!r.offsets.defined() && (r.experts.defined() || few)) {
     ok(qmoe_mxfp4_gather_qmv(ptr<uint16_t>(x), x.size(0), x.size(1), ptr<int32_t>(r.x_rows), (int32_t)r.div,
                              ptr<int32_t>(r.experts), r.n, ptr<uint32_t>(g.w), ptr<uint8_t>(g.s), (int32_t)g.E, g.N, g.K,
                              transpose, t, out.data_ptr(), stream(x)),
