@@ -526,17 +526,17 @@ int qmoe_mxfp4_gather_qqmm(const uint32_t* xq, const uint8_t* xs, int64_t n_x,
 /* ------------------------------------------- tokens to experts, gradients --
  * The row movement of switch_layers.py:13-25 and moe_weighted_sum.py:44-98
  * with gradients, for QMOE_BF16, _FP16 and _FP32 rows of any length.  Pair
- * p = t * top_k + j is slot j of token t; order [n] and inv [n] are inverse
- * permutations of the n = T * top_k pairs (qmoe_route).  Sums are fp32, in
- * slot order, rounded once.
- *   qmoe_sort_rows    out[i] = x[order[i] / top_k]
+ * p = t * top_k + j is slot j of token t; inv [n] is a permutation of the
+ * n = T * top_k pairs, the sorted row of each (qmoe_route's inv_order).  Sums
+ * are fp32, in slot order, rounded once.
+ *   qmoe_sort_rows    out[inv[p]] = x[t]
  *   qmoe_unsort_sum   y[t] = sum_j s[p] xs[inv[p]]; scores NULL: s = 1; inv
  *                     NULL: the identity.  first [T + 1]: the pairs of y[t]
  *                     are first[t] .. first[t + 1] - 1 instead (top_k unused,
  *                     scores by pair).  fp32 rows may have a bf16 sum.
  *   qmoe_unsort_grad  dxs[inv[p]] = s[p] dy[t]; dscores[p] = <dy[t], xs[inv[p]]>;
  *                     either may be NULL: not wanted. */
-int qmoe_sort_rows(const void* x, int64_t T, const int32_t* order,
+int qmoe_sort_rows(const void* x, int64_t T, const int32_t* inv,
                    int64_t top_k, int64_t D, int dtype, void* out,
                    void* stream);
 int qmoe_unsort_sum(const void* xs, int64_t n, int dtype, const int32_t* inv,

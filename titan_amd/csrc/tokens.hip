@@ -1,9 +1,8 @@
 // Tokens sorted by expert and back, with the scores applied, and the gradients
-// of both.  Pair p = t * k + j is slot j of token t; order[i] is the pair of
-// sorted row i and inv[p] its sorted row, two permutations inverse to each
-// other (qmoe_route).
+// of both.  Pair p = t * k + j is slot j of token t, inv[p] its sorted row, a
+// permutation of the pairs (qmoe_route).
 //
-//   sort              xs[i] = x[order[i] / k]
+//   sort              xs[inv[t k + j]] = x[t]
 //   its gradient      dx[t] = sum_j dxs[inv[t k + j]]
 //   back              y[t]  = sum_j s[t, j] xs[inv[t k + j]]
 //   its gradients     dxs[inv[p]] = s[p] dy[t],  ds[p] = <dy[t], xs[inv[p]]>
@@ -63,15 +62,18 @@ __device__ __forceinline__ void set(typename Vec<T, N>::V& v, int i, T x) {
 
 constexpr int kBatch = 8;  // rows in flight per thread
 
+// One block per token, whose row is read once and written to its k places.
 template <typename U>
-__global__ __launch_bounds__(256) void sort_rows_kernel(const U* __restrict__ x, int64_t n_src,
-                                                        const int32_t* __restrict__ order, int64_t n, uint32_t k,
-                                                        int64_t units, U* __restrict__ out) {
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (u >= n * units) return;
-  const int64_t i = u / units, c = u - i * units;
-  const int64_t t = min((int64_t)((uint32_t)max(order[i], 0) / k), n_src - 1);
-  __builtin_nontemporal_store(x[t * units + c], out + u);
+__global__ __launch_bounds__(256) void sort_rows_kernel(const U* __restrict__ x, const int32_t* __restrict__ inv,
+                                                        int64_t n, int k, int64_t units, U* __restrict__ out) {
+  const int64_t t = blockIdx.x;
+  for (int64_t c = threadIdx.x; c < units; c += blockDim.x) {
+    const U v = x[t * units + c];
+    for (int j = 0; j < k; ++j) {
+      const int64_t i = min(max((int64_t)inv[t * k + j], (int64_t)0), n - 1);
+      __builtin_nontemporal_store(v, out + i * units + c);
+    }
+  }
 }
 
 // y[t] = sum of the rows of token t's pairs, weighted by `scores` if given.
@@ -224,30 +226,27 @@ int launch_grad(const void* dy, const void* xs, int64_t n, const int32_t* inv, c
 
 }  // namespace
 
-extern "C" int qmoe_sort_rows(const void* x, int64_t T, const int32_t* order, int64_t top_k, int64_t D, int dtype,
+extern "C" int qmoe_sort_rows(const void* x, int64_t T, const int32_t* inv, int64_t top_k, int64_t D, int dtype,
                               void* out, void* stream) {
   const int size = size_of(dtype);
   if (!size) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "dtype=%d", dtype);
   if (T < 0 || top_k < 0 || D < 0) return qmoe::fail(QMOE_ERR_INVALID, "bad sizes");
   if (T == 0 || top_k == 0 || D == 0) return QMOE_OK;
-  if (!x || !order || !out) return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
+  if (!x || !inv || !out) return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
   if (!qmoe::aligned16(x) || !qmoe::aligned16(out)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "rows must be 16-byte aligned");
   if (T > 0x7FFFFFFF / top_k) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "too many pairs");
   const int64_t n = T * top_k, bytes = D * size;
   const int unit = bytes % 16 == 0 ? 16 : size;
   const int64_t units = bytes / unit;
-  if (n > (int64_t)0x7FFFFFFF * 256 / units) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "too many rows");
-  const dim3 grid((unsigned)((n * units + 255) / 256)), block(256);
+  const dim3 grid((unsigned)T), block(row_threads(units));
   hipStream_t st = qmoe::as_stream(stream);
+  const int k = (int)top_k;
   if (unit == 16)
-    sort_rows_kernel<<<grid, block, 0, st>>>(static_cast<const i32x4_t*>(x), T, order, n, (uint32_t)top_k, units,
-                                             static_cast<i32x4_t*>(out));
+    sort_rows_kernel<<<grid, block, 0, st>>>(static_cast<const i32x4_t*>(x), inv, n, k, units, static_cast<i32x4_t*>(out));
   else if (unit == 4)
-    sort_rows_kernel<<<grid, block, 0, st>>>(static_cast<const uint32_t*>(x), T, order, n, (uint32_t)top_k, units,
-                                             static_cast<uint32_t*>(out));
+    sort_rows_kernel<<<grid, block, 0, st>>>(static_cast<const uint32_t*>(x), inv, n, k, units, static_cast<uint32_t*>(out));
   else
-    sort_rows_kernel<<<grid, block, 0, st>>>(static_cast<const uint16_t*>(x), T, order, n, (uint32_t)top_k, units,
-                                             static_cast<uint16_t*>(out));
+    sort_rows_kernel<<<grid, block, 0, st>>>(static_cast<const uint16_t*>(x), inv, n, k, units, static_cast<uint16_t*>(out));
   return qmoe::launch_status("sort_rows_kernel");
 }
 

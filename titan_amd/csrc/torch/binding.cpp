@@ -146,10 +146,10 @@ py::object dequantize(py::handle w_, py::handle s_, int type, bool must) {
 
 // --------------------------------------------------------------- token sort
 
-Tensor sort_run(const Tensor& x, const Tensor& order) {
-  const int64_t n = order.numel(), T = x.size(0), D = x.size(1);
+Tensor sort_run(const Tensor& x, const Tensor& inv) {
+  const int64_t n = inv.numel(), T = x.size(0), D = x.size(1);
   Tensor xs = at::empty({n, D}, x.options().requires_grad(false));
-  ok(qmoe_sort_rows(x.const_data_ptr(), T, ptr<int32_t>(order), T ? n / T : 0, D, type_of(x), xs.data_ptr(), stream(x)),
+  ok(qmoe_sort_rows(x.const_data_ptr(), T, ptr<int32_t>(inv), T ? n / T : 0, D, type_of(x), xs.data_ptr(), stream(x)),
      "qmoe_sort_rows");
   return xs;
 }
@@ -163,10 +163,10 @@ Tensor sum_run(const Tensor& rows, const Tensor& inv, const Tensor& scores, cons
 }
 
 struct Sort : torch::autograd::Function<Sort> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& order, const Tensor& inv) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& inv) {
     ctx->save_for_backward({inv});
     ctx->saved_data["T"] = x.size(0);
-    return sort_run(x, order);
+    return sort_run(x, inv);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const Tensor inv = ctx->get_saved_variables()[0];
@@ -174,7 +174,7 @@ struct Sort : torch::autograd::Function<Sort> {
     const Tensor d = ready(grads[0]);
     const c10::hip::HIPGuard guard(d.get_device());
     Tensor dx = sum_run(d, inv, {}, {}, T, T ? d.size(0) / T : 0, d.scalar_type());
-    return first_order({dx, Tensor(), Tensor()}, grads);
+    return first_order({dx, Tensor()}, grads);
   }
 };
 
@@ -217,7 +217,7 @@ py::object sort_tokens(py::handle x_, py::handle order_, py::handle inv_, bool m
   const int64_t n = order.numel(), T = x.size(0);
   if ((T ? n % T : n) || !pairs(order, x, n) || !pairs(inv, x, n)) return none(must);
   const c10::hip::HIPGuard guard(x.get_device());
-  return give(records(x) ? Sort::apply(x, order, inv) : sort_run(x, order));
+  return give(records(x) ? Sort::apply(x, inv) : sort_run(x, inv));
 }
 
 py::object unsort_tokens(py::handle xs_, py::handle order_, py::handle inv_, py::handle scores_, bool must) {
