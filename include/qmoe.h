@@ -514,14 +514,23 @@ int qmoe_mxfp4_gather_qmm(const uint16_t* x, int64_t n_x, int64_t ldx,
                           int out_dtype, void* out, void* stream);
 
 /* Both operands in mxfp4: out [n_rows, N] (bf16) = deq(xq)[xr] W[e]^T, xq
- * [n_x, K/8] and xs [n_x, K/32] from qmoe_mxfp4_quantize, rows as above. */
+ * [n_x, K/8] and xs [n_x, K/32] from qmoe_mxfp4_quantize, rows as above.
+ * lines NULL, or the scales of both operands laid out for the kernel with xq
+ * (xs is then not read) by qmoe_mxfp4_quantize_lines from bf16 x [n_x, K]:
+ * (num_experts * N + n_x) * ceil(K / 128) words, worth their making for many
+ * rows. */
+int qmoe_mxfp4_quantize_lines(const uint16_t* x, int64_t n_x, int64_t K,
+                              uint32_t* xq, const uint8_t* scales,
+                              int32_t num_experts, int64_t N, uint32_t* lines,
+                              int64_t line_words, void* stream);
 int qmoe_mxfp4_gather_qqmm(const uint32_t* xq, const uint8_t* xs, int64_t n_x,
                            const int32_t* x_rows, int64_t n_rows,
                            const uint32_t* w, const uint8_t* scales,
                            int32_t num_experts, int64_t N, int64_t K,
                            const int32_t* offsets, const int32_t* tile_row,
                            const int32_t* tile_exp, const int32_t* ntiles,
-                           int64_t max_tiles, void* out, void* stream);
+                           int64_t max_tiles, const uint32_t* lines, void* out,
+                           void* stream);
 
 /* ------------------------------------------- tokens to experts, gradients --
  * The row movement of switch_layers.py:13-25 and moe_weighted_sum.py:44-98

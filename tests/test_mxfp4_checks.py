@@ -207,10 +207,17 @@ def test_bad_arguments_at_the_entry_points():
     assert qmm(tab=(one,) * 4) == INV and qmm(ldx=68) == UNS and qmm(ldx=32) == UNS and qmm(K=48) == UNS
     assert qmm(tr=0, N=72) == UNS and qmm(n=0) == _lib.OK and qmm(dt=1) == UNS
 
-    def qq(xq=one, n_x=4, n=4, E=1, K=64):
-        return L.qmoe_mxfp4_gather_qqmm(xq, one, n_x, None, n, one, one, E, 8, K, None, None, None, None, 0, one, None)
+    def qq(xq=one, n_x=4, n=4, E=1, K=64, lines=None):
+        return L.qmoe_mxfp4_gather_qqmm(xq, one, n_x, None, n, one, one, E, 8, K, None, None, None, None, 0, lines, one, None)
 
     assert qq(xq=None) == INV and qq(E=3) == INV and qq(n=5) == INV and qq(K=16) == UNS and qq(xq=one + 4) == UNS
+    assert qq(lines=one + 2) == UNS
+
+    def lines(x=one, n_x=4, K=64, xq=one, s=one, E=2, N=8, at=one, words=20):
+        return L.qmoe_mxfp4_quantize_lines(x, n_x, K, xq, s, E, N, at, words, None)
+
+    assert lines(x=None) == INV and lines(at=None) == INV and lines(N=-1) == INV and lines(K=48) == UNS
+    assert lines(words=19) == _lib.ERR_WORKSPACE and lines(x=one + 2) == UNS and lines(n_x=0) == _lib.OK
     assert L.qmoe_sort_rows(one, 3, None, 2, 8, 0, one, None) == INV
     assert L.qmoe_sort_rows(one, 3, one, 2, 8, 7, one, None) == UNS
     assert L.qmoe_sort_rows(one, 1 << 30, one, 4, 8, 0, one, None) == UNS

@@ -92,7 +92,8 @@ SIGNATURES: dict[str, tuple] = {
     "qmoe_mxfp4_dequantize": (INT, [P, P, I64, I64, INT, P, P]),
     "qmoe_mxfp4_gather_qmv": (INT, [P, I64, I64, P, I32, P, I64, P, P, I32, I64, I64, INT, INT, P, P]),
     "qmoe_mxfp4_gather_qmm": (INT, [P, I64, I64, P, I64, P, P, I32, I64, I64, INT, P, P, P, P, I64, INT, P, P]),
-    "qmoe_mxfp4_gather_qqmm": (INT, [P, P, I64, P, I64, P, P, I32, I64, I64, P, P, P, P, I64, P, P]),
+    "qmoe_mxfp4_quantize_lines": (INT, [P, I64, I64, P, P, I32, I64, P, I64, P]),
+    "qmoe_mxfp4_gather_qqmm": (INT, [P, P, I64, P, I64, P, P, I32, I64, I64, P, P, P, P, I64, P, P, P]),
     "qmoe_sort_rows": (INT, [P, I64, P, I64, I64, INT, P, P]),
     "qmoe_unsort_sum": (INT, [P, I64, INT, P, P, P, I64, I64, I64, INT, P, P]),
     "qmoe_unsort_grad": (INT, [P, P, I64, INT, P, P, I64, I64, I64, P, P, P]),

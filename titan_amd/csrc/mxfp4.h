@@ -20,6 +20,11 @@ namespace qmoe_mx {
 
 constexpr int kBlock = 32;  // elements per scale
 
+// Scales in lines: per group of 128 columns a line of one word per row, the
+// row's four scale bytes (0 past the last block), so that copies of
+// consecutive rows' scales read consecutive words: word [e][g][n] of [experts]
+// [ceil(K/128)][N], and after those of the weights [g][row] of the activations.
+
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 // Byte b of four scale bytes as the conversions' operand, in one rotation: they
 // use the exponent field alone, whatever the sign and the mantissa bits are.

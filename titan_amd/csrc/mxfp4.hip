@@ -51,14 +51,9 @@ __device__ __forceinline__ void load8(const void* x, int64_t u, float (&f)[8]) {
   }
 }
 
-// One thread per word of codes, four neighbouring lanes per block.
-template <int DT>
-__global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict__ x, int64_t words,
-                                                          uint32_t* __restrict__ w, uint8_t* __restrict__ s) {
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (u >= words) return;  // whole quads: words is a multiple of four
-  float f[8];
-  load8<DT>(x, u, f);
+// The scale byte of the block that four neighbouring lanes hold, eight elements
+// each.
+__device__ __forceinline__ uint32_t quad_scale(const float (&f)[8]) {
   // magnitudes compare as integers; an infinity or a NaN is past all finite ones
   uint32_t m = 0;
 #pragma unroll
@@ -67,15 +62,82 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict
   // the exponent field of a normal m is floor(log2 m) + 127; a subnormal one
   // (field 0) and fields up to 2 clamp to byte 0, a non-finite one is 255
   const int field = (int)(m >> 23);
-  const uint32_t byte = field == 255 ? 255u : (uint32_t)max(field - 2, 0);
+  return field == 255 ? 255u : (uint32_t)max(field - 2, 0);
+}
+// The word of codes of eight elements under a scale byte.
+__device__ __forceinline__ uint32_t quantize8(const float (&f)[8], uint32_t byte) {
   const float sc = scale_of(byte);
   uint32_t q = 0;
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[0], f[1], sc, 0);
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2], f[3], sc, 1);
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4], f[5], sc, 2);
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6], f[7], sc, 3);
-  w[u] = byte == 255u ? 0u : q;
+  return byte == 255u ? 0u : q;
+}
+
+// One thread per word of codes, four neighbouring lanes per block.
+template <int DT>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const void* __restrict__ x, int64_t words,
+                                                          uint32_t* __restrict__ w, uint8_t* __restrict__ s) {
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= words) return;  // whole quads: words is a multiple of four
+  float f[8];
+  load8<DT>(x, u, f);
+  const uint32_t byte = quad_scale(f);
+  w[u] = quantize8(f, byte);
   if ((threadIdx.x & 3) == 0) s[u >> 2] = (uint8_t)byte;
+}
+
+// Quantises bf16 rows and lays their scales and the weights' out in lines: the
+// first blocks take sixteen threads per row and group of 128 columns, each one
+// word of codes; the others 64 weight rows each, a lane per row.  Bound by the
+// weights' scales, a 17th of their bytes read and written.
+__global__ __launch_bounds__(256) void mx_quantize_lines_kernel(const uint4* __restrict__ x, int64_t n_x, int64_t K,
+                                                                uint32_t* __restrict__ xq, uint32_t* __restrict__ xl,
+                                                                int64_t xblocks, const uint8_t* __restrict__ s,
+                                                                int64_t rows, int64_t N, uint32_t* __restrict__ sl) {
+  const int64_t G = (K + 127) / 128, units = K / kBlock;
+  if ((int64_t)blockIdx.x < xblocks) {
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t line = u / 16;  // row * G + group
+    const int l = (int)(u % 16);
+    const int64_t row = min(line / G, n_x - 1), g = line % G;
+    const int64_t word = g * 16 + l;  // of the row
+    const bool in = line < n_x * G && word < K / 8;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (in) load8<QMOE_BF16>(x, row * (K / 8) + word, f);
+    const uint32_t byte = in ? quad_scale(f) : 0u;
+    if (in) xq[row * (K / 8) + word] = quantize8(f, byte);
+    // lane 0 of sixteen collects the four blocks' bytes
+    uint32_t four = byte;
+#pragma unroll
+    for (int b = 1; b < 4; ++b) four |= (uint32_t)__shfl_down((int)byte, 4 * b, 64) << (8 * b);
+    if (l == 0 && line < n_x * G) xl[g * n_x + row] = four;
+    return;
+  }
+  const int64_t r = ((int64_t)blockIdx.x - xblocks) * 64 + threadIdx.x % 64;
+  if (r >= rows) return;
+  const int64_t e = r / N, n = r - e * N;
+  const uint8_t* src = s + r * units;
+  uint32_t* dst = sl + e * G * N + n;
+  const bool whole = units % 16 == 0 && (reinterpret_cast<uintptr_t>(s) & 15) == 0;
+  for (int64_t g0 = threadIdx.x / 64 * 4; g0 < G; g0 += 16) {
+    uint32_t v[4];
+    if (whole) {
+      const uint4 q = *reinterpret_cast<const uint4*>(src + 4 * g0);
+      v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = 0;
+        for (int b = 0; b < 4; ++b)
+          if (4 * (g0 + i) + b < units) v[i] |= (uint32_t)src[4 * (g0 + i) + b] << (8 * b);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (g0 + i < G) dst[(g0 + i) * N] = v[i];
+  }
 }
 
 // A thread makes 16 bytes of values at a time, so that a wave's stores are
@@ -154,4 +216,24 @@ extern "C" int qmoe_mxfp4_dequantize(const uint32_t* w, const uint8_t* scales, i
   else if (dtype == QMOE_FP16) mx_dequantize_kernel<QMOE_FP16><<<grid, block, 0, st>>>(w, scales, pieces, o);
   else mx_dequantize_kernel<QMOE_FP32><<<grid, block, 0, st>>>(w, scales, pieces, o);
   return qmoe::launch_status("mx_dequantize_kernel");
+}
+
+extern "C" int qmoe_mxfp4_quantize_lines(const uint16_t* x, int64_t n_x, int64_t K, uint32_t* xq, const uint8_t* scales,
+                                         int32_t num_experts, int64_t N, uint32_t* lines, int64_t line_words,
+                                         void* stream) {
+  const int rc = check(x, xq, scales, QMOE_BF16, n_x, K);
+  if (rc != QMOE_OK) return rc;
+  if (num_experts < 0 || N < 0 || line_words < 0) return qmoe::fail(QMOE_ERR_INVALID, "bad sizes");
+  if (n_x == 0 || K == 0) return QMOE_OK;
+  const int64_t G = (K + 127) / 128;
+  if (N > 0x7FFFFFFF || K > 0x7FFFFFFF || num_experts * N > ((int64_t)1 << 40) / G || n_x > ((int64_t)1 << 40) / G)
+    return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
+  const int64_t rows = num_experts * N;
+  if (!lines || !qmoe::aligned4(lines)) return qmoe::fail(QMOE_ERR_INVALID, "lines must be 4-byte aligned");
+  if (line_words < (rows + n_x) * G) return qmoe::fail(QMOE_ERR_WORKSPACE, "lines hold %lld words, %lld are needed", (long long)line_words, (long long)((rows + n_x) * G));
+  const int64_t xblocks = (n_x * G + 15) / 16, blocks = xblocks + (rows + 63) / 64;
+  if (blocks > 0x7FFFFFFF) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
+  mx_quantize_lines_kernel<<<dim3((unsigned)blocks), dim3(256), 0, qmoe::as_stream(stream)>>>(
+      reinterpret_cast<const uint4*>(x), n_x, K, xq, lines + rows * G, xblocks, scales, rows, N, lines);
+  return qmoe::launch_status("mx_quantize_lines_kernel");
 }

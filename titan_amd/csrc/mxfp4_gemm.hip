@@ -26,6 +26,8 @@ struct GemmArgs {
   const uint8_t* s;
   int num_experts;
   int64_t N, K;
+  // kQQ: scales in lines (mxfp4.h), null: as they are in s and xs
+  const uint32_t *sl, *xl;
   const int32_t *offsets, *tile_row, *tile_exp, *ntiles;  // all null: one expert, rows in order
   void* out;
   int out_f32;
@@ -762,8 +764,16 @@ struct Trn {
 // Contraction in groups of 128.  A lane's scale byte at step kk is block 2kk +
 // h of its row: the row's four bytes shifted by h, byte 2kk picked by the
 // instruction.
-template <bool S4, int MSUB, bool SPLIT>
+//
+// Where the scales are copied from rows, every lane of a copy reads a cache
+// line of its own, as many lines for a group's 1.5 KiB of scales as for its 24
+// KiB of codes; kLines reads them from lines of consecutive rows (4096^3: 68 ->
+// 49 us; 1531 tokens x top-10 of 256 experts: 104 -> 92 us; the lines are made
+// with the activations' codes, 12 and 10 us where the codes alone take 9 and 5).
+enum { kBytes = 0, kWords = 1, kLines = 2 };
+template <int SC, int MSUB, bool SPLIT>
 struct QQ {
+  static constexpr bool S4 = SC != kBytes;  // a group's four scale bytes of a row at a time
   typedef Geo<SPLIT> Way;
   static constexpr int kCols = Way::kCols, kRows = (SPLIT ? 32 : 64) * MSUB;
   static constexpr int kScaleRows = SPLIT ? 64 : kTileRows;  // rows whose scales are copied: whole waves' worth
@@ -779,14 +789,16 @@ struct QQ {
   struct Ctx {
     RowSrc<kACopies, 4, Way::kWaves> x;
     const char *w, *s, *xs;
+    int64_t sline, xline;  // kLines: bytes from a group's line to the next one's
+    uint32_t xoff;
     uint32_t woff[kBCopies], soff[kSCopies];
     int wunit;
     uint32_t lds;
     int wave, lane, units;  // wave: of those that fill the ring
   };
 
-  static __device__ __forceinline__ void copy(const Ctx& c, int g) {
-    const uint32_t st = c.lds + (g % NS) * kStage;
+  static __device__ __forceinline__ void copy(const Ctx& c, int g, int stage) {
+    const uint32_t st = c.lds + stage * kStage;
     const bool whole = 4 * (g + 1) <= c.units;
 #pragma unroll
     for (int d = 0; d < kACopies; ++d) {
@@ -806,7 +818,11 @@ struct QQ {
       }
     }
     const uint32_t sa = st + kSAOff + (c.wave & 1) * 256, sb = st + kSBOff + c.wave * 256;
-    if constexpr (S4) {
+    if constexpr (SC == kLines) {
+      qmoe_gemm::dma4s(c.xs + g * c.xline, c.xoff, sa);
+#pragma unroll
+      for (int d = 0; d < kSCopies; ++d) qmoe_gemm::dma4s(c.s + g * c.sline, c.soff[d], sb + d * 256);
+    } else if constexpr (S4) {
       qmoe_gemm::dma4(c.xs + (size_t)g * 4, sa);
 #pragma unroll
       for (int d = 0; d < kSCopies; ++d) qmoe_gemm::dma4s(c.s + (size_t)g * 4, c.soff[d], sb + d * 256);
@@ -833,6 +849,13 @@ struct QQ {
       const uint32_t hi = *reinterpret_cast<const uint32_t*>(st + ((2 + h) * rows + row) * 4);
       return (int)(lo | (hi << 16));
     }
+  }
+  static __device__ __forceinline__ void read_scales(const char* st, int row, int col, int h, int (&sa)[MSUB],
+                                                     int (&sb)[4]) {
+#pragma unroll
+    for (int i = 0; i < MSUB; ++i) sa[i] = scales(st + kSAOff, kScaleRows, row + 32 * i, h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sb[j] = scales(st + kSBOff, kCols, col + 32 * j, h);
   }
   struct Frag {
     i32x4_t a[MSUB], b[4];
@@ -875,12 +898,22 @@ struct QQ {
     {
       const int64_t i = u.row0 + min((c.wave & 1) * 64 + c.lane, u.valid - 1);
       const int64_t x = min(max(a.x_rows ? (int64_t)a.x_rows[i] : i, (int64_t)0), a.n_x - 1);
-      c.xs = reinterpret_cast<const char*>(a.xs) + x * c.units;
+      if constexpr (SC == kLines) {
+        c.xs = reinterpret_cast<const char*>(a.xl);
+        c.xoff = (uint32_t)x * 4;
+        c.xline = a.n_x * 4;
+        c.sline = a.N * 4;
+      } else {
+        c.xs = reinterpret_cast<const char*>(a.xs) + x * c.units;
+      }
     }
     const int64_t row = (int64_t)u.e * a.N + u.o0;
     const int cols = (int)min((int64_t)kCols, a.N - u.o0);
     c.w = reinterpret_cast<const char*>(a.w) + qmoe_gemm::uniform64(row * c.units * 16);
-    c.s = reinterpret_cast<const char*>(a.s) + qmoe_gemm::uniform64(row * c.units);
+    if constexpr (SC == kLines)
+      c.s = reinterpret_cast<const char*>(a.sl) + qmoe_gemm::uniform64(((int64_t)u.e * ((c.units + 3) / 4) * a.N + u.o0) * 4);
+    else
+      c.s = reinterpret_cast<const char*>(a.s) + qmoe_gemm::uniform64(row * c.units);
     c.wunit = (c.lane % 4) ^ swz4(c.lane / 4);  // swz4 repeats every 16 columns
 #pragma unroll
     for (int d = 0; d < kBCopies; ++d) {
@@ -889,7 +922,7 @@ struct QQ {
     }
 #pragma unroll
     for (int d = 0; d < kSCopies; ++d)
-      c.soff[d] = (uint32_t)(min((d * Way::kWaves + c.wave) * 64 + c.lane, cols - 1) * c.units);
+      c.soff[d] = (uint32_t)(min((d * Way::kWaves + c.wave) * 64 + c.lane, cols - 1) * (SC == kLines ? 4 : c.units));
     int g0, G;  // this wave's groups
     Way::template part<1>((c.units + 3) / 4, wave, &g0, &G);
     const int row0 = 32 * MSUB * wm, col0 = 128 * wn;
@@ -897,35 +930,38 @@ struct QQ {
 
     f32x16_t acc[MSUB][4] = {};
     if (!SPLIT || g0 < G) {
+      // past the end: the last group again, into stages that nothing reads any more
 #pragma unroll
-    for (int i = 0; i < NS; ++i) copy(c, min(g0 + i, G - 1));
-    qmoe_gemm::wait_vmem<(NS - 1) * kCopies>();
-    Way::barrier();
-    Frag fa, fb;
-    int sa[MSUB], sb[4];
-    read(c, smem + (g0 % NS) * kStage, 0, row0, col0, fa);
-    for (int g = g0; g < G; ++g) {
-      const char* st = smem + (g % NS) * kStage;
-#pragma unroll
-      for (int i = 0; i < MSUB; ++i) sa[i] = scales(st + kSAOff, kScaleRows, row0 + 32 * i + l32, h);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sb[j] = scales(st + kSBOff, kCols, col0 + 32 * j + l32, h);
-      read(c, st, 1, row0, col0, fb);
-      products<0>(fa, sa, sb, acc);
-      if (g + 1 < G) {
-        qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        Way::barrier();
-        copy(c, min(g + NS, G - 1));
-        read(c, smem + ((g + 1) % NS) * kStage, 0, row0, col0, fa);
+      for (int i = 0; i < NS; ++i) copy(c, min(g0 + i, G - 1), i);
+      qmoe_gemm::wait_vmem<(NS - 1) * kCopies>();
+      Way::barrier();
+      Frag fa, fb;
+      int sa[MSUB], sb[4];
+      read(c, smem, 0, row0, col0, fa);
+      int at = 0;
+      for (int g = g0; g < G; ++g) {
+        const char* st = smem + at * kStage;
+        read_scales(st, row0 + l32, col0 + l32, h, sa, sb);
+        read(c, st, 1, row0, col0, fb);
+        products<0>(fa, sa, sb, acc);
+        __builtin_amdgcn_sched_barrier(0);
+        at = at + 1 == NS ? 0 : at + 1;
+        if (g + 1 < G) {
+          qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          Way::barrier();
+          copy(c, min(g + NS, G - 1), at == 0 ? NS - 1 : at - 1);
+          read(c, smem + at * kStage, 0, row0, col0, fa);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        products<1>(fb, sa, sb, acc);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      products<1>(fb, sa, sb, acc);
-    }
     }
     qmoe_gemm::wait_vmem<0>();
     const int el = fresh_tid() % 64, e32 = el % 32, eh = el / 32;
     if constexpr (SPLIT) {
-      Fwd<S4, 1, MSUB, true>::put_parts(block_smem + wave * kRows * 512, e32, eh, acc);
+      Fwd<true, 1, MSUB, true>::put_parts(block_smem + wave * kRows * 512, e32, eh, acc);
       __syncthreads();
       store_parts<kRows>(a, block_smem, u, a.N);
       return;
@@ -966,32 +1002,32 @@ struct Pick<F, G, Rest...> {
     else Next::run(a, u, smem);
   }
 };
-template <int MODE, bool S4, bool SPLIT>
+template <int MODE, int SC, bool SPLIT>
 struct Kernel;
-template <bool S4>
-struct Kernel<kFwd, S4, false> {
-  typedef Pick<Fwd<S4, 2, 2, false>, Fwd<S4, 1, 3, false>, Fwd<S4, 1, 2, false>, Fwd<S4, 1, 1, false>> Forms;
+template <int SC>
+struct Kernel<kFwd, SC, false> {
+  typedef Pick<Fwd<SC == kWords, 2, 2, false>, Fwd<SC == kWords, 1, 3, false>, Fwd<SC == kWords, 1, 2, false>, Fwd<SC == kWords, 1, 1, false>> Forms;
 };
-template <bool S4>
-struct Kernel<kFwd, S4, true> {
-  typedef Pick<Fwd<S4, 1, 2, true>, Fwd<S4, 1, 1, true>> Forms;
+template <int SC>
+struct Kernel<kFwd, SC, true> {
+  typedef Pick<Fwd<SC == kWords, 1, 2, true>, Fwd<SC == kWords, 1, 1, true>> Forms;
 };
-template <bool S4>
-struct Kernel<kT, S4, false> {
-  typedef Pick<Trn<S4, 4, false>, Trn<S4, 3, false>, Trn<S4, 2, false>, Trn<S4, 1, false>> Forms;
+template <int SC>
+struct Kernel<kT, SC, false> {
+  typedef Pick<Trn<SC == kWords, 4, false>, Trn<SC == kWords, 3, false>, Trn<SC == kWords, 2, false>, Trn<SC == kWords, 1, false>> Forms;
 };
-template <bool S4>
-struct Kernel<kT, S4, true> {
-  typedef Pick<Trn<S4, 4, true>, Trn<S4, 2, true>, Trn<S4, 1, true>> Forms;
+template <int SC>
+struct Kernel<kT, SC, true> {
+  typedef Pick<Trn<SC == kWords, 4, true>, Trn<SC == kWords, 2, true>, Trn<SC == kWords, 1, true>> Forms;
 };
-template <bool S4, bool SPLIT>
-struct Kernel<kQQ, S4, SPLIT> {
-  typedef Pick<QQ<S4, 2, SPLIT>, QQ<S4, 1, SPLIT>> Forms;
+template <int SC, bool SPLIT>
+struct Kernel<kQQ, SC, SPLIT> {
+  typedef Pick<QQ<SC, 2, SPLIT>, QQ<SC, 1, SPLIT>> Forms;
 };
 
-template <int MODE, bool S4, bool SPLIT>
+template <int MODE, int SC, bool SPLIT>
 __global__ __launch_bounds__(256, SPLIT ? 1 : 2) void mx_gemm_kernel(GemmArgs a, int64_t dense_tiles, int NB) {
-  typedef typename Kernel<MODE, S4, SPLIT>::Forms Forms;
+  typedef typename Kernel<MODE, SC, SPLIT>::Forms Forms;
   typedef Geo<SPLIT> Way;
   constexpr int kEnd = SPLIT ? 4 * 64 * 512 : 64 * 512;  // the epilogue's rows
   constexpr int kRing = Way::kRings * Forms::kRing > kEnd ? Way::kRings * Forms::kRing : kEnd;
@@ -1037,9 +1073,15 @@ void launch_way(const GemmArgs& a, int64_t max_tiles, hipStream_t st) {
   const int64_t NB = (O + Geo<SPLIT>::kCols - 1) / Geo<SPLIT>::kCols;
   const int64_t units = (a.offsets ? max_tiles : dense) * NB * (SPLIT ? 2 : 1);
   const dim3 grid((unsigned)qmoe_gemm::grid_blocks(units, SPLIT ? 1 : 2)), block(256);
+  if constexpr (MODE == kQQ) {
+    if (a.sl) {
+      mx_gemm_kernel<MODE, kLines, SPLIT><<<grid, block, 0, st>>>(a, dense, (int)NB);
+      return;
+    }
+  }
   const bool s4 = a.K % 128 == 0 && qmoe::aligned4(a.s) && (MODE != kQQ || qmoe::aligned4(a.xs));
-  if (s4) mx_gemm_kernel<MODE, true, SPLIT><<<grid, block, 0, st>>>(a, dense, (int)NB);
-  else mx_gemm_kernel<MODE, false, SPLIT><<<grid, block, 0, st>>>(a, dense, (int)NB);
+  if (s4) mx_gemm_kernel<MODE, kWords, SPLIT><<<grid, block, 0, st>>>(a, dense, (int)NB);
+  else mx_gemm_kernel<MODE, kBytes, SPLIT><<<grid, block, 0, st>>>(a, dense, (int)NB);
 }
 
 // Wide units from this many on: below, split ones are faster.  At 64, 128 and
@@ -1076,7 +1118,7 @@ int check(const GemmArgs& a, int mode, int64_t max_tiles, int out_dtype, bool* r
   if (a.n_rows == 0 || O == 0) return QMOE_OK;
   if (C == 0) return qmoe::fail(QMOE_ERR_INVALID, "an empty contraction");
   if (a.n_x == 0 || a.num_experts == 0) return qmoe::fail(QMOE_ERR_INVALID, "no activation rows or no experts");
-  if (!a.w || !a.s || !a.out || (mode == kQQ ? !a.xq || !a.xs : !a.x)) return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
+  if (!a.w || !a.s || !a.out || (mode == kQQ ? !a.xq || (!a.xs && !a.sl) : !a.x)) return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
   const bool any = a.offsets || a.tile_row || a.tile_exp || a.ntiles;
   if (any && !(a.offsets && a.tile_row && a.tile_exp && a.ntiles)) return qmoe::fail(QMOE_ERR_INVALID, "half a tile table");
   if (!any && a.num_experts != 1) return qmoe::fail(QMOE_ERR_INVALID, "several experts need a tile table");
@@ -1099,7 +1141,7 @@ extern "C" int qmoe_mxfp4_gather_qmm(const uint16_t* x, int64_t n_x, int64_t ldx
                                      int64_t K, int transpose, const int32_t* offsets, const int32_t* tile_row,
                                      const int32_t* tile_exp, const int32_t* ntiles, int64_t max_tiles, int out_dtype,
                                      void* out, void* stream) {
-  GemmArgs a{x, nullptr, nullptr, x_rows, n_rows, n_x, ldx, w, scales, num_experts, N, K,
+  GemmArgs a{x, nullptr, nullptr, x_rows, n_rows, n_x, ldx, w, scales, num_experts, N, K, nullptr, nullptr,
              offsets, tile_row, tile_exp, ntiles, out, out_dtype == QMOE_FP32};
   bool run;
   const int rc = check(a, transpose ? kFwd : kT, max_tiles, out_dtype, &run);
@@ -1112,13 +1154,19 @@ extern "C" int qmoe_mxfp4_gather_qmm(const uint16_t* x, int64_t n_x, int64_t ldx
 extern "C" int qmoe_mxfp4_gather_qqmm(const uint32_t* xq, const uint8_t* xs, int64_t n_x, const int32_t* x_rows,
                                       int64_t n_rows, const uint32_t* w, const uint8_t* scales, int32_t num_experts,
                                       int64_t N, int64_t K, const int32_t* offsets, const int32_t* tile_row,
-                                      const int32_t* tile_exp, const int32_t* ntiles, int64_t max_tiles, void* out,
-                                      void* stream) {
-  GemmArgs a{nullptr, xq, xs, x_rows, n_rows, n_x, 0, w, scales, num_experts, N, K,
+                                      const int32_t* tile_exp, const int32_t* ntiles, int64_t max_tiles,
+                                      const uint32_t* lines, void* out, void* stream) {
+  GemmArgs a{nullptr, xq, xs, x_rows, n_rows, n_x, 0, w, scales, num_experts, N, K, lines, nullptr,
              offsets, tile_row, tile_exp, ntiles, out, 0};
   bool run;
   const int rc = check(a, kQQ, max_tiles, QMOE_BF16, &run);
   if (rc != QMOE_OK || !run) return rc;
-  if (!offsets && n_rows <= kFewRows) return rows_product(rows_of(a), true, qmoe::as_stream(stream));
+  if (lines) {
+    if (!qmoe::aligned4(lines)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "lines must be 4-byte aligned");
+    if (n_x > (1 << 29)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "n_x=%lld: too many rows for lines", (long long)n_x);
+    a.xl = lines + (int64_t)num_experts * ((K + 127) / 128) * N;
+  } else if (!offsets && n_rows <= kFewRows) {
+    return rows_product(rows_of(a), true, qmoe::as_stream(stream));
+  }
   return launch<kQQ>(a, max_tiles, qmoe::as_stream(stream));
 }

@@ -38,6 +38,10 @@ constexpr int64_t kSortedMinRows = 64;  // gathered rows from which the grouped 
 // products take the GEMM from one row on (4096 x 2048: 20 and 14.6 us).
 constexpr int64_t kQmvMaxRows = 4, kQmvMaxWork = int64_t(1) << 24;
 
+// Rows above which products of two mxfp4 operands leave the kernel for few rows,
+// and rows per expert from which laying the scales out in lines pays.
+constexpr int64_t kFewRows = 64, kLineRows = 32;
+
 struct Failure : std::runtime_error {
   int code;
   Failure(int c, const char* what)
@@ -316,14 +320,26 @@ Tensor product(const Tensor& x, const Weights& g, const Rows& r, bool transpose)
 }
 
 Tensor qq_run(const Tensor& x, const Weights& g, const Rows& r) {
-  const auto [xq, xs] = quantize_run(x);
   Tensor out = at::empty({r.n, g.N}, x.options().requires_grad(false));
   if (out.numel() == 0) return out;
   if (g.K == 0) return out.zero_();
+  Tensor xq, xs, lines;
+  if (r.n > kFewRows && r.n >= kLineRows * g.E) {
+    const int64_t words = (g.E * g.N + x.size(0)) * ((g.K + 127) / 128);
+    xq = at::empty({x.size(0), g.K / 8}, x.options().dtype(at::kInt).requires_grad(false));
+    lines = at::empty({words}, xq.options());
+    ok(qmoe_mxfp4_quantize_lines(ptr<uint16_t>(x), x.size(0), g.K, static_cast<uint32_t*>(xq.data_ptr()),
+                                 ptr<uint8_t>(g.s), (int32_t)g.E, g.N, static_cast<uint32_t*>(lines.data_ptr()), words,
+                                 stream(x)),
+       "qmoe_mxfp4_quantize_lines");
+  } else {
+    std::tie(xq, xs) = quantize_run(x);
+  }
   const Tensor rows = gemm_rows(r, x);
   ok(qmoe_mxfp4_gather_qqmm(ptr<uint32_t>(xq), ptr<uint8_t>(xs), x.size(0), ptr<int32_t>(rows), r.n, ptr<uint32_t>(g.w),
                             ptr<uint8_t>(g.s), (int32_t)g.E, g.N, g.K, ptr<int32_t>(r.offsets), ptr<int32_t>(r.tile_row),
-                            ptr<int32_t>(r.tile_exp), ptr<int32_t>(r.ntiles), r.maxt, out.data_ptr(), stream(x)),
+                            ptr<int32_t>(r.tile_exp), ptr<int32_t>(r.ntiles), r.maxt, ptr<uint32_t>(lines),
+                            out.data_ptr(), stream(x)),
      "qmoe_mxfp4_gather_qqmm");
   return out;
 }
