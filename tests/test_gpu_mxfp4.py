@@ -293,6 +293,35 @@ def test_sorted_rows_with_empty_and_full_experts(dev, n):
         check_sum(got.squeeze(1), *_by_expert(x, W, e, True), K)
 
 
+@pytest.mark.parametrize("n", [5, 70, 300])
+@pytest.mark.parametrize("is_sorted", [False, True])
+def test_indices_out_of_range_are_clamped(dev, n, is_sorted):
+    """Memory stays in bounds and every row is computed, forward and backward, few rows and many."""
+    say("clamped", n, is_sorted)
+    g = _gen(41)
+    E, K, N = 4, 64, 40
+    w, s = codes(g, E, N, K)
+    W = dequantize_ref(w, s)
+    e = torch.randint(-3, E + 3, (n,), generator=g)
+    lhs = torch.randint(-2, n + 2, (n,), generator=g)
+    if is_sorted:
+        e = torch.sort(e)[0]
+    x = _acts(g, n, K)
+    inside = e.clamp(0, E - 1)
+    xd = x.to(dev).unsqueeze(1).requires_grad_(True)
+    for kw, xi in (({}, torch.arange(n)), ({"lhs_indices": lhs.to(dev)}, lhs.clamp(0, n - 1))):
+        for ids in (e.to(dev), e.to(torch.int32).to(dev)):
+            y = ops.gather_qmm(xd, w.to(dev), s.to(dev), rhs_indices=ids, mode="mxfp4", sorted_indices=is_sorted, **kw)
+            check_sum(y.squeeze(1), *_by_expert(x[xi], W, inside, True), K)
+            q = ops.gather_qqmm(xd.detach(), w.to(dev), s.to(dev), rhs_indices=ids, sorted_indices=is_sorted, **kw)
+            check_sum(q.squeeze(1), *_by_expert(quantize_ref(x)[0][xi], W, inside, True), K)
+        dy = _acts(g, n, N)
+        (dx,) = torch.autograd.grad(y, xd, dy.to(dev).unsqueeze(1))
+        ref, mag = _by_expert(dy, W, inside, False)
+        zero = torch.zeros(n, K, dtype=torch.float64)
+        check_sum(dx.squeeze(1), zero.index_add(0, xi, ref), zero.index_add(0, xi, mag), N + n)
+
+
 # -------------------------------------------------------------- gradients
 
 

@@ -456,7 +456,8 @@ __global__ __launch_bounds__(kScanThreads) void tiles_from_sorted_kernel(const i
                                                                          int32_t* __restrict__ tile_row,
                                                                          int32_t* __restrict__ tile_exp,
                                                                          int32_t* __restrict__ ntiles,
-                                                                         int64_t max_tiles) {
+                                                                         int64_t max_tiles, bool all) {
+  // all: ids below 0 are expert 0's, ids from E on expert E - 1's, so that every row has a tile
   // first row whose id >= e, in two levels: a search over every stride-th id,
   // read by the block at once, then one inside a stride.  (Each step of a
   // search in memory is a dependent read, 15 of them at 20,480 rows: 4.8 -> 4.5
@@ -480,6 +481,8 @@ __global__ __launch_bounds__(kScanThreads) void tiles_from_sorted_kernel(const i
       if (sorted_ids[mid] < e) lo = mid + 1;
       else hi = mid;
     }
+    if (all && e == 0) lo = 0;
+    if (all && e == E) lo = n;
     offsets[e] = (int32_t)lo;
   }
   __syncthreads();
@@ -706,17 +709,30 @@ extern "C" int qmoe_route_block(const int32_t* ids, int64_t n_pairs, int32_t top
                       BlockRows{x_rows, (uint32_t)top_k, shared_rows});
 }
 
-extern "C" int qmoe_build_tiles(const int32_t* sorted_ids, int64_t n_rows, int32_t num_experts,
-                                int32_t tile_rows, int32_t* offsets, int32_t* tile_row, int32_t* tile_exp,
-                                int32_t* ntiles, int64_t max_tiles, void* stream) {
+static int build_tiles(const int32_t* sorted_ids, int64_t n_rows, int32_t num_experts, int32_t tile_rows,
+                       int32_t* offsets, int32_t* tile_row, int32_t* tile_exp, int32_t* ntiles, int64_t max_tiles,
+                       bool all, void* stream) {
   if (n_rows < 0 || num_experts <= 0 || tile_rows <= 0 || max_tiles < 0)
     return qmoe::fail(QMOE_ERR_INVALID, "bad sizes");
   if (n_rows > 0x7FFFFFFF) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "too many rows");
   if (!offsets || !tile_row || !tile_exp || !ntiles || (n_rows > 0 && !sorted_ids))
     return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
   tiles_from_sorted_kernel<<<dim3(1), dim3(kScanThreads), 0, qmoe::as_stream(stream)>>>(
-      sorted_ids, n_rows, num_experts, tile_rows, offsets, tile_row, tile_exp, ntiles, max_tiles);
+      sorted_ids, n_rows, num_experts, tile_rows, offsets, tile_row, tile_exp, ntiles, max_tiles, all);
   return qmoe::launch_status("tiles_from_sorted_kernel");
+}
+
+extern "C" int qmoe_build_tiles(const int32_t* sorted_ids, int64_t n_rows, int32_t num_experts,
+                                int32_t tile_rows, int32_t* offsets, int32_t* tile_row, int32_t* tile_exp,
+                                int32_t* ntiles, int64_t max_tiles, void* stream) {
+  return build_tiles(sorted_ids, n_rows, num_experts, tile_rows, offsets, tile_row, tile_exp, ntiles, max_tiles, false,
+                     stream);
+}
+extern "C" int qmoe_build_tiles_clamped(const int32_t* sorted_ids, int64_t n_rows, int32_t num_experts,
+                                        int32_t tile_rows, int32_t* offsets, int32_t* tile_row, int32_t* tile_exp,
+                                        int32_t* ntiles, int64_t max_tiles, void* stream) {
+  return build_tiles(sorted_ids, n_rows, num_experts, tile_rows, offsets, tile_row, tile_exp, ntiles, max_tiles, true,
+                     stream);
 }
 
 // ------------------------------------------------------------------------

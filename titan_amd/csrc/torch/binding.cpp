@@ -392,10 +392,10 @@ bool table(const Tensor& experts, int64_t E, Rows* r) {
   r->tile_row = all.narrow(0, a, r->maxt);
   r->tile_exp = all.narrow(0, a + b, r->maxt);
   r->ntiles = all.narrow(0, a + 2 * b, 1);
-  ok(qmoe_build_tiles(ptr<int32_t>(experts), n, (int32_t)E, (int32_t)tr, r->offsets.data_ptr<int32_t>(),
+  ok(qmoe_build_tiles_clamped(ptr<int32_t>(experts), n, (int32_t)E, (int32_t)tr, r->offsets.data_ptr<int32_t>(),
                       r->tile_row.data_ptr<int32_t>(), r->tile_exp.data_ptr<int32_t>(), r->ntiles.data_ptr<int32_t>(),
                       r->maxt, stream(experts)),
-     "qmoe_build_tiles");
+     "qmoe_build_tiles_clamped");
   return true;
 }
 

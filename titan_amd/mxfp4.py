@@ -210,7 +210,7 @@ def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
     if n >= min_rows:
         if sorted_indices:
             if tiles is None or tiles.rows != n:
-                tiles = ops.build_tiles(experts, E)
+                tiles = ops.build_tiles(experts.clamp(0, E - 1), E)
             elif tiles.num_experts != E or tiles.tile_rows != ops.tile_rows():
                 raise ValueError("tile table does not match this call")
         else:
@@ -249,7 +249,8 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=No
     """:func:`titan_amd.ops.gather_qmm` for codes w [E, N, K/8]: x [.., M, K]
     times W^T, or x [.., M, N] times W without ``transpose``.  From 64 rows on
     the rows run through the grouped GEMM: as they are with ``sorted_indices``
-    (ascending ``rhs_indices``), else sorted by expert first."""
+    (ascending ``rhs_indices``), else sorted by expert first.  Indices outside
+    their range are clamped into it."""
     _format(group_size, bits, biases)
     if tiles is None:
         y = _lib.binding().gather(x, w, scales, lhs_indices, rhs_indices, bool(transpose), bool(sorted_indices), False)
