@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define QMOE_ABI_VERSION 4
+#define QMOE_ABI_VERSION 5
 
 enum {
   QMOE_OK = 0,
