@@ -488,3 +488,106 @@ def test_repeats_on_streams_and_in_graphs(dev, M):
         assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
         if seed == 1:
             assert all(torch.equal(a, b) for a, b in zip(first, want))
+
+
+def _indexed(dev, seed, n_x, n, E, K):
+    g = _gen(seed)
+    lhs = torch.randint(0, n_x, (n,), generator=g)
+    lhs[: n // 4] = lhs[n // 4: n // 4 * 2]  # the same row by several indices
+    return lhs, torch.randint(0, E, (n,), generator=g), _acts(g, n_x, K), _acts(g, n, 40)
+
+
+@pytest.mark.parametrize("is_sorted", [False, True])
+@pytest.mark.parametrize("n_x,n", [(1, 90), (300, 700), (2049, 64), (5000, 700)])
+def test_gradient_of_indexed_rows(dev, n_x, n, is_sorted):
+    """Activation rows taken by index, few and many, in any order: eager, and captured and replayed with new inputs."""
+    say("indexed rows", n_x, n, is_sorted)
+    E, K, N = 5, 64, 40
+    w, s = codes(_gen(43), E, N, K)
+    W = dequantize_ref(w, s)
+    wd, sd = w.to(dev), s.to(dev)
+
+    def prepared(seed):
+        lhs, e, x, dy = _indexed(dev, seed, n_x, n, E, K)
+        return lhs, torch.sort(e)[0] if is_sorted else e, x, dy
+
+    lhs, e, x, dy = (t.to(dev) for t in prepared(1))
+
+    def step():
+        xd = x.detach().unsqueeze(1).requires_grad_(True)
+        y = ops.gather_qmm(xd, wd, sd, lhs_indices=lhs, rhs_indices=e, mode="mxfp4", sorted_indices=is_sorted)
+        return torch.autograd.grad(y, xd, dy.unsqueeze(1))[0].squeeze(1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2, 3):
+        fresh = prepared(seed)
+        for t, f in zip((lhs, e, x, dy), fresh):
+            t.copy_(f)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), seed
+        ref, mag = _by_expert(fresh[3], W, fresh[1], False)
+        zero = torch.zeros(n_x, K, dtype=torch.float64)
+        check_sum(want, zero.index_add(0, fresh[0], ref), zero.index_add(0, fresh[0], mag), N + n)
+
+
+@pytest.mark.parametrize("k", [1, 3])
+def test_gradient_of_an_unsorted_call_in_a_graph(dev, k):
+    """Rows that the call sorts by itself, each token's for k pairs: eager and replayed alike."""
+    say("unsorted graph", k)
+    T, E, K, N = 80, 6, 96, 33
+    g = _gen(47)
+    w, s = codes(g, E, N, K)
+    W = dequantize_ref(w, s)
+    wd, sd = w.to(dev), s.to(dev)
+    x, ids, dy = _acts(g, T, K).to(dev), torch.zeros(T, k, dtype=torch.int32, device=dev), _acts(g, T * k, N).to(dev)
+
+    def step():
+        xd = x.detach().requires_grad_(True)
+        y = ops.gather_qmm(xd.reshape(T, 1, 1, K), wd, sd, rhs_indices=ids, mode="mxfp4")
+        return torch.autograd.grad(y, xd, dy.reshape(y.shape))[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2, 3):
+        new = torch.randint(0, E, (T, k), generator=_gen(seed))
+        ids.copy_(new)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), seed
+        ref, mag = _by_expert(dy.cpu(), W, new.reshape(-1), False)
+        tok = torch.arange(T).repeat_interleave(k)
+        zero = torch.zeros(T, K, dtype=torch.float64)
+        check_sum(want, zero.index_add(0, tok, ref), zero.index_add(0, tok, mag), N + k)
+
+
+def test_refuses_forward_mode(dev):
+    """A tangent is refused, not lost."""
+    from torch.autograd import forward_ad
+
+    w, s = (t.to(dev) for t in codes(_gen(1), 8, 32))
+    x = torch.ones(2, 32, dtype=BF, device=dev)
+    one = torch.arange(2, dtype=torch.int32, device=dev)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.quantized_matmul(d, w, s, mode="mxfp4"), lambda: ops.qqmm(d, w, s),
+                     lambda: ops.gather_qmm(d.unsqueeze(1), w[None], s[None], rhs_indices=one * 0, mode="mxfp4"),
+                     lambda: ops.sort_tokens(d, one, one), lambda: ops.unsort_tokens(d, one, one),
+                     lambda: ops.unsort_tokens(d, one, one, torch.ones(2, 1, device=dev))):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()

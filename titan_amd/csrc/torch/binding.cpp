@@ -14,8 +14,9 @@
 #include <torch/extension.h>
 
 #include <ATen/ops/arange.h>
+#include <ATen/ops/index_select.h>
 #include <ATen/ops/searchsorted.h>
-#include <ATen/ops/sort.h>
+#include <ATen/ops/zeros.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -81,10 +82,15 @@ const T* ptr(const Tensor& t) {
 }
 void* stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 Tensor ready(Tensor t) {
-  t = t.contiguous();
+  t = t.resolve_neg().contiguous();
   return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 ? t.clone() : t;
 }
-bool records(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+// A gradient of t is asked for.  Tangents (forward mode) would be lost: refused.
+bool records(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(),
+                              "forward-mode automatic differentiation is not supported here");
+  return t.requires_grad() && at::GradMode::is_enabled();
+}
 
 py::object none(bool must) {
   TORCH_CHECK(!must, "the arguments are not what the kernels read");
@@ -242,10 +248,11 @@ py::object unsort_tokens(py::handle xs_, py::handle order_, py::handle inv_, py:
 
 // Which activation row and which expert each of n output rows takes: x_rows,
 // or row i / div; experts (undefined: expert 0 for all); and the tile table of
-// sorted rows (undefined: not sorted, or one expert).
+// sorted rows (undefined: not sorted, or one expert).  With inv activation row
+// t's rows are known to be inv[t div .. (t + 1) div).
 struct Rows {
   int64_t n = 0, div = 1, maxt = 0;
-  Tensor x_rows, experts, offsets, tile_row, tile_exp, ntiles;
+  Tensor x_rows, experts, offsets, tile_row, tile_exp, ntiles, inv;
 };
 struct Weights {
   Tensor w, s;
@@ -282,9 +289,36 @@ Tensor product_run(const Tensor& x_, const Weights& g, const Rows& r, bool trans
   return out;
 }
 
+// The rows of each of n_x activation rows, in ascending order: (order, first),
+// activation row t's being order[first[t] .. first[t + 1]).  A stable radix sort
+// of the rows' activation rows by the routing's counting sort, eleven bits a
+// pass: no library sort, whose cleared counters a captured graph must not hold.
+std::pair<Tensor, Tensor> rows_of(const Tensor& x_rows, int64_t n_x) {
+  constexpr int64_t kBits = 11, kBins = 1 << kBits;
+  const int64_t n = x_rows.numel(), maxt = kBins + 1;
+  if (n == 0) return {x_rows, at::zeros({n_x + 1}, x_rows.options())};
+  const Tensor at_ = x_rows.clamp(0, std::max<int64_t>(n_x - 1, 0));
+  const int64_t bytes = qmoe_route_workspace_size(n, kBins);
+  Tensor order;
+  for (int64_t bit = 0; bit == 0 || (n_x - 1) >> bit; bit += kBits) {
+    Tensor digit = at_.__rshift__(bit).bitwise_and_(kBins - 1);
+    if (order.defined()) digit = digit.index_select(0, order);
+    Tensor by = at::empty({n}, at_.options()), tmp = at::empty({2 * n + kBins + 1 + 2 * maxt + 1}, at_.options()),
+           ws = at::empty({bytes}, at_.options().dtype(at::kByte));
+    int32_t* p = tmp.data_ptr<int32_t>();
+    // tiles as long as all the rows: one per bin at most
+    ok(qmoe_route(digit.data_ptr<int32_t>(), n, kBins, (int32_t)n, by.data_ptr<int32_t>(), p, p + n, p + 2 * n,
+                  p + 2 * n + kBins + 1, p + 2 * n + kBins + 1 + maxt, p + 2 * n + kBins + 1 + 2 * maxt, maxt,
+                  ws.data_ptr(), bytes, stream(at_)),
+       "qmoe_route");
+    order = order.defined() ? order.index_select(0, by) : by;
+  }
+  return {order, at::searchsorted(at_.index_select(0, order), at::arange(n_x + 1, at_.options()), /*out_int32=*/true)};
+}
+
 struct Product : torch::autograd::Function<Product> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Weights& g, const Rows& r, bool transpose) {
-    ctx->save_for_backward({g.w, g.s, r.x_rows, r.experts, r.offsets, r.tile_row, r.tile_exp, r.ntiles});
+    ctx->save_for_backward({g.w, g.s, r.x_rows, r.experts, r.offsets, r.tile_row, r.tile_exp, r.ntiles, r.inv});
     ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), g.E, g.N, g.K, r.n, r.div, r.maxt, transpose};
     return product_run(x, g, r, transpose, at::kBFloat16);
   }
@@ -303,12 +337,11 @@ struct Product : torch::autograd::Function<Product> {
       dx = product_run(dy, g, own, !z[7], at::kBFloat16);
     } else {  // several rows share an activation row: their gradients are added in fp32, rounded once
       const Tensor dr = product_run(dy, g, own, !z[7], at::kFloat);
-      if (!v[2].defined()) {
-        dx = sum_run(dr, {}, {}, {}, n_x, div, at::kBFloat16);
+      if (!v[2].defined() || v[8].defined()) {
+        dx = sum_run(dr, v[8], {}, {}, n_x, div, at::kBFloat16);
       } else {
-        const auto [at_, order] = v[2].clamp(0, std::max<int64_t>(n_x - 1, 0)).sort(/*stable=*/true, 0, false);
-        const Tensor first = at::searchsorted(at_, at::arange(n_x + 1, v[2].options()), /*out_int32=*/true);
-        dx = sum_run(dr, order.to(at::kInt), {}, first, n_x, 0, at::kBFloat16);
+        const auto [order, first] = rows_of(v[2], n_x);
+        dx = sum_run(dr, order, {}, first, n_x, 0, at::kBFloat16);
       }
     }
     return first_order({dx, Tensor(), Tensor(), Tensor()}, grads);
@@ -440,23 +473,26 @@ py::object gather(py::handle x_, py::handle w_, py::handle s_, py::handle lhs_, 
   return give(y.reshape(sizes));
 }
 
-// Rows already arranged by the wrapper: x [rows, C], x_rows / experts int32 or None, a tile table or None.
+// Rows already arranged by the wrapper: x [rows, C], x_rows / experts int32 or None, a tile table or None, and
+// where the rows of activation row t are known, their places inv[t div .. (t + 1) div).
 py::object rows_product(const Tensor& x, const Tensor& w, const Tensor& s, const std::optional<Tensor>& x_rows,
                         int64_t div, const std::optional<Tensor>& experts,
                         const std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, int64_t>>& tiles, int64_t n,
-                        bool transpose, bool qq) {
+                        bool transpose, bool qq, const std::optional<Tensor>& inv) {
   Weights g{w, s, w.size(0), w.size(1), w.size(2) * 8};
   Rows r;
   r.n = n;
   r.div = div;
   if (x_rows) r.x_rows = *x_rows;
   if (experts) r.experts = *experts;
+  if (inv) r.inv = *inv;
   if (tiles) std::tie(r.offsets, r.tile_row, r.tile_exp, r.ntiles, r.maxt) = *tiles;
   TORCH_CHECK(plain(x, at::kBFloat16) && words(w) && bytes(s), "the arguments are not what the kernels read");
-  for (const Tensor* t : {&r.x_rows, &r.experts, &r.offsets, &r.tile_row, &r.tile_exp, &r.ntiles})
+  for (const Tensor* t : {&r.x_rows, &r.experts, &r.offsets, &r.tile_row, &r.tile_exp, &r.ntiles, &r.inv})
     TORCH_CHECK(!t->defined() || (t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == x.device()),
                 "the arguments are not what the kernels read");
-  TORCH_CHECK((!x_rows || r.x_rows.numel() == n) && (!experts || r.experts.numel() == n), "the rows disagree");
+  TORCH_CHECK((!x_rows || r.x_rows.numel() == n) && (!experts || r.experts.numel() == n) &&
+                  (!inv || (r.inv.numel() == n && x.size(0) * div == n)), "the rows disagree");
   const c10::hip::HIPGuard guard(x.get_device());
   return give(qq ? qq_run(x, g, r) : product(x, g, r, transpose));
 }

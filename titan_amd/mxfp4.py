@@ -108,12 +108,13 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases=None, group_size: i
 class _Rows:
     """Which activation row and which expert each output row takes: ``x_rows``
     (or row i // div), ``experts``, and the tile table of sorted rows (None: not
-    sorted)."""
+    sorted).  With ``inv``, ``x_rows`` is the sorted form of row i // div, whose
+    rows are at ``inv[i]``."""
 
-    __slots__ = ("n", "x_rows", "div", "experts", "tiles")
+    __slots__ = ("n", "x_rows", "div", "experts", "tiles", "inv")
 
-    def __init__(self, n, x_rows=None, div=1, experts=None, tiles=None):
-        self.n, self.x_rows, self.div, self.experts, self.tiles = n, x_rows, div, experts, tiles
+    def __init__(self, n, x_rows=None, div=1, experts=None, tiles=None, inv=None):
+        self.n, self.x_rows, self.div, self.experts, self.tiles, self.inv = n, x_rows, div, experts, tiles, inv
 
 
 def _product(x, w, scales, transpose, rows: _Rows, qq: bool = False):
@@ -121,7 +122,8 @@ def _product(x, w, scales, transpose, rows: _Rows, qq: bool = False):
     says, recorded where a gradient of x may be asked for; ``qq``: x in mxfp4."""
     t = rows.tiles
     table = None if t is None else (t.offsets, t.tile_row, t.tile_exp, t.ntiles, t.maxt)
-    return _lib.binding().rows_product(x, w, scales, rows.x_rows, rows.div, rows.experts, table, rows.n, bool(transpose), qq)
+    return _lib.binding().rows_product(x, w, scales, rows.x_rows, rows.div, rows.experts, table, rows.n, bool(transpose), qq,
+                                        rows.inv)
 
 
 def _x_rows(rows: _Rows, device):
@@ -204,7 +206,7 @@ def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
         x_rows = None if base is None else (base[:, None] * M + ar).reshape(-1)
         div = 1
         experts = experts.repeat_interleave(M)
-    n, order = nb * M, None
+    n, order, known = nb * M, None, None
     if n and (E == 0 or math.prod(x.shape[:-1]) == 0):
         raise ValueError("rows are asked for, but there are no experts or no activation rows")
     if n >= min_rows:
@@ -217,13 +219,16 @@ def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
             r = ops.route(experts, E)
             order, inv, tiles = r.order, r.inv_order, r.tiles
             experts = r.sorted_ids
-            x_rows = _x_rows(_Rows(n, x_rows, div), dev)
-            x_rows = order if x_rows is None else x_rows[order.long()]
+            if x_rows is None:
+                known = inv
+                x_rows = order if div == 1 else torch.div(order, div, rounding_mode="floor")
+            else:
+                x_rows = x_rows[order.long()]
+                div = 1
             order = order, inv
-            div = 1
     else:
         tiles = None
-    return batch, _Rows(n, x_rows, div, experts, tiles), order
+    return batch, _Rows(n, x_rows, div, experts, tiles, known), order
 
 
 def _check_gather(x, w, scales, transpose, lhs, rhs):
