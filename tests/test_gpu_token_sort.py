@@ -105,6 +105,17 @@ def test_no_tokens(dev):
     assert x.grad.shape == (0, 16)
 
 
+def test_rows_without_elements(dev):
+    """D = 0: the scores' gradients are empty sums."""
+    ids = torch.arange(6, dtype=torch.int32, device=dev)
+    xs = torch.empty(6, 0, device=dev, requires_grad=True)
+    scores = torch.ones(3, 2, device=dev, requires_grad=True)
+    y = ops.unsort_tokens(xs, ids, ids, scores)
+    assert y.shape == (3, 0) and ops.sort_tokens(y.detach(), ids, ids).shape == (6, 0)
+    y.sum().backward()
+    assert xs.grad.shape == (6, 0) and torch.equal(scores.grad, torch.zeros(3, 2, device=dev))
+
+
 def test_gradients_against_differences(dev):
     """In fp32 the sums are linear in xs and in scores."""
     g, ids, order, inv, x, ys, scores = _setup(dev, 5, 3, 6, 37, torch.float32)

@@ -229,6 +229,22 @@ def test_bad_arguments_at_the_entry_points():
     assert L.qmoe_unsort_grad(one, one, 6, 0, one, None, 3, 2, 8, one, one, None) == INV
 
 
+def test_more_than_one_launch_holds():
+    """A grid of 2^32 threads or more is refused, not cut off."""
+    L = _lib.load()
+    one, UNS = 4096, _lib.ERR_UNSUPPORTED
+    many = 1 << 31
+    assert L.qmoe_mxfp4_quantize(one, 0, many, 32, one, one, None) == UNS
+    assert L.qmoe_mxfp4_dequantize(one, one, many // 4, 32, 2, one, None) == UNS
+    assert L.qmoe_mxfp4_quantize_lines(one, 1 << 29, 32, one, one, 1, 8, one, 1 << 40, None) == UNS
+    assert L.qmoe_mxfp4_gather_qmv(one, 4, 64, None, 1, None, 65535, one, one, 1, 1 << 20, 64, 1, 0, one, None) == UNS
+    assert L.qmoe_mxfp4_gather_qmv(one, 4, 64, None, 1, None, 65535, one, one, 1, 64, 1 << 20, 0, 0, one, None) == UNS
+    assert L.qmoe_mxfp4_gather_qmm(one, 9, 64, None, 9, one, one, 1, many - 1, 64, 1, *(None,) * 4, 0, 0, one, None) == UNS
+    assert L.qmoe_sort_rows(one, 1 << 25, one, 2, 4096, 0, one, None) == UNS
+    assert L.qmoe_unsort_sum(one, 1 << 25, 0, one, one, None, 1 << 25, 1, 4096, 0, one, None) == UNS
+    assert L.qmoe_unsort_grad(one, one, 1 << 25, 0, one, one, 1 << 25, 1, 4096, one, one, None) == UNS
+
+
 def test_the_binding_declines_what_is_not_on_the_gpu():
     """Without a GPU tensor every function answers None, and says so where it must not."""
     B = _lib_binding()

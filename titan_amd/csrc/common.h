@@ -15,6 +15,8 @@ int launch_status(const char* what);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+// Does a launch of `blocks` blocks of `threads` exceed what one may hold (a grid's threads are counted in 32 bits)?
+inline bool too_many(int64_t blocks, int64_t threads) { return blocks > (int64_t)0xFFFFFFFF / threads; }
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 }  // namespace qmoe

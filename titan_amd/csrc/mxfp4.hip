@@ -176,7 +176,8 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __re
   __builtin_nontemporal_store(v, out + u);
 }
 
-int check(const void* x, const void* w, const void* s, int dtype, int64_t rows, int64_t K) {
+// per: threads per word of codes
+int check(const void* x, const void* w, const void* s, int dtype, int64_t rows, int64_t K, int per) {
   if (dtype != QMOE_BF16 && dtype != QMOE_FP16 && dtype != QMOE_FP32)
     return qmoe::fail(QMOE_ERR_UNSUPPORTED, "dtype=%d", dtype);
   if (rows < 0 || K < 0) return qmoe::fail(QMOE_ERR_INVALID, "bad sizes rows=%lld K=%lld", (long long)rows, (long long)K);
@@ -185,7 +186,7 @@ int check(const void* x, const void* w, const void* s, int dtype, int64_t rows, 
   if (!x || !w || !s) return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
   if (!qmoe::aligned16(x) || !qmoe::aligned4(w))
     return qmoe::fail(QMOE_ERR_UNSUPPORTED, "the values must be 16-byte aligned, the codes 4-byte aligned");
-  if (rows > (int64_t)0x7FFFFFFF * 128 / (K / 8)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "too many elements");
+  if (rows > ((int64_t)0xFFFFFFFF - 255) / per / (K / 8)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "too many elements");
   return QMOE_OK;
 }
 
@@ -193,7 +194,7 @@ int check(const void* x, const void* w, const void* s, int dtype, int64_t rows, 
 
 extern "C" int qmoe_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t K, uint32_t* w, uint8_t* scales,
                                    void* stream) {
-  const int rc = check(x, w, scales, dtype, rows, K);
+  const int rc = check(x, w, scales, dtype, rows, K, 1);
   if (rc != QMOE_OK || rows == 0 || K == 0) return rc;
   const int64_t words = rows * (K / 8);
   const dim3 grid((unsigned)((words + 255) / 256)), block(256);
@@ -206,7 +207,7 @@ extern "C" int qmoe_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64
 
 extern "C" int qmoe_mxfp4_dequantize(const uint32_t* w, const uint8_t* scales, int64_t rows, int64_t K, int dtype,
                                      void* out, void* stream) {
-  const int rc = check(out, w, scales, dtype, rows, K);
+  const int rc = check(out, w, scales, dtype, rows, K, dtype == QMOE_FP32 ? 2 : 1);
   if (rc != QMOE_OK || rows == 0 || K == 0) return rc;
   const int64_t pieces = rows * (K / 8) * (dtype == QMOE_FP32 ? 2 : 1);
   const dim3 grid((unsigned)((pieces + 255) / 256)), block(256);
@@ -221,7 +222,7 @@ extern "C" int qmoe_mxfp4_dequantize(const uint32_t* w, const uint8_t* scales, i
 extern "C" int qmoe_mxfp4_quantize_lines(const uint16_t* x, int64_t n_x, int64_t K, uint32_t* xq, const uint8_t* scales,
                                          int32_t num_experts, int64_t N, uint32_t* lines, int64_t line_words,
                                          void* stream) {
-  const int rc = check(x, xq, scales, QMOE_BF16, n_x, K);
+  const int rc = check(x, xq, scales, QMOE_BF16, n_x, K, 1);
   if (rc != QMOE_OK) return rc;
   if (num_experts < 0 || N < 0 || line_words < 0) return qmoe::fail(QMOE_ERR_INVALID, "bad sizes");
   if (n_x == 0 || K == 0) return QMOE_OK;
@@ -232,7 +233,7 @@ extern "C" int qmoe_mxfp4_quantize_lines(const uint16_t* x, int64_t n_x, int64_t
   if (!lines || !qmoe::aligned4(lines)) return qmoe::fail(QMOE_ERR_INVALID, "lines must be 4-byte aligned");
   if (line_words < (rows + n_x) * G) return qmoe::fail(QMOE_ERR_WORKSPACE, "lines hold %lld words, %lld are needed", (long long)line_words, (long long)((rows + n_x) * G));
   const int64_t xblocks = (n_x * G + 15) / 16, blocks = xblocks + (rows + 63) / 64;
-  if (blocks > 0x7FFFFFFF) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
+  if (qmoe::too_many(blocks, 256)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
   mx_quantize_lines_kernel<<<dim3((unsigned)blocks), dim3(256), 0, qmoe::as_stream(stream)>>>(
       reinterpret_cast<const uint4*>(x), n_x, K, xq, lines + rows * G, xblocks, scales, rows, N, lines);
   return qmoe::launch_status("mx_quantize_lines_kernel");

@@ -164,11 +164,19 @@ __global__ __launch_bounds__(64 * kTWaves) void mx_qmv_t_kernel(QmvArgs a) {
   }
 }
 
+int too_large(int64_t blocks, int64_t n_rows, int threads) {
+  if (!qmoe::too_many(blocks * n_rows, threads)) return QMOE_OK;
+  return qmoe::fail(QMOE_ERR_UNSUPPORTED, "n_rows=%lld: too many for weights of this size", (long long)n_rows);
+}
+
 template <int LPR, int NR>
-void launch_fwd(const QmvArgs& a, hipStream_t st) {
+int launch_fwd(const QmvArgs& a, hipStream_t st) {
   constexpr int kRows = (64 / LPR) * NR * kWaves;
-  const dim3 grid((unsigned)((a.N + kRows - 1) / kRows), (unsigned)a.n_rows);
-  mx_qmv_kernel<LPR, NR><<<grid, dim3(64 * kWaves), 0, st>>>(a);
+  const int64_t blocks = (a.N + kRows - 1) / kRows;
+  const int rc = too_large(blocks, a.n_rows, 64 * kWaves);
+  if (rc != QMOE_OK) return rc;
+  mx_qmv_kernel<LPR, NR><<<dim3((unsigned)blocks, (unsigned)a.n_rows), dim3(64 * kWaves), 0, st>>>(a);
+  return qmoe::launch_status("mx_qmv_kernel");
 }
 
 }  // namespace
@@ -195,6 +203,8 @@ extern "C" int qmoe_mxfp4_gather_qmv(const uint16_t* x, int64_t n_x, int64_t ldx
   hipStream_t st = qmoe::as_stream(stream);
   if (!transpose) {
     const dim3 grid((unsigned)((K + kTOut - 1) / kTOut), (unsigned)n_rows);
+    const int rc = too_large(grid.x, n_rows, 64 * kTWaves);
+    if (rc != QMOE_OK) return rc;
     mx_qmv_t_kernel<<<grid, dim3(64 * kTWaves), 0, st>>>(a);
     return qmoe::launch_status("mx_qmv_t_kernel");
   }
@@ -207,8 +217,7 @@ extern "C" int qmoe_mxfp4_gather_qmv(const uint16_t* x, int64_t n_x, int64_t ldx
   // the pairs do (one token x top-10 of 1024 x 2048 5.7 / 6.1 us, two 8.9 / 8.2,
   // six 18.9 / 16.2).
   const bool many = n_rows >= 16;
-  if (lpr == 64) many ? launch_fwd<64, 4>(a, st) : launch_fwd<64, 2>(a, st);
-  else if (lpr == 32) many ? launch_fwd<32, 4>(a, st) : launch_fwd<32, 2>(a, st);
-  else many ? launch_fwd<16, 4>(a, st) : launch_fwd<16, 2>(a, st);
-  return qmoe::launch_status("mx_qmv_kernel");
+  if (lpr == 64) return many ? launch_fwd<64, 4>(a, st) : launch_fwd<64, 2>(a, st);
+  if (lpr == 32) return many ? launch_fwd<32, 4>(a, st) : launch_fwd<32, 2>(a, st);
+  return many ? launch_fwd<16, 4>(a, st) : launch_fwd<16, 2>(a, st);
 }

@@ -165,9 +165,12 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(RowsArgs a) {
 }
 
 template <bool QQ, int MT, int BK>
-void launch(const RowsArgs& a, hipStream_t st) {
+int launch(const RowsArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
+  if (qmoe::too_many((int64_t)grid.x * grid.y, 64 * kWaves))
+    return qmoe::fail(QMOE_ERR_UNSUPPORTED, "N=%lld: too large", (long long)a.N);
   mx_rows_kernel<QQ, MT, BK><<<grid, dim3(64 * kWaves), 0, st>>>(a);
+  return qmoe::launch_status("mx_rows_kernel");
 }
 
 }  // namespace
@@ -176,14 +179,10 @@ int qmoe_mx::rows_product(const RowsArgs& a, bool qq, hipStream_t st) {
   // row tiles of 16 as many as there are rows for; batches as long as eight waves' buffers leave room for
   const int mt = (int)((a.M + 15) / 16);
   if (qq) {
-    if (mt <= 1) launch<true, 1, 256>(a, st);
-    else if (mt == 2) launch<true, 2, 256>(a, st);
-    else launch<true, 4, 256>(a, st);
-  } else {
-    if (mt <= 1) launch<false, 1, 256>(a, st);
-    else if (mt == 2) launch<false, 2, 256>(a, st);
-    else if (mt == 3) launch<false, 3, 128>(a, st);
-    else launch<false, 4, 128>(a, st);
+    if (mt <= 1) return launch<true, 1, 256>(a, st);
+    return mt == 2 ? launch<true, 2, 256>(a, st) : launch<true, 4, 256>(a, st);
   }
-  return qmoe::launch_status("mx_rows_kernel");
+  if (mt <= 1) return launch<false, 1, 256>(a, st);
+  if (mt == 2) return launch<false, 2, 256>(a, st);
+  return mt == 3 ? launch<false, 3, 128>(a, st) : launch<false, 4, 128>(a, st);
 }

@@ -194,8 +194,12 @@ __global__ __launch_bounds__(256) void unsort_grad_kernel(const void* __restrict
 
 int size_of(int dtype) { return dtype == QMOE_FP32 ? 4 : dtype == QMOE_BF16 || dtype == QMOE_FP16 ? 2 : 0; }
 
-// Threads for `units` work items along a row: whole waves, at most 256.
-unsigned row_threads(int64_t units) { return (unsigned)(units >= 256 ? 256 : (units + 63) / 64 * 64); }
+// Threads for `units` work items along a row: whole waves, one at least, at most 256.
+unsigned row_threads(int64_t units) { return (unsigned)(units >= 256 ? 256 : units <= 64 ? 64 : (units + 63) / 64 * 64); }
+int too_large(int64_t blocks, unsigned threads) {
+  if (!qmoe::too_many(blocks, threads)) return QMOE_OK;
+  return qmoe::fail(QMOE_ERR_UNSUPPORTED, "too many rows of this length");
+}
 
 template <int IN, int OUT>
 int launch_sum(const void* xs, int64_t n, const int32_t* inv, const float* scores, const int32_t* first, int64_t T,
@@ -207,6 +211,7 @@ int launch_sum(const void* xs, int64_t n, const int32_t* inv, const float* score
   const int64_t cols = (units + threads - 1) / threads;
   if (cols > 65535) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "D=%lld too large", (long long)D);
   const dim3 grid((unsigned)T, (unsigned)cols);
+  if (const int rc = too_large(T * cols, threads)) return rc;
   if (vec) unsort_sum_kernel<IN, OUT, N><<<grid, dim3(threads), 0, st>>>(xs, n, inv, scores, first, k, units, y);
   else unsort_sum_kernel<IN, OUT, 1><<<grid, dim3(threads), 0, st>>>(xs, n, inv, scores, first, k, units, y);
   return qmoe::launch_status("unsort_sum_kernel");
@@ -219,6 +224,7 @@ int launch_grad(const void* dy, const void* xs, int64_t n, const int32_t* inv, c
   const bool vec = D % N == 0;
   const int64_t units = vec ? D / N : D;
   const dim3 grid((unsigned)T), block(row_threads(units));
+  if (const int rc = too_large(T, block.x)) return rc;
   if (vec) unsort_grad_kernel<DT, N><<<grid, block, 0, st>>>(dy, xs, n, inv, scores, k, units, dxs, ds);
   else unsort_grad_kernel<DT, 1><<<grid, block, 0, st>>>(dy, xs, n, inv, scores, k, units, dxs, ds);
   return qmoe::launch_status("unsort_grad_kernel");
@@ -239,6 +245,7 @@ extern "C" int qmoe_sort_rows(const void* x, int64_t T, const int32_t* inv, int6
   const int unit = bytes % 16 == 0 ? 16 : size;
   const int64_t units = bytes / unit;
   const dim3 grid((unsigned)T), block(row_threads(units));
+  if (const int rc = too_large(T, block.x)) return rc;
   hipStream_t st = qmoe::as_stream(stream);
   const int k = (int)top_k;
   if (unit == 16)

@@ -516,5 +516,7 @@ PYBIND11_MODULE(_binding, m) {
   m.def("unsort_tokens", &unsort_tokens);
   m.def("matmul", &matmul);
   m.def("gather", &gather);
-  m.def("rows_product", &rows_product);
+  m.def("rows_product", &rows_product, py::arg("x"), py::arg("w"), py::arg("s"), py::arg("x_rows"), py::arg("div"),
+        py::arg("experts"), py::arg("tiles"), py::arg("n"), py::arg("transpose"), py::arg("qq"),
+        py::arg("inv") = py::none());
 }
