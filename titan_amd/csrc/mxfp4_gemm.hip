@@ -52,9 +52,18 @@ __device__ __forceinline__ qmoe_gemm::TileRows tile_of(const GemmArgs& a, int64_
 // tile's rows and 128 of the outputs, so weights are converted twice per tile
 // and activations read twice from LDS (one by four would halve the first and
 // double the second, and LDS reads are the scarcer: at 128 B a clock and CU
-// they take 55% of the matrix cores' time as it is).  Blocks are persistent,
-// two per CU, and take the units heavy-first (gemm_common.h).  Tiles of at
-// most 64 rows run with half the row subtiles.
+// they take 55% of the matrix cores' time as it is; measured, either way takes
+// 61 us for 4096 x 2048 x 4096).  Blocks are persistent, two per CU, and take
+// the units heavy-first (gemm_common.h).  Shorter tiles run in forms of 32, 64
+// and 96 rows (the last up to 128 in steps of 32; both mxfp4: 64 and 128): with
+// 64 and 128 alone 40,960 rows of 256 experts pay for 20% more rows than they
+// have, with these for 10%.
+//
+// What bounds it: a product of 68.7 GFLOP takes 61 us (1.1 PFLOP/s) forward,
+// 72 to 80 transposed, both at the card's power limit (a loop of nothing but
+// these instructions runs at 1.8 GHz of 2.4): blocks alone on their CU are as
+// fast as two, copies five groups ahead as fast as three.  4096^3 in mxfp4
+// takes 49 us (2.8 PFLOP/s), bound by the copies into LDS.
 //
 // Operands reach LDS by asynchronous copies into a ring of NS stages and are
 // read from there as matrix fragments; the fragments of a step are prepared
@@ -499,7 +508,9 @@ struct Fwd {
 // output that the matrix instruction wants.  With v_mfma_f32_16x16x32 the
 // sixteen words of a wave's 128 outputs are the sixteen lanes of a quarter
 // wave and the four quarters the four octets of n, so no value crosses lanes:
-// the sixteen outputs of subtile j are 8c + j, c = 0 .. 15.
+// the sixteen outputs of subtile j are 8c + j, c = 0 .. 15.  Eight conversions
+// and eight permutes go with eight products of 64 rows, spread between them (in
+// runs of their own: 1 to 2% slower).
 template <bool S4, int MSUB, bool SPLIT>  // MSUB: 16-row subtiles per wave
 struct Trn {
   typedef Geo<SPLIT> Way;
@@ -592,15 +603,12 @@ struct Trn {
     }
     return r;
   }
-  // Fragments of outputs 8c + 2T and 8c + 2T + 1.
+  // Four values of the fragments of outputs 8c + 2T and 8c + 2T + 1, those of rows n 2i and 2i + 1.
   template <int T>
-  static __device__ __forceinline__ void pair(const Words& q, i32x4_t (&b)[2]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = pair_of<T>(q.w[2 * i], q.s[2 * i]), hi = pair_of<T>(q.w[2 * i + 1], q.s[2 * i + 1]);
-      b[0][i] = (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u);
-      b[1][i] = (int)__builtin_amdgcn_perm(hi, lo, 0x07060302u);
-    }
+  static __device__ __forceinline__ void pair(const Words& q, int i, i32x4_t (&b)[2]) {
+    const uint32_t lo = pair_of<T>(q.w[2 * i], q.s[2 * i]), hi = pair_of<T>(q.w[2 * i + 1], q.s[2 * i + 1]);
+    b[0][i] = (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    b[1][i] = (int)__builtin_amdgcn_perm(hi, lo, 0x07060302u);
   }
   static __device__ __forceinline__ void read_x(const Ctx& c, const char* smem, int g, int s, int row0,
                                                 i32x4_t (&f)[MSUB]) {
@@ -610,32 +618,40 @@ struct Trn {
     for (int i = 0; i < MSUB; ++i)
       f[i] = *reinterpret_cast<const i32x4_t*>(st + (16 * i + l16) * 128 + ((4 * s + q) ^ swz8(l16)) * 16);
   }
+  // The products of outputs 8c + 2t and 8c + 2t + 1, with `pieces` calls of more(i) spread between them.
+  template <int PIECES, class More>
   static __device__ __forceinline__ void products(const i32x4_t (&x)[MSUB], const i32x4_t (&b)[2],
-                                                  f32x4_t (&acc)[MSUB][8], int t) {
+                                                  f32x4_t (&acc)[MSUB][8], int t, More more) {
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
+    for (int m = 0; m < 2 * MSUB; ++m) {
+      const int v = m / MSUB, i = m % MSUB;
+      acc[i][2 * t + v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b[v]),
+                                                                  __builtin_bit_cast(bf16x8_t, x[i]),
+                                                                  acc[i][2 * t + v], 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < MSUB; ++i)
-        acc[i][2 * t + v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b[v]),
-                                                                    __builtin_bit_cast(bf16x8_t, x[i]),
-                                                                    acc[i][2 * t + v], 0, 0, 0);
+      for (int p = 0; p < PIECES; ++p)
+        if (p * 2 * MSUB / PIECES == m) more(p);
+      if (PIECES) __builtin_amdgcn_sched_barrier(0);
+    }
   }
-  // One step: the pairs of outputs in turn, each prepared during the one before.  next() reads the next step's
-  // words and activations, late, when the current words are used up: 128 accumulators leave few registers.
+  // One step, its first outputs' fragments in b0: the others are prepared during the first half of its products, so
+  // that the current words are used up when next() reads the next step's words and activations, and the next step's
+  // first fragments, into b1, during the last quarter.
   template <class Next>
   static __device__ __forceinline__ void step(const i32x4_t (&x)[MSUB], Words& w, i32x4_t (&b0)[2], i32x4_t (&b1)[2],
-                                              f32x4_t (&acc)[MSUB][8], Next next) {
-    pair<1>(w, b1);
-    products(x, b0, acc, 0);
-    pair<2>(w, b0);
-    products(x, b1, acc, 1);
-    pair<3>(w, b1);
-    __builtin_amdgcn_sched_barrier(0);
+                                              i32x4_t (&b2)[2], f32x4_t (&acc)[MSUB][8], Next next) {
+    products<6>(x, b0, acc, 0, [&](int p) {
+      if (p < 4) pair<1>(w, p, b1);
+      else pair<2>(w, p - 4, b2);
+    });
+    products<6>(x, b1, acc, 1, [&](int p) {
+      if (p < 2) pair<2>(w, p + 2, b2);
+      else pair<3>(w, p - 2, b0);
+    });
     next();
-    products(x, b0, acc, 2);
-    pair<0>(w, b0);
-    products(x, b1, acc, 3);
+    products<0>(x, b2, acc, 2, [](int) {});
     __builtin_amdgcn_sched_barrier(0);
+    products<4>(x, b0, acc, 3, [&](int p) { pair<0>(w, p, b1); });
   }
 
   static __device__ __forceinline__ void run(const GemmArgs& a, const Unit& u, char* block_smem) {
@@ -675,16 +691,17 @@ struct Trn {
     for (int i = 0; i < NS; ++i) copy(c, min(g0 + i, G - 1));
     qmoe_gemm::wait_vmem<(NS - 1) * kCopies>();
     Way::barrier();
-    i32x4_t xa[MSUB], xb[MSUB], b0[2], b1[2];
+    i32x4_t xa[MSUB], xb[MSUB], b0[2], b1[2], b2[2];
     Words w = read_words(c, smem, g0, 0, wn);
     read_x(c, smem, g0, 0, row0, xa);
-    pair<0>(w, b0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pair<0>(w, i, b0);
     for (int g = g0; g < G - 1; ++g) {
-      step(xa, w, b0, b1, acc, [&] {
+      step(xa, w, b0, b1, b2, acc, [&] {
         w = read_words(c, smem, g, 1, wn);
         read_x(c, smem, g, 1, row0, xb);
       });
-      step(xb, w, b0, b1, acc, [&] {
+      step(xb, w, b1, b0, b2, acc, [&] {
         // group g + 1 landed (copies of NS - 2 groups after it may be in flight); all reads of stage g are done
         qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -694,11 +711,11 @@ struct Trn {
         read_x(c, smem, g + 1, 0, row0, xa);
       });
     }
-    step(xa, w, b0, b1, acc, [&] {
+    step(xa, w, b0, b1, b2, acc, [&] {
       w = read_words(c, smem, G - 1, 1, wn);
       read_x(c, smem, G - 1, 1, row0, xb);
     });
-    step(xb, w, b0, b1, acc, [] {});
+    step(xb, w, b1, b0, b2, acc, [] {});
     }
     qmoe_gemm::wait_vmem<0>();
     const int lane = fresh_tid() % 64, l16 = lane % 16, q = lane / 16;
@@ -1085,10 +1102,10 @@ void launch_way(const GemmArgs& a, int64_t max_tiles, hipStream_t st) {
 }
 
 // Wide units from this many on: below, split ones are faster.  At 64, 128 and
-// 256 wide units (us, wide / split; 512 to 4096 rows of 4096 x 2048 and 1024 x
-// 2048 weights): forward 35.6 / 20.3, 37.5 / 36.9, 41.6 / 68.0; transposed
-// 74.8 / 28.2, 75.6 / 54.8, 83.0 / 102.9; both mxfp4 18.6 / 15.9, 19.9 / 27.3,
-// 22.3 / 46.9.
+// 256 wide units of 4096 x 2048 weights (us, wide / split): forward 29.9 / 18.4,
+// 31.0 / 32.0, 33.6 / 56.4; transposed 69.6 / 26.0, 69.6 / 46.5
+// (256 units of 1024 x 2048: 24.2 / 41.7); both mxfp4 17.1 / 15.0, 17.7 / 25.3,
+// 18.6 / 43.7 (at 96 units 17.5 / 24.6).
 constexpr int64_t kWideUnits = 160, kWideUnitsQQ = 96;
 
 template <int MODE>

@@ -12,6 +12,9 @@
 // lane / 16) holds block q of four of row n: v_mfma_f32_16x16x32_bf16 takes a
 // word of it at a time, converted, against the same columns of x;
 // v_mfma_scale_f32_16x16x128_f8f6f4 (QQ) the block as it is against x's codes.
+//
+// Bound by the two or three dependent round trips to HBM of a launch: 4096 x
+// 2048 weights (4.5 MB) take 4.7 us at 5 rows, 6.7 at 32, 8.6 at 64 in a graph.
 #include "gemm_common.h"
 #include "mxfp4.h"
 #include "mxfp4_rows.h"

@@ -10,8 +10,10 @@
 // Sums run in fp32 in slot order, whatever the rows' type, and are rounded
 // once; nothing is added atomically, so results do not depend on timing.
 // All of it is bound by memory: every row is read once and written once, and
-// the gradients of a token's k rows are formed together, so that dy[t] is read
-// once for the k of them.
+// work goes by token, so that x[t] and dy[t] are read once for its k rows.  4096
+// tokens x top-10 of 2048 bf16: the sort 34 us (5.4 TB/s; one wave per sorted
+// row, which reads x[t] k times, 44), each sum 33 us (5.6 TB/s), both gradients
+// of the way back 75 us (4.7 TB/s).
 //
 // A thread takes 16 bytes of a row where the row length is a multiple of 16
 // bytes, one element otherwise (VEC).
