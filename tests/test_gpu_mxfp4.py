@@ -591,3 +591,105 @@ def test_refuses_forward_mode(dev):
                      lambda: ops.unsort_tokens(d, one, one, torch.ones(2, 1, device=dev))):
             with pytest.raises(NotImplementedError, match="forward"):
                 call()
+
+
+# ------------------------------------------------- offsets past 32 bits
+
+
+@pytest.fixture
+def room(dev):
+    """These tests hold 10 to 25 GB for a moment."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("less than 40 GiB of GPU memory free")
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_experts_past_four_gigabytes(dev, room, rows):
+    say("experts past 4 GB", rows)
+    E, N, K = 1100, 1024, 8192
+    g = torch.Generator(device=dev).manual_seed(5)
+    w = torch.randint(-(1 << 31), 1 << 31, (E, N, K // 8), generator=g, device=dev, dtype=torch.int32)
+    s = torch.randint(116, 124, (E, N, K // 32), generator=g, device=dev, dtype=torch.int32).to(torch.uint8)
+    assert w.numel() * 4 > 1 << 32
+    used = torch.tensor([0, 511, 1030, 1099])  # the last two lie behind it
+    e = torch.sort(used[torch.randint(0, 4, (rows,), generator=_gen(3))])[0]
+    e[-1] = 1099
+    W = dequantize_ref(w[used.to(dev)], s[used.to(dev)])
+    at = (e.unsqueeze(1) == used).int().argmax(1)
+    for transpose, C in ((True, K), (False, N)):
+        x = _acts(_gen(9), rows, C)
+        for is_sorted in (True, False):
+            y = ops.gather_qmm(x.to(dev).unsqueeze(1), w, s, rhs_indices=e.to(dev), transpose=transpose, mode="mxfp4",
+                               sorted_indices=is_sorted)
+            check_sum(y.squeeze(1), *_by_expert(x, W, at, transpose), C)
+    x = _acts(_gen(9), rows, K)
+    y = ops.gather_qqmm(x.to(dev).unsqueeze(1), w, s, rhs_indices=e.to(dev), sorted_indices=True)
+    check_sum(y.squeeze(1), *_by_expert(quantize_ref(x)[0], W, at, True), K)
+
+
+def test_rows_past_four_gigabytes(dev, room):
+    say("rows past 4 GB")
+    M, N, K = 300_000, 8192, 32
+    w, s = codes(_gen(51), N, K)
+    W, wd, sd = dequantize_ref(w, s), w.to(dev), s.to(dev)
+    some = torch.tensor([0, 131_071, 262_144, 262_145, M - 1])
+    few = _acts(_gen(53), len(some), K)
+    x = torch.zeros(M, K, dtype=BF, device=dev)
+    x[some.to(dev)] = few.to(dev)
+    for y, v in ((ops.quantized_matmul(x, wd, sd, mode="mxfp4"), few), (ops.qqmm(x, wd, sd), quantize_ref(few)[0])):
+        check_sum(y[some.to(dev)], *_dense(v, W, True), K)
+        assert not y[1:131_071].any()
+        del y
+    few = _acts(_gen(57), len(some), N)
+    x = torch.zeros(M, N, dtype=BF, device=dev)
+    x[some.to(dev)] = few.to(dev)
+    y = ops.quantized_matmul(x, wd, sd, transpose=False, mode="mxfp4")
+    check_sum(y[some.to(dev)], *_dense(few, W, False), N)
+    q, b = ops.quantize(x)
+    ref, ref_b = quantize_ref(few)
+    assert torch.equal(b[some.to(dev)].cpu(), ref_b)
+    back = ops.dequantize(q, b, mode="mxfp4", dtype=torch.float32)
+    assert torch.equal(back[some.to(dev)].cpu().double(), ref) and not back[1:131_071].any()
+
+
+def test_two_threads_at_once(dev):
+    """Calls with gradients from two threads, each on a stream of its own, agree with the same calls alone."""
+    import threading
+
+    say("threads")
+    w, s = (t.to(dev) for t in codes(_gen(61), 6, 72, 96))
+    e = torch.sort(torch.randint(0, 6, (150,), generator=_gen(62)))[0].to(torch.int32).to(dev)
+    xs = [_acts(_gen(63 + i), 150, 96).to(dev) for i in range(2)]
+    dy = _acts(_gen(65), 150, 72).to(dev)
+
+    def step(x):
+        x = x.detach().requires_grad_(True)
+        y = ops.gather_qmm(x.unsqueeze(1), w, s, rhs_indices=e, mode="mxfp4", sorted_indices=True)
+        z = ops.gather_qqmm(x.detach().unsqueeze(1), w, s, rhs_indices=e, sorted_indices=True)
+        return y.detach(), z, torch.autograd.grad(y, x, dy.unsqueeze(1))[0]
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i].append(step(xs[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as err:  # noqa: BLE001 - reported by the test's own thread
+            errors.append(err)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i in range(2):
+        assert len(got[i]) == 20
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))

@@ -197,3 +197,33 @@ def test_second_derivatives_are_refused(dev):
     assert torch.equal(dx.cpu(), 2 * 2 * x)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.sum().backward()
+
+
+def test_rows_past_four_gigabytes(dev):
+    """Sorted rows of 5 GB, there and back and their gradients, with a weight of one on each slot."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("less than 40 GiB of GPU memory free")
+    T, k, D = 150_000, 8, 2048
+    g = torch.Generator(device=dev).manual_seed(3)
+    ids = torch.randint(0, 64, (T, k), generator=g, device=dev, dtype=torch.int32)
+    r = ops.route(ids, 64)
+    x = torch.randn(T, D, generator=g, device=dev).to(torch.bfloat16)
+    xs = ops.sort_tokens(x, r.order, r.inv_order)
+    assert xs.numel() * 2 > 1 << 32
+    some = torch.tensor([0, 1, T * k // 2, T * k - 2, T * k - 1], device=dev)
+    assert torch.equal(xs[some], x[r.order.long()[some] // k])
+    scores = torch.zeros(T, k, device=dev)
+    scores[:, k - 1] = 2.0
+    xs.requires_grad_(True)
+    scores.requires_grad_(True)
+    y = ops.unsort_tokens(xs, r.order, r.inv_order, scores)
+    assert torch.equal(y, 2 * x)
+    dxs, ds = torch.autograd.grad(y, (xs, scores), x)
+    last = r.order.long() % k == k - 1
+    assert torch.equal(dxs[some], torch.where(last[some, None], 2 * x[r.order.long()[some] // k], 0))
+    # each slot's row is the token's: the same dot product, D fp32 terms that are all positive
+    want = x[-3:].double().square().sum(-1)
+    assert ((ds[-3:].double() - want[:, None]).abs() <= (D + 8) * 2.0 ** -24 * want[:, None]).all()
+    assert torch.equal(ds, ds[:, :1].expand(T, k))
+    del xs, dxs, y
+    torch.cuda.empty_cache()
