@@ -133,6 +133,19 @@ def test_quantized_matmul(dev, M, K, N, transpose):
     check_sum(got, ref, mag, x.shape[1], (M, K, N, transpose))
 
 
+@pytest.mark.parametrize("K", [1056, 2080, 2176, 2560, 3200, 4128, 6144])
+@pytest.mark.parametrize("M", [5, 23, 40, 64])
+def test_few_rows_past_whole_rounds(dev, M, K):
+    """Contractions that end in every part of a round of the waves' batches, both kinds of activations."""
+    say("few rows", M, K)
+    g = _gen(67)
+    w, s = codes(g, 35, K)
+    x = _acts(g, M, K)
+    W = dequantize_ref(w, s)
+    check_sum(ops.quantized_matmul(x.to(dev), w.to(dev), s.to(dev), mode="mxfp4"), *_dense(x, W, True), K)
+    check_sum(ops.qqmm(x.to(dev), w.to(dev), s.to(dev)), *_dense(quantize_ref(x)[0], W, True), K)
+
+
 @pytest.mark.parametrize("transpose", [True, False])
 @pytest.mark.parametrize("shape", [(0,), (3, 0), (2, 5), (1, 1, 70)])
 def test_quantized_matmul_batch_shapes(dev, shape, transpose):

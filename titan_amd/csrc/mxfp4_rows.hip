@@ -8,13 +8,13 @@
 // whole lines of each row, into a buffer of its own (read straight into the
 // matrix instructions' layout, 16 rows under 16 neighbouring lanes, a load
 // costs its lanes a cycle each), so nothing waits on a barrier, and with K =
-// 2048 all of a call's bytes are requested at once.  Lane (n = lane % 16, q =
+// 2048 all of a call's bytes are requested in one or two rounds.  Lane (n = lane % 16, q =
 // lane / 16) holds block q of four of row n: v_mfma_f32_16x16x32_bf16 takes a
 // word of it at a time, converted, against the same columns of x;
 // v_mfma_scale_f32_16x16x128_f8f6f4 (QQ) the block as it is against x's codes.
 //
 // Bound by the two or three dependent round trips to HBM of a launch: 4096 x
-// 2048 weights (4.5 MB) take 4.7 us at 5 rows, 6.7 at 32, 8.6 at 64 in a graph.
+// 2048 weights (4.5 MB) take 4.7 us at 5 rows, 5.7 at 32, 8.6 at 64 in a graph.
 #include "gemm_common.h"
 #include "mxfp4.h"
 #include "mxfp4_rows.h"
@@ -179,13 +179,15 @@ int launch(const RowsArgs& a, hipStream_t st) {
 }  // namespace
 
 int qmoe_mx::rows_product(const RowsArgs& a, bool qq, hipStream_t st) {
-  // row tiles of 16 as many as there are rows for; batches as long as eight waves' buffers leave room for
+  // Row tiles of 16 as many as there are rows for.  Batches of 256 where two blocks still fit a CU: with one, blocks
+  // past the 256th wait for a round of their own (23 rows, batches of 256 / 128: 4099 x 2080 10.2 / 6.8 us, 8192 x
+  // 2048 10.7 / 7.6, 4096 x 2048 6.2 / 5.6; in smaller forms either is within 8% of the other).
   const int mt = (int)((a.M + 15) / 16);
   if (qq) {
     if (mt <= 1) return launch<true, 1, 256>(a, st);
     return mt == 2 ? launch<true, 2, 256>(a, st) : launch<true, 4, 256>(a, st);
   }
   if (mt <= 1) return launch<false, 1, 256>(a, st);
-  if (mt == 2) return launch<false, 2, 256>(a, st);
+  if (mt == 2) return launch<false, 2, 128>(a, st);
   return mt == 3 ? launch<false, 3, 128>(a, st) : launch<false, 4, 128>(a, st);
 }
