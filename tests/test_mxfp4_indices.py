@@ -1,0 +1,36 @@
+"""Which activation row and which expert each output row of a gather call takes,
+on the CPU: the rows before any launch, where the kernels clamp what is left."""
+
+import pytest
+import torch
+
+from titan_amd import mxfp4, ops
+
+BF = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def on_the_cpu(monkeypatch):
+    monkeypatch.setattr(ops, "_dev", lambda t, name: None)
+
+
+def _taken(x, E, lhs, rhs):
+    """(activation row, expert) of each output row as the kernels read them."""
+    _, rows, order = mxfp4._gathered(x, E, lhs, rhs, False, None, 1 << 40)
+    assert order is None
+    n_x = x[..., 0].numel()
+    xr = mxfp4._x_rows(rows, x.device)
+    xr = torch.arange(rows.n, dtype=torch.int32) if xr is None else xr
+    assert xr.dtype == rows.experts.dtype == torch.int32
+    return xr.clamp(0, n_x - 1).tolist(), rows.experts.clamp(0, E - 1).tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64, torch.int16])
+@pytest.mark.parametrize("M", [1, 2, 5])
+def test_an_index_out_of_range_takes_the_nearest_batch(M, dtype):
+    """All M rows of the nearest batch of x, not its nearest row M times."""
+    B, E = 4, 3
+    lhs, rhs = [4, -1, 2, 9, -7, 3, 0], [0, 1, 2, 3, -1, 0, 7]
+    got = _taken(torch.zeros(B, M, 32, dtype=BF), E, torch.tensor(lhs, dtype=dtype), torch.tensor(rhs, dtype=dtype))
+    assert got == ([min(max(i, 0), B - 1) * M + m for i in lhs for m in range(M)],
+                   [min(max(i, 0), E - 1) for i in rhs for _ in range(M)])

@@ -202,6 +202,8 @@ def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
     experts = _flat(rhs, batch)
     if M != 1 and nb:  # rows of one batch index: M activation rows, one expert
         ar = torch.arange(M, device=dev, dtype=torch.int32)
+        if lhs is not None:  # clamped here as a batch: the kernels clamp each of its rows
+            x_rows = x_rows.clamp(0, max(math.prod(x.shape[:-2]) - 1, 0))
         base = x_rows if x_rows is not None else None if div == 1 else _x_rows(_Rows(nb, None, div), dev)
         x_rows = None if base is None else (base[:, None] * M + ar).reshape(-1)
         div = 1
