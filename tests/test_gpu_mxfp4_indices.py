@@ -50,3 +50,24 @@ def test_batches_of_several_rows(dev, M, n, is_sorted):
     ref, mag = _by_expert(dy, W.transpose(1, 2), ei)
     zero = torch.zeros(B, M, K, dtype=torch.float64)
     check_sum(dx, zero.index_add(0, xi, ref), zero.index_add(0, xi, mag), N + n)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint32, torch.uint64])
+@pytest.mark.parametrize("n", [5, 90])
+def test_past_32_bits(dev, n, dtype):
+    say("past 32 bits", n, dtype)
+    g = _gen(n)
+    E, K, N = 4, 64, 40
+    w, s = codes(g, E, N, K)
+    W = dequantize_ref(w, s).transpose(1, 2)
+    x = torch.randn(n, 1, K, generator=g).to(BF)
+    far = (1 << 31) + 1 if dtype == torch.uint32 else (1 << 32) + 1
+    e = torch.sort(torch.randint(0, E, (n,), generator=g))[0]
+    lhs = torch.randint(0, n, (n,), generator=g)
+    e[-2:] = far
+    lhs[1] = far
+    xi, ei = lhs.clamp(0, n - 1), e.clamp(0, E - 1)
+    for is_sorted in (True, False):
+        kw = {"lhs_indices": lhs.to(dtype).to(dev), "rhs_indices": e.to(dtype).to(dev), "sorted_indices": is_sorted}
+        check_sum(ops.gather_qmm(x.to(dev), w.to(dev), s.to(dev), mode="mxfp4", **kw), *_by_expert(x[xi], W, ei), K)
+        check_sum(ops.gather_qqmm(x.to(dev), w.to(dev), s.to(dev), **kw), *_by_expert(quantize_ref(x)[0][xi], W, ei), K)

@@ -34,3 +34,30 @@ def test_an_index_out_of_range_takes_the_nearest_batch(M, dtype):
     got = _taken(torch.zeros(B, M, 32, dtype=BF), E, torch.tensor(lhs, dtype=dtype), torch.tensor(rhs, dtype=dtype))
     assert got == ([min(max(i, 0), B - 1) * M + m for i in lhs for m in range(M)],
                    [min(max(i, 0), E - 1) for i in rhs for _ in range(M)])
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint32, torch.uint64])
+@pytest.mark.parametrize("M", [1, 3])
+def test_an_index_past_32_bits_takes_the_last_batch(M, dtype):
+    """What 32 bits do not hold is out of range, not some other index."""
+    B, E = 4, 3
+    far = [1 << 31, (1 << 31) + 1, (1 << 32) - 1]
+    if dtype != torch.uint32:
+        far += [1 << 32, (1 << 32) + 2, (1 << 62) + 1]
+    if dtype == torch.uint64:
+        far += [1 << 63, (1 << 64) - 1]
+    t = lambda v: torch.tensor(v, dtype=dtype)  # noqa: E731
+    n = len(far)
+    got = _taken(torch.zeros(B, M, 32, dtype=BF), E, t([*far, 1]), t([*far, 2]))
+    assert got == ([B * M - M + m for _ in far for m in range(M)] + list(range(M, 2 * M)), [E - 1] * (n * M) + [2] * M)
+    if dtype == torch.int64:
+        got = _taken(torch.zeros(B, M, 32, dtype=BF), E, t([-i for i in far]), t([-i for i in far]))
+        assert got == (list(range(M)) * n, [0] * (n * M))
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.uint16])
+def test_narrow_indices(dtype):
+    B, E = 300, 400
+    v = [0, 5, 100]
+    t = torch.tensor(v, dtype=dtype)
+    assert _taken(torch.zeros(B, 2, 32, dtype=BF), E, t, t) == ([2 * i + m for i in v for m in (0, 1)], [i for i in v for _ in (0, 1)])

@@ -157,10 +157,9 @@ def _broadcast(a, b) -> tuple:
     return tuple(j if i == 1 else i for i, j in zip(a, b))
 
 
-def _flat(t, batch):
-    """Indices over the batch as a contiguous int32 vector."""
-    if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+def _flat(t, batch, n):
+    """Indices into ``n`` over the batch as a contiguous int32 vector."""
+    t = ops._narrow(t, n)
     if t.shape != batch:
         t = t.expand(batch)
     return ops._ready(t if t.dim() == 1 else t.reshape(-1))
@@ -198,12 +197,12 @@ def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
         ops._same_device(lhs, "lhs_indices", dev)
         batch = lhs.shape if lhs.shape == rhs.shape else torch.Size(_broadcast(lhs.shape, rhs.shape))
         nb = math.prod(batch)
-        x_rows = _flat(lhs, batch)
-    experts = _flat(rhs, batch)
+        x_rows = _flat(lhs, batch, math.prod(xb))
+    experts = _flat(rhs, batch, E)
     if M != 1 and nb:  # rows of one batch index: M activation rows, one expert
         ar = torch.arange(M, device=dev, dtype=torch.int32)
         if lhs is not None:  # clamped here as a batch: the kernels clamp each of its rows
-            x_rows = x_rows.clamp(0, max(math.prod(x.shape[:-2]) - 1, 0))
+            x_rows = x_rows.clamp(0, max(math.prod(xb) - 1, 0))
         base = x_rows if x_rows is not None else None if div == 1 else _x_rows(_Rows(nb, None, div), dev)
         x_rows = None if base is None else (base[:, None] * M + ar).reshape(-1)
         div = 1
