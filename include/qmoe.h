@@ -143,7 +143,8 @@ int qmoe_build_tiles(const int32_t* sorted_ids, int64_t n_rows,
                      int32_t* tile_row, int32_t* tile_exp, int32_t* ntiles,
                      int64_t max_tiles, void* stream);
 /* The same with every row in a tile: ids below 0 count as expert 0, ids from
- * num_experts on as the last one (qmoe_build_tiles leaves their rows out). */
+ * num_experts on as the last one (qmoe_build_tiles leaves their rows out, and
+ * the products leave those rows of their results as they were). */
 int qmoe_build_tiles_clamped(const int32_t* sorted_ids, int64_t n_rows,
                              int32_t num_experts, int32_t tile_rows,
                              int32_t* offsets, int32_t* tile_row,

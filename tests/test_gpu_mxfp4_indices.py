@@ -71,3 +71,41 @@ def test_past_32_bits(dev, n, dtype):
         kw = {"lhs_indices": lhs.to(dtype).to(dev), "rhs_indices": e.to(dtype).to(dev), "sorted_indices": is_sorted}
         check_sum(ops.gather_qmm(x.to(dev), w.to(dev), s.to(dev), mode="mxfp4", **kw), *_by_expert(x[xi], W, ei), K)
         check_sum(ops.gather_qqmm(x.to(dev), w.to(dev), s.to(dev), **kw), *_by_expert(quantize_ref(x)[0][xi], W, ei), K)
+
+
+@pytest.mark.parametrize("n", [64, 300])
+def test_with_a_table_of_the_callers(dev, n):
+    """Rows whose ids are out of range are in the table too: computed, none left as its memory was."""
+    say("table", n)
+    g = _gen(n)
+    E, K, N = 4, 64, 40
+    w, s = codes(g, E, N, K)
+    W = dequantize_ref(w, s).transpose(1, 2)
+    x, dy = torch.randn(n, 1, K, generator=g).to(BF), torch.randn(n, 1, N, generator=g).to(BF)
+    for e in (torch.sort(torch.randint(-3, E + 3, (n,), generator=g))[0], torch.full((n,), -1), torch.full((n,), E),
+              torch.cat([torch.zeros(n - 2, dtype=torch.int64), torch.tensor([1 << 31, (1 << 32) + 1])])):
+        ei = e.clamp(0, E - 1)
+        for ids in (e, e.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)):
+            tiles = ops.build_tiles(ids.to(dev), E)
+            for width in (N, K):  # what the results' memory held before
+                torch.full((n, width), float("nan"), dtype=BF, device=dev)
+            xd = x.to(dev).requires_grad_(True)
+            y = ops.gather_qmm(xd, w.to(dev), s.to(dev), rhs_indices=ids.to(dev), mode="mxfp4", sorted_indices=True, tiles=tiles)
+            check_sum(y, *_by_expert(x, W, ei), K)
+            (dx,) = torch.autograd.grad(y, xd, dy.to(dev))
+            check_sum(dx, *_by_expert(dy, W.transpose(1, 2), ei), N)
+            q = ops.gather_qqmm(x.to(dev), w.to(dev), s.to(dev), rhs_indices=ids.to(dev), sorted_indices=True, tiles=tiles)
+            check_sum(q, *_by_expert(quantize_ref(x)[0], W, ei), K)
+
+
+def test_a_table_covers_every_row(dev):
+    say("tables")
+    for ids, E in (([-5, -1, 0, 2, 2, 3, 9], 4), ([7] * 130, 3), ([-1] * 130, 3), ([], 3), ([1, 1], 1)):
+        t = ops.build_tiles(torch.tensor(ids, dtype=torch.int32, device=dev), E)
+        inside = torch.tensor(ids, dtype=torch.int64).clamp(0, E - 1)
+        want = torch.searchsorted(inside, torch.arange(E + 1))
+        assert t.offsets.tolist() == want.tolist()
+        k = int(t.ntiles)
+        rows = [(int(r) + i, int(x)) for r, x in zip(t.tile_row[:k], t.tile_exp[:k])
+                for i in range(min(t.tile_rows, int(want[int(x) + 1]) - int(r)))]
+        assert rows == list(enumerate(inside.tolist()))

@@ -213,7 +213,7 @@ def _gathered(x, E, lhs, rhs, sorted_indices, tiles, min_rows):
     if n >= min_rows:
         if sorted_indices:
             if tiles is None or tiles.rows != n:
-                tiles = ops.build_tiles(experts.clamp(0, E - 1), E)
+                tiles = ops.build_tiles(experts, E)
             elif tiles.num_experts != E or tiles.tile_rows != ops.tile_rows():
                 raise ValueError("tile table does not match this call")
         else:

@@ -196,10 +196,11 @@ class Routing:
 
 
 def build_tiles(sorted_ids: torch.Tensor, num_experts: int, tile_rows_: int | None = None) -> TileTable:
-    """Tile table over ids already sorted ascending."""
+    """Tile table over ids already sorted ascending.  Every row is in it: ids out
+    of range count as the nearest expert's, as :func:`route` has them."""
     _dev(sorted_ids, "sorted_ids")
     dev = sorted_ids.device
-    ids = _i32(sorted_ids.reshape(-1), "sorted_ids", dev)
+    ids = _ready(_narrow(sorted_ids.reshape(-1), num_experts))
     tr = tile_rows() if tile_rows_ is None else int(tile_rows_)
     n = ids.numel()
     mt = max_tiles(n, num_experts, tr)
@@ -207,7 +208,7 @@ def build_tiles(sorted_ids: torch.Tensor, num_experts: int, tile_rows_: int | No
     trow = torch.empty(mt, dtype=torch.int32, device=dev)
     texp = torch.empty(mt, dtype=torch.int32, device=dev)
     nt = torch.empty(1, dtype=torch.int32, device=dev)
-    _lib.call("qmoe_build_tiles", ids.data_ptr(), n, num_experts, tr, offsets.data_ptr(),
+    _lib.call("qmoe_build_tiles_clamped", ids.data_ptr(), n, num_experts, tr, offsets.data_ptr(),
               trow.data_ptr(), texp.data_ptr(), nt.data_ptr(), mt, _stream(ids))
     return TileTable(offsets, trow, texp, nt, mt, tr, num_experts, n)
 
