@@ -47,6 +47,7 @@ struct Failure : std::runtime_error {
   int code;
   Failure(int c, const char* what)
       : std::runtime_error(std::string(what) + ": " + qmoe_last_error() + " (code " + std::to_string(c) + ")"), code(c) {}
+  explicit Failure(const char* refused) : std::runtime_error(refused), code(QMOE_ERR_UNSUPPORTED) {}
 };
 void ok(int rc, const char* what) {
   if (rc != QMOE_OK) throw Failure(rc, what);
@@ -479,6 +480,8 @@ py::object rows_product(const Tensor& x, const Tensor& w, const Tensor& s, const
                         int64_t div, const std::optional<Tensor>& experts,
                         const std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, int64_t>>& tiles, int64_t n,
                         bool transpose, bool qq, const std::optional<Tensor>& inv) {
+  if (records(x) && qq)
+    throw Failure("the products of quantised activations have no gradient: detach x, or use quantized_matmul / gather_qmm");
   Weights g{w, s, w.size(0), w.size(1), w.size(2) * 8};
   Rows r;
   r.n = n;
