@@ -33,3 +33,31 @@ def test_a_gradient_of_quantised_rows():
     x = torch.ones(3, 32, dtype=BF, requires_grad=True)
     with pytest.raises(QmoeUnsupported, match="gradient"):
         B.rows_product(x, w, s, None, 1, None, None, 3, True, True)
+
+
+def _calls():
+    B = _lib.binding()
+    x, od, (w, s) = torch.zeros(4, 64, dtype=BF), torch.arange(4, dtype=torch.int32), _w(5, 64)
+    return [lambda v: B.quantize(v, False), lambda v: B.dequantize(w, s, 0, False), lambda v: B.sort_tokens(v, od, od, False),
+            lambda v: B.unsort_tokens(v, od, od, torch.ones(4, 1), False), lambda v: B.matmul(v, w, s, True, False, False),
+            lambda v: B.gather(v, w[None], s[None], None, od, True, True, False),
+            lambda v: B.rows_product(v, w[None], s[None], None, 1, None, None, 4, True, False)], x
+
+
+@pytest.mark.parametrize("i", range(7))
+def test_recorders(i):
+    """A recorded call would hold the result's allocation and no kernel."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    calls, x = _calls()
+    refusals = []
+
+    def call(v):
+        with pytest.raises(QmoeUnsupported, match="record"):
+            calls[i](v)
+        refusals.append(i)
+        return v + 1
+
+    torch.jit.trace(call, (x,), check_trace=False)
+    make_fx(call)(x)
+    assert refusals == [i, i]

@@ -17,10 +17,12 @@
 #include <ATen/ops/index_select.h>
 #include <ATen/ops/searchsorted.h>
 #include <ATen/ops/zeros.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "qmoe.h"
 
@@ -93,6 +95,14 @@ bool records(const Tensor& t) {
   return t.requires_grad() && at::GradMode::is_enabled();
 }
 
+// A tracer sees the allocation of a result and not the launch that fills it: refused.
+void refuse_recorders() {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  if (torch::jit::tracer::isTracing() || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value())
+    throw Failure("torch.jit.trace and make_fx cannot record these kernels");
+}
+
 py::object none(bool must) {
   TORCH_CHECK(!must, "the arguments are not what the kernels read");
   return py::none();
@@ -130,6 +140,7 @@ std::pair<Tensor, Tensor> quantize_run(const Tensor& x) {
 }
 
 py::object quantize(py::handle x_, bool must) {
+  refuse_recorders();
   Tensor x;
   if (!get(x_, &x) || type_of(x) < 0 || x.dim() < 1 || x.size(-1) % 32 || !plain(x)) return none(must);
   const c10::hip::HIPGuard guard(x.get_device());
@@ -138,6 +149,7 @@ py::object quantize(py::handle x_, bool must) {
 }
 
 py::object dequantize(py::handle w_, py::handle s_, int type, bool must) {
+  refuse_recorders();
   Tensor w, s;
   if (!get(w_, &w) || !get(s_, &s) || !words(w) || !bytes(s) || w.dim() < 1 || w.dim() != s.dim() ||
       w.device() != s.device() || w.size(-1) % 4 || s.size(-1) != w.size(-1) / 4 ||
@@ -222,6 +234,7 @@ bool pairs(const Tensor& t, const Tensor& rows, int64_t n) {
 }
 
 py::object sort_tokens(py::handle x_, py::handle order_, py::handle inv_, bool must) {
+  refuse_recorders();
   Tensor x, order, inv;
   if (!get(x_, &x) || !get(order_, &order) || !get(inv_, &inv) || type_of(x) < 0 || x.dim() != 2 || !plain(x))
     return none(must);
@@ -232,6 +245,7 @@ py::object sort_tokens(py::handle x_, py::handle order_, py::handle inv_, bool m
 }
 
 py::object unsort_tokens(py::handle xs_, py::handle order_, py::handle inv_, py::handle scores_, bool must) {
+  refuse_recorders();
   Tensor xs, order, inv, scores;
   if (!get(xs_, &xs) || !get(order_, &order) || !get(inv_, &inv) || !get(scores_, &scores) || type_of(xs) < 0 ||
       xs.dim() != 2 || !plain(xs))
@@ -396,6 +410,7 @@ Tensor as_rows(const Tensor& x) {
 
 // x [.., C] times the weights of one matrix; qq: x quantised as well.
 py::object matmul(py::handle x_, py::handle w_, py::handle s_, bool transpose, bool qq, bool must) {
+  refuse_recorders();
   Tensor x;
   Weights g;
   if (!get(x_, &x) || !plain(x, at::kBFloat16) || x.dim() < 1 || !weights(w_, s_, x, 2, &g) ||
@@ -438,6 +453,7 @@ bool table(const Tensor& experts, int64_t E, Rows* r) {
 // lhs's; and either sorted or fewer rows than are worth sorting.
 py::object gather(py::handle x_, py::handle w_, py::handle s_, py::handle lhs_, py::handle rhs_, bool transpose,
                   bool is_sorted, bool qq) {
+  refuse_recorders();
   Tensor x, lhs, rhs;
   Weights g;
   if (!get(x_, &x) || !plain(x, at::kBFloat16) || x.dim() < 2 || x.size(-2) != 1 || !get(rhs_, &rhs) ||
@@ -480,6 +496,7 @@ py::object rows_product(const Tensor& x, const Tensor& w, const Tensor& s, const
                         int64_t div, const std::optional<Tensor>& experts,
                         const std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, int64_t>>& tiles, int64_t n,
                         bool transpose, bool qq, const std::optional<Tensor>& inv) {
+  refuse_recorders();
   if (records(x) && qq)
     throw Failure("the products of quantised activations have no gradient: detach x, or use quantized_matmul / gather_qmm");
   Weights g{w, s, w.size(0), w.size(1), w.size(2) * 8};
