@@ -224,3 +224,23 @@ def test_repeats_in_graphs(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
+
+
+def test_more_rows_than_one_launch_lays_out_in_lines(dev):
+    """Rows that are quantised in one launch but whose scales fill more than one in lines."""
+    say("rows past the lines")
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("less than 60 GiB of GPU memory free")
+    M, K, N = (1 << 28) + 77, 32, 8
+    g = _gen(7)
+    w, s = codes(g, N, K)
+    some = torch.tensor([0, 127, 1 << 27, (1 << 28) - 1, 1 << 28, M - 1])
+    few = _acts(g, len(some), K)
+    x = torch.zeros(M, K, dtype=BF, device=dev)
+    x[some.to(dev)] = few.to(dev)
+    y = ops.qqmm(x, w.to(dev), s.to(dev))
+    del x
+    check_sum(y[some.to(dev)], *_product(quantize_ref(few)[0].to(dev), dequantize_ref(w, s).t().to(dev)), K)
+    assert not y[1:127].any() and not y[(1 << 27) + 1:(1 << 27) + 5000].any()
+    del y
+    torch.cuda.empty_cache()

@@ -376,13 +376,13 @@ Tensor qq_run(const Tensor& x, const Weights& g, const Rows& r) {
     const int64_t words = (g.E * g.N + x.size(0)) * ((g.K + 127) / 128);
     xq = at::empty({x.size(0), g.K / 8}, x.options().dtype(at::kInt).requires_grad(false));
     lines = at::empty({words}, xq.options());
-    ok(qmoe_mxfp4_quantize_lines(ptr<uint16_t>(x), x.size(0), g.K, static_cast<uint32_t*>(xq.data_ptr()),
-                                 ptr<uint8_t>(g.s), (int32_t)g.E, g.N, static_cast<uint32_t*>(lines.data_ptr()), words,
-                                 stream(x)),
-       "qmoe_mxfp4_quantize_lines");
-  } else {
-    std::tie(xq, xs) = quantize_run(x);
+    const int rc = qmoe_mxfp4_quantize_lines(ptr<uint16_t>(x), x.size(0), g.K, static_cast<uint32_t*>(xq.data_ptr()),
+                                             ptr<uint8_t>(g.s), (int32_t)g.E, g.N,
+                                             static_cast<uint32_t*>(lines.data_ptr()), words, stream(x));
+    if (rc == QMOE_ERR_UNSUPPORTED) lines = xq = Tensor();  // more than one launch holds: the scales stay in their rows
+    else ok(rc, "qmoe_mxfp4_quantize_lines");
   }
+  if (!lines.defined()) std::tie(xq, xs) = quantize_run(x);
   const Tensor rows = gemm_rows(r, x);
   ok(qmoe_mxfp4_gather_qqmm(ptr<uint32_t>(xq), ptr<uint8_t>(xs), x.size(0), ptr<int32_t>(rows), r.n, ptr<uint32_t>(g.w),
                             ptr<uint8_t>(g.s), (int32_t)g.E, g.N, g.K, ptr<int32_t>(r.offsets), ptr<int32_t>(r.tile_row),
