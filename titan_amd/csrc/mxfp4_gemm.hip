@@ -59,11 +59,13 @@ __device__ __forceinline__ qmoe_gemm::TileRows tile_of(const GemmArgs& a, int64_
 // 64 and 128 alone 40,960 rows of 256 experts pay for 20% more rows than they
 // have, with these for 10%.
 //
-// What bounds it: a product of 68.7 GFLOP takes 61 us (1.1 PFLOP/s) forward,
-// 72 to 80 transposed, both at the card's power limit (a loop of nothing but
-// these instructions runs at 1.8 GHz of 2.4): blocks alone on their CU are as
-// fast as two, copies five groups ahead as fast as three.  4096^3 in mxfp4
-// takes 49 us (2.8 PFLOP/s), bound by the copies into LDS.
+// What bounds it: a product of 68.7 GFLOP takes 61 us (1.1 PFLOP/s) forward, at
+// the card's power limit (a loop of nothing but these instructions runs at 1.8
+// GHz of 2.4).  Transposed it takes 72 to 80 back to back (82 to 90 where each
+// is waited for): for the same products it issues twice the matrix
+// instructions, and a permute besides each conversion; blocks alone on their
+// CU are as fast as two, copies five groups ahead as fast as three.  4096^3 in
+// mxfp4 takes 49 us (2.8 PFLOP/s), bound by the copies into LDS.
 //
 // Operands reach LDS by asynchronous copies into a ring of NS stages and are
 // read from there as matrix fragments; the fragments of a step are prepared

@@ -6,8 +6,9 @@
 // side by side cover one weight row.  Codes become bf16 pairs by the scaled
 // conversion (exact) and go through v_dot2_f32_bf16 with the activation's
 // pairs: 32 instructions per 32 codes.  Bound by the latency of one dependent
-// HBM round trip at one token (4096 x 2048: 4.0 us for 4.5 MB; top-10 of 1024 x
-// 2048: 5.7 us for 11 MB), by the caches and HBM at more (six tokens 16.2 us).
+// HBM round trip at one token (per call in a graph, 4096 x 2048: 4.0 us for 4.5
+// MB; top-10 of 1024 x 2048: 5.7 us for 11 MB), by the caches and HBM at more
+// (six tokens 16.2 us).
 //
 // Transposed, out[r, k] = sum_n x[r, n] W[e_r, n, k]: a lane owns the 32
 // outputs of one block column and walks n, four rows' loads ahead; sixteen

@@ -14,7 +14,8 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4 (QQ) the block as it is against x's codes.
 //
 // Bound by the two or three dependent round trips to HBM of a launch: 4096 x
-// 2048 weights (4.5 MB) take 4.7 us at 5 rows, 5.7 at 32, 8.6 at 64 in a graph.
+// 2048 weights (4.5 MB) take 4.8 us per call in a graph at 5 rows, 6.4 at 32,
+// 8.7 at 64.
 #include "gemm_common.h"
 #include "mxfp4.h"
 #include "mxfp4_rows.h"
@@ -180,7 +181,7 @@ int launch(const RowsArgs& a, hipStream_t st) {
 
 int qmoe_mx::rows_product(const RowsArgs& a, bool qq, hipStream_t st) {
   // Row tiles of 16 as many as there are rows for.  Batches of 256 where two blocks still fit a CU: with one, blocks
-  // past the 256th wait for a round of their own (23 rows, batches of 256 / 128: 4099 x 2080 10.2 / 6.8 us, 8192 x
+  // past the 256th wait for a round of their own (us per call in a graph, 23 rows, batches of 256 / 128: 4099 x 2080 10.2 / 6.8 us, 8192 x
   // 2048 10.7 / 7.6, 4096 x 2048 6.2 / 5.6; in smaller forms either is within 8% of the other).
   const int mt = (int)((a.M + 15) / 16);
   if (qq) {

@@ -5,9 +5,11 @@
 // without it, it returns None for anything but tensors the entry points can
 // read as they are (GPU, contiguous, aligned, of the right types and sizes),
 // and the wrapper then checks, converts or refuses; with it, such a call is an
-// error.  A call made this way costs the host about 5 us where ctypes and
-// Python autograd nodes cost 11 us (one product) to 68 us (a forward and
-// backward pass), which is what a small call's time is made of.
+// error.  Tracers, which would not see a launch, and tangents are refused.  A
+// call made this way costs the host about 5 us where ctypes cost 11, and the
+// token sort and the way back with their gradients 46 to 79 from run to run
+// where Python autograd nodes cost 136, which is what a small call's time is
+// made of.
 //
 // Launches go to the tensors' device and its current stream; nothing
 // synchronises; outputs and tables come from torch's allocator.
@@ -38,7 +40,7 @@ constexpr int64_t kSortedMinRows = 64;  // gathered rows from which the grouped 
 // once per row, mostly from the caches after the first, the kernel for few rows
 // once in all but with a longer start.  Two rows of 4096 x 2048 take 4.7 us
 // either way, four 6.4 and 4.7, four of 1024 x 2048 3.4 and 4.0.  Transposed
-// products take the GEMM from one row on (4096 x 2048: 20 and 14.6 us).
+// products take the GEMM from one row on (4096 x 2048: 20 and 14.2 us).
 constexpr int64_t kQmvMaxRows = 4, kQmvMaxWork = int64_t(1) << 24;
 
 // Rows above which products of two mxfp4 operands leave the kernel for few rows,

@@ -10,7 +10,8 @@ bf16, products and sums fp32, results bf16.
 The products are differentiable in x: with ``transpose`` (x W^T) dx = dy W, and
 without (x W) dx = dy W^T, by the same kernels over the same codes.  The codes
 and scales are constants of the graph.  ``qqmm`` and ``gather_qqmm`` quantise x
-as well and have no gradient.
+as well and have no gradient.  Forward-mode tangents, torch.jit.trace and
+make_fx are refused.
 
 The calls and their autograd nodes are csrc/torch/binding.cpp's.  It takes what
 the kernels can read as it is; the functions here check, convert, arrange or
@@ -256,7 +257,9 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases=No
     times W^T, or x [.., M, N] times W without ``transpose``.  From 64 rows on
     the rows run through the grouped GEMM: as they are with ``sorted_indices``
     (ascending ``rhs_indices``), else sorted by expert first.  Indices outside
-    their range are clamped into it."""
+    their range are clamped into it.  ``tiles``: the table of sorted rows
+    (:func:`titan_amd.ops.build_tiles` of ``rhs_indices``, or the routing's), which
+    then says what expert a row takes."""
     _format(group_size, bits, biases)
     if tiles is None:
         y = _lib.binding().gather(x, w, scales, lhs_indices, rhs_indices, bool(transpose), bool(sorted_indices), False)

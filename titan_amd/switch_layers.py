@@ -11,10 +11,11 @@ gate_up projection (gate rows first, loader.py:19-27), SwiGLU, the down
 projection, and un-sorts.
 
 Tensors stay on their device.  For ROCm tensors the sort is the HIP counting
-sort, which also yields the tile table both projections share, and the row
-gather, the default activation and the un-sort are one kernel each (at 512
-tokens x top-10, hidden 2048, 13 torch launches of 75 us before); CPU tensors
-use torch's stable argsort and the stock gather.
+sort, which also yields the tile table that affine projections share (mxfp4
+ones make their own), and the row gather, the default activation and the
+un-sort are one kernel each (at 512 tokens x top-10, hidden 2048, 13 torch
+launches of 75 us before); CPU tensors use torch's stable argsort and the stock
+gather.
 """
 
 from __future__ import annotations

@@ -6,7 +6,9 @@ Pair ``p = t * k + j`` is slot j of token t.  ``order`` (the pair of each sorted
 row) and ``inv_order`` (the sorted row of each pair) are inverse permutations of
 the T * k pairs, as :func:`titan_amd.ops.route` gives them.  Rows are bf16, fp16
 or fp32, of any length; sums run in fp32 in slot order and are rounded once, so
-results repeat bit for bit.
+results repeat bit for bit.  Where they are not inverse permutations, rows that no
+pair is sent to stay as their memory was; nothing is read or written out of bounds.
+Forward-mode tangents, torch.jit.trace and make_fx are refused.
 
 The calls and their autograd nodes are csrc/torch/binding.cpp's.  It takes what
 the kernels can read as it is; the functions here check, convert or refuse the
@@ -43,8 +45,9 @@ def _pairs(t: torch.Tensor, name: str, device, n: int | None = None) -> torch.Te
 
 
 def sort_tokens(x: torch.Tensor, order: torch.Tensor, inv_order: torch.Tensor) -> torch.Tensor:
-    """x [T, D] -> [T * k, D], row i the token of pair ``order[i]``; the gradient
-    of a token is the sum over its k rows, formed from ``inv_order``."""
+    """x [T, D] -> [T * k, D], row i the token of pair ``order[i]``: each token's
+    row is written to its k places ``inv_order``, and its gradient is the sum over
+    them."""
     y = _lib.binding().sort_tokens(x, order, inv_order, False)
     if y is not None:
         return y
