@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define QMOE_ABI_VERSION 5
+#define QMOE_ABI_VERSION 6
 
 enum {
   QMOE_OK = 0,
@@ -135,6 +135,11 @@ int qmoe_route_noalloc(const int32_t* ids, int64_t n_pairs, int32_t num_experts,
                        int32_t* sorted_ids, int32_t* offsets, int32_t* tile_row,
                        int32_t* tile_exp, int32_t* ntiles, int64_t max_tiles,
                        int32_t* n_bad, void* stream);
+
+/* int64 ids to int32 ones, clamped into [0, n) (all 0 where n is 0): what 32
+ * bits do not hold is out of range and not some other id. */
+int qmoe_narrow_ids(const int64_t* ids, int64_t count, int32_t n, int32_t* out,
+                    void* stream);
 
 /* build_tiles over ids that are already sorted ascending
  * (titan/kernels/moe_gather_ws.py:133-156,181-202). */

@@ -109,3 +109,47 @@ def test_a_table_covers_every_row(dev):
         rows = [(int(r) + i, int(x)) for r, x in zip(t.tile_row[:k], t.tile_exp[:k])
                 for i in range(min(t.tile_rows, int(want[int(x) + 1]) - int(r)))]
         assert rows == list(enumerate(inside.tolist()))
+
+
+@pytest.mark.parametrize("count", [0, 1, 255, 256, 5000])
+def test_narrowed_ids(dev, count):
+    """int64 ids in memory of every order: as they are, strided, expanded, of several dimensions."""
+    say("narrow", count)
+    g = _gen(count)
+    v = torch.randint(-(1 << 62), 1 << 62, (count,), generator=g) >> torch.randint(0, 63, (count,), generator=g)
+    for n in (0, 1, 7, 1 << 20, (1 << 31) - 1, 1 << 31):
+        t = v.to(dev)
+        for s in (t, torch.stack([t, t], 1)[:, 1], t[None].expand(2, -1), t.reshape(1, -1, 1)):
+            got = ops._narrow(s, n)
+            assert got.dtype == torch.int32 and got.shape == s.shape
+            assert torch.equal(got.cpu().long(), s.cpu().clamp(0, min(max(n - 1, 0), (1 << 31) - 1)))
+
+
+def test_int64_ids_in_a_graph(dev):
+    say("graph")
+    g = _gen(1)
+    E, K, N = 6, 64, 40
+    w, s = (t.to(dev) for t in codes(g, E, N, K))
+    W = dequantize_ref(w, s).transpose(1, 2)
+    x, ids = torch.randn(9, 1, K, generator=g).to(BF).to(dev), torch.zeros(9, dtype=torch.int64, device=dev)
+
+    def step():
+        return ops.gather_qmm(x, w, s, rhs_indices=ids, mode="mxfp4"), ops.gather_qqmm(x, w, s, rhs_indices=ids)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2, 3):
+        new = torch.randint(-2, E + 2, (9,), generator=_gen(seed))
+        new[seed] = (1 << 32) + 1
+        ids.copy_(new)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
+        check_sum(want[0], *_by_expert(x, W, new.clamp(0, E - 1)), K)

@@ -61,3 +61,15 @@ def test_narrow_indices(dtype):
     v = [0, 5, 100]
     t = torch.tensor(v, dtype=dtype)
     assert _taken(torch.zeros(B, 2, 32, dtype=BF), E, t, t) == ([2 * i + m for i in v for m in (0, 1)], [i for i in v for _ in (0, 1)])
+
+
+def test_bad_arguments_of_the_narrowing():
+    from titan_amd import _lib
+
+    L, one = _lib.load(), 4096
+    assert L.qmoe_narrow_ids(one, -1, 4, one, None) == _lib.ERR_INVALID
+    assert L.qmoe_narrow_ids(one, 3, -1, one, None) == _lib.ERR_INVALID
+    assert L.qmoe_narrow_ids(None, 3, 4, one, None) == _lib.ERR_INVALID
+    assert L.qmoe_narrow_ids(one, 3, 4, None, None) == _lib.ERR_INVALID
+    assert L.qmoe_narrow_ids(None, 0, 4, None, None) == _lib.OK
+    assert L.qmoe_narrow_ids(one, 1 << 40, 4, one, None) == _lib.ERR_UNSUPPORTED

@@ -63,7 +63,25 @@ __global__ void dequant_kernel(const uint32_t* __restrict__ w, const uint16_t* _
   }
 }
 
+// One thread per id.  One launch, as the cast alone is: clamped and cast by two
+// of torch's, a one-token gather with int64 ids takes 7.3 us in a graph, not 6.0.
+__global__ void narrow_ids_kernel(const int64_t* __restrict__ ids, int64_t count, int64_t last,
+                                  int32_t* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < count) out[i] = (int32_t)min(max(ids[i], (int64_t)0), last);
+}
+
 }  // namespace
+
+extern "C" int qmoe_narrow_ids(const int64_t* ids, int64_t count, int32_t n, int32_t* out, void* stream) {
+  if (count < 0 || n < 0) return qmoe::fail(QMOE_ERR_INVALID, "bad sizes");
+  if (count == 0) return QMOE_OK;
+  if (!ids || !out) return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
+  const int64_t blocks = (count + 255) / 256;
+  if (qmoe::too_many(blocks, 256)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "too many ids");
+  narrow_ids_kernel<<<dim3((unsigned)blocks), dim3(256), 0, qmoe::as_stream(stream)>>>(ids, count, n > 0 ? n - 1 : 0, out);
+  return qmoe::launch_status("narrow_ids_kernel");
+}
 
 extern "C" int qmoe_unpack(const uint32_t* w, int64_t n_words, int bits, uint8_t* codes,
                            void* stream) {

@@ -492,6 +492,16 @@ py::object gather(py::handle x_, py::handle w_, py::handle s_, py::handle lhs_, 
   return give(y.reshape(sizes));
 }
 
+// int64 ids as int32 ones clamped into [0, n).
+Tensor narrow(const Tensor& ids, int64_t n) {
+  TORCH_CHECK(ids.scalar_type() == at::kLong && ids.is_cuda() && ids.is_contiguous() && n >= 0 && n <= INT32_MAX,
+              "the arguments are not what the kernels read");
+  const c10::hip::HIPGuard guard(ids.get_device());
+  Tensor out = at::empty(ids.sizes(), ids.options().dtype(at::kInt));
+  ok(qmoe_narrow_ids(ptr<int64_t>(ids), ids.numel(), (int32_t)n, out.data_ptr<int32_t>(), stream(ids)), "qmoe_narrow_ids");
+  return out;
+}
+
 // Rows already arranged by the wrapper: x [rows, C], x_rows / experts int32 or None, a tile table or None, and
 // where the rows of activation row t are known, their places inv[t div .. (t + 1) div).
 py::object rows_product(const Tensor& x, const Tensor& w, const Tensor& s, const std::optional<Tensor>& x_rows,
@@ -538,6 +548,7 @@ PYBIND11_MODULE(_binding, m) {
   m.def("unsort_tokens", &unsort_tokens);
   m.def("matmul", &matmul);
   m.def("gather", &gather);
+  m.def("narrow", &narrow);
   m.def("rows_product", &rows_product, py::arg("x"), py::arg("w"), py::arg("s"), py::arg("x_rows"), py::arg("div"),
         py::arg("experts"), py::arg("tiles"), py::arg("n"), py::arg("transpose"), py::arg("qq"),
         py::arg("inv") = py::none());

@@ -100,12 +100,16 @@ def _i32(t: torch.Tensor, name: str, device) -> torch.Tensor:
 def _narrow(t: torch.Tensor, n: int) -> torch.Tensor:
     """Indices into ``n`` as int32; those of the types that 32 bits do not hold
     are clamped into range first, so that none becomes another index."""
+    if t.dtype == torch.int32:
+        return t
+    if t.dtype == torch.int64 and t.is_cuda and t.is_contiguous() and n <= 0x7FFFFFFF:
+        return _lib.binding().narrow(t, n)
     if t.dtype == torch.uint64:
         t = t.view(torch.int64)
         t = torch.where(t < 0, n, t)  # 2^63 and more
     if t.dtype in (torch.int64, torch.uint32):
         t = t.to(torch.int64).clamp(0, max(n - 1, 0))
-    return t if t.dtype == torch.int32 else t.to(torch.int32)
+    return t.to(torch.int32)
 
 
 def _f32(t: torch.Tensor, name: str, device) -> torch.Tensor:
