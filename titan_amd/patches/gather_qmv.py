@@ -6,7 +6,8 @@ The reference leaves these shapes on MLX's own gather_qmv
 drop-in.  It also takes every call of both with ``mode="mxfp4"`` and bf16
 activations on the GPU, sorted or not, either way round and with gradients
 (:mod:`titan_amd.mxfp4`): the prefill overlays above it take affine weights
-alone; what the kernels refuse (a trace, a tangent) is handed down.  Affine calls are routed when: ``sorted_indices`` false, affine ``transpose=True``
+alone; what the kernels refuse (a trace, a tangent) is handed down.  Affine
+calls are routed when: ``sorted_indices`` false, affine ``transpose=True``
 weights with biases, bf16 activations on the GPU.  Shapes the kernels do not
 take (bits other than 4 and 8, group sizes other than 32/64/128, K outside the
 kernels' range: 8-bit codes up to K = 4096) raise
