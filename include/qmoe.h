@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define QMOE_ABI_VERSION 6
+#define QMOE_ABI_VERSION 7
 
 enum {
   QMOE_OK = 0,
@@ -569,6 +569,80 @@ int qmoe_unsort_grad(const void* dy, const void* xs, int64_t n, int dtype,
                      const int32_t* inv, const float* scores, int64_t T,
                      int64_t top_k, int64_t D, void* dxs, float* dscores,
                      void* stream);
+
+/* ------------------------------------------------ both operands in 8 bits --
+ * Rows of signed 8-bit codes with one fp32 scale each: activations by token,
+ * weights by output channel (the mode="int8" of quantize, dequantize, qqmm and
+ * gather_qqmm; an extension, the reference has int8 activations against int4
+ * weights only).  A row v has scale s = max|v| / 127 (fp32, correctly rounded)
+ * and codes rint(v / s) in [-127, 127], those of qmoe_quantize_act_int8; a row
+ * of zeros has scale 0, a row with a NaN or an infinity scale NaN and codes 0.
+ * Rows of any length; x and what dequantise writes are QMOE_BF16, _FP16 or
+ * _FP32; all but the scales 16-byte aligned. */
+int qmoe_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K,
+                       int8_t* codes, float* scales, void* stream);
+int qmoe_int8_dequantize(const int8_t* codes, const float* scales,
+                         int64_t rows, int64_t K, int dtype, void* out,
+                         void* stream);
+
+/* RMS norm into that form (an extension): h = x + residual, rounded to the
+ * rows' type (residual NULL: h = x), v = h / sqrt(mean(h^2) + eps) * weight
+ * [D] (of the rows' type or fp32; NULL: ones) in fp32, the squares summed in
+ * 64 bits; codes and scales of v; sum = h and norm = v in the rows' type,
+ * either NULL: not written.  sum may be x or residual, and norm may be x or
+ * residual where sum is not the same buffer. */
+int qmoe_int8_rms_norm(const void* x, const void* residual, const void* weight,
+                       int weight_dtype, int dtype, int64_t rows, int64_t D,
+                       double eps, int8_t* codes, float* scales, void* sum,
+                       void* norm, void* stream);
+
+/* Products: out[r, n] = sx[xr] sw[e, n] sum_k x[xr, k] w[e, n, k], summed
+ * exactly in 32 bits, rounded once to out_dtype; codes [-128, 127].  K is a
+ * multiple of 16, at most 131056.  Indices are clamped into range.
+ *   qmoe_int8_gather_qqmv  few rows (at most 65535), xr = x_rows[r], or r /
+ *                          x_div where x_rows is NULL; experts NULL: expert 0
+ *   qmoe_int8_gather_qqmm  many rows, sorted by expert, as described by a tile
+ *                          table (qmoe_route / qmoe_build_tiles with
+ *                          qmoe_gemm_tile_rows() rows per tile), or with the
+ *                          four tables NULL rows of one expert; x_rows NULL:
+ *                          row r reads x[r] */
+int qmoe_int8_gather_qqmv(const int8_t* x, const float* sx, int64_t n_x,
+                          const int32_t* x_rows, int32_t x_div,
+                          const int32_t* experts, int64_t n_rows,
+                          const int8_t* w, const float* sw,
+                          int32_t num_experts, int64_t N, int64_t K,
+                          int out_dtype, void* out, void* stream);
+int qmoe_int8_gather_qqmm(const int8_t* x, const float* sx, int64_t n_x,
+                          const int32_t* x_rows, int64_t n_rows,
+                          const int8_t* w, const float* sw,
+                          int32_t num_experts, int64_t N, int64_t K,
+                          const int32_t* offsets, const int32_t* tile_row,
+                          const int32_t* tile_exp, const int32_t* ntiles,
+                          int64_t max_tiles, int out_dtype, void* out,
+                          void* stream);
+
+/* ------------------------------------------------- the router's balance loss --
+ * An extension for training a router (the reference serves only).  Over the
+ * tokens with mask[t] != 0 (mask NULL: all T), n of them, with p = softmax of
+ * their logits [T, E] (a row of -inf: zeros) and ids [T, k] (int32, or int64
+ * with ids64; clamped into range) their experts:
+ *   counts[e]  pairs of those tokens routed to e
+ *   loss       E sum_e counts[e] / (n k) * mean_t p[t, e]; 0 where n = 0
+ *   n          those tokens
+ * and the gradient of dloss * loss by the logits, the counts being constants:
+ * exactly 0 for masked tokens.  logits and dlogits are QMOE_BF16, _FP16 or
+ * _FP32 and 16-byte aligned, E <= 1024; sums over tokens go in a fixed order.
+ * The workspace has qmoe_router_balance_workspace_size(T, E) bytes. */
+size_t qmoe_router_balance_workspace_size(int64_t T, int64_t E);
+int qmoe_router_balance(const void* logits, int dtype, int64_t T, int64_t E,
+                        const void* ids, int ids64, int64_t k,
+                        const uint8_t* mask, float* loss, int32_t* counts,
+                        int32_t* n, void* workspace, size_t workspace_bytes,
+                        void* stream);
+int qmoe_router_balance_grad(const void* logits, int dtype, int64_t T,
+                             int64_t E, int64_t k, const uint8_t* mask,
+                             const int32_t* counts, const int32_t* n,
+                             const float* dloss, void* dlogits, void* stream);
 
 #ifdef __cplusplus
 }

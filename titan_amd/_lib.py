@@ -99,6 +99,14 @@ SIGNATURES: dict[str, tuple] = {
     "qmoe_sort_rows": (INT, [P, I64, P, I64, I64, INT, P, P]),
     "qmoe_unsort_sum": (INT, [P, I64, INT, P, P, P, I64, I64, I64, INT, P, P]),
     "qmoe_unsort_grad": (INT, [P, P, I64, INT, P, P, I64, I64, I64, P, P, P]),
+    "qmoe_int8_quantize": (INT, [P, INT, I64, I64, P, P, P]),
+    "qmoe_int8_dequantize": (INT, [P, P, I64, I64, INT, P, P]),
+    "qmoe_int8_rms_norm": (INT, [P, P, P, INT, INT, I64, I64, ctypes.c_double, P, P, P, P, P]),
+    "qmoe_int8_gather_qqmv": (INT, [P, P, I64, P, I32, P, I64, P, P, I32, I64, I64, INT, P, P]),
+    "qmoe_int8_gather_qqmm": (INT, [P, P, I64, P, I64, P, P, I32, I64, I64, P, P, P, P, I64, INT, P, P]),
+    "qmoe_router_balance_workspace_size": (SZ, [I64, I64]),
+    "qmoe_router_balance": (INT, [P, INT, I64, I64, P, INT, I64, P, P, P, P, P, SZ, P]),
+    "qmoe_router_balance_grad": (INT, [P, INT, I64, I64, I64, P, P, P, P, P, P]),
 }
 
 _lock = threading.Lock()
@@ -127,7 +135,7 @@ def load() -> ctypes.CDLL:
 
 
 def binding():
-    """The torch binding of the mxfp4 and token-sort operators
+    """The torch binding of the mxfp4, 8-bit, token-sort and balance-loss operators
     (csrc/torch/binding.cpp), which carries their autograd nodes."""
     global _binding
     if _binding is None:

@@ -17,50 +17,9 @@
 //
 // A thread takes 16 bytes of a row where the row length is a multiple of 16
 // bytes, one element otherwise (VEC).
-#include "common.h"
+#include "elem.h"
 
 namespace {
-
-template <int DT>
-struct Elem;
-template <>
-struct Elem<QMOE_BF16> {
-  typedef uint16_t T;
-  static __device__ __forceinline__ float load(T v) { return bf16_to_f32(v); }
-  static __device__ __forceinline__ T store(float f) { return (T)f32_to_bf16(f); }
-};
-template <>
-struct Elem<QMOE_FP16> {
-  typedef _Float16 T;
-  static __device__ __forceinline__ float load(T v) { return (float)v; }
-  static __device__ __forceinline__ T store(float f) { return (_Float16)f; }
-};
-template <>
-struct Elem<QMOE_FP32> {
-  typedef float T;
-  static __device__ __forceinline__ float load(T v) { return v; }
-  static __device__ __forceinline__ T store(float f) { return f; }
-};
-
-// N consecutive elements, moved as one access of N * sizeof(T) bytes.
-template <typename T, int N>
-struct Vec {
-  typedef T V __attribute__((ext_vector_type(N)));
-};
-template <typename T>
-struct Vec<T, 1> {
-  typedef T V;
-};
-template <typename T, int N>
-__device__ __forceinline__ T at(const typename Vec<T, N>::V& v, int i) {
-  if constexpr (N == 1) return v;
-  else return v[i];
-}
-template <typename T, int N>
-__device__ __forceinline__ void set(typename Vec<T, N>::V& v, int i, T x) {
-  if constexpr (N == 1) v = x;
-  else v[i] = x;
-}
 
 constexpr int kBatch = 8;  // rows in flight per thread
 
@@ -194,7 +153,7 @@ __global__ __launch_bounds__(256) void unsort_grad_kernel(const void* __restrict
   }
 }
 
-int size_of(int dtype) { return dtype == QMOE_FP32 ? 4 : dtype == QMOE_BF16 || dtype == QMOE_FP16 ? 2 : 0; }
+using qmoe::size_of;
 
 // Threads for `units` work items along a row: whole waves, one at least, at most 256.
 unsigned row_threads(int64_t units) { return (unsigned)(units >= 256 ? 256 : units <= 64 ? 64 : (units + 63) / 64 * 64); }

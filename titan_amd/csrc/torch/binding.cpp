@@ -1,5 +1,6 @@
-// Python binding of the mxfp4 products, the quantisation and the token sort,
-// with their autograd nodes, over the C ABI of libqmoe.so.
+// Python binding of the mxfp4 and 8-bit products, their quantisations, the
+// token sort and the router's balance loss, with their autograd nodes, over the
+// C ABI of libqmoe.so.
 //
 // Every function takes its arguments as the Python wrappers do and a flag:
 // without it, it returns None for anything but tensors the entry points can
@@ -65,6 +66,7 @@ int type_of(const Tensor& t) {
     default: return -1;
   }
 }
+constexpr at::ScalarType kTypes[] = {at::kBFloat16, at::kHalf, at::kFloat};  // by the entry points' numbers
 // A tensor the kernels can read as it is.
 bool plain(const Tensor& t) {
   return t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() && !t.is_neg() && !t.is_conj() &&
@@ -161,8 +163,7 @@ py::object dequantize(py::handle w_, py::handle s_, int type, bool must) {
   const int64_t K = w.size(-1) * 8;
   auto sizes = w.sizes().vec();
   sizes.back() = K;
-  const at::ScalarType types[] = {at::kBFloat16, at::kHalf, at::kFloat};
-  Tensor out = at::empty(sizes, w.options().dtype(types[type]));
+  Tensor out = at::empty(sizes, w.options().dtype(kTypes[type]));
   ok(qmoe_mxfp4_dequantize(ptr<uint32_t>(w), ptr<uint8_t>(s), K ? w.numel() / w.size(-1) : 0, K, type, out.data_ptr(),
                            stream(w)),
      "qmoe_mxfp4_dequantize");
@@ -452,37 +453,45 @@ bool table(const Tensor& experts, int64_t E, Rows* r) {
 
 // The gather calls whose rows need no arranging: one row per batch index; the
 // batch that of rhs, x's own or x's with its last dimensions broadcast, or
-// lhs's; and either sorted or fewer rows than are worth sorting.
+// lhs's; and either sorted or fewer rows than are worth sorting (sorted_only:
+// sorted).  False: not one of them.
+bool arranged(const Tensor& x, int64_t E, py::handle lhs_, py::handle rhs_, bool is_sorted, bool sorted_only, Rows* r,
+              Tensor* rhs) {
+  Tensor lhs;
+  if (!get(rhs_, rhs) || !plain(*rhs, at::kInt) || rhs->device() != x.device()) return false;
+  r->n = rhs->numel();
+  const int64_t n_x = x.numel() && x.size(-1) ? x.numel() / x.size(-1) : 0;
+  if (r->n == 0 || n_x == 0 || E == 0) return false;
+  if (lhs_.is_none()) {
+    const int64_t bd = x.dim() - 2;
+    if (bd != rhs->dim()) return false;
+    int64_t d = 0;
+    while (d < bd && x.size(d) == rhs->size(d)) ++d;
+    for (int64_t i = d; i < bd; ++i) {
+      if (x.size(i) != 1) return false;
+      r->div *= rhs->size(i);
+    }
+  } else {
+    if (!get(lhs_, &lhs) || !plain(lhs, at::kInt) || lhs.sizes() != rhs->sizes() || lhs.device() != x.device())
+      return false;
+    r->x_rows = lhs.reshape({-1});
+  }
+  if (!is_sorted && (sorted_only || r->n >= kSortedMinRows)) return false;
+  r->experts = rhs->reshape({-1});
+  return true;
+}
+
 py::object gather(py::handle x_, py::handle w_, py::handle s_, py::handle lhs_, py::handle rhs_, bool transpose,
                   bool is_sorted, bool qq) {
   refuse_recorders();
-  Tensor x, lhs, rhs;
+  Tensor x, rhs;
   Weights g;
-  if (!get(x_, &x) || !plain(x, at::kBFloat16) || x.dim() < 2 || x.size(-2) != 1 || !get(rhs_, &rhs) ||
-      !plain(rhs, at::kInt) || rhs.device() != x.device() || !weights(w_, s_, x, 3, &g) ||
-      x.size(-1) != (transpose ? g.K : g.N) || (qq && records(x)))
-    return py::none();
   Rows r;
-  r.n = rhs.numel();
-  const int64_t n_x = x.numel() && x.size(-1) ? x.numel() / x.size(-1) : 0;
-  if (r.n == 0 || n_x == 0 || g.E == 0) return py::none();
-  if (lhs_.is_none()) {
-    const int64_t bd = x.dim() - 2;
-    if (bd != rhs.dim()) return py::none();
-    int64_t d = 0;
-    while (d < bd && x.size(d) == rhs.size(d)) ++d;
-    for (int64_t i = d; i < bd; ++i) {
-      if (x.size(i) != 1) return py::none();
-      r.div *= rhs.size(i);
-    }
-  } else {
-    if (!get(lhs_, &lhs) || !plain(lhs, at::kInt) || lhs.sizes() != rhs.sizes() || lhs.device() != x.device())
-      return py::none();
-    r.x_rows = lhs.reshape({-1});
-  }
-  if (!is_sorted && (qq || r.n >= kSortedMinRows)) return py::none();
+  if (!get(x_, &x) || !plain(x, at::kBFloat16) || x.dim() < 2 || x.size(-2) != 1 || !weights(w_, s_, x, 3, &g) ||
+      x.size(-1) != (transpose ? g.K : g.N) || (qq && records(x)) ||
+      !arranged(x, g.E, lhs_, rhs_, is_sorted, qq, &r, &rhs))
+    return py::none();
   const c10::hip::HIPGuard guard(x.get_device());
-  r.experts = rhs.reshape({-1});
   if ((qq || r.n >= kSortedMinRows) && !table(r.experts, g.E, &r)) return py::none();
   const Tensor x2 = as_rows(x);
   Tensor y = qq ? qq_run(x2, g, r) : product(x2, g, r, transpose);
@@ -529,6 +538,242 @@ py::object rows_product(const Tensor& x, const Tensor& w, const Tensor& s, const
   return give(qq ? qq_run(x, g, r) : product(x, g, r, transpose));
 }
 
+// ------------------------------------------------- both operands in 8 bits
+
+int64_t row_count(const Tensor& t) {  // rows along the last dimension
+  int64_t n = 1;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) n *= t.size(d);
+  return n;
+}
+at::IntArrayRef batch_of(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
+bool scales32(const Tensor& t) {  // scales need no alignment past their own
+  return t.scalar_type() == at::kFloat && t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() && !t.is_neg();
+}
+
+std::pair<Tensor, Tensor> int8_run(const Tensor& x) {
+  Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar).requires_grad(false));
+  Tensor s = at::empty(batch_of(x), x.options().dtype(at::kFloat).requires_grad(false));
+  ok(qmoe_int8_quantize(x.const_data_ptr(), type_of(x), row_count(x), x.size(-1), q.data_ptr<int8_t>(), s.data_ptr<float>(),
+                        stream(x)),
+     "qmoe_int8_quantize");
+  return {q, s};
+}
+
+py::object int8_quantize(py::handle x_, bool must) {
+  refuse_recorders();
+  Tensor x;
+  if (!get(x_, &x) || type_of(x) < 0 || x.dim() < 1 || !plain(x)) return none(must);
+  const c10::hip::HIPGuard guard(x.get_device());
+  const auto [q, s] = int8_run(x);
+  return py::make_tuple(give(q), give(s));
+}
+
+py::object int8_dequantize(py::handle q_, py::handle s_, int type, bool must) {
+  refuse_recorders();
+  Tensor q, s;
+  if (!get(q_, &q) || !get(s_, &s) || !plain(q, at::kChar) || !scales32(s) || q.dim() < 1 || s.sizes() != batch_of(q) ||
+      s.device() != q.device())
+    return none(must);
+  const c10::hip::HIPGuard guard(q.get_device());
+  Tensor out = at::empty(q.sizes(), q.options().dtype(kTypes[type]));
+  ok(qmoe_int8_dequantize(ptr<int8_t>(q), ptr<float>(s), row_count(q), q.size(-1), type, out.data_ptr(), stream(q)),
+     "qmoe_int8_dequantize");
+  return give(out);
+}
+
+py::object rms_norm_quantize(py::handle x_, py::handle w_, double eps, py::handle r_, bool norm, bool must) {
+  refuse_recorders();
+  Tensor x, w, r;
+  if (!get(x_, &x) || type_of(x) < 0 || x.dim() < 1 || !plain(x) || records(x)) return none(must);
+  if (!w_.is_none() && (!get(w_, &w) || !(plain(w, x.scalar_type()) || plain(w, at::kFloat)) || w.dim() != 1 ||
+                        w.size(0) != x.size(-1) || w.device() != x.device() || records(w)))
+    return none(must);
+  if (!r_.is_none() && (!get(r_, &r) || !plain(r, x.scalar_type()) || r.sizes() != x.sizes() ||
+                        r.device() != x.device() || records(r)))
+    return none(must);
+  const c10::hip::HIPGuard guard(x.get_device());
+  const auto like = x.options().requires_grad(false);
+  Tensor q = at::empty(x.sizes(), like.dtype(at::kChar)), s = at::empty(batch_of(x), like.dtype(at::kFloat)), sum, v;
+  if (r.defined()) sum = at::empty(x.sizes(), like);
+  if (norm) v = at::empty(x.sizes(), like);
+  ok(qmoe_int8_rms_norm(x.const_data_ptr(), r.defined() ? r.const_data_ptr() : nullptr,
+                        w.defined() ? w.const_data_ptr() : nullptr, w.defined() ? type_of(w) : type_of(x), type_of(x),
+                        row_count(x), x.size(-1), eps, q.data_ptr<int8_t>(), s.data_ptr<float>(),
+                        sum.defined() ? sum.data_ptr() : nullptr, v.defined() ? v.data_ptr() : nullptr, stream(x)),
+     "qmoe_int8_rms_norm");
+  return py::make_tuple(give(q), give(s), sum.defined() ? give(sum) : py::none(), v.defined() ? give(v) : py::none());
+}
+
+// Activations: codes and scales, or (scales None) values to be quantised here.
+struct Acts {
+  Tensor x, s;
+  bool get_from(py::handle x_, py::handle s_) {
+    if (!get(x_, &x) || x.dim() < 1) return false;
+    if (s_.is_none()) return type_of(x) >= 0 && plain(x) && !records(x);
+    return plain(x, at::kChar) && get(s_, &s) && scales32(s) && s.sizes() == batch_of(x) && s.device() == x.device() &&
+           !records(s);
+  }
+  int type(int asked) const { return asked >= 0 ? asked : s.defined() ? QMOE_BF16 : type_of(x); }
+  void quantized() {
+    if (!s.defined()) std::tie(x, s) = int8_run(x);
+  }
+};
+struct Weights8 {
+  Tensor w, s;
+  int64_t E, N, K;
+  bool get_from(py::handle w_, py::handle s_, const Tensor& x, int64_t dims) {
+    if (!get(w_, &w) || !get(s_, &s) || !plain(w, at::kChar) || !scales32(s) || w.dim() != dims || s.sizes() != batch_of(w) ||
+        w.device() != x.device() || s.device() != x.device() || records(s))
+      return false;
+    E = dims == 3 ? w.size(0) : 1;
+    N = w.size(-2);
+    K = w.size(-1);
+    return K % 16 == 0 && x.size(-1) == K;
+  }
+};
+
+Tensor int8_product_run(const Acts& a, const Weights8& g, const Rows& r, int type) {
+  Tensor out = at::empty({r.n, g.N}, a.x.options().dtype(kTypes[type]).requires_grad(false));
+  if (out.numel() == 0) return out;
+  if (g.K == 0) return out.zero_();
+  const int64_t n_x = row_count(a.x);
+  if (!r.offsets.defined() && (r.experts.defined() || r.n <= kQmvMaxRows)) {
+    ok(qmoe_int8_gather_qqmv(ptr<int8_t>(a.x), ptr<float>(a.s), n_x, ptr<int32_t>(r.x_rows), (int32_t)r.div,
+                             ptr<int32_t>(r.experts), r.n, ptr<int8_t>(g.w), ptr<float>(g.s), (int32_t)g.E, g.N, g.K, type,
+                             out.data_ptr(), stream(a.x)),
+       "qmoe_int8_gather_qqmv");
+    return out;
+  }
+  const Tensor rows = gemm_rows(r, a.x);
+  ok(qmoe_int8_gather_qqmm(ptr<int8_t>(a.x), ptr<float>(a.s), n_x, ptr<int32_t>(rows), r.n, ptr<int8_t>(g.w), ptr<float>(g.s),
+                           (int32_t)g.E, g.N, g.K, ptr<int32_t>(r.offsets), ptr<int32_t>(r.tile_row),
+                           ptr<int32_t>(r.tile_exp), ptr<int32_t>(r.ntiles), r.maxt, type, out.data_ptr(), stream(a.x)),
+     "qmoe_int8_gather_qqmm");
+  return out;
+}
+
+// x [.., K] times the weights of one matrix.
+py::object int8_matmul(py::handle x_, py::handle sx_, py::handle w_, py::handle s_, int type, bool must) {
+  refuse_recorders();
+  Acts a;
+  Weights8 g;
+  if (!a.get_from(x_, sx_) || !g.get_from(w_, s_, a.x, 2)) return none(must);
+  const c10::hip::HIPGuard guard(a.x.get_device());
+  type = a.type(type);
+  auto sizes = a.x.sizes().vec();
+  sizes.back() = g.N;
+  Rows r;
+  r.n = row_count(a.x);
+  a.quantized();
+  return give(int8_product_run(a, g, r, type).reshape(sizes));
+}
+
+py::object int8_gather(py::handle x_, py::handle sx_, py::handle w_, py::handle s_, py::handle lhs_, py::handle rhs_,
+                       bool is_sorted, int type) {
+  refuse_recorders();
+  Acts a;
+  Weights8 g;
+  Rows r;
+  Tensor rhs;
+  if (!a.get_from(x_, sx_) || a.x.dim() < 2 || a.x.size(-2) != 1 || !g.get_from(w_, s_, a.x, 3) ||
+      !arranged(a.x, g.E, lhs_, rhs_, is_sorted, false, &r, &rhs))
+    return py::none();
+  const c10::hip::HIPGuard guard(a.x.get_device());
+  if (r.n >= kSortedMinRows && !table(r.experts, g.E, &r)) return py::none();
+  type = a.type(type);
+  a.quantized();
+  auto sizes = rhs.sizes().vec();
+  sizes.push_back(1);
+  sizes.push_back(g.N);
+  return give(int8_product_run(a, g, r, type).reshape(sizes));
+}
+
+// Rows already arranged by the wrapper, as rows_product has them.
+py::object int8_rows_product(py::handle x_, py::handle sx_, py::handle w_, py::handle s_,
+                             const std::optional<Tensor>& x_rows, int64_t div, const std::optional<Tensor>& experts,
+                             const std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, int64_t>>& tiles, int64_t n,
+                             int type) {
+  refuse_recorders();
+  Acts a;
+  Weights8 g;
+  TORCH_CHECK(a.get_from(x_, sx_) && g.get_from(w_, s_, a.x, 3), "the arguments are not what the kernels read");
+  Rows r;
+  r.n = n;
+  r.div = div;
+  if (x_rows) r.x_rows = *x_rows;
+  if (experts) r.experts = *experts;
+  if (tiles) std::tie(r.offsets, r.tile_row, r.tile_exp, r.ntiles, r.maxt) = *tiles;
+  for (const Tensor* t : {&r.x_rows, &r.experts, &r.offsets, &r.tile_row, &r.tile_exp, &r.ntiles})
+    TORCH_CHECK(!t->defined() || (t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == a.x.device()),
+                "the arguments are not what the kernels read");
+  TORCH_CHECK((!x_rows || r.x_rows.numel() == n) && (!experts || r.experts.numel() == n), "the rows disagree");
+  const c10::hip::HIPGuard guard(a.x.get_device());
+  type = a.type(type);
+  a.quantized();
+  return give(int8_product_run(a, g, r, type));
+}
+
+// ------------------------------------------------- the router's balance loss
+
+struct Balance : torch::autograd::Function<Balance> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& ids,
+                               const std::optional<Tensor>& mask) {
+    const auto [loss, counts, n] = run(logits, ids, mask.value_or(Tensor()));
+    ctx->mark_non_differentiable({counts});
+    ctx->save_for_backward({logits, mask.value_or(Tensor()), counts, n});
+    ctx->saved_data["k"] = ids.size(-1);
+    return {loss, counts};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &mask = saved[1], &counts = saved[2], &n = saved[3];
+    const Tensor g = ready(grads[0]);
+    const c10::hip::HIPGuard guard(logits.get_device());
+    Tensor d = at::empty(logits.sizes(), logits.options().requires_grad(false));
+    ok(qmoe_router_balance_grad(logits.const_data_ptr(), type_of(logits), row_count(logits), logits.size(-1),
+                                ctx->saved_data["k"].toInt(), bytes_of(mask), ptr<int32_t>(counts), ptr<int32_t>(n),
+                                ptr<float>(g), d.data_ptr(), stream(logits)),
+       "qmoe_router_balance_grad");
+    auto from = grads;
+    from.push_back(logits);
+    return first_order({d, Tensor(), Tensor()}, from);
+  }
+  static const uint8_t* bytes_of(const Tensor& mask) {
+    return mask.defined() ? static_cast<const uint8_t*>(mask.const_data_ptr()) : nullptr;
+  }
+  static std::tuple<Tensor, Tensor, Tensor> run(const Tensor& logits, const Tensor& ids, const Tensor& mask) {
+    const int64_t T = row_count(logits), E = logits.size(-1);
+    const auto like = logits.options().requires_grad(false);
+    const size_t bytes = qmoe_router_balance_workspace_size(T, E);
+    Tensor loss = at::empty({}, like.dtype(at::kFloat)), counts = at::empty({E}, like.dtype(at::kInt)),
+           n = at::empty({}, like.dtype(at::kInt)), ws = at::empty({(int64_t)bytes}, like.dtype(at::kByte));
+    ok(qmoe_router_balance(logits.const_data_ptr(), type_of(logits), T, E, ids.const_data_ptr(),
+                           ids.scalar_type() == at::kLong, ids.size(-1), bytes_of(mask), loss.data_ptr<float>(),
+                           counts.data_ptr<int32_t>(), n.data_ptr<int32_t>(), ws.data_ptr(), bytes, stream(logits)),
+       "qmoe_router_balance");
+    return {loss, counts, n};
+  }
+};
+
+py::object router_balance(py::handle logits_, py::handle ids_, py::handle mask_, bool must) {
+  refuse_recorders();
+  Tensor logits, ids, mask;
+  if (!get(logits_, &logits) || !get(ids_, &ids) || type_of(logits) < 0 || !plain(logits) || logits.dim() < 1 ||
+      !(plain(ids, at::kInt) || plain(ids, at::kLong)) || ids.dim() != logits.dim() || batch_of(ids) != batch_of(logits) ||
+      ids.device() != logits.device())
+    return none(must);
+  if (!mask_.is_none() && (!get(mask_, &mask) || mask.scalar_type() != at::kBool || !mask.is_cuda() ||
+                           !mask.is_contiguous() || mask.sizes() != batch_of(logits) || mask.device() != logits.device()))
+    return none(must);
+  const c10::hip::HIPGuard guard(logits.get_device());
+  if (records(logits)) {
+    const auto out = Balance::apply(logits, ids, mask.defined() ? std::optional<Tensor>(mask) : std::nullopt);
+    return py::make_tuple(give(out[0]), give(out[1]));
+  }
+  const auto [loss, counts, n] = Balance::run(logits, ids, mask);
+  return py::make_tuple(give(loss), give(counts));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_binding, m) {
@@ -549,6 +794,13 @@ PYBIND11_MODULE(_binding, m) {
   m.def("matmul", &matmul);
   m.def("gather", &gather);
   m.def("narrow", &narrow);
+  m.def("int8_quantize", &int8_quantize);
+  m.def("int8_dequantize", &int8_dequantize);
+  m.def("rms_norm_quantize", &rms_norm_quantize);
+  m.def("int8_matmul", &int8_matmul);
+  m.def("int8_gather", &int8_gather);
+  m.def("int8_rows_product", &int8_rows_product);
+  m.def("router_balance", &router_balance);
   m.def("rows_product", &rows_product, py::arg("x"), py::arg("w"), py::arg("s"), py::arg("x_rows"), py::arg("div"),
         py::arg("experts"), py::arg("tiles"), py::arg("n"), py::arg("transpose"), py::arg("qq"),
         py::arg("inv") = py::none());

@@ -25,6 +25,9 @@ Call-surface parity with the reference (paths relative to its root):
 * :func:`sort_tokens` / :func:`unsort_tokens`   _gather_sort, _scatter_unsort
   (switch_layers.py:13-25) and the weighted sum, with gradients
   (:mod:`titan_amd.token_sort`)
+* ``mode="int8"`` of :func:`quantize`, :func:`dequantize`, :func:`qqmm` and
+  :func:`gather_qqmm`, :func:`rms_norm_quantize` (:mod:`titan_amd.int8`) and
+  :func:`router_balance_loss` (:mod:`titan_amd.balance`): extensions
 """
 
 from __future__ import annotations
@@ -132,9 +135,12 @@ def _same_device(t: torch.Tensor, name: str, device) -> None:
 # ------------------------------------------------------------------ layout
 
 
-def quantize(w: torch.Tensor, group_size: int | None = None, bits: int = BITS, mode: str = "mxfp4"):
-    """mx.quantize into mxfp4 (:func:`titan_amd.mxfp4.quantize`): (codes, scales)."""
-    return mxfp4.quantize(w, group_size, bits, mode)
+def quantize(w: torch.Tensor, group_size: int | None = None, bits: int | None = None, mode: str = "mxfp4"):
+    """mx.quantize into mxfp4 (:func:`titan_amd.mxfp4.quantize`): (codes, scales);
+    mode "int8": rows with one scale each (:func:`titan_amd.int8.quantize`)."""
+    if mode == "int8":
+        return int8.quantize(w, group_size, bits)
+    return mxfp4.quantize(w, group_size, BITS if bits is None else bits, mode)
 
 
 def unpack(w: torch.Tensor, bits: int = BITS) -> torch.Tensor:
@@ -147,10 +153,14 @@ def unpack(w: torch.Tensor, bits: int = BITS) -> torch.Tensor:
 
 
 def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor | None = None,
-               group_size: int | None = None, bits: int = BITS, mode: str = "affine",
+               group_size: int | None = None, bits: int | None = None, mode: str = "affine",
                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """bf16_rne(fmaf(q, s, b)) for every element (mx.dequantize); mode "mxfp4":
-    :func:`titan_amd.mxfp4.dequantize`, into bf16, fp16 or fp32."""
+    :func:`titan_amd.mxfp4.dequantize`, mode "int8":
+    :func:`titan_amd.int8.dequantize`, into bf16, fp16 or fp32."""
+    if mode == "int8":
+        return int8.dequantize(w, scales, biases, group_size, bits, dtype)
+    bits = BITS if bits is None else bits
     if mode == "mxfp4":
         return mxfp4.dequantize(w, scales, biases, group_size, bits, dtype=dtype)
     group_size = _affine(mode, biases, group_size)
@@ -619,18 +629,34 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
     return out.reshape(*batch, M, N)
 
 
-def qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, group_size: int | None = None, bits: int = BITS,
-         mode: str = "mxfp4") -> torch.Tensor:
-    """mx.qqmm: both operands in mxfp4 (:func:`titan_amd.mxfp4.qqmm`)."""
-    return mxfp4.qqmm(x, w, scales, group_size, bits, mode)
+def _bf16_result(dtype: torch.dtype | None) -> None:
+    if dtype not in (None, torch.bfloat16):
+        raise QmoeUnsupported(_lib.ERR_UNSUPPORTED, f"dtype={dtype}: products in mxfp4 are bfloat16")
 
 
-def gather_qqmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, lhs_indices: torch.Tensor | None = None,
-                rhs_indices: torch.Tensor | None = None, group_size: int | None = None, bits: int = BITS,
-                mode: str = "mxfp4", sorted_indices: bool = False, *, tiles: TileTable | None = None) -> torch.Tensor:
+def qqmm(x, w: torch.Tensor, scales: torch.Tensor, group_size: int | None = None, bits: int | None = None,
+         mode: str = "mxfp4", dtype: torch.dtype | None = None) -> torch.Tensor:
+    """mx.qqmm: both operands in mxfp4 (:func:`titan_amd.mxfp4.qqmm`); mode "int8":
+    both in 8-bit integers with scales by token and channel
+    (:func:`titan_amd.int8.qqmm`), x quantised already or not."""
+    if mode == "int8":
+        return int8.qqmm(x, w, scales, group_size, bits, dtype)
+    _bf16_result(dtype)
+    return mxfp4.qqmm(x, w, scales, group_size, BITS if bits is None else bits, mode)
+
+
+def gather_qqmm(x, w: torch.Tensor, scales: torch.Tensor, lhs_indices: torch.Tensor | None = None,
+                rhs_indices: torch.Tensor | None = None, group_size: int | None = None, bits: int | None = None,
+                mode: str = "mxfp4", sorted_indices: bool = False, *, tiles: TileTable | None = None,
+                dtype: torch.dtype | None = None) -> torch.Tensor:
     """:func:`gather_qmm` with the activations quantised to mxfp4 too
-    (:func:`titan_amd.mxfp4.gather_qqmm`)."""
-    return mxfp4.gather_qqmm(x, w, scales, lhs_indices, rhs_indices, group_size, bits, mode, sorted_indices, tiles)
+    (:func:`titan_amd.mxfp4.gather_qqmm`); mode "int8": both operands in 8-bit
+    integers (:func:`titan_amd.int8.gather_qqmm`)."""
+    if mode == "int8":
+        return int8.gather_qqmm(x, w, scales, lhs_indices, rhs_indices, group_size, bits, sorted_indices, tiles, dtype)
+    _bf16_result(dtype)
+    return mxfp4.gather_qqmm(x, w, scales, lhs_indices, rhs_indices, group_size, BITS if bits is None else bits, mode,
+                             sorted_indices, tiles)
 
 
 def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor | None = None,
@@ -935,6 +961,19 @@ def router_topk(logits: torch.Tensor, k: int, norm: bool = True):
     return idx.reshape(*lg.shape[:-1], k), scores.reshape(*lg.shape[:-1], k)
 
 
+def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6,
+                      residual: torch.Tensor | None = None, norm: bool = False):
+    """The RMS norm of x + residual in 8 bits with a scale per token, for
+    :func:`qqmm` and :func:`gather_qqmm` (:func:`titan_amd.int8.rms_norm_quantize`)."""
+    return int8.rms_norm_quantize(x, weight, eps, residual, norm)
+
+
+def router_balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: torch.Tensor | None = None):
+    """(loss, counts): how unevenly tokens use the experts, with its gradient
+    (:func:`titan_amd.balance.router_balance_loss`)."""
+    return balance.router_balance_loss(logits, ids, mask)
+
+
 def router_logits(x: torch.Tensor, router, group_size: int = GROUP, bits: int = BITS) -> torch.Tensor:
     """fp32 router logits [T, E] for tokens x [T, K]: ``router`` a dense bf16
     [E, K] weight, or an affine-quantized (w, scales, biases) triple, whose
@@ -960,8 +999,8 @@ def router_logits(x: torch.Tensor, router, group_size: int = GROUP, bits: int = 
     return out
 
 
-# at the end: both are written over the functions above
-from . import mxfp4, token_sort  # noqa: E402
+# at the end: all are written over the functions above
+from . import balance, int8, mxfp4, token_sort  # noqa: E402
 
 __all__ = [
     "GROUP", "BITS", "QmoeError", "QmoeUnsupported", "TileTable", "TileWeights", "Routing", "build_tiles", "route",
@@ -971,4 +1010,5 @@ __all__ = [
     "gate_up_silu_topk", "gate_up_topk_supported", "gather_rows", "swiglu", "shared_combine", "max_tiles", "tile_rows", "unpack", "dequantize", "gather_qmv", "gather_qmm_sorted", "gather_qmm",
     "gemm_supported", "quantized_matmul", "gate_up_silu", "down_wsum", "moe_weighted_sum",
     "quantize_act_int8", "gather_qmm_int8_sorted", "quantize", "qqmm", "gather_qqmm", "sort_tokens", "unsort_tokens",
+    "rms_norm_quantize", "router_balance_loss",
 ]
