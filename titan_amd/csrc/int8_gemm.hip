@@ -2,17 +2,22 @@
 // (int8_product.h).  Rows are those of a tile table (sorted by expert), or of
 // one expert without a table.
 //
-// A unit is a block of up to kRows rows of one expert times kCols outputs.  Its
-// WM x WN waves hold MSUB x NSUB subtiles of v_mfma_i32_32x32x32_i8 each.  Both
-// operands reach LDS by asynchronous copies into a ring of NS stages of KB
-// bytes of the contraction, and are read from there as fragments, those of a
-// step during the step before.  The barrier that hands over a stage stands
-// before a group's last step, whose operands are in registers by then; the
-// copies into the stage that it frees are spread between the matrix
-// instructions that follow, since a run of them would hold up the wave that
-// issues them.  Blocks are persistent; units of a table go heavy-first
-// (gemm_common.h), those of one matrix in bands of columns, so that the blocks
-// of an XCD share rows and columns in its L2.
+// A unit is a block of up to 256 rows of one expert times 256 outputs, computed
+// by a block of eight waves, one block per CU.  Its form by its rows: WM x WN
+// waves of MSUB x NSUB subtiles of v_mfma_i32_32x32x32_i8 each.  Both operands
+// reach LDS by asynchronous copies, 128 bytes of a row at a time (a whole line;
+// with 64, twice the requests for the same bytes), into a ring of NS stages, and
+// are read from there as fragments, those of a step during the step before.  The
+// barrier that hands over a stage stands before a group's last step, whose
+// operands are in registers by then; the copies into the stage that it frees are
+// spread between the matrix instructions that follow, since a run of them would
+// hold up the wave that issues them.
+//
+// Blocks are persistent.  Units of a table take two tiles of an expert where it
+// has them, so that its weights are read once for up to 256 rows, and go
+// heavy-first; those of one matrix go in bands of columns, so that the blocks of
+// an XCD share rows and columns in its L2.  A unit's first copies are issued
+// before the results of the one before it are stored.
 #include <algorithm>
 
 #include "gemm_common.h"
@@ -23,7 +28,17 @@ namespace {
 using namespace qmoe_i8;
 using qmoe_gemm::kTileRows;
 
+constexpr int kWaves = 8, kThreads = 64 * kWaves;
+constexpr int kCols = 256;               // outputs of a unit
+constexpr int kPairRows = 2 * kTileRows;  // rows of a unit, at most
+constexpr int kGroup = 128;              // bytes of the contraction per stage
+constexpr int kUnits = kGroup / 16;      // and its 16-byte units
+constexpr int kSteps = kGroup / 32;
+constexpr int kRound = kWaves * (1024 / kGroup);  // rows that one copy of every wave fills
+constexpr int kBCopies = kCols / kRound, kMaxACopies = kPairRows / kRound;
 constexpr int kLdsCU = 160 * 1024;
+// The results are staged in the ring's second 64 KiB: the first stage of the next unit is filled meanwhile.
+constexpr int kStaging = 64 * 1024, kRing = 144 * 1024;
 __device__ __attribute__((aligned(16))) uint32_t zero_unit[4];  // what copies past the contraction's end read
 
 // The thread's index through an empty asm, so that what is computed from it is
@@ -34,8 +49,15 @@ __device__ __forceinline__ int fresh_tid() {
   return tid;
 }
 
+// All waves of the block are here, and their accesses to LDS are done; memory operations may be under way.
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 struct Unit {
-  int e, valid;
+  int e, valid;      // valid 0: none
   int64_t row0, o0;  // first row; first output
 };
 
@@ -44,75 +66,124 @@ __device__ __forceinline__ int64_t row_of(const Product& a, const Unit& u, int r
   const int64_t r = u.row0 + min(row, u.valid - 1);
   return min(max(a.x_rows ? (int64_t)a.x_rows[r] : r, (int64_t)0), a.n_x - 1);
 }
+// Copies of activation rows per wave and group: the forms' rows in rounds.
+__device__ __forceinline__ int a_copies(int valid) { return (valid + kRound - 1) / kRound; }
 
-// Swizzle of a row's 16-byte units in LDS, KB / 16 of them: one unit of sixteen
+// Swizzle of a row's eight 16-byte units in LDS: one unit of sixteen
 // consecutive rows is read without bank conflicts.
-template <int KB>
-__device__ __forceinline__ int swz(int row) {
-  if constexpr (KB == 128) return (row & 7) ^ ((row >> 3) & 1);
-  else return (row >> 2) & 3;
-}
+__device__ __forceinline__ int swz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
 // Sixteen bytes stored at any element's address.
 struct __attribute__((packed)) Loose16 {
   i32x4_t v __attribute__((aligned(2)));
 };
 
-template <int WM_, int WN_, int MSUB_, int NSUB_, int KB_, int NS_>
-struct Form {
-  static constexpr int WM = WM_, WN = WN_, MSUB = MSUB_, NSUB = NSUB_, KB = KB_, NS = NS_;
-  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr int kRows = 32 * WM * MSUB, kCols = 32 * WN * NSUB;
-  static constexpr int kA = kRows * KB, kB = kCols * KB, kStage = kA + kB, kRing = NS * kStage;
-  static constexpr int kPer = 1024 / KB;  // rows per copy
-  static constexpr int kACopies = kRows / kPer / kWaves, kBCopies = kCols / kPer / kWaves;
-  static constexpr int kCopies = kACopies + kBCopies;  // per wave and group
-  static constexpr int kSteps = KB / 32;
-  static_assert(kRows % (kPer * kWaves) == 0 && kCols % (kPer * kWaves) == 0, "whole copies");
+// The activation rows of a unit that a lane copies from, and whose scale it copies.
+struct Rows {
+  int x[kMaxACopies], scale;
+};
+__device__ __forceinline__ Rows rows_of(const Product& a, const Unit& u) {
+  const int tid = fresh_tid(), lane = tid % 64, wave = tid / 64;
+  Rows r;
+#pragma unroll
+  for (int d = 0; d < kMaxACopies; ++d) r.x[d] = (int)row_of(a, u, d * kRound + wave * (kRound / kWaves) + lane / kUnits);
+  r.scale = (int)row_of(a, u, min(tid, kPairRows - 1));
+  return r;
+}
 
-  struct Ctx {
-    const char* x[kACopies];  // the lane's unit of each copy's row
-    const char* w;            // the unit's columns
-    uint32_t woff[kBCopies];
-    int unit;  // the lane's unit within a group (the rows of its copies swizzle alike)
-    uint32_t lds;
-    int wave, lane, units;
-  };
+struct Ctx {
+  const char* x[kMaxACopies];  // the lane's unit of each copy's row
+  const char* w;               // the unit's columns
+  uint32_t woff[kBCopies];
+  int unit;  // the lane's unit within a group: the rows of its copies swizzle alike
+  uint32_t lds;
+  int wave, lane, units;
+  // What is alike for all lanes of a wave, in scalar registers.
+  __device__ __forceinline__ void settle(const Product& a, const char* smem) {
+    const int tid = fresh_tid();
+    units = (int)(a.K / 16);
+    lane = tid % 64;
+    wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)smem);
+    w = reinterpret_cast<const char*>(qmoe_gemm::uniform64((int64_t)w));
+  }
+};
+
+// Copy d of group g into the stage at `st`, of the wave's NA of x and kBCopies
+// of w.  Units past the contraction's end are zeros of x, and of w the group's
+// first unit, whatever it holds.
+__device__ __forceinline__ void copy_x(const Ctx& c, int g, uint32_t st, int d) {
+  const bool in = g * kUnits + c.unit < c.units;
+  const char* p = c.x[d] + (size_t)g * kGroup;
+  qmoe_gemm::dma16(in ? p : reinterpret_cast<const char*>(zero_unit), st + (d * kWaves + c.wave) * 1024);
+}
+__device__ __forceinline__ void copy_w(const Ctx& c, int g, uint32_t st, int na, int d) {
+  const bool in = g * kUnits + c.unit < c.units;
+  qmoe_gemm::dma16s(c.w + (size_t)g * kGroup, c.woff[d] - (in ? 0u : (uint32_t)c.unit * 16),
+                    st + ((na + d) * kWaves + c.wave) * 1024);
+}
+
+// A unit's addresses, and the copies of its scales (into s: rows', then columns') and of its first group.
+__device__ __forceinline__ Ctx begin(const Product& a, const Unit& u, const Rows& rows, char* smem, float* s) {
+  Ctx c;
+  const int tid = fresh_tid();
+  const int64_t n0 = (int64_t)u.e * a.N + u.o0;
+  const int cols = (int)min((int64_t)kCols, a.N - u.o0);
+  c.w = reinterpret_cast<const char*>(a.w) + n0 * a.K;
+  c.settle(a, smem);
+  c.unit = (c.lane % kUnits) ^ swz(c.wave * (kRound / kWaves) + c.lane / kUnits);
+  static_assert(kRound % 16 == 0, "the copies' rows swizzle alike");
+#pragma unroll
+  for (int d = 0; d < kMaxACopies; ++d)
+    c.x[d] = reinterpret_cast<const char*>(a.x) + (int64_t)rows.x[d] * a.K + c.unit * 16;
+#pragma unroll
+  for (int d = 0; d < kBCopies; ++d)
+    c.woff[d] = (uint32_t)(min(d * kRound + c.wave * (kRound / kWaves) + c.lane / kUnits, cols - 1) * (int)a.K + c.unit * 16);
+  const uint32_t ls = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)s);
+  if (c.wave < kPairRows / 64) {
+    qmoe_gemm::dma4(a.sx + rows.scale, ls + c.wave * 256);
+    qmoe_gemm::dma4(a.sw + n0 + min(tid, cols - 1), ls + kPairRows * 4 + c.wave * 256);
+  }
+  static_assert(kCols == kPairRows, "the same waves copy both scales");
+  const int na = a_copies(u.valid);
+#pragma unroll
+  for (int d = 0; d < kMaxACopies; ++d)
+    if (d < na) copy_x(c, 0, c.lds, d);
+#pragma unroll
+  for (int d = 0; d < kBCopies; ++d) copy_w(c, 0, c.lds, na, d);
+  return c;
+}
+
+template <int WM_, int WN_, int MSUB_, int NSUB_, int NS_>
+struct Form {
+  static constexpr int WM = WM_, WN = WN_, MSUB = MSUB_, NSUB = NSUB_, NS = NS_;
+  static constexpr int kRows = 32 * WM * MSUB;
+  static constexpr int kACopies = (kRows + kRound - 1) / kRound, kCopies = kACopies + kBCopies;  // per wave and group
+  static constexpr int kA = kACopies * kWaves * 1024, kStage = kA + kCols * kGroup;
+  static_assert(WM * WN == kWaves && 32 * WN * NSUB == kCols, "eight waves, the unit's columns");
+  static_assert(NS * kStage <= kRing && kStage <= kStaging, "the ring");
+  typedef i32x16_t Acc[MSUB][NSUB];
+
   struct Frag {
     i32x4_t a[MSUB], b[NSUB];
   };
-
-  // Copy d of group g, of the wave's kCopies.
   static __device__ __forceinline__ void copy(const Ctx& c, int g, int stage, int d) {
     const uint32_t st = c.lds + stage * kStage;
-    const bool in = g * (KB / 16) + c.unit < c.units;
-    const bool whole = (g + 1) * (KB / 16) <= c.units;
-    if (d < kACopies) {
-      const char* p = c.x[d] + (size_t)g * KB;
-      qmoe_gemm::dma16(whole || in ? p : reinterpret_cast<const char*>(zero_unit), st + (d * kWaves + c.wave) * 1024);
-    } else {
-      const int b = d - kACopies;
-      const uint32_t dst = st + kA + (b * kWaves + c.wave) * 1024;
-      if (whole) {
-        qmoe_gemm::dma16s(c.w + (size_t)g * KB, c.woff[b], dst);
-      } else {
-        const char* p = c.w + (size_t)g * KB + c.woff[b];
-        qmoe_gemm::dma16(in ? p : reinterpret_cast<const char*>(zero_unit), dst);
-      }
-    }
+    if (d < kACopies) copy_x(c, g, st, d);
+    else copy_w(c, g, st, kACopies, d - kACopies);
   }
   static __device__ __forceinline__ void read(const Ctx& c, const char* st, int kk, int row0, int col0, Frag& f) {
-    const int l32 = c.lane % 32, unit = (2 * kk + c.lane / 32) ^ swz<KB>(l32);  // swz repeats every 16 rows
+    const int l32 = c.lane % 32, unit = (2 * kk + c.lane / 32) ^ swz(l32);  // swz repeats every 16 rows
 #pragma unroll
     for (int i = 0; i < MSUB; ++i)
-      f.a[i] = *reinterpret_cast<const i32x4_t*>(st + (row0 + 32 * i + l32) * KB + unit * 16);
+      f.a[i] = *reinterpret_cast<const i32x4_t*>(st + (row0 + 32 * i + l32) * kGroup + unit * 16);
 #pragma unroll
     for (int j = 0; j < NSUB; ++j)
-      f.b[j] = *reinterpret_cast<const i32x4_t*>(st + kA + (col0 + 32 * j + l32) * KB + unit * 16);
+      f.b[j] = *reinterpret_cast<const i32x4_t*>(st + kA + (col0 + 32 * j + l32) * kGroup + unit * 16);
   }
   // A step's products with PIECES calls of more(i) spread between them.
   template <int PIECES, class More>
-  static __device__ __forceinline__ void products(const Frag& f, i32x16_t (&acc)[MSUB][NSUB], More more) {
+  static __device__ __forceinline__ void products(const Frag& f, Acc& acc, More more) {
 #pragma unroll
     for (int j = 0; j < NSUB; ++j)
 #pragma unroll
@@ -127,46 +198,22 @@ struct Form {
       }
   }
 
-  static __device__ __forceinline__ void run(const Product& a, const Unit& u, char* smem, float* sx, float* sw) {
-    Ctx c;
-    const int tid = fresh_tid();
-    c.lane = tid % 64;
-    c.wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const int wm = c.wave / WN, wn = c.wave % WN;
-    c.units = (int)(a.K / 16);
-    c.lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)smem);
-    constexpr int kUnits = KB / 16;
-    // a wave's copies are kWaves * kPer rows apart, a multiple of 16: their swizzle is one
-    static_assert(kWaves * kPer % 16 == 0, "the copies' rows swizzle alike");
-    c.unit = (c.lane % kUnits) ^ swz<KB>(c.wave * kPer + c.lane / kUnits);
-#pragma unroll
-    for (int d = 0; d < kACopies; ++d) {
-      const int row = (d * kWaves + c.wave) * kPer + c.lane / kUnits;
-      c.x[d] = reinterpret_cast<const char*>(a.x) + row_of(a, u, row) * a.K + c.unit * 16;
-    }
-    const int64_t n0 = (int64_t)u.e * a.N + u.o0;
-    const int cols = (int)min((int64_t)kCols, a.N - u.o0);
-    c.w = reinterpret_cast<const char*>(a.w) + qmoe_gemm::uniform64(n0 * a.K);
-#pragma unroll
-    for (int d = 0; d < kBCopies; ++d)
-      c.woff[d] = (uint32_t)(min((d * kWaves + c.wave) * kPer + c.lane / kUnits, cols - 1) * (int)a.K + c.unit * 16);
+  // The sums of a unit whose first group is under way; between() is called once nothing reads the ring any more.
+  template <class Between>
+  static __device__ __forceinline__ void run(const Product& a, const Unit& u, Ctx& c, char* smem, const float* s,
+                                             Between between) {
+    c.settle(a, smem);
+    const int row0 = 32 * MSUB * (c.wave / WN), col0 = 32 * NSUB * (c.wave % WN);
     const int G = (c.units + kUnits - 1) / kUnits;
-    const int row0 = 32 * MSUB * wm, col0 = 32 * NSUB * wn;
-
-    // the scales, the rows' and the columns', into LDS ahead of everything else
-    const uint32_t lsx = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)sx);
-    const uint32_t lsw = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)sw);
-    for (int i = c.wave * 64; i < kRows; i += kThreads) qmoe_gemm::dma4(a.sx + row_of(a, u, i + c.lane), lsx + i * 4);
-    for (int i = c.wave * 64; i < kCols; i += kThreads) qmoe_gemm::dma4(a.sw + n0 + min(i + c.lane, cols - 1), lsw + i * 4);
-
-    i32x16_t acc[MSUB][NSUB] = {};
+    Acc acc = {};
+    if (NS > 2) meet();  // the staging of the unit before, which other stages overlap, is read
     // past the end: the last group again, into stages that nothing reads any more
 #pragma unroll
-    for (int i = 0; i < NS - 1; ++i)
+    for (int i = 1; i < NS - 1; ++i)
 #pragma unroll
       for (int d = 0; d < kCopies; ++d) copy(c, min(i, G - 1), i, d);
     qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
-    __builtin_amdgcn_s_barrier();
+    meet();
     Frag f[2];
     read(c, smem, 0, row0, col0, f[0]);
     int at = 0;  // the stage of group g
@@ -184,8 +231,7 @@ struct Form {
       if (g + 1 < G) {
         // the next group landed (copies of NS - 2 groups after it may be in flight); this one's reads are done
         qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
+        meet();
         read(c, smem + at * kStage, 0, row0, col0, f[kSteps & 1]);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -193,32 +239,45 @@ struct Form {
       __builtin_amdgcn_sched_barrier(0);
     }
     qmoe_gemm::wait_vmem<0>();
-    store(a, u, smem, sx, sw, acc);
+    meet();
+    between();
+    if (a.dtype == QMOE_FP32) store<4>(a, u, smem + kStaging, s, acc);
+    else store<2>(a, u, smem + kStaging, s, acc);
   }
 
-  // The results through LDS, a row subtile of every wave at a time, so that rows leave in whole lines.
-  static __device__ __forceinline__ void store(const Product& a, const Unit& u, char* smem, const float* sx,
-                                               const float* sw, i32x16_t (&acc)[MSUB][NSUB]) {
+  // The results through LDS, a row subtile of every wave at a time, so that rows
+  // leave in whole lines.  Passes of 2-byte results take the staging's halves in
+  // turn: a half is written again only past the barrier of the pass between.
+  template <int SIZE>
+  static __device__ __forceinline__ void store(const Product& a, const Unit& u, char* staging, const float* s, Acc& acc) {
+    constexpr int kPitch = kCols * SIZE, kPer = 16 / SIZE, kRowUnits = kCols / kPer;
+    constexpr int kReads = 32 * WM * kRowUnits / kThreads;  // per thread and pass
     const int tid = fresh_tid(), lane = tid % 64, l32 = lane % 32, h = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64), wm = wave / WN, wn = wave % WN;
-    const int size = a.dtype == QMOE_FP32 ? 4 : 2;
+    const int lr = 32 * wm + l32;
     const int64_t left = a.N - u.o0;
 #pragma unroll
     for (int i = 0; i < MSUB; ++i) {
-      __syncthreads();
-      const int lr = 32 * wm + l32;
-      const float s1 = sx[32 * MSUB * wm + 32 * i + l32];
+      char* ep = staging + (SIZE == 2 ? (i & 1) * (kStaging / 2) : 0);
+      if (SIZE == 4 && i) meet();
+      const float sx = s[32 * MSUB * wm + 32 * i + l32];
+      const bool plain = __all(ordinary(sx));
 #pragma unroll
       for (int j = 0; j < NSUB; ++j)
 #pragma unroll
         for (int v = 0; v < 16; v += 4) {
           const int gi = (32 * NSUB * wn + 32 * j + 2 * v + 4 * h) / 4;  // four outputs
-          const f32x4_t s = *reinterpret_cast<const f32x4_t*>(sw + 4 * gi);
+          const f32x4_t sw = *reinterpret_cast<const f32x4_t*>(s + kPairRows + 4 * gi);
           f32x4_t y;
+          if (plain) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) y[k] = scaled(acc[i][j][v + k], s1, s[k]);
-          if (size == 4) {
-            *reinterpret_cast<f32x4_t*>(smem + lr * (kCols * 4) + (gi ^ l32) * 16) = y;
+            for (int k = 0; k < 4; ++k) y[k] = (float)acc[i][j][v + k] * sx * sw[k];
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = scaled(acc[i][j][v + k], sx, sw[k]);
+          }
+          if constexpr (SIZE == 4) {
+            *reinterpret_cast<f32x4_t*>(ep + lr * kPitch + (gi ^ l32) * 16) = y;
           } else {
             uint2 o;
             if (a.dtype == QMOE_BF16) {
@@ -227,31 +286,46 @@ struct Form {
               typedef _Float16 h4 __attribute__((ext_vector_type(4)));
               o = __builtin_bit_cast(uint2, h4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]});
             }
-            *reinterpret_cast<uint2*>(smem + lr * (kCols * 2) + (gi ^ (2 * l32)) * 8) = o;
+            *reinterpret_cast<uint2*>(ep + lr * kPitch + (gi ^ (2 * l32)) * 8) = o;
           }
         }
-      __syncthreads();
-      const int per = 16 / size, row_units = kCols / per;  // outputs of a 16-byte unit; units of a row
-      for (int t = tid; t < 32 * WM * row_units; t += kThreads) {
-        const int r = t / row_units, unit = t % row_units;
-        const int row = 32 * MSUB * (r / 32) + 32 * i + r % 32;
-        const int64_t n = per * unit;
+      meet();
+      uint32_t from[kReads];
+      i32x4_t v[kReads];
+#pragma unroll
+      for (int t = 0; t < kReads; ++t) {
+        const int r = (t * kThreads + tid) / kRowUnits, unit = (t * kThreads + tid) % kRowUnits;
+        from[t] = (uint32_t)(uintptr_t)ep + r * kPitch + (unit ^ (r % 32)) * 16;
+      }
+      lds_read16(v, from);
+#pragma unroll
+      for (int t = 0; t < kReads; ++t) {
+        const int r = (t * kThreads + tid) / kRowUnits, unit = (t * kThreads + tid) % kRowUnits;
+        const int row = 32 * MSUB * (r / 32) + 32 * i + r % 32, n = kPer * unit;
         if (row >= u.valid || n >= left) continue;
-        const int at = size == 4 ? (unit ^ (r % 32)) * 16 : ((2 * unit) ^ (2 * (r % 32))) * 8;
-        const char* from = smem + r * (kCols * size) + at;
-        char* to = static_cast<char*>(a.out) + ((u.row0 + row) * a.N + u.o0 + n) * size;
-        const i32x4_t v = *reinterpret_cast<const i32x4_t*>(from);
-        if (a.N % per == 0) {
-          __builtin_nontemporal_store(v, reinterpret_cast<i32x4_t*>(to));
-        } else if (n + per <= left) {
-          reinterpret_cast<Loose16*>(to)->v = v;
+        char* to = static_cast<char*>(a.out) + ((u.row0 + row) * a.N + u.o0 + n) * SIZE;
+        if (a.N % kPer == 0) {
+          __builtin_nontemporal_store(v[t], reinterpret_cast<i32x4_t*>(to));
+        } else if (n + kPer <= left) {
+          reinterpret_cast<Loose16*>(to)->v = v[t];
         } else {
-          for (int k = 0; k < left - n; ++k) {
-            if (size == 4) reinterpret_cast<int*>(to)[k] = reinterpret_cast<const int*>(from)[k];
-            else reinterpret_cast<uint16_t*>(to)[k] = reinterpret_cast<const uint16_t*>(from)[k];
+#pragma unroll
+          for (int k = 0; k < kPer - 1; ++k) {
+            if (n + k >= left) break;
+            if constexpr (SIZE == 4) reinterpret_cast<int*>(to)[k] = v[t][k];
+            else reinterpret_cast<uint16_t*>(to)[k] = (uint16_t)((uint32_t)v[t][k / 2] >> (16 * (k % 2)));
           }
         }
       }
+    }
+  }
+  template <int N>
+  static __device__ __forceinline__ void lds_read16(i32x4_t (&v)[N], const uint32_t (&a)[N]) {
+    if constexpr (N == 2) {
+      asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(v[0]), "=&v"(v[1]) : "v"(a[0]), "v"(a[1]) : "memory");
+    } else {
+      qmoe_gemm::lds_read16_all(v, a);
     }
   }
 };
@@ -261,77 +335,141 @@ template <class... Forms>
 struct Pick;
 template <class F>
 struct Pick<F> {
-  static constexpr int kRing = F::kRing, kStaged = 32 * F::WM * F::kCols * 4;
-  static __device__ __forceinline__ void run(const Product& a, const Unit& u, char* smem, float* sx, float* sw) {
-    F::run(a, u, smem, sx, sw);
-  }
+  template <class... A>
+  static __device__ __forceinline__ void run(const Product& a, const Unit& u, A&&... rest) { F::run(a, u, rest...); }
 };
 template <class F, class G, class... Rest>
 struct Pick<F, G, Rest...> {
-  typedef Pick<G, Rest...> Next;
-  static constexpr int kRing = F::kRing > Next::kRing ? F::kRing : Next::kRing;
-  static constexpr int kStaged = Pick<F>::kStaged > Next::kStaged ? Pick<F>::kStaged : Next::kStaged;
-  static __device__ __forceinline__ void run(const Product& a, const Unit& u, char* smem, float* sx, float* sw) {
-    if (u.valid > G::kRows) F::run(a, u, smem, sx, sw);
-    else Next::run(a, u, smem, sx, sw);
+  template <class... A>
+  static __device__ __forceinline__ void run(const Product& a, const Unit& u, A&&... rest) {
+    if (u.valid > G::kRows) F::run(a, u, rest...);
+    else Pick<G, Rest...>::run(a, u, rest...);
   }
 };
+typedef Pick<Form<2, 4, 4, 2, 2>, Form<2, 4, 3, 2, 2>, Form<2, 4, 2, 2, 3>, Form<1, 8, 3, 1, 3>, Form<1, 8, 2, 1, 3>,
+             Form<1, 8, 1, 1, 3>> Forms;
 
-// ROWS: rows of a unit; BLOCKS per CU.
-template <class Forms, int ROWS, int COLS, int BLOCKS>
-__global__ __launch_bounds__(256, BLOCKS) void int8_gemm_kernel(Product a, int64_t row_units, int NB) {
-  constexpr int kSmem = Forms::kRing > Forms::kStaged ? Forms::kRing : Forms::kStaged;
-  constexpr bool kTable = ROWS == kTileRows;  // a tile table's units are its tiles
-  constexpr int kOrder = kTable ? qmoe_gemm::kMaxOrder : 1;
-  static_assert(BLOCKS * (kSmem + 4 * (ROWS + COLS + kOrder)) <= kLdsCU, "LDS per CU");
-  __shared__ __attribute__((aligned(16))) char smem[kSmem];
-  __shared__ __attribute__((aligned(16))) float sx[ROWS], sw[COLS];
-  __shared__ int order[kOrder];
+// The rows of tile t's unit, 0 for the second tile of a pair.
+__device__ __forceinline__ qmoe_gemm::TileRows pair_rows_of(const qmoe_gemm::Tiles& t, int tile) {
+  qmoe_gemm::TileRows r = qmoe_gemm::tile_rows_of(t, tile);
+  const int64_t first = t.offsets[r.e], end = min((int64_t)t.offsets[r.e + 1], t.n_rows);
+  r.valid = r.valid <= 0 || ((r.row0 - first) / kTileRows) % 2 ? 0 : (int)min((int64_t)kPairRows, end - r.row0);
+  return r;
+}
+
+// Ranks the units of `tiles` (<= kMaxRanked) tiles by their 32-row subtiles,
+// largest first and stable in tile order; returns how many there are.  cls is
+// scratch of kMaxRanked + 1 ints.  Called by the whole block.
+constexpr int kMaxRanked = 1024;
+__device__ inline int rank_pairs(const qmoe_gemm::Tiles& t, int tiles, int* order, int* cls) {
+  for (int i = threadIdx.x; i < tiles; i += kThreads) cls[i] = (pair_rows_of(t, i).valid + 31) / 32;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+    constexpr int kClasses = kPairRows / 32;
+    int start[kClasses + 1] = {};
+    for (int i = 0; i < tiles; i += 64) {
+      const int m = i + lane < tiles ? cls[i + lane] : 0;
+#pragma unroll
+      for (int k = 1; k <= kClasses; ++k) start[k] += __popcll(__ballot(m == k));
+    }
+    int sum = 0;
+#pragma unroll
+    for (int k = kClasses; k >= 1; --k) {
+      const int n = start[k];
+      start[k] = sum;
+      sum += n;
+    }
+    if (lane == 0) cls[kMaxRanked] = sum;
+    for (int i = 0; i < tiles; i += 64) {
+      const int m = i + lane < tiles ? cls[i + lane] : 0;
+#pragma unroll
+      for (int k = 1; k <= kClasses; ++k) {
+        const uint64_t same = __ballot(m == k);
+        if (m == k) order[start[k] + __popcll(same & below)] = i + lane;
+        start[k] += __popcll(same);
+      }
+    }
+  }
+  __syncthreads();
+  const int units = cls[kMaxRanked];
+  __syncthreads();  // cls is free
+  return units;
+}
+
+// row_units, unit_rows: of one matrix (unit_rows <= kPairRows); a table's units are its own.
+__global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t row_units, int unit_rows, int NB) {
+  __shared__ __attribute__((aligned(16))) char smem[kRing];
+  __shared__ __attribute__((aligned(16))) float scales[2][kPairRows + kCols];  // of this unit and the next
+  __shared__ int order[kMaxRanked];
+  static_assert(kRing + sizeof(scales) + sizeof(order) <= kLdsCU, "LDS per CU");
+  static_assert(2 * kStaging <= kRing && kRing >= 4 * (kMaxRanked + 1), "the staged results; the ranking's scratch");
   const qmoe_gemm::Tiles table{a.offsets, a.tile_row, a.tile_exp, a.ntiles, a.n_rows, a.num_experts};
   bool ranked = false;
-  if (kTable && a.offsets) {
+  if (a.offsets) {
     row_units = max(a.ntiles[0], 0);
-    ranked = row_units <= kOrder;
-    if (ranked) qmoe_gemm::rank_tiles(table, (int)row_units, order, reinterpret_cast<int*>(smem));
+    ranked = row_units <= kMaxRanked;
+    if (ranked) row_units = rank_pairs(table, (int)row_units, order, reinterpret_cast<int*>(smem));
   }
   const qmoe_gemm::Snake snake(row_units * NB);
-  constexpr int kBand = 2048 / COLS;  // column blocks of a band
-  for (int64_t k = 0;; ++k) {
-    const int64_t at = snake.unit(k);
-    if (at < 0) break;
-    Unit u;
-    int col;
-    if (kTable && a.offsets) {
-      const int64_t tile = at / NB;
-      col = (int)(at % NB);
-      const qmoe_gemm::TileRows t = qmoe_gemm::tile_rows_of(table, ranked ? order[tile] : (int)tile);
-      u.e = __builtin_amdgcn_readfirstlane(t.e);
-      u.valid = __builtin_amdgcn_readfirstlane(t.valid);
-      u.row0 = qmoe_gemm::uniform64(t.row0);
-    } else {
-      const int64_t band = at / (row_units * kBand), in = at % (row_units * kBand);
-      const int wide = (int)min((int64_t)kBand, NB - band * kBand);
-      col = (int)(band * kBand + in % wide);
-      u.e = 0;
-      u.row0 = in / wide * ROWS;
-      u.valid = (int)min((int64_t)ROWS, a.n_rows - u.row0);
+  constexpr int kBand = 8;  // column blocks of a band
+  // Every second XCD takes its units lightest first, from four rounds on: long
+  // units are bound by the matrix cores, short ones by their weights' way from
+  // HBM, and so both kinds are under way at once (five rounds, 4096 tokens x
+  // top-10 of 256: 174 -> 167 us; two rounds: 60 -> 62).
+  const int64_t rounds = (snake.units + snake.P - 1) / snake.P;
+  const bool reversed = a.offsets && rounds >= 4 && snake.q / (snake.P / 8) % 2;
+  int64_t round = 0;
+  const auto next = [&] {  // this block's next unit
+    Unit u{0, 0, 0, 0};
+    for (;;) {
+      if (round == rounds) return u;
+      const int64_t at = snake.unit(reversed ? rounds - 1 - round : round);
+      ++round;
+      if (at < 0) continue;
+      int col;
+      if (a.offsets) {
+        const int64_t tile = at / NB;
+        col = (int)(at % NB);
+        const qmoe_gemm::TileRows t = pair_rows_of(table, ranked ? order[tile] : (int)tile);
+        u.e = __builtin_amdgcn_readfirstlane(t.e);
+        u.valid = __builtin_amdgcn_readfirstlane(t.valid);
+        u.row0 = qmoe_gemm::uniform64(t.row0);
+      } else {
+        const int64_t band = at / (row_units * kBand), in = at % (row_units * kBand);
+        const int wide = (int)min((int64_t)kBand, NB - band * kBand);
+        col = (int)(band * kBand + in % wide);
+        u.row0 = in / wide * unit_rows;
+        u.valid = (int)min((int64_t)unit_rows, a.n_rows - u.row0);
+      }
+      u.o0 = (int64_t)__builtin_amdgcn_readfirstlane(col) * kCols;
+      if (u.valid > 0) return u;
     }
-    if (u.valid <= 0) continue;
-    u.o0 = (int64_t)__builtin_amdgcn_readfirstlane(col) * COLS;
-    Forms::run(a, u, smem, sx, sw);
-    __syncthreads();  // the ring and the scales are free for the next unit
+  };
+  Unit u = next();
+  if (u.valid <= 0) return;
+  Ctx c = begin(a, u, rows_of(a, u), smem, scales[0]);
+  for (int s = 0;; s ^= 1) {
+    // the next unit's rows, while this one's first copies are under way
+    const Unit v = next();
+    Rows rows = {};
+    if (v.valid > 0) rows = rows_of(a, v);
+    Ctx d;
+    Forms::run(a, u, c, smem, scales[s], [&] {
+      if (v.valid > 0) d = begin(a, v, rows, smem, scales[s ^ 1]);
+    });
+    if (v.valid <= 0) break;
+    u = v;
+    c = d;
   }
 }
 
-// 256 x 256 outputs, one block per CU; 128 x 256, two, with shorter forms for the ends of segments.
-typedef Pick<Form<2, 2, 4, 4, 128, 2>> Wide;
-typedef Pick<Form<2, 2, 2, 4, 64, 3>, Form<1, 4, 2, 2, 64, 3>> Tile;
-
-template <class Forms, int ROWS, int BLOCKS>
-void launch(const Product& a, int64_t max_tiles, hipStream_t st) {
-  const int64_t NB = (a.N + 255) / 256, rows = a.offsets ? max_tiles : (a.n_rows + ROWS - 1) / ROWS;
-  const dim3 grid((unsigned)qmoe_gemm::grid_blocks(rows * NB, BLOCKS));
-  int8_gemm_kernel<Forms, ROWS, 256, BLOCKS><<<grid, dim3(256), 0, st>>>(a, rows, (int)NB);
+int launch(const Product& a, int64_t max_tiles, int unit_rows, hipStream_t st) {
+  const int64_t NB = (a.N + kCols - 1) / kCols, rows = a.offsets ? max_tiles : (a.n_rows + unit_rows - 1) / unit_rows;
+  const dim3 grid((unsigned)qmoe_gemm::grid_blocks(rows * NB, 1));
+  int8_gemm_kernel<<<grid, dim3(kThreads), 0, st>>>(a, rows, unit_rows, (int)NB);
+  return qmoe::launch_status("int8_gemm_kernel");
 }
 
 }  // namespace
@@ -350,9 +488,6 @@ extern "C" int qmoe_int8_gather_qqmm(const int8_t* x, const float* sx, int64_t n
   if (!any && !x_rows && n_x < n_rows) return qmoe::fail(QMOE_ERR_INVALID, "fewer activation rows than rows");
   if (any && max_tiles <= 0) return qmoe::fail(QMOE_ERR_INVALID, "an empty tile table");
   if (max_tiles > 0x7FFFFFFF) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
-  hipStream_t st = qmoe::as_stream(stream);
-  const int64_t wide = (n_rows + 255) / 256 * ((N + 255) / 256);
-  if (!any && wide >= 192) launch<Wide, 256, 1>(a, max_tiles, st);
-  else launch<Tile, kTileRows, 2>(a, max_tiles, st);
-  return qmoe::launch_status("int8_gemm_kernel");
+  const int64_t wide = (n_rows + kPairRows - 1) / kPairRows * ((N + kCols - 1) / kCols);
+  return launch(a, max_tiles, any || wide >= 192 ? kPairRows : kTileRows, qmoe::as_stream(stream));
 }

@@ -33,11 +33,16 @@ __device__ __forceinline__ int64_t x_row_of(const Product& a, int64_t r) {
   return min(max(t, (int64_t)0), a.n_x - 1);
 }
 
-// A sum times both scales, the smaller first: the product of the sum and the
-// smaller scale overflows only where the result does, and loses nothing to
-// underflow that the result keeps.
+// A sum times both scales: the row's first where it is of ordinary size, so
+// that the product with it neither overflows nor underflows, else the smaller
+// one first, whose product overflows only where the result does and loses
+// nothing to underflow that the result keeps.
+__device__ __forceinline__ bool ordinary(float sx) {
+  const float v = fabsf(sx);
+  return (v >= 0x1p-60f && v <= 0x1p60f) || v == 0.f;
+}
 __device__ __forceinline__ float scaled(int acc, float sx, float sw) {
-  const bool first = fabsf(sx) < fabsf(sw);
+  const bool first = ordinary(sx) || fabsf(sx) < fabsf(sw);
   return (float)acc * (first ? sx : sw) * (first ? sw : sx);
 }
 __device__ __forceinline__ void put(const Product& a, int64_t i, float v) {
