@@ -589,8 +589,7 @@ int qmoe_int8_dequantize(const int8_t* codes, const float* scales,
  * rows' type (residual NULL: h = x), v = h / sqrt(mean(h^2) + eps) * weight
  * [D] (of the rows' type or fp32; NULL: ones) in fp32, the squares summed in
  * 64 bits; codes and scales of v; sum = h and norm = v in the rows' type,
- * either NULL: not written.  sum may be x or residual, and norm may be x or
- * residual where sum is not the same buffer. */
+ * either NULL: not written.  No output may overlap an input. */
 int qmoe_int8_rms_norm(const void* x, const void* residual, const void* weight,
                        int weight_dtype, int dtype, int64_t rows, int64_t D,
                        double eps, int8_t* codes, float* scales, void* sum,

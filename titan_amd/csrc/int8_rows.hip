@@ -8,11 +8,18 @@
 // A row that holds a NaN or an infinity has the scale NaN and codes 0, so that
 // it reads back as NaN throughout and spoils no other row.  The squares are
 // summed in 64 bits: no value of the types overflows or vanishes there.
+//
+// A row belongs to a wave, four waves or sixteen, whose threads keep it in
+// registers between its passes (the sum of squares, the largest value, the
+// codes); longer rows are read again for each.  Threads move 16 bytes at a time
+// at whatever address a row begins.  Bound by HBM from some thousands of rows
+// on (norm of 8192 x 2048 bf16 with the residual, its sum and the norm written:
+// 21 us, 7.2 TB/s, some of it from the caches; 65536 x 2048 fp32 to codes:
+// 126 us, 5.3 TB/s), by one chain of loads, two reductions and the stores below
+// (one row of 2048: 2.9 us per call in a graph, quantised alone 2.2).
 #include "elem.h"
 
 namespace {
-
-constexpr int kThreads = 256;
 
 // Larger |v| have larger bits, infinities and NaN the largest.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
@@ -26,12 +33,137 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return top >= kInfinite ? __uint_as_float(0x7FC00000u) : __fdiv_rn(__uint_as_float(top), 127.f);
 }
 
+// v combined over the wave, in every lane: DPP moves within a row of sixteen
+// lanes, then swaps of rows and of halves.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <class T, class Op>
+__device__ __forceinline__ T over_wave(T v, Op op) {
+  constexpr int W = sizeof(T) / 4;
+  struct Words {
+    uint32_t w[W];
+  };
+  const auto step = [&](auto move) {
+    const Words a = __builtin_bit_cast(Words, v);
+    Words b;
+#pragma unroll
+    for (int i = 0; i < W; ++i) b.w[i] = move(a.w[i]);
+    v = op(v, __builtin_bit_cast(T, b));
+  };
+  step([](uint32_t x) { return dpp<0xB1>(x); });   // quad_perm 1,0,3,2
+  step([](uint32_t x) { return dpp<0x4E>(x); });   // quad_perm 2,3,0,1
+  step([](uint32_t x) { return dpp<0x141>(x); });  // row_half_mirror
+  step([](uint32_t x) { return dpp<0x128>(x); });  // row_ror:8
+  const auto swap = [&](auto pair) {  // pair gives both rows' (halves') values to both
+    const Words a = __builtin_bit_cast(Words, v);
+    Words b, c;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const auto p = pair(a.w[i]);
+      b.w[i] = p[0], c.w[i] = p[1];
+    }
+    v = op(__builtin_bit_cast(T, b), __builtin_bit_cast(T, c));
+  };
+  swap([](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+  swap([](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+  return v;
+}
+// .. and over the TPR threads of a row (whole waves; the whole block from two waves on).
+template <int TPR, class T, class Op>
+__device__ __forceinline__ T over_row(T v, T* shared, Op op) {
+  v = over_wave(v, op);
+  if constexpr (TPR > 64) {
+    constexpr int kW = TPR / 64;
+    if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = shared[0];
+#pragma unroll
+    for (int i = 1; i < kW; ++i) v = op(v, shared[i]);
+  }
+  return v;
+}
+
+// N elements at any element's address.
+template <class T, int N>
+struct __attribute__((packed)) Loose {
+  typename Vec<T, N>::V v __attribute__((aligned(1)));
+};
+template <class T, int N>
+__device__ __forceinline__ typename Vec<T, N>::V get(const T* p) {
+  return reinterpret_cast<const Loose<T, N>*>(p)->v;
+}
+template <class T, int N>
+__device__ __forceinline__ void put(T* p, typename Vec<T, N>::V v) {
+  reinterpret_cast<Loose<T, N>*>(p)->v = v;
+}
+// .. the first `there` of which exist.
+template <class T, int N>
+__device__ __forceinline__ typename Vec<T, N>::V get(const T* p, int there) {
+  if (there >= N) return get<T, N>(p);
+  typename Vec<T, N>::V v = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < there) v[i] = p[i];
+  return v;
+}
+template <class T, int N>
+__device__ __forceinline__ void put(T* p, int there, typename Vec<T, N>::V v) {
+  if (there >= N) return put<T, N>(p, v);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < there) p[i] = v[i];
+}
+
+// The codes of N values, four to a word.  Within |scale| limits the quotient is
+// taken as v times the scale's reciprocal, which is off by less than 3e-5 of a
+// code from the rounded quotient: where that could matter, the division decides.
+struct Coder {
+  float s, inv;
+  bool quick;
+  __device__ __forceinline__ explicit Coder(float scale)
+      : s(scale), inv(1.f / scale), quick(scale >= 0x1p-100f && scale <= 0x1p100f) {}
+  template <int N>
+  __device__ __forceinline__ void codes(const float (&v)[N], uint32_t (&out)[N / 4]) const {
+    constexpr float kMagic = 0x1.8p23f;  // added to a small number: its nearest integer in the low bits
+    float off = 1.f;
+    if (quick) {
+      off = 0.f;
+      uint32_t b[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float t = __builtin_fmaf(v[i], inv, kMagic);
+        b[i] = __float_as_uint(t);
+        off = fmaxf(off, fabsf(__builtin_fmaf(v[i], inv, kMagic - t)));
+      }
+#pragma unroll
+      for (int i = 0; i < N; i += 4)
+        out[i / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[i + 3], b[i + 2], 0x0C0C0400u),
+                                           __builtin_amdgcn_perm(b[i + 1], b[i], 0x0C0C0400u), 0x05040100u);
+    }
+    if (__any(!(off <= 0.5f - 3e-5f))) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4)
+        out[i / 4] = (uint32_t)(code_of(v[i], s) & 255) | (uint32_t)(code_of(v[i + 1], s) & 255) << 8 |
+                     (uint32_t)(code_of(v[i + 2], s) & 255) << 16 | (uint32_t)code_of(v[i + 3], s) << 24;
+    }
+  }
+};
+
+// The rounding to the type in one instruction.
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::T rounded(float f) {
+  if constexpr (DT == QMOE_BF16) return __builtin_bit_cast(uint16_t, (__bf16)f);
+  else return Elem<DT>::store(f);
+}
+
 struct RowArgs {
   const void* x;
   const void* r;  // the residual; null: none
   const void* w;  // the norm's weight, of the rows' type or fp32; null: ones
   int w_f32;
-  int64_t D;
+  int64_t rows, D;
   double eps;
   int8_t* q;
   float* s;
@@ -39,79 +171,182 @@ struct RowArgs {
   void* norm;  // v in the rows' type; null: not written
 };
 
-// One block per row.
-template <int DT, bool NORM>
-__global__ __launch_bounds__(kThreads) void int8_rows_kernel(RowArgs a) {
+template <int DT>
+constexpr int kVec = 16 / sizeof(typename Elem<DT>::T);
+
+// TPR threads per row, blocks of at least 256; NV vectors of N elements per
+// thread in registers, 0: rows of any length, read again.  A row's last vector
+// ends with it: where N does not divide D it overlaps the one before, whose
+// elements it has as well (they are counted once).  No load stands in a branch,
+// so that all of a thread's are under way together.  D < N: one vector of which
+// D elements exist (SHORT).
+template <int DT, bool NORM, int TPR, int NV, bool SHORT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(RowArgs a) {
   typedef typename Elem<DT>::T T;
-  __shared__ double sums[kThreads / 64];
-  __shared__ uint32_t tops[kThreads / 64];
-  const int64_t row = blockIdx.x, base = row * a.D;
+  constexpr int N = kVec<DT>, kKept = NV ? NV : 1;
+  typedef typename Vec<T, N>::V V;
+  __shared__ double sums[TPR / 64];
+  __shared__ uint32_t tops[TPR / 64];
+  const int64_t row = TPR < 256 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x;
+  if (row >= a.rows) return;
+  const int lane = threadIdx.x % TPR, D = (int)a.D, there = SHORT ? D : N;
+  const int64_t base = row * a.D;
   const T* x = static_cast<const T*>(a.x) + base;
-  const T* r = a.r ? static_cast<const T*>(a.r) + base : nullptr;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const auto h_of = [&](int64_t c) {
-    const float v = Elem<DT>::load(x[c]);
-    return r ? Elem<DT>::load(Elem<DT>::store(v + Elem<DT>::load(r[c]))) : v;
+  const T* r = NORM && a.r ? static_cast<const T*>(a.r) + base : nullptr;
+  const int64_t vecs = (a.D + N - 1) / N;
+  const auto place = [&](int64_t i) { return SHORT ? 0 : (int)min(i * N, (int64_t)D - N); };
+  // f(place in the registers, first element, element that the vector begins with as its own) for this thread's vectors
+  const auto each = [&](auto f) {
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) f(k, place(lane + k * TPR), (int64_t)(lane + k * TPR) * N);
+    } else {
+      for (int64_t i = lane; i < vecs; i += TPR) f(0, place(i), i * N);
+    }
   };
+  V xv[kKept], rv[kKept];
+  const auto load = [&](int k, int c) {
+    xv[k] = get<T, N>(x + c, there);
+    if (NORM && r) rv[k] = get<T, N>(r + c, there);
+  };
+  float kept[kKept][N];
+  const auto h = [&](int k, int c) {
+    if (!NV) load(k, c);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      kept[k][i] = Elem<DT>::load(xv[k][i]);
+      if (NORM && r) kept[k][i] = Elem<DT>::load(rounded<DT>(kept[k][i] + Elem<DT>::load(rv[k][i])));
+    }
+  };
+  const auto narrow = [&](int k) {
+    V o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = rounded<DT>(kept[k][i]);
+    return o;
+  };
+  each([&](int k, int c, int64_t) {
+    if (NV) load(k, c);
+  });
+  if constexpr (NV > 0) each([&](int k, int c, int64_t) { h(k, c); });
   float rstd = 1.f;
   if constexpr (NORM) {
     double ss = 0.0;
-    for (int64_t c = threadIdx.x; c < a.D; c += kThreads) {
-      const float h = h_of(c);
-      if (a.sum) static_cast<T*>(a.sum)[base + c] = Elem<DT>::store(h);
-      ss = fma((double)h, (double)h, ss);
-    }
+    each([&](int k, int c, int64_t own) {
+      if (!NV) h(k, c);
+      if (a.sum && own < a.D) put<T, N>(static_cast<T*>(a.sum) + base + c, there, narrow(k));
+      if (__any(own != c)) {
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
-    if (lane == 0) sums[wave] = ss;
-    __syncthreads();
-    ss = sums[0];
+        for (int i = 0; i < N; ++i)
+          if (c + i >= own && i < there) ss = fma((double)kept[k][i], (double)kept[k][i], ss);
+      } else {
 #pragma unroll
-    for (int i = 1; i < kThreads / 64; ++i) ss += sums[i];
+        for (int i = 0; i < N; ++i) ss = fma((double)kept[k][i], (double)kept[k][i], ss);
+      }
+    });
+    ss = over_row<TPR>(ss, sums, [](double p, double q) { return p + q; });
     rstd = (float)(1.0 / sqrt(ss / (double)a.D + a.eps));
   }
-  const auto v_of = [&](int64_t c) {
-    float v = h_of(c);
-    if constexpr (NORM) {
-      v *= rstd;
-      if (a.w) v *= a.w_f32 ? static_cast<const float*>(a.w)[c] : Elem<DT>::load(static_cast<const T*>(a.w)[c]);
+  const auto normed = [&](int k, int c) {
+    if constexpr (!NORM) return;
+    if (!a.w) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) kept[k][i] *= rstd;
+    } else if (a.w_f32) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const typename Vec<float, 4>::V q = get<float, 4>(static_cast<const float*>(a.w) + c + i, there - i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kept[k][i + j] = kept[k][i + j] * rstd * q[j];
+      }
+    } else {
+      const V q = get<T, N>(static_cast<const T*>(a.w) + c, there);
+#pragma unroll
+      for (int i = 0; i < N; ++i) kept[k][i] = kept[k][i] * rstd * Elem<DT>::load(q[i]);
     }
-    return v;
   };
   uint32_t top = 0;
-  for (int64_t c = threadIdx.x; c < a.D; c += kThreads) top = max(top, magnitude(v_of(c)));
+  each([&](int k, int c, int64_t) {
+    if (!NV) h(k, c);
+    normed(k, c);
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
-  if (lane == 0) tops[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) top = max(top, tops[i]);
+    for (int i = 0; i < N; ++i) top = max(top, i < there ? magnitude(kept[k][i]) : 0u);
+  });
+  top = over_row<TPR>(top, tops, [](uint32_t p, uint32_t q) { return max(p, q); });
   const float s = scale_of(top);
-  if (threadIdx.x == 0) a.s[row] = s;
-  for (int64_t c = threadIdx.x; c < a.D; c += kThreads) {
-    const float v = v_of(c);
-    a.q[base + c] = (int8_t)code_of(v, s);
-    if (NORM && a.norm) static_cast<T*>(a.norm)[base + c] = Elem<DT>::store(v);
+  if (lane == 0) a.s[row] = s;
+  const Coder coder(s);
+  each([&](int k, int c, int64_t own) {
+    if (!NV) {
+      h(k, c);
+      normed(k, c);
+    }
+    uint32_t code[N / 4];
+    coder.codes(kept[k], code);
+    if (own >= a.D) return;
+    if (NORM && a.norm) put<T, N>(static_cast<T*>(a.norm) + base + c, there, narrow(k));
+    put<uint8_t, N>(reinterpret_cast<uint8_t*>(a.q) + base + c, there, __builtin_bit_cast(typename Vec<uint8_t, N>::V, code));
+  });
+}
+
+// Codes times their row's scale: TPR threads per row, 256 per block.
+template <int DT, int TPR>
+__global__ __launch_bounds__(256) void int8_values_kernel(const int8_t* __restrict__ q, const float* __restrict__ s,
+                                                          int64_t rows, int64_t D, typename Elem<DT>::T* __restrict__ out) {
+  typedef typename Elem<DT>::T T;
+  constexpr int N = kVec<DT>;
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (row >= rows) return;
+  const int64_t base = row * D;
+  const float sc = s[row];
+  for (int64_t own = (threadIdx.x % TPR) * N; own < D; own += TPR * N) {
+    const int64_t c = D < N ? 0 : min(own, D - N);  // the last vector ends with the row
+    const int there = (int)min(D, (int64_t)N);
+    const typename Vec<int8_t, N>::V v = get<int8_t, N>(q + base + c, there);
+    typename Vec<T, N>::V o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = rounded<DT>((float)v[i] * sc);
+    put<T, N>(out + base + c, there, o);
   }
 }
 
-// One block per row: codes times the row's scale.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void int8_values_kernel(const int8_t* __restrict__ q, const float* __restrict__ s,
-                                                               int64_t D, typename Elem<DT>::T* __restrict__ out) {
-  const int64_t base = (int64_t)blockIdx.x * D;
-  const float sc = s[blockIdx.x];
-  for (int64_t c = threadIdx.x; c < D; c += kThreads) out[base + c] = Elem<DT>::store((float)q[base + c] * sc);
+template <int DT, bool NORM, int TPR, int NV, bool SHORT = false>
+void launch_form(const RowArgs& a, hipStream_t st) {
+  constexpr int kPer = TPR < 256 ? 256 / TPR : 1;
+  int8_rows_kernel<DT, NORM, TPR, NV, SHORT><<<dim3((unsigned)((a.rows + kPer - 1) / kPer)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(a);
 }
-
+// A wave per row where the rows alone fill the chip and a thread holds up to
+// four vectors, else a vector per thread where that is possible: a thread's
+// vectors cost 1 to 2 us each one after the other.  Norms of bf16 rows, wave /
+// four waves per row (us): 1024 x 1000 5.1 / 5.9, 512 x 2048 6.9 / 5.0, 2048 x
+// 2048 8.9 / 9.1, 4096 x 4096 (eight vectors a thread / two) 24.5 / 20.6.
+template <int DT, bool NORM>
+void launch_type(const RowArgs& a, hipStream_t st) {
+  const int64_t vecs = (a.D + kVec<DT> - 1) / kVec<DT>;
+  if (a.D < kVec<DT>) launch_form<DT, NORM, 64, 1, true>(a, st);
+  else if (vecs <= 64) launch_form<DT, NORM, 64, 1>(a, st);
+  else if (vecs <= 128 && a.rows >= 1024) launch_form<DT, NORM, 64, 2>(a, st);
+  else if (vecs <= 256 && a.rows >= 2048) launch_form<DT, NORM, 64, 4>(a, st);
+  else if (vecs <= 256) launch_form<DT, NORM, 256, 1>(a, st);
+  else if (vecs <= 512) launch_form<DT, NORM, 256, 2>(a, st);
+  else if (vecs <= 1024) launch_form<DT, NORM, 1024, 1>(a, st);
+  else if (vecs <= 4096) launch_form<DT, NORM, 1024, 4>(a, st);
+  else launch_form<DT, NORM, 1024, 0>(a, st);
+}
 template <bool NORM>
-int launch_rows(const RowArgs& a, int64_t rows, int dtype, hipStream_t st) {
-  const dim3 grid((unsigned)rows), block(kThreads);
-  if (dtype == QMOE_BF16) int8_rows_kernel<QMOE_BF16, NORM><<<grid, block, 0, st>>>(a);
-  else if (dtype == QMOE_FP16) int8_rows_kernel<QMOE_FP16, NORM><<<grid, block, 0, st>>>(a);
-  else int8_rows_kernel<QMOE_FP32, NORM><<<grid, block, 0, st>>>(a);
+int launch_rows(const RowArgs& a, int dtype, hipStream_t st) {
+  if (dtype == QMOE_BF16) launch_type<QMOE_BF16, NORM>(a, st);
+  else if (dtype == QMOE_FP16) launch_type<QMOE_FP16, NORM>(a, st);
+  else launch_type<QMOE_FP32, NORM>(a, st);
   return qmoe::launch_status("int8_rows_kernel");
 }
+template <int DT>
+void launch_values(const int8_t* q, const float* s, int64_t rows, int64_t D, void* out, hipStream_t st) {
+  typedef typename Elem<DT>::T T;
+  if (D <= 64 * kVec<DT>) int8_values_kernel<DT, 64><<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st>>>(q, s, rows, D, static_cast<T*>(out));
+  else int8_values_kernel<DT, 256><<<dim3((unsigned)rows), dim3(256), 0, st>>>(q, s, rows, D, static_cast<T*>(out));
+}
+
+constexpr int kThreads = 1024;  // of a block, at most
 
 // QMOE_OK with *run = false: nothing to do.
 int check_rows(int64_t rows, int64_t D, int dtype, const void* in, const int8_t* q, const float* s, bool* run) {
@@ -134,7 +369,7 @@ extern "C" int qmoe_int8_quantize(const void* x, int dtype, int64_t rows, int64_
   const int rc = check_rows(rows, K, dtype, x, codes, scales, &run);
   if (rc != QMOE_OK || !run) return rc;
   if (!qmoe::aligned16(x) || !qmoe::aligned16(codes)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "x and codes must be 16-byte aligned");
-  return launch_rows<false>({x, nullptr, nullptr, 0, K, 0.0, codes, scales, nullptr, nullptr}, rows, dtype,
+  return launch_rows<false>({x, nullptr, nullptr, 0, rows, K, 0.0, codes, scales, nullptr, nullptr}, dtype,
                             qmoe::as_stream(stream));
 }
 
@@ -145,10 +380,9 @@ extern "C" int qmoe_int8_dequantize(const int8_t* codes, const float* scales, in
   if (rc != QMOE_OK || !run || K == 0) return rc;
   if (!qmoe::aligned16(out) || !qmoe::aligned16(codes)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "codes and out must be 16-byte aligned");
   hipStream_t st = qmoe::as_stream(stream);
-  const dim3 grid((unsigned)rows), block(kThreads);
-  if (dtype == QMOE_BF16) int8_values_kernel<QMOE_BF16><<<grid, block, 0, st>>>(codes, scales, K, static_cast<uint16_t*>(out));
-  else if (dtype == QMOE_FP16) int8_values_kernel<QMOE_FP16><<<grid, block, 0, st>>>(codes, scales, K, static_cast<_Float16*>(out));
-  else int8_values_kernel<QMOE_FP32><<<grid, block, 0, st>>>(codes, scales, K, static_cast<float*>(out));
+  if (dtype == QMOE_BF16) launch_values<QMOE_BF16>(codes, scales, rows, K, out, st);
+  else if (dtype == QMOE_FP16) launch_values<QMOE_FP16>(codes, scales, rows, K, out, st);
+  else launch_values<QMOE_FP32>(codes, scales, rows, K, out, st);
   return qmoe::launch_status("int8_values_kernel");
 }
 
@@ -165,6 +399,6 @@ extern "C" int qmoe_int8_rms_norm(const void* x, const void* residual, const voi
   if (D == 0) return qmoe::fail(QMOE_ERR_INVALID, "rows without elements have no norm");
   for (const void* p : {x, residual, weight, (const void*)codes, (const void*)sum, (const void*)norm})
     if (!qmoe::aligned16(p)) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "the rows and the weight must be 16-byte aligned");
-  return launch_rows<true>({x, residual, weight, weight_dtype == QMOE_FP32, D, eps, codes, scales, sum, norm}, rows,
-                           dtype, qmoe::as_stream(stream));
+  return launch_rows<true>({x, residual, weight, weight_dtype == QMOE_FP32, rows, D, eps, codes, scales, sum, norm}, dtype,
+                           qmoe::as_stream(stream));
 }
