@@ -631,7 +631,8 @@ int qmoe_int8_gather_qqmm(const int8_t* x, const float* sx, int64_t n_x,
  * and the gradient of dloss * loss by the logits, the counts being constants:
  * exactly 0 for masked tokens.  logits and dlogits are QMOE_BF16, _FP16 or
  * _FP32 and 16-byte aligned, E <= 1024; sums over tokens go in a fixed order.
- * The workspace has qmoe_router_balance_workspace_size(T, E) bytes. */
+ * The workspace has qmoe_router_balance_workspace_size(T, E) bytes, 8-byte
+ * aligned, and is one call's at a time. */
 size_t qmoe_router_balance_workspace_size(int64_t T, int64_t E);
 int qmoe_router_balance(const void* logits, int dtype, int64_t T, int64_t E,
                         const void* ids, int ids64, int64_t k,

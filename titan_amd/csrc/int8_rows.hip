@@ -18,6 +18,7 @@
 // 126 us, 5.3 TB/s), by one chain of loads, two reductions and the stores below
 // (one row of 2048: 2.9 us per call in a graph, quantised alone 2.2).
 #include "elem.h"
+#include "lanes.h"
 
 namespace {
 
@@ -33,47 +34,10 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   return top >= kInfinite ? __uint_as_float(0x7FC00000u) : __fdiv_rn(__uint_as_float(top), 127.f);
 }
 
-// v combined over the wave, in every lane: DPP moves within a row of sixteen
-// lanes, then swaps of rows and of halves.
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
-}
-template <class T, class Op>
-__device__ __forceinline__ T over_wave(T v, Op op) {
-  constexpr int W = sizeof(T) / 4;
-  struct Words {
-    uint32_t w[W];
-  };
-  const auto step = [&](auto move) {
-    const Words a = __builtin_bit_cast(Words, v);
-    Words b;
-#pragma unroll
-    for (int i = 0; i < W; ++i) b.w[i] = move(a.w[i]);
-    v = op(v, __builtin_bit_cast(T, b));
-  };
-  step([](uint32_t x) { return dpp<0xB1>(x); });   // quad_perm 1,0,3,2
-  step([](uint32_t x) { return dpp<0x4E>(x); });   // quad_perm 2,3,0,1
-  step([](uint32_t x) { return dpp<0x141>(x); });  // row_half_mirror
-  step([](uint32_t x) { return dpp<0x128>(x); });  // row_ror:8
-  const auto swap = [&](auto pair) {  // pair gives both rows' (halves') values to both
-    const Words a = __builtin_bit_cast(Words, v);
-    Words b, c;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const auto p = pair(a.w[i]);
-      b.w[i] = p[0], c.w[i] = p[1];
-    }
-    v = op(__builtin_bit_cast(T, b), __builtin_bit_cast(T, c));
-  };
-  swap([](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
-  swap([](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
-  return v;
-}
-// .. and over the TPR threads of a row (whole waves; the whole block from two waves on).
+// v combined over the TPR threads of a row (whole waves; the whole block from two waves on).
 template <int TPR, class T, class Op>
 __device__ __forceinline__ T over_row(T v, T* shared, Op op) {
-  v = over_wave(v, op);
+  v = qmoe_lanes::over<64>(v, op);
   if constexpr (TPR > 64) {
     constexpr int kW = TPR / 64;
     if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = v;
