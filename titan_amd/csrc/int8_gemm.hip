@@ -21,7 +21,7 @@
 #include <algorithm>
 
 #include "gemm_common.h"
-#include "int8_product.h"
+#include "int8_few.h"
 
 namespace {
 
@@ -29,13 +29,12 @@ using namespace qmoe_i8;
 using qmoe_gemm::kTileRows;
 
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
-constexpr int kCols = 256;               // outputs of a unit
 constexpr int kPairRows = 2 * kTileRows;  // rows of a unit, at most
 constexpr int kGroup = 128;              // bytes of the contraction per stage
 constexpr int kUnits = kGroup / 16;      // and its 16-byte units
 constexpr int kSteps = kGroup / 32;
 constexpr int kRound = kWaves * (1024 / kGroup);  // rows that one copy of every wave fills
-constexpr int kBCopies = kCols / kRound, kMaxACopies = kPairRows / kRound;
+constexpr int kMaxACopies = kPairRows / kRound;
 constexpr int kLdsCU = 160 * 1024;
 // The results are staged in the ring's second 64 KiB: the first stage of the next unit is filled meanwhile.
 constexpr int kStaging = 64 * 1024, kRing = 144 * 1024;
@@ -91,10 +90,11 @@ __device__ __forceinline__ Rows rows_of(const Product& a, const Unit& u) {
   return r;
 }
 
+template <int COLS>
 struct Ctx {
   const char* x[kMaxACopies];  // the lane's unit of each copy's row
   const char* w;               // the unit's columns
-  uint32_t woff[kBCopies];
+  uint32_t woff[COLS / kRound];
   int unit;  // the lane's unit within a group: the rows of its copies swizzle alike
   uint32_t lds;
   int wave, lane, units;
@@ -109,26 +109,30 @@ struct Ctx {
   }
 };
 
-// Copy d of group g into the stage at `st`, of the wave's NA of x and kBCopies
+// Copy d of group g into the stage at `st`, of the wave's NA of x and those
 // of w.  Units past the contraction's end are zeros of x, and of w the group's
 // first unit, whatever it holds.
-__device__ __forceinline__ void copy_x(const Ctx& c, int g, uint32_t st, int d) {
+template <int COLS>
+__device__ __forceinline__ void copy_x(const Ctx<COLS>& c, int g, uint32_t st, int d) {
   const bool in = g * kUnits + c.unit < c.units;
   const char* p = c.x[d] + (size_t)g * kGroup;
   qmoe_gemm::dma16(in ? p : reinterpret_cast<const char*>(zero_unit), st + (d * kWaves + c.wave) * 1024);
 }
-__device__ __forceinline__ void copy_w(const Ctx& c, int g, uint32_t st, int na, int d) {
+template <int COLS>
+__device__ __forceinline__ void copy_w(const Ctx<COLS>& c, int g, uint32_t st, int na, int d) {
   const bool in = g * kUnits + c.unit < c.units;
   qmoe_gemm::dma16s(c.w + (size_t)g * kGroup, c.woff[d] - (in ? 0u : (uint32_t)c.unit * 16),
                     st + ((na + d) * kWaves + c.wave) * 1024);
 }
 
 // A unit's addresses, and the copies of its scales (into s: rows', then columns') and of its first group.
-__device__ __forceinline__ Ctx begin(const Product& a, const Unit& u, const Rows& rows, char* smem, float* s) {
-  Ctx c;
+template <int COLS>
+__device__ __forceinline__ Ctx<COLS> begin(const Product& a, const Unit& u, const Rows& rows, char* smem, float* s) {
+  constexpr int kBCopies = COLS / kRound;
+  Ctx<COLS> c;
   const int tid = fresh_tid();
   const int64_t n0 = (int64_t)u.e * a.N + u.o0;
-  const int cols = (int)min((int64_t)kCols, a.N - u.o0);
+  const int cols = (int)min((int64_t)COLS, a.N - u.o0);
   c.w = reinterpret_cast<const char*>(a.w) + n0 * a.K;
   c.settle(a, smem);
   c.unit = (c.lane % kUnits) ^ swz(c.wave * (kRound / kWaves) + c.lane / kUnits);
@@ -144,7 +148,7 @@ __device__ __forceinline__ Ctx begin(const Product& a, const Unit& u, const Rows
     qmoe_gemm::dma4(a.sx + rows.scale, ls + c.wave * 256);
     qmoe_gemm::dma4(a.sw + n0 + min(tid, cols - 1), ls + kPairRows * 4 + c.wave * 256);
   }
-  static_assert(kCols == kPairRows, "the same waves copy both scales");
+  static_assert(COLS <= kPairRows, "the same waves copy both scales");
   const int na = a_copies(u.valid);
 #pragma unroll
   for (int d = 0; d < kMaxACopies; ++d)
@@ -157,12 +161,13 @@ __device__ __forceinline__ Ctx begin(const Product& a, const Unit& u, const Rows
 template <int WM_, int WN_, int MSUB_, int NSUB_, int NS_>
 struct Form {
   static constexpr int WM = WM_, WN = WN_, MSUB = MSUB_, NSUB = NSUB_, NS = NS_;
-  static constexpr int kRows = 32 * WM * MSUB;
-  static constexpr int kACopies = (kRows + kRound - 1) / kRound, kCopies = kACopies + kBCopies;  // per wave and group
+  static constexpr int kRows = 32 * WM * MSUB, kCols = 32 * WN * NSUB;
+  static constexpr int kBCopies = kCols / kRound, kACopies = (kRows + kRound - 1) / kRound, kCopies = kACopies + kBCopies;  // per wave and group
   static constexpr int kA = kACopies * kWaves * 1024, kStage = kA + kCols * kGroup;
-  static_assert(WM * WN == kWaves && 32 * WN * NSUB == kCols, "eight waves, the unit's columns");
+  static_assert(WM * WN == kWaves, "eight waves");
   static_assert(NS * kStage <= kRing && kStage <= kStaging, "the ring");
   typedef i32x16_t Acc[MSUB][NSUB];
+  typedef ::Ctx<kCols> Ctx;
 
   struct Frag {
     i32x4_t a[MSUB], b[NSUB];
@@ -277,7 +282,7 @@ struct Form {
             for (int k = 0; k < 4; ++k) y[k] = scaled(acc[i][j][v + k], sx, sw[k]);
           }
           if constexpr (SIZE == 4) {
-            *reinterpret_cast<f32x4_t*>(ep + lr * kPitch + (gi ^ l32) * 16) = y;
+            *reinterpret_cast<f32x4_t*>(ep + lr * kPitch + (gi ^ (l32 % kRowUnits)) * 16) = y;
           } else {
             uint2 o;
             if (a.dtype == QMOE_BF16) {
@@ -286,7 +291,7 @@ struct Form {
               typedef _Float16 h4 __attribute__((ext_vector_type(4)));
               o = __builtin_bit_cast(uint2, h4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]});
             }
-            *reinterpret_cast<uint2*>(ep + lr * kPitch + (gi ^ (2 * l32)) * 8) = o;
+            *reinterpret_cast<uint2*>(ep + lr * kPitch + (gi ^ (2 * (l32 % kRowUnits))) * 8) = o;
           }
         }
       meet();
@@ -295,7 +300,7 @@ struct Form {
 #pragma unroll
       for (int t = 0; t < kReads; ++t) {
         const int r = (t * kThreads + tid) / kRowUnits, unit = (t * kThreads + tid) % kRowUnits;
-        from[t] = (uint32_t)(uintptr_t)ep + r * kPitch + (unit ^ (r % 32)) * 16;
+        from[t] = (uint32_t)(uintptr_t)ep + r * kPitch + (unit ^ (r % 32 % kRowUnits)) * 16;
       }
       lds_read16(v, from);
 #pragma unroll
@@ -335,11 +340,14 @@ template <class... Forms>
 struct Pick;
 template <class F>
 struct Pick<F> {
+  static constexpr int kCols = F::kCols;
   template <class... A>
   static __device__ __forceinline__ void run(const Product& a, const Unit& u, A&&... rest) { F::run(a, u, rest...); }
 };
 template <class F, class G, class... Rest>
 struct Pick<F, G, Rest...> {
+  static constexpr int kCols = F::kCols;
+  static_assert(kCols == G::kCols, "forms of one unit");
   template <class... A>
   static __device__ __forceinline__ void run(const Product& a, const Unit& u, A&&... rest) {
     if (u.valid > G::kRows) F::run(a, u, rest...);
@@ -347,7 +355,12 @@ struct Pick<F, G, Rest...> {
   }
 };
 typedef Pick<Form<2, 4, 4, 2, 2>, Form<2, 4, 3, 2, 2>, Form<2, 4, 2, 2, 3>, Form<1, 8, 3, 1, 3>, Form<1, 8, 2, 1, 3>,
-             Form<1, 8, 1, 1, 3>> Forms;
+             Form<1, 8, 1, 1, 3>> Wide;
+// 64 x 128 and 128 x 128 outputs, for products of few units: five and three
+// groups ahead, where it is the copies' way that takes the time.
+constexpr int kNarrowRows = 64;
+typedef Pick<Form<2, 4, 1, 1, 6>> Narrow;
+typedef Pick<Form<2, 4, 2, 1, 4>> Middle;
 
 // The rows of tile t's unit, 0 for the second tile of a pair.
 __device__ __forceinline__ qmoe_gemm::TileRows pair_rows_of(const qmoe_gemm::Tiles& t, int tile) {
@@ -399,9 +412,11 @@ __device__ inline int rank_pairs(const qmoe_gemm::Tiles& t, int tiles, int* orde
 }
 
 // row_units, unit_rows: of one matrix (unit_rows <= kPairRows); a table's units are its own.
+template <class Forms>
 __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t row_units, int unit_rows, int NB) {
+  constexpr int kCols = Forms::kCols;
   __shared__ __attribute__((aligned(16))) char smem[kRing];
-  __shared__ __attribute__((aligned(16))) float scales[2][kPairRows + kCols];  // of this unit and the next
+  __shared__ __attribute__((aligned(16))) float scales[2][2 * kPairRows];  // of this unit and the next
   __shared__ int order[kMaxRanked];
   static_assert(kRing + sizeof(scales) + sizeof(order) <= kLdsCU, "LDS per CU");
   static_assert(2 * kStaging <= kRing && kRing >= 4 * (kMaxRanked + 1), "the staged results; the ranking's scratch");
@@ -449,15 +464,15 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
   };
   Unit u = next();
   if (u.valid <= 0) return;
-  Ctx c = begin(a, u, rows_of(a, u), smem, scales[0]);
+  Ctx<kCols> c = begin<kCols>(a, u, rows_of(a, u), smem, scales[0]);
   for (int s = 0;; s ^= 1) {
     // the next unit's rows, while this one's first copies are under way
     const Unit v = next();
     Rows rows = {};
     if (v.valid > 0) rows = rows_of(a, v);
-    Ctx d;
+    Ctx<kCols> d;
     Forms::run(a, u, c, smem, scales[s], [&] {
-      if (v.valid > 0) d = begin(a, v, rows, smem, scales[s ^ 1]);
+      if (v.valid > 0) d = begin<kCols>(a, v, rows, smem, scales[s ^ 1]);
     });
     if (v.valid <= 0) break;
     u = v;
@@ -465,11 +480,34 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
   }
 }
 
+template <class Forms>
 int launch(const Product& a, int64_t max_tiles, int unit_rows, hipStream_t st) {
-  const int64_t NB = (a.N + kCols - 1) / kCols, rows = a.offsets ? max_tiles : (a.n_rows + unit_rows - 1) / unit_rows;
+  const int64_t NB = (a.N + Forms::kCols - 1) / Forms::kCols, rows = a.offsets ? max_tiles : (a.n_rows + unit_rows - 1) / unit_rows;
   const dim3 grid((unsigned)qmoe_gemm::grid_blocks(rows * NB, 1));
-  int8_gemm_kernel<<<grid, dim3(kThreads), 0, st>>>(a, rows, unit_rows, (int)NB);
+  int8_gemm_kernel<Forms><<<grid, dim3(kThreads), 0, st>>>(a, rows, unit_rows, (int)NB);
   return qmoe::launch_status("int8_gemm_kernel");
+}
+
+// One matrix.  Up to kFewBlocks blocks of 32 x 32 outputs are the few-rows
+// kernel's, which splits the contraction (4096 x 2048 weights, 128 / 192 / 256
+// rows: 9.1 / 11.4 / 13.6 us, in 64 x 128 units 12.2 / 12.2 / 12.1; 2048 x 8192,
+// 128 rows: 13.4 and 31).  Beyond, the form whose rounds of 256 units cost least.
+// A round's cost, as measured with K = 2048: 64 x 128 units 9.5 us, 128 x 128 13,
+// 128 x 256 19, 256 x 256 33; a product of one round takes 3 more (N = 4096: 512
+// rows 12.4 / 14.4 / 19.7 / 35.5 us, 1024 rows 22.6 / 15.8 / 20.0 / 34.8, 4096 rows
+// 76 / 55 / 43 / 40).
+constexpr int64_t kFewBlocks = 768, kRoundUnits = 256;
+int dense(const Product& a, hipStream_t st) {
+  const auto blocks = [&](int64_t rows, int64_t cols) { return (a.n_rows + rows - 1) / rows * ((a.N + cols - 1) / cols); };
+  if (blocks(32, 32) <= kFewBlocks) return few_product(a, st);
+  const auto cost = [&](int64_t rows, int64_t cols, int64_t round) {
+    return (blocks(rows, cols) + kRoundUnits - 1) / kRoundUnits * round;
+  };
+  const int64_t narrow = cost(kNarrowRows, 128, 19), middle = cost(kTileRows, 128, 26), tall = cost(kTileRows, 256, 38),
+                wide = cost(kPairRows, 256, 66), least = std::min({narrow, middle, tall, wide});
+  if (least == wide) return launch<Wide>(a, 0, kPairRows, st);
+  if (least == tall) return launch<Wide>(a, 0, kTileRows, st);
+  return least == middle ? launch<Middle>(a, 0, kTileRows, st) : launch<Narrow>(a, 0, kNarrowRows, st);
 }
 
 }  // namespace
@@ -488,6 +526,6 @@ extern "C" int qmoe_int8_gather_qqmm(const int8_t* x, const float* sx, int64_t n
   if (!any && !x_rows && n_x < n_rows) return qmoe::fail(QMOE_ERR_INVALID, "fewer activation rows than rows");
   if (any && max_tiles <= 0) return qmoe::fail(QMOE_ERR_INVALID, "an empty tile table");
   if (max_tiles > 0x7FFFFFFF) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
-  const int64_t wide = (n_rows + kPairRows - 1) / kPairRows * ((N + kCols - 1) / kCols);
-  return launch(a, max_tiles, any || wide >= 192 ? kPairRows : kTileRows, qmoe::as_stream(stream));
+  hipStream_t st = qmoe::as_stream(stream);
+  return any ? launch<Wide>(a, max_tiles, kPairRows, st) : dense(a, st);
 }
