@@ -600,6 +600,10 @@ int qmoe_int8_rms_norm(const void* x, const void* residual, const void* weight,
  * multiple of 16, at most 131056.  Indices are clamped into range.
  *   qmoe_int8_gather_qqmv  few rows (at most 65535), xr = x_rows[r], or r /
  *                          x_div where x_rows is NULL; experts NULL: expert 0
+ *   qmoe_int8_gather_qmv   the same for rows of x that are values of QMOE_BF16,
+ *                          _FP16 or _FP32 (dtype): qmoe_int8_quantize and the
+ *                          product in one launch, the same results; K at most
+ *                          16384
  *   qmoe_int8_gather_qqmm  many rows, sorted by expert, as described by a tile
  *                          table (qmoe_route / qmoe_build_tiles with
  *                          qmoe_gemm_tile_rows() rows per tile), or with the
@@ -611,6 +615,12 @@ int qmoe_int8_gather_qqmv(const int8_t* x, const float* sx, int64_t n_x,
                           const int8_t* w, const float* sw,
                           int32_t num_experts, int64_t N, int64_t K,
                           int out_dtype, void* out, void* stream);
+int qmoe_int8_gather_qmv(const void* x, int dtype, int64_t n_x,
+                         const int32_t* x_rows, int32_t x_div,
+                         const int32_t* experts, int64_t n_rows,
+                         const int8_t* w, const float* sw,
+                         int32_t num_experts, int64_t N, int64_t K,
+                         int out_dtype, void* out, void* stream);
 int qmoe_int8_gather_qqmm(const int8_t* x, const float* sx, int64_t n_x,
                           const int32_t* x_rows, int64_t n_rows,
                           const int8_t* w, const float* sw,

@@ -299,3 +299,23 @@ def test_gradients_and_recorders_are_refused(dev):
 
     with fw.dual_level(), pytest.raises(NotImplementedError):
         ops.qqmm(fw.make_dual(x.detach(), x.detach()), w, sw, mode="int8")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F4])
+@pytest.mark.parametrize("K", [16, 112, 1024, 2048, 4096, 6160, 16384, 20480])
+def test_values_quantised_in_the_product(dev, K, dtype):
+    """Few rows of values: the codes, and so the bits, of the product of rows quantised before."""
+    g = torch.Generator().manual_seed(K)
+    x = (torch.randn(4, K, generator=g) * torch.tensor([1.0, 30.0, 1e-3, 0.0]).unsqueeze(-1)).to(dtype)
+    x[1, K // 2] = float("inf")
+    w, sw = (t.to(dev) for t in _codes((3, 21, K), 27))
+    pair = ops.quantize(x.to(dev), mode="int8")
+    for m in (1, 4):
+        a = ops.qqmm(x[:m].to(dev), w[0], sw[0], mode="int8", dtype=F4)
+        b = ops.qqmm((pair[0][:m], pair[1][:m]), w[0], sw[0], mode="int8", dtype=F4)
+        assert torch.equal(a.nan_to_num(7), b.nan_to_num(7)) and torch.equal(torch.isnan(a), torch.isnan(b))
+    ids = torch.tensor([[0, 2], [1, 1], [2, 0], [0, 1]], dtype=torch.int32, device=dev)
+    a = ops.gather_qqmm(x.reshape(4, 1, 1, K).to(dev), w, sw, rhs_indices=ids, mode="int8")
+    b = ops.gather_qqmm((pair[0].reshape(4, 1, 1, K), pair[1].reshape(4, 1, 1)), w, sw, rhs_indices=ids, mode="int8", dtype=dtype)
+    assert a.dtype == dtype and torch.equal(a.nan_to_num(7), b.nan_to_num(7))
+    assert torch.isnan(a[1]).all() and not a[3].any()

@@ -219,6 +219,10 @@ def test_product_entries():
                        ({"x": ODD}, _lib.ERR_UNSUPPORTED), ({"out": ODD}, _lib.ERR_UNSUPPORTED), ({"n": 65536}, _lib.ERR_UNSUPPORTED),
                        ({"N": 1 << 31}, _lib.ERR_UNSUPPORTED), ({"n": 0}, _lib.OK), ({"N": 0}, _lib.OK)):
         assert _rc("qmoe_int8_gather_qqmv", *{**few, **change}.values(), None) == rc, change
+    val = dict(x=P, xdt=0, **{k: v for k, v in few.items() if k not in ("x", "sx")})
+    for change, rc in (({"xdt": 3}, _lib.ERR_UNSUPPORTED), ({"K": 16400}, _lib.ERR_UNSUPPORTED), ({"x": None}, _lib.ERR_INVALID),
+                       ({"n": 65536}, _lib.ERR_UNSUPPORTED), ({"x": ODD}, _lib.ERR_UNSUPPORTED), ({"n": 0}, _lib.OK)):
+        assert _rc("qmoe_int8_gather_qmv", *{**val, **change}.values(), None) == rc, change
     many = dict(x=P, sx=P, n_x=2, rows=None, n=2, w=P, sw=P, E=1, N=8, K=32, off=None, tr=None, te=None, nt=None, maxt=0, dt=0,
                 out=P)
     for change, rc in (({"E": 2}, _lib.ERR_INVALID), ({"off": P}, _lib.ERR_INVALID), ({"n": 3}, _lib.ERR_INVALID),

@@ -103,6 +103,7 @@ SIGNATURES: dict[str, tuple] = {
     "qmoe_int8_dequantize": (INT, [P, P, I64, I64, INT, P, P]),
     "qmoe_int8_rms_norm": (INT, [P, P, P, INT, INT, I64, I64, ctypes.c_double, P, P, P, P, P]),
     "qmoe_int8_gather_qqmv": (INT, [P, P, I64, P, I32, P, I64, P, P, I32, I64, I64, INT, P, P]),
+    "qmoe_int8_gather_qmv": (INT, [P, INT, I64, P, I32, P, I64, P, P, I32, I64, I64, INT, P, P]),
     "qmoe_int8_gather_qqmm": (INT, [P, P, I64, P, I64, P, P, I32, I64, I64, P, P, P, P, I64, INT, P, P]),
     "qmoe_router_balance_workspace_size": (SZ, [I64, I64]),
     "qmoe_router_balance": (INT, [P, INT, I64, I64, P, INT, I64, P, P, P, P, P, SZ, P]),

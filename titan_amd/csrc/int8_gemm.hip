@@ -518,7 +518,7 @@ extern "C" int qmoe_int8_gather_qqmm(const int8_t* x, const float* sx, int64_t n
                                      const int32_t* ntiles, int64_t max_tiles, int out_dtype, void* out, void* stream) {
   Product a{x, sx, x_rows, n_rows, n_x, 1, nullptr, w, sw, num_experts, N, K, offsets, tile_row, tile_exp, ntiles, out, out_dtype};
   bool run;
-  const int rc = check(a, &run);
+  const int rc = check(a, false, &run);
   if (rc != QMOE_OK || !run) return rc;
   const bool any = offsets || tile_row || tile_exp || ntiles;
   if (any && !(offsets && tile_row && tile_exp && ntiles)) return qmoe::fail(QMOE_ERR_INVALID, "half a tile table");

@@ -52,6 +52,7 @@ __device__ __forceinline__ void put(const Product& a, int64_t i, float v) {
 }
 
 // Argument checks of the entry points; QMOE_OK with *run = false: nothing to do.
-int check(const Product& a, bool* run);
+// values: x has no scales yet.
+int check(const Product& a, bool values, bool* run);
 
 }  // namespace qmoe_i8

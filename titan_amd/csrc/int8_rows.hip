@@ -17,22 +17,12 @@
 // 21 us, 7.2 TB/s, some of it from the caches; 65536 x 2048 fp32 to codes:
 // 126 us, 5.3 TB/s), by one chain of loads, two reductions and the stores below
 // (one row of 2048: 2.9 us per call in a graph, quantised alone 2.2).
-#include "elem.h"
+#include "int8_codes.h"
 #include "lanes.h"
 
 namespace {
 
-// Larger |v| have larger bits, infinities and NaN the largest.
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-constexpr uint32_t kInfinite = 0x7F800000u;
-
-__device__ __forceinline__ int code_of(float v, float s) {
-  if (!(s > 0.f)) return 0;
-  return (int)fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.f), 127.f);
-}
-__device__ __forceinline__ float scale_of(uint32_t top) {
-  return top >= kInfinite ? __uint_as_float(0x7FC00000u) : __fdiv_rn(__uint_as_float(top), 127.f);
-}
+using namespace qmoe_i8;
 
 // v combined over the TPR threads of a row (whole waves; the whole block from two waves on).
 template <int TPR, class T, class Op>
@@ -48,72 +38,6 @@ __device__ __forceinline__ T over_row(T v, T* shared, Op op) {
   }
   return v;
 }
-
-// N elements at any element's address.
-template <class T, int N>
-struct __attribute__((packed)) Loose {
-  typename Vec<T, N>::V v __attribute__((aligned(1)));
-};
-template <class T, int N>
-__device__ __forceinline__ typename Vec<T, N>::V get(const T* p) {
-  return reinterpret_cast<const Loose<T, N>*>(p)->v;
-}
-template <class T, int N>
-__device__ __forceinline__ void put(T* p, typename Vec<T, N>::V v) {
-  reinterpret_cast<Loose<T, N>*>(p)->v = v;
-}
-// .. the first `there` of which exist.
-template <class T, int N>
-__device__ __forceinline__ typename Vec<T, N>::V get(const T* p, int there) {
-  if (there >= N) return get<T, N>(p);
-  typename Vec<T, N>::V v = {};
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < there) v[i] = p[i];
-  return v;
-}
-template <class T, int N>
-__device__ __forceinline__ void put(T* p, int there, typename Vec<T, N>::V v) {
-  if (there >= N) return put<T, N>(p, v);
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < there) p[i] = v[i];
-}
-
-// The codes of N values, four to a word.  Within |scale| limits the quotient is
-// taken as v times the scale's reciprocal, which is off by less than 3e-5 of a
-// code from the rounded quotient: where that could matter, the division decides.
-struct Coder {
-  float s, inv;
-  bool quick;
-  __device__ __forceinline__ explicit Coder(float scale)
-      : s(scale), inv(1.f / scale), quick(scale >= 0x1p-100f && scale <= 0x1p100f) {}
-  template <int N>
-  __device__ __forceinline__ void codes(const float (&v)[N], uint32_t (&out)[N / 4]) const {
-    constexpr float kMagic = 0x1.8p23f;  // added to a small number: its nearest integer in the low bits
-    float off = 1.f;
-    if (quick) {
-      off = 0.f;
-      uint32_t b[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float t = __builtin_fmaf(v[i], inv, kMagic);
-        b[i] = __float_as_uint(t);
-        off = fmaxf(off, fabsf(__builtin_fmaf(v[i], inv, kMagic - t)));
-      }
-#pragma unroll
-      for (int i = 0; i < N; i += 4)
-        out[i / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[i + 3], b[i + 2], 0x0C0C0400u),
-                                           __builtin_amdgcn_perm(b[i + 1], b[i], 0x0C0C0400u), 0x05040100u);
-    }
-    if (__any(!(off <= 0.5f - 3e-5f))) {
-#pragma unroll
-      for (int i = 0; i < N; i += 4)
-        out[i / 4] = (uint32_t)(code_of(v[i], s) & 255) | (uint32_t)(code_of(v[i + 1], s) & 255) << 8 |
-                     (uint32_t)(code_of(v[i + 2], s) & 255) << 16 | (uint32_t)code_of(v[i + 3], s) << 24;
-    }
-  }
-};
 
 // The rounding to the type in one instruction.
 template <int DT>

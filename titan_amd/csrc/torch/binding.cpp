@@ -604,6 +604,7 @@ py::object rms_norm_quantize(py::handle x_, py::handle w_, double eps, py::handl
   return py::make_tuple(give(q), give(s), sum.defined() ? give(sum) : py::none(), v.defined() ? give(v) : py::none());
 }
 
+constexpr int64_t kMaxValues = 16384;  // longest row of values that the matrix-vector kernel quantises itself
 // Activations: codes and scales, or (scales None) values to be quantised here.
 struct Acts {
   Tensor x, s;
@@ -614,9 +615,6 @@ struct Acts {
            !records(s);
   }
   int type(int asked) const { return asked >= 0 ? asked : s.defined() ? QMOE_BF16 : type_of(x); }
-  void quantized() {
-    if (!s.defined()) std::tie(x, s) = int8_run(x);
-  }
 };
 struct Weights8 {
   Tensor w, s;
@@ -632,12 +630,24 @@ struct Weights8 {
   }
 };
 
-Tensor int8_product_run(const Acts& a, const Weights8& g, const Rows& r, int type) {
+Tensor int8_product_run(Acts& a, const Weights8& g, const Rows& r, int type) {
   Tensor out = at::empty({r.n, g.N}, a.x.options().dtype(kTypes[type]).requires_grad(false));
   if (out.numel() == 0) return out;
   if (g.K == 0) return out.zero_();
   const int64_t n_x = row_count(a.x);
-  if (!r.offsets.defined() && (r.experts.defined() || r.n <= kQmvMaxRows)) {
+  // codes: two rows of 4096 x 2048 take 5.1 us here and 5.0 by the kernel for few rows, four 5.7 and 5.0; values are
+  // quantised on the way (four 6.5, a launch less)
+  const bool few = !r.offsets.defined() && (r.experts.defined() || r.n == 1 ||
+                                            (r.n <= kQmvMaxRows && (!a.s.defined() || r.n * g.N * g.K <= kQmvMaxWork)));
+  if (few && !a.s.defined() && g.K <= kMaxValues) {
+    ok(qmoe_int8_gather_qmv(a.x.const_data_ptr(), type_of(a.x), n_x, ptr<int32_t>(r.x_rows), (int32_t)r.div,
+                            ptr<int32_t>(r.experts), r.n, ptr<int8_t>(g.w), ptr<float>(g.s), (int32_t)g.E, g.N, g.K, type,
+                            out.data_ptr(), stream(a.x)),
+       "qmoe_int8_gather_qmv");
+    return out;
+  }
+  if (!a.s.defined()) std::tie(a.x, a.s) = int8_run(a.x);
+  if (few) {
     ok(qmoe_int8_gather_qqmv(ptr<int8_t>(a.x), ptr<float>(a.s), n_x, ptr<int32_t>(r.x_rows), (int32_t)r.div,
                              ptr<int32_t>(r.experts), r.n, ptr<int8_t>(g.w), ptr<float>(g.s), (int32_t)g.E, g.N, g.K, type,
                              out.data_ptr(), stream(a.x)),
@@ -664,7 +674,6 @@ py::object int8_matmul(py::handle x_, py::handle sx_, py::handle w_, py::handle 
   sizes.back() = g.N;
   Rows r;
   r.n = row_count(a.x);
-  a.quantized();
   return give(int8_product_run(a, g, r, type).reshape(sizes));
 }
 
@@ -681,7 +690,6 @@ py::object int8_gather(py::handle x_, py::handle sx_, py::handle w_, py::handle 
   const c10::hip::HIPGuard guard(a.x.get_device());
   if (r.n >= kSortedMinRows && !table(r.experts, g.E, &r)) return py::none();
   type = a.type(type);
-  a.quantized();
   auto sizes = rhs.sizes().vec();
   sizes.push_back(1);
   sizes.push_back(g.N);
@@ -709,7 +717,6 @@ py::object int8_rows_product(py::handle x_, py::handle sx_, py::handle w_, py::h
   TORCH_CHECK((!x_rows || r.x_rows.numel() == n) && (!experts || r.experts.numel() == n), "the rows disagree");
   const c10::hip::HIPGuard guard(a.x.get_device());
   type = a.type(type);
-  a.quantized();
   return give(int8_product_run(a, g, r, type));
 }
 
