@@ -319,3 +319,78 @@ def test_values_quantised_in_the_product(dev, K, dtype):
     b = ops.gather_qqmm((pair[0].reshape(4, 1, 1, K), pair[1].reshape(4, 1, 1)), w, sw, rhs_indices=ids, mode="int8", dtype=dtype)
     assert a.dtype == dtype and torch.equal(a.nan_to_num(7), b.nan_to_num(7))
     assert torch.isnan(a[1]).all() and not a[3].any()
+
+
+@pytest.mark.parametrize("E,n,N,K", [(1100, 1500, 40, 32),   # more tiles than are ranked
+                                     (300, 2000, 1030, 64),  # four rounds of units and more: every second XCD's order reversed
+                                     (2, 3000, 333, 144)])   # pairs of tiles
+@pytest.mark.parametrize("out", [BF, HF, F4])
+def test_orders_of_units(dev, E, n, N, K, out):
+    g = torch.Generator().manual_seed(n)
+    x, sx = _codes((90, K), 28)
+    w, sw = _codes((E, N, K), 29)
+    ids, rows = torch.randint(0, E, (n,), generator=g).sort().values, torch.randint(0, 90, (n,), generator=g)
+    y = ops.gather_qqmm((x.to(dev).unsqueeze(1), sx.to(dev).unsqueeze(1)), w.to(dev), sw.to(dev), lhs_indices=rows.to(dev),
+                        rhs_indices=ids.to(dev), mode="int8", sorted_indices=True, dtype=out)
+    o.assert_rounded(y.squeeze(1), _gather_oracle(x, sx, w, sw, rows, ids))
+
+
+@pytest.mark.parametrize("M,N,K", [(96, 8190, 48),    # blocks of few rows, the most of them
+                                   (100, 9001, 80),   # 64 x 128
+                                   (520, 4100, 400),  # 128 x 128
+                                   (1030, 4098, 272), # 128 x 256
+                                   (4000, 4091, 144)])  # 256 x 256
+def test_dense_forms(dev, M, N, K):
+    """Each form of a unit with odd rows and columns, in every type."""
+    for out in (BF, HF, F4):
+        _dense(dev, M, K, N, out, M)
+
+
+def test_a_table_larger_than_its_buffers(dev):
+    """More tiles than there is room for: those that fit are computed, nothing is read behind them."""
+    from titan_amd import _lib
+
+    x, sx = (t.to(dev) for t in _codes((256, 64), 31))
+    w, sw = (t.to(dev) for t in _codes((2, 48, 64), 32))
+    t = ops.build_tiles(torch.tensor([0] * 128 + [1] * 128, dtype=torch.int32, device=dev), 2)
+    out = torch.full((256, 48), 7.0, dtype=BF, device=dev)
+    _lib.call("qmoe_int8_gather_qqmm", x.data_ptr(), sx.data_ptr(), 256, None, 256, w.data_ptr(), sw.data_ptr(), 2, 48, 64,
+              t.offsets.data_ptr(), t.tile_row.data_ptr(), t.tile_exp.data_ptr(), t.ntiles.data_ptr(), 1, 0,
+              out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    ids = torch.tensor([0] * 128)
+    o.assert_rounded(out[:128], _gather_oracle(x.cpu(), sx.cpu(), w.cpu(), sw.cpu(), torch.arange(128), ids))
+    assert bool((out[128:] == 7).all())
+
+
+def test_calls_of_two_threads(dev):
+    """Each on a stream of its own: no state is shared."""
+    import threading
+
+    w, sw = (t.to(dev) for t in _codes((8, 256, 512), 33))
+    v = [torch.randn(200, 512, generator=torch.Generator().manual_seed(40 + i)).to(dev, BF) for i in range(2)]
+    ids = [torch.randint(0, 8, (200,), generator=torch.Generator().manual_seed(50 + i)).sort().values.to(dev) for i in range(2)]
+    logits = [torch.randn(5000, 64, generator=torch.Generator().manual_seed(60 + i)).to(dev) for i in range(2)]
+
+    def run(i):
+        n = ops.rms_norm_quantize(v[i], None, residual=v[i])
+        return (ops.qqmm(n, w[i], sw[i], mode="int8"), ops.qqmm(v[i][:3], w[i], sw[i], mode="int8"),
+                ops.gather_qqmm(v[i].unsqueeze(1), w, sw, rhs_indices=ids[i], mode="int8", sorted_indices=True),
+                *ops.router_balance_loss(logits[i], ids[i][:100].repeat(50).reshape(5000, 1)))
+
+    want = [run(i) for i in range(2)]
+    got, streams = [None, None], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(30):
+                got[i] = run(i)
+            streams[i].synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(want[i], got[i]))

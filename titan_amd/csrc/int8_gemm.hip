@@ -65,8 +65,6 @@ __device__ __forceinline__ int64_t row_of(const Product& a, const Unit& u, int r
   const int64_t r = u.row0 + min(row, u.valid - 1);
   return min(max(a.x_rows ? (int64_t)a.x_rows[r] : r, (int64_t)0), a.n_x - 1);
 }
-// Copies of activation rows per wave and group: the forms' rows in rounds.
-__device__ __forceinline__ int a_copies(int valid) { return (valid + kRound - 1) / kRound; }
 
 // Swizzle of a row's eight 16-byte units in LDS: one unit of sixteen
 // consecutive rows is read without bank conflicts.
@@ -126,9 +124,9 @@ __device__ __forceinline__ void copy_w(const Ctx<COLS>& c, int g, uint32_t st, i
 }
 
 // A unit's addresses, and the copies of its scales (into s: rows', then columns') and of its first group.
-template <int COLS>
-__device__ __forceinline__ Ctx<COLS> begin(const Product& a, const Unit& u, const Rows& rows, char* smem, float* s) {
-  constexpr int kBCopies = COLS / kRound;
+template <class Forms>
+__device__ __forceinline__ Ctx<Forms::kCols> begin(const Product& a, const Unit& u, const Rows& rows, char* smem, float* s) {
+  constexpr int COLS = Forms::kCols, kBCopies = COLS / kRound;
   Ctx<COLS> c;
   const int tid = fresh_tid();
   const int64_t n0 = (int64_t)u.e * a.N + u.o0;
@@ -149,7 +147,7 @@ __device__ __forceinline__ Ctx<COLS> begin(const Product& a, const Unit& u, cons
     qmoe_gemm::dma4(a.sw + n0 + min(tid, cols - 1), ls + kPairRows * 4 + c.wave * 256);
   }
   static_assert(COLS <= kPairRows, "the same waves copy both scales");
-  const int na = a_copies(u.valid);
+  const int na = Forms::copies(u.valid);
 #pragma unroll
   for (int d = 0; d < kMaxACopies; ++d)
     if (d < na) copy_x(c, 0, c.lds, d);
@@ -341,6 +339,8 @@ struct Pick;
 template <class F>
 struct Pick<F> {
   static constexpr int kCols = F::kCols;
+  // Copies of activation rows per wave and group of the form for so many rows.
+  static __device__ __forceinline__ int copies(int) { return F::kACopies; }
   template <class... A>
   static __device__ __forceinline__ void run(const Product& a, const Unit& u, A&&... rest) { F::run(a, u, rest...); }
 };
@@ -348,6 +348,9 @@ template <class F, class G, class... Rest>
 struct Pick<F, G, Rest...> {
   static constexpr int kCols = F::kCols;
   static_assert(kCols == G::kCols, "forms of one unit");
+  static __device__ __forceinline__ int copies(int valid) {
+    return valid > G::kRows ? F::kACopies : Pick<G, Rest...>::copies(valid);
+  }
   template <class... A>
   static __device__ __forceinline__ void run(const Product& a, const Unit& u, A&&... rest) {
     if (u.valid > G::kRows) F::run(a, u, rest...);
@@ -423,7 +426,7 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
   const qmoe_gemm::Tiles table{a.offsets, a.tile_row, a.tile_exp, a.ntiles, a.n_rows, a.num_experts};
   bool ranked = false;
   if (a.offsets) {
-    row_units = max(a.ntiles[0], 0);
+    row_units = min((int64_t)max(a.ntiles[0], 0), row_units);  // of as many as the caller says there is room for
     ranked = row_units <= kMaxRanked;
     if (ranked) row_units = rank_pairs(table, (int)row_units, order, reinterpret_cast<int*>(smem));
   }
@@ -464,7 +467,7 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
   };
   Unit u = next();
   if (u.valid <= 0) return;
-  Ctx<kCols> c = begin<kCols>(a, u, rows_of(a, u), smem, scales[0]);
+  Ctx<kCols> c = begin<Forms>(a, u, rows_of(a, u), smem, scales[0]);
   for (int s = 0;; s ^= 1) {
     // the next unit's rows, while this one's first copies are under way
     const Unit v = next();
@@ -472,7 +475,7 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
     if (v.valid > 0) rows = rows_of(a, v);
     Ctx<kCols> d;
     Forms::run(a, u, c, smem, scales[s], [&] {
-      if (v.valid > 0) d = begin<kCols>(a, v, rows, smem, scales[s ^ 1]);
+      if (v.valid > 0) d = begin<Forms>(a, v, rows, smem, scales[s ^ 1]);
     });
     if (v.valid <= 0) break;
     u = v;
