@@ -142,6 +142,17 @@ def test_norm_extremes(dev):
     assert not zero.codes.any() and not zero.scales.any() and not zero.norm.any()
 
 
+@pytest.mark.parametrize("shape", [(2, 300), (2, 2048), (1, 70000)])
+def test_norm_factors_past_32_bits(dev, shape):
+    """Rows whose factor 1 / rms, or the precision of it, 32 bits do not hold; the norm itself is ordinary."""
+    x = _rows(shape, F4, 15).clamp(-8, 8)
+    for size in (2.0 ** -145, 2.0 ** -130, 2.0 ** -99, 2.0 ** 99, 2.0 ** 124):
+        for dtype in (BF, F4) if size > 2.0 ** -133 else (F4,):  # bf16's least value
+            v = (x * size).to(dtype)
+            got = ops.rms_norm_quantize(v.to(dev), None, 0.0, norm=True)
+            _check_norm(got, v, None, 0.0, None, dtype)
+
+
 def test_layouts_types_and_empty(dev):
     x = _rows((4, 6, 130), BF, 11).to(dev)
     want = ops.quantize(x.contiguous(), mode="int8")
@@ -212,6 +223,16 @@ def test_refusals_on_the_gpu(dev):
         ops.rms_norm_quantize(x, None, residual=leaf)
     with pytest.raises(ops.QmoeUnsupported, match="gradient"):
         ops.rms_norm_quantize(x, leaf[0].detach().requires_grad_(True))
+    q, s = ops.quantize(leaf, mode="int8")  # the codes of a layer's weight, say
+    assert not q.requires_grad and not s.requires_grad
+    with pytest.raises(ops.QmoeUnsupported, match="gradient"):
+        ops.dequantize(q, s.requires_grad_(True), mode="int8")
+    import torch.autograd.forward_ad as fw
+
+    with fw.dual_level():
+        for call in (lambda t: ops.quantize(t, mode="int8"), lambda t: ops.rms_norm_quantize(t, None)):
+            with pytest.raises(NotImplementedError):
+                call(fw.make_dual(x, x))
     with torch.no_grad():
         assert ops.rms_norm_quantize(leaf, None, residual=leaf).sum.shape == x.shape
     with pytest.raises(ops.QmoeUnsupported):

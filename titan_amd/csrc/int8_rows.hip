@@ -116,7 +116,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(RowArg
     if (NV) load(k, c);
   });
   if constexpr (NV > 0) each([&](int k, int c, int64_t) { h(k, c); });
-  float rstd = 1.f;
+  float rstd = 1.f, lift = 1.f;
   if constexpr (NORM) {
     double ss = 0.0;
     each([&](int k, int c, int64_t own) {
@@ -132,10 +132,18 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(RowArg
       }
     });
     ss = over_row<TPR>(ss, sums, [](double p, double q) { return p + q; });
-    rstd = (float)(1.0 / sqrt(ss / (double)a.D + a.eps));
+    const double r64 = 1.0 / sqrt(ss / (double)a.D + a.eps);
+    // past fp32's range in rows near its ends: the row takes a part of the factor, a power of two
+    if (r64 > 0x1p100) lift = 0x1p64f;
+    else if (r64 < 0x1p-100) lift = 0x1p-64f;
+    rstd = (float)(r64 / lift);
   }
   const auto normed = [&](int k, int c) {
     if constexpr (!NORM) return;
+    if (lift != 1.f) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) kept[k][i] *= lift;
+    }
     if (!a.w) {
 #pragma unroll
       for (int i = 0; i < N; ++i) kept[k][i] *= rstd;

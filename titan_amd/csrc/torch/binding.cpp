@@ -563,6 +563,7 @@ py::object int8_quantize(py::handle x_, bool must) {
   refuse_recorders();
   Tensor x;
   if (!get(x_, &x) || type_of(x) < 0 || x.dim() < 1 || !plain(x)) return none(must);
+  records(x);  // codes have no gradient, which loses nothing to one that asks; a tangent is refused
   const c10::hip::HIPGuard guard(x.get_device());
   const auto [q, s] = int8_run(x);
   return py::make_tuple(give(q), give(s));
@@ -572,7 +573,7 @@ py::object int8_dequantize(py::handle q_, py::handle s_, int type, bool must) {
   refuse_recorders();
   Tensor q, s;
   if (!get(q_, &q) || !get(s_, &s) || !plain(q, at::kChar) || !scales32(s) || q.dim() < 1 || s.sizes() != batch_of(q) ||
-      s.device() != q.device())
+      s.device() != q.device() || records(s))
     return none(must);
   const c10::hip::HIPGuard guard(q.get_device());
   Tensor out = at::empty(q.sizes(), q.options().dtype(kTypes[type]));
