@@ -14,15 +14,27 @@
 // codes); longer rows are read again for each.  Threads move 16 bytes at a time
 // at whatever address a row begins.  Bound by HBM from some thousands of rows
 // on (norm of 8192 x 2048 bf16 with the residual, its sum and the norm written:
-// 21 us, 7.2 TB/s, some of it from the caches; 65536 x 2048 fp32 to codes:
-// 126 us, 5.3 TB/s), by one chain of loads, two reductions and the stores below
-// (one row of 2048: 2.9 us per call in a graph, quantised alone 2.2).
+// 28 us, 5.4 TB/s; 65536 x 2048 fp32 to codes: 114 us, 5.9
+// TB/s; the values back: 58 us, 6.9 TB/s), by one chain of loads, two reductions and
+// the stores below (one row of 2048: 2.6 us per call in a graph, quantised alone
+// 2.4, its values 2.2).
 #include "int8_codes.h"
 #include "lanes.h"
 
 namespace {
 
 using namespace qmoe_i8;
+// As put, past the caches: for what is written whole and read later, if at all.
+// The values of 65536 x 2048 in bf16 take 58 us so and 71 without, in fp32 92 and
+// 144; the norm of 4096 x 2048 with its residual's sum and itself 11.3 and 14.1.
+// Not for codes, which a product reads next (quantisation and product of 16384
+// rows: 163 us so, 157 without).
+template <class T, int N>
+__device__ __forceinline__ void put_nt(T* p, int there, typename Vec<T, N>::V v) {
+  typedef typename Vec<T, N>::V At __attribute__((aligned(1)));
+  if (there >= N) __builtin_nontemporal_store(v, reinterpret_cast<At*>(p));
+  else put<T, N>(p, there, v);
+}
 
 // v combined over the TPR threads of a row (whole waves; the whole block from two waves on).
 template <int TPR, class T, class Op>
@@ -121,7 +133,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(RowArg
     double ss = 0.0;
     each([&](int k, int c, int64_t own) {
       if (!NV) h(k, c);
-      if (a.sum && own < a.D) put<T, N>(static_cast<T*>(a.sum) + base + c, there, narrow(k));
+      if (a.sum && own < a.D) put_nt<T, N>(static_cast<T*>(a.sum) + base + c, there, narrow(k));
       if (__any(own != c)) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -179,29 +191,36 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void int8_rows_kernel(RowArg
     uint32_t code[N / 4];
     coder.codes(kept[k], code);
     if (own >= a.D) return;
-    if (NORM && a.norm) put<T, N>(static_cast<T*>(a.norm) + base + c, there, narrow(k));
+    if (NORM && a.norm) put_nt<T, N>(static_cast<T*>(a.norm) + base + c, there, narrow(k));
     put<uint8_t, N>(reinterpret_cast<uint8_t*>(a.q) + base + c, there, __builtin_bit_cast(typename Vec<uint8_t, N>::V, code));
   });
 }
 
-// Codes times their row's scale: TPR threads per row, 256 per block.
-template <int DT, int TPR>
+// Codes times their row's scale: TPR threads per row, 256 per block, NV vectors of a thread under way together.
+template <int DT, int TPR, int NV>
 __global__ __launch_bounds__(256) void int8_values_kernel(const int8_t* __restrict__ q, const float* __restrict__ s,
                                                           int64_t rows, int64_t D, typename Elem<DT>::T* __restrict__ out) {
   typedef typename Elem<DT>::T T;
   constexpr int N = kVec<DT>;
+  typedef typename Vec<int8_t, N>::V C;
   const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   if (row >= rows) return;
   const int64_t base = row * D;
   const float sc = s[row];
-  for (int64_t own = (threadIdx.x % TPR) * N; own < D; own += TPR * N) {
-    const int64_t c = D < N ? 0 : min(own, D - N);  // the last vector ends with the row
-    const int there = (int)min(D, (int64_t)N);
-    const typename Vec<int8_t, N>::V v = get<int8_t, N>(q + base + c, there);
-    typename Vec<T, N>::V o;
+  const int there = (int)min(D, (int64_t)N);
+  const auto place = [&](int64_t own) { return D < N ? 0 : min(own, D - N); };  // the last vector ends with the row
+  for (int64_t own = (threadIdx.x % TPR) * N; own < D; own += NV * TPR * N) {
+    C v[NV];
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = rounded<DT>((float)v[i] * sc);
-    put<T, N>(out + base + c, there, o);
+    for (int k = 0; k < NV; ++k) v[k] = get<int8_t, N>(q + base + place(own + k * TPR * N), there);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (own + k * TPR * N >= D) break;
+      typename Vec<T, N>::V o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = rounded<DT>((float)v[k][i] * sc);
+      put_nt<T, N>(out + base + place(own + k * TPR * N), there, o);
+    }
   }
 }
 
@@ -214,7 +233,8 @@ void launch_form(const RowArgs& a, hipStream_t st) {
 // four vectors, else a vector per thread where that is possible: a thread's
 // vectors cost 1 to 2 us each one after the other.  Norms of bf16 rows, wave /
 // four waves per row (us): 1024 x 1000 5.1 / 5.9, 512 x 2048 6.9 / 5.0, 2048 x
-// 2048 8.9 / 9.1, 4096 x 4096 (eight vectors a thread / two) 24.5 / 20.6.
+// 2048 8.9 / 9.1, 4096 x 4096 (eight vectors a thread / two) 24.5 / 20.6 (measured
+// with the norm's stores through the caches).
 template <int DT, bool NORM>
 void launch_type(const RowArgs& a, hipStream_t st) {
   const int64_t vecs = (a.D + kVec<DT> - 1) / kVec<DT>;
@@ -235,11 +255,19 @@ int launch_rows(const RowArgs& a, int dtype, hipStream_t st) {
   else launch_type<QMOE_FP32, NORM>(a, st);
   return qmoe::launch_status("int8_rows_kernel");
 }
+// A wave per row and four vectors a thread where the rows fill the chip (4096 x
+// 2048: 4.5 us, by four waves 5.4 with stores through the caches), else threads enough for one or two each.
 template <int DT>
 void launch_values(const int8_t* q, const float* s, int64_t rows, int64_t D, void* out, hipStream_t st) {
   typedef typename Elem<DT>::T T;
-  if (D <= 64 * kVec<DT>) int8_values_kernel<DT, 64><<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st>>>(q, s, rows, D, static_cast<T*>(out));
-  else int8_values_kernel<DT, 256><<<dim3((unsigned)rows), dim3(256), 0, st>>>(q, s, rows, D, static_cast<T*>(out));
+  T* o = static_cast<T*>(out);
+  const int64_t vecs = (D + kVec<DT> - 1) / kVec<DT>;
+  const auto wave = dim3((unsigned)((rows + 3) / 4)), block = dim3((unsigned)rows);
+  if (vecs <= 64) int8_values_kernel<DT, 64, 1><<<wave, dim3(256), 0, st>>>(q, s, rows, D, o);
+  else if (vecs <= 256 && rows >= 2048) int8_values_kernel<DT, 64, 4><<<wave, dim3(256), 0, st>>>(q, s, rows, D, o);
+  else if (vecs <= 256) int8_values_kernel<DT, 256, 1><<<block, dim3(256), 0, st>>>(q, s, rows, D, o);
+  else if (vecs <= 512) int8_values_kernel<DT, 256, 2><<<block, dim3(256), 0, st>>>(q, s, rows, D, o);
+  else int8_values_kernel<DT, 256, 4><<<block, dim3(256), 0, st>>>(q, s, rows, D, o);
 }
 
 constexpr int kThreads = 1024;  // of a block, at most
