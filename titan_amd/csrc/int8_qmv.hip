@@ -6,7 +6,7 @@
 // for itself, the first weights on their way meanwhile: a launch less, and the
 // same codes as int8_rows.hip's.  Bound by the latency of one dependent HBM round
 // trip at one token (per call in a graph, 4096 x 2048: 4.6 us for 8.4 MB, from
-// bf16 values 5.1; top-10 of 1024 x 2048 6.4 and 6.6), by HBM and the caches at
+// bf16 values 4.8; top-10 of 1024 x 2048 6.4 and 6.6), by HBM and the caches at
 // more (six tokens 21).
 #include "int8_codes.h"
 #include "int8_product.h"

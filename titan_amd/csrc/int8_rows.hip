@@ -17,7 +17,7 @@
 // 28 us, 5.4 TB/s; 65536 x 2048 fp32 to codes: 114 us, 5.9
 // TB/s; the values back: 58 us, 6.9 TB/s), by one chain of loads, two reductions and
 // the stores below (one row of 2048: 2.6 us per call in a graph, quantised alone
-// 2.4, its values 2.2).
+// 2.2, its values 2.2).
 #include "int8_codes.h"
 #include "lanes.h"
 
@@ -26,7 +26,7 @@ namespace {
 using namespace qmoe_i8;
 // As put, past the caches: for what is written whole and read later, if at all.
 // The values of 65536 x 2048 in bf16 take 58 us so and 71 without, in fp32 92 and
-// 144; the norm of 4096 x 2048 with its residual's sum and itself 11.3 and 14.1.
+// 144; the norm of 4096 x 2048 with its residual's sum and itself 10.6 and 13.4.
 // Not for codes, which a product reads next (quantisation and product of 16384
 // rows: 163 us so, 157 without).
 template <class T, int N>
