@@ -15,6 +15,11 @@
 // their columns' probabilities in registers.  A row's last vector ends with it:
 // where V does not divide E it overlaps the one before, and what it has as well
 // is not its own: computed alike, stored twice, counted once.
+//
+// Bound by HBM and by the exponentials' issue, then by the join's launch: 32768
+// tokens of 256 fp32 logits, per call in a graph, 10.3 us for the sums (3.3 TB/s),
+// 6.1 for the join, 12.0 for the gradient (5.6 TB/s); 61 tokens of 60 in one launch
+// of 4.2, gradient 3.0.
 #include "elem.h"
 #include "lanes.h"
 

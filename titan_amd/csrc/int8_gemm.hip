@@ -18,6 +18,18 @@
 // heavy-first; those of one matrix go in bands of columns, so that the blocks of
 // an XCD share rows and columns in its L2.  A unit's first copies are issued
 // before the results of the one before it are stored.
+//
+// 256 x 256 by eight waves: a wave's 128 x 64 outputs read 6 KiB of fragments for
+// 8 matrix instructions (with four waves of 128 x 128 4 for 8, but one wave per
+// SIMD waits alone: 75 us at 4096^3, this 60), and a unit copies half the bytes
+// per product that 128 x 128 does (both operands pass L2 -> LDS at up to 33 TB/s
+// in 128-byte pieces, 17 in 64-byte ones).  Large products are bound by power: 60
+// us at 4096^3 (2.3 POP/s), 445 at 8192^3 (2.5), where a loop of the matrix
+// instructions alone reaches 3.45.  Experts are bound by their weights' way from
+// HBM and by the chains of units: 4096 tokens x top-10 of 256, 2048 -> 1024, take
+// 164 us (537 MB of weights: 109 at a copy's rate), 512 tokens 104 (5.3 TB/s).
+// Three stages of 128-column units for experts, more in flight but more units:
+// 185 us instead of 164.
 #include <algorithm>
 
 #include "gemm_common.h"
@@ -492,9 +504,10 @@ int launch(const Product& a, int64_t max_tiles, int unit_rows, hipStream_t st) {
 }
 
 // One matrix.  Up to kFewBlocks blocks of 32 x 32 outputs are the few-rows
-// kernel's, which splits the contraction (4096 x 2048 weights, 128 / 192 / 256
-// rows: 9.1 / 11.4 / 13.6 us, in 64 x 128 units 12.2 / 12.2 / 12.1; 2048 x 8192,
-// 128 rows: 13.4 and 31).  Beyond, the form whose rounds of 256 units cost least.
+// kernel's, which splits the contraction (4096 x 2048 weights, 128 / 160 / 192 / 224
+// rows: 9.4 / 10.9 / 11.7 / 12.9 us, in 64 x 128 units 11.7 / 11.4 / 11.7 / 11.3; 8192
+// x 2048, 64 / 96 rows: 10.4 / 12.6 and 12.1 / 11.6; 2048 x 8192, 128 rows: 14.9 and
+// 31).  Beyond, the form whose rounds of 256 units cost least.
 // A round's cost, as measured with K = 2048: 64 x 128 units 9.5 us, 128 x 128 13,
 // 128 x 256 19, 256 x 256 33; a product of one round takes 3 more (N = 4096: 512
 // rows 12.4 / 14.4 / 19.7 / 35.5 us, 1024 rows 22.6 / 15.8 / 20.0 / 34.8, 4096 rows
