@@ -394,3 +394,15 @@ def test_calls_of_two_threads(dev):
         t.join()
     for i in range(2):
         assert all(torch.equal(a, b) for a, b in zip(want[i], got[i]))
+
+
+def test_more_rounds_of_units_than_are_planned_at_once(dev):
+    """80 rounds of a table's units on 256 CUs."""
+    E, n, N, K = 1000, 1300, 5120, 16
+    g = torch.Generator().manual_seed(34)
+    x, sx = _codes((50, K), 35)
+    w, sw = _codes((E, N, K), 36)
+    ids, rows = torch.cat([torch.arange(E), torch.randint(0, E, (n - E,), generator=g)]).sort().values, torch.randint(0, 50, (n,), generator=g)
+    y = ops.gather_qqmm((x.to(dev).unsqueeze(1), sx.to(dev).unsqueeze(1)), w.to(dev), sw.to(dev), lhs_indices=rows.to(dev),
+                        rhs_indices=ids.to(dev), mode="int8", sorted_indices=True, dtype=F4)
+    o.assert_rounded(y.squeeze(1), _gather_oracle(x, sx, w, sw, rows, ids))

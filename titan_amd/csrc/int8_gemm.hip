@@ -27,9 +27,10 @@
 // us at 4096^3 (2.3 POP/s), 445 at 8192^3 (2.5), where a loop of the matrix
 // instructions alone reaches 3.45.  Experts are bound by their weights' way from
 // HBM and by the chains of units: 4096 tokens x top-10 of 256, 2048 -> 1024, take
-// 164 us (537 MB of weights: 109 at a copy's rate), 512 tokens 104 (5.3 TB/s).
+// 164 us (537 MB of weights and 84 of results: 130 at a copy's rate), 512 tokens 102 (5.4 TB/s).
 // Three stages of 128-column units for experts, more in flight but more units:
-// 185 us instead of 164.
+// 185 us instead of 164; results stored from the registers, with the ring filled
+// meanwhile, 170.
 #include <algorithm>
 
 #include "gemm_common.h"
@@ -213,10 +214,11 @@ struct Form {
       }
   }
 
-  // The sums of a unit whose first group is under way; between() is called once nothing reads the ring any more.
-  template <class Between>
+  // The sums of a unit whose first group is under way; last() is called before the last group's products, between() once
+  // nothing reads the ring any more.
+  template <class Last, class Between>
   static __device__ __forceinline__ void run(const Product& a, const Unit& u, Ctx& c, char* smem, const float* s,
-                                             Between between) {
+                                             Last last, Between between) {
     c.settle(a, smem);
     const int row0 = 32 * MSUB * (c.wave / WN), col0 = 32 * NSUB * (c.wave % WN);
     const int G = (c.units + kUnits - 1) / kUnits;
@@ -233,6 +235,7 @@ struct Form {
     read(c, smem, 0, row0, col0, f[0]);
     int at = 0;  // the stage of group g
     for (int g = 0; g < G; ++g) {
+      if (g + 1 == G) last();
       const char* st = smem + at * kStage;
       const int freed = at == 0 ? NS - 1 : at - 1, from = min(g + NS - 1, G - 1);
 #pragma unroll
@@ -450,43 +453,53 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
   // top-10 of 256: 174 -> 167 us; two rounds: 60 -> 62).
   const int64_t rounds = (snake.units + snake.P - 1) / snake.P;
   const bool reversed = a.offsets && rounds >= 4 && snake.q / (snake.P / 8) % 2;
+  // A table's units of 64 rounds, a lane each, so that the chain of loads that
+  // leads to them is waited for once (512 tokens x top-10 of 256: 104 -> 102 us;
+  // 4096 tokens of 512 values 132 -> 125).
+  struct Planned {
+    int e, valid, row0, col;
+  };
+  const auto plan = [&](int64_t first) {
+    const int64_t r = first + threadIdx.x % 64, at = r < rounds ? snake.unit(reversed ? rounds - 1 - r : r) : -1;
+    if (at < 0) return Planned{0, 0, 0, 0};
+    const int64_t tile = at / NB;
+    const qmoe_gemm::TileRows t = pair_rows_of(table, ranked ? order[tile] : (int)tile);
+    return Planned{t.e, t.valid, (int)t.row0, (int)(at % NB)};
+  };
+  Planned planned{0, 0, 0, 0};
   int64_t round = 0;
   const auto next = [&] {  // this block's next unit
-    Unit u{0, 0, 0, 0};
-    for (;;) {
-      if (round == rounds) return u;
-      const int64_t at = snake.unit(reversed ? rounds - 1 - round : round);
-      ++round;
-      if (at < 0) continue;
-      int col;
+    while (round < rounds) {
+      const int64_t r = round++;
+      Planned p;
       if (a.offsets) {
-        const int64_t tile = at / NB;
-        col = (int)(at % NB);
-        const qmoe_gemm::TileRows t = pair_rows_of(table, ranked ? order[tile] : (int)tile);
-        u.e = __builtin_amdgcn_readfirstlane(t.e);
-        u.valid = __builtin_amdgcn_readfirstlane(t.valid);
-        u.row0 = qmoe_gemm::uniform64(t.row0);
+        const int lane = (int)(r % 64);
+        if (lane == 0) planned = plan(r);
+        p = {__builtin_amdgcn_readlane(planned.e, lane), __builtin_amdgcn_readlane(planned.valid, lane),
+             __builtin_amdgcn_readlane(planned.row0, lane), __builtin_amdgcn_readlane(planned.col, lane)};
       } else {
+        const int64_t at = snake.unit(r);
+        if (at < 0) continue;
         const int64_t band = at / (row_units * kBand), in = at % (row_units * kBand);
         const int wide = (int)min((int64_t)kBand, NB - band * kBand);
-        col = (int)(band * kBand + in % wide);
-        u.row0 = in / wide * unit_rows;
-        u.valid = (int)min((int64_t)unit_rows, a.n_rows - u.row0);
+        const int64_t row0 = in / wide * unit_rows;
+        p = {0, (int)min((int64_t)unit_rows, a.n_rows - row0), (int)row0, (int)(band * kBand + in % wide)};
       }
-      u.o0 = (int64_t)__builtin_amdgcn_readfirstlane(col) * kCols;
-      if (u.valid > 0) return u;
+      p.valid = __builtin_amdgcn_readfirstlane(p.valid);
+      if (p.valid > 0)
+        return Unit{__builtin_amdgcn_readfirstlane(p.e), p.valid, (int64_t)__builtin_amdgcn_readfirstlane(p.row0),
+                    (int64_t)__builtin_amdgcn_readfirstlane(p.col) * kCols};
     }
+    return Unit{0, 0, 0, 0};
   };
   Unit u = next();
   if (u.valid <= 0) return;
   Ctx<kCols> c = begin<Forms>(a, u, rows_of(a, u), smem, scales[0]);
   for (int s = 0;; s ^= 1) {
-    // the next unit's rows, while this one's first copies are under way
     const Unit v = next();
     Rows rows = {};
-    if (v.valid > 0) rows = rows_of(a, v);
     Ctx<kCols> d;
-    Forms::run(a, u, c, smem, scales[s], [&] {
+    Forms::run(a, u, c, smem, scales[s], [&] { if (v.valid > 0) rows = rows_of(a, v); }, [&] {
       if (v.valid > 0) d = begin<Forms>(a, v, rows, smem, scales[s ^ 1]);
     });
     if (v.valid <= 0) break;
