@@ -406,3 +406,21 @@ def test_more_rounds_of_units_than_are_planned_at_once(dev):
     y = ops.gather_qqmm((x.to(dev).unsqueeze(1), sx.to(dev).unsqueeze(1)), w.to(dev), sw.to(dev), lhs_indices=rows.to(dev),
                         rhs_indices=ids.to(dev), mode="int8", sorted_indices=True, dtype=F4)
     o.assert_rounded(y.squeeze(1), _gather_oracle(x, sx, w, sw, rows, ids))
+
+
+@pytest.mark.parametrize("E,n,N,K", [(6, 700, 300, 272),    # half tiles by 128 columns
+                                     (5, 6000, 333, 144),   # tiles by 128
+                                     (3, 9000, 500, 64),    # tiles by 256
+                                     (3, 20000, 600, 48)])  # pairs of tiles by 256
+def test_units_of_tables(dev, E, n, N, K):
+    """Each shape of a table's units, with experts of every share of rows and one without, in every type."""
+    g = torch.Generator().manual_seed(n)
+    x, sx = _codes((900, K), 37)
+    w, sw = _codes((E, N, K), 38)
+    p = torch.linspace(0, 1, E)  # expert 0: no rows
+    ids, rows = torch.multinomial(p, n, replacement=True, generator=g).sort().values, torch.randint(0, 900, (n,), generator=g)
+    want = _gather_oracle(x, sx, w, sw, rows, ids)
+    for out in (BF, HF, F4):
+        y = ops.gather_qqmm((x.to(dev).unsqueeze(1), sx.to(dev).unsqueeze(1)), w.to(dev), sw.to(dev), lhs_indices=rows.to(dev),
+                            rhs_indices=ids.to(dev), mode="int8", sorted_indices=True, dtype=out)
+        o.assert_rounded(y.squeeze(1), want, what=out)

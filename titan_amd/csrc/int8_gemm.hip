@@ -14,8 +14,8 @@
 // hold up the wave that issues them.
 //
 // Blocks are persistent.  Units of a table take two tiles of an expert where it
-// has them, so that its weights are read once for up to 256 rows, and go
-// heavy-first; those of one matrix go in bands of columns, so that the blocks of
+// has them and they fill the chip, so that its weights are read once for up to 256
+// rows, and go heavy-first; those of one matrix go in bands of columns, so that the blocks of
 // an XCD share rows and columns in its L2.  A unit's first copies are issued
 // before the results of the one before it are stored.
 //
@@ -378,30 +378,39 @@ typedef Pick<Form<2, 4, 4, 2, 2>, Form<2, 4, 3, 2, 2>, Form<2, 4, 2, 2, 3>, Form
 // groups ahead, where it is the copies' way that takes the time.
 constexpr int kNarrowRows = 64;
 typedef Pick<Form<2, 4, 1, 1, 6>> Narrow;
-typedef Pick<Form<2, 4, 2, 1, 4>> Middle;
+typedef Pick<Form<2, 4, 2, 1, 4>, Form<2, 4, 1, 1, 6>> Middle;
 
-// The rows of tile t's unit, 0 for the second tile of a pair.
-__device__ __forceinline__ qmoe_gemm::TileRows pair_rows_of(const qmoe_gemm::Tiles& t, int tile) {
-  qmoe_gemm::TileRows r = qmoe_gemm::tile_rows_of(t, tile);
+// The rows of a table's row unit: two tiles of an expert (none for the second of
+// them), a tile or half of one.
+__device__ __forceinline__ qmoe_gemm::TileRows unit_rows_of(const qmoe_gemm::Tiles& t, int unit, int unit_rows) {
+  if (unit_rows == kTileRows) return qmoe_gemm::tile_rows_of(t, unit);
+  if (unit_rows < kTileRows) {
+    qmoe_gemm::TileRows r = qmoe_gemm::tile_rows_of(t, unit / 2);
+    const int first = unit % 2 * unit_rows;
+    r.row0 += first;
+    r.valid = min(r.valid - first, unit_rows);
+    return r;
+  }
+  qmoe_gemm::TileRows r = qmoe_gemm::tile_rows_of(t, unit);
   const int64_t first = t.offsets[r.e], end = min((int64_t)t.offsets[r.e + 1], t.n_rows);
   r.valid = r.valid <= 0 || ((r.row0 - first) / kTileRows) % 2 ? 0 : (int)min((int64_t)kPairRows, end - r.row0);
   return r;
 }
 
-// Ranks the units of `tiles` (<= kMaxRanked) tiles by their 32-row subtiles,
-// largest first and stable in tile order; returns how many there are.  cls is
-// scratch of kMaxRanked + 1 ints.  Called by the whole block.
+// Ranks a table's row units (<= kMaxRanked) by their 32-row subtiles, largest
+// first and stable in their order; returns how many have rows.  cls is scratch of
+// kMaxRanked + 1 ints.  Called by the whole block.
 constexpr int kMaxRanked = 1024;
-__device__ inline int rank_pairs(const qmoe_gemm::Tiles& t, int tiles, int* order, int* cls) {
-  for (int i = threadIdx.x; i < tiles; i += kThreads) cls[i] = (pair_rows_of(t, i).valid + 31) / 32;
+__device__ inline int rank_units(const qmoe_gemm::Tiles& t, int row_units, int unit_rows, int* order, int* cls) {
+  for (int i = threadIdx.x; i < row_units; i += kThreads) cls[i] = (max(unit_rows_of(t, i, unit_rows).valid, 0) + 31) / 32;
   __syncthreads();
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
     const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
     constexpr int kClasses = kPairRows / 32;
     int start[kClasses + 1] = {};
-    for (int i = 0; i < tiles; i += 64) {
-      const int m = i + lane < tiles ? cls[i + lane] : 0;
+    for (int i = 0; i < row_units; i += 64) {
+      const int m = i + lane < row_units ? cls[i + lane] : 0;
 #pragma unroll
       for (int k = 1; k <= kClasses; ++k) start[k] += __popcll(__ballot(m == k));
     }
@@ -413,8 +422,8 @@ __device__ inline int rank_pairs(const qmoe_gemm::Tiles& t, int tiles, int* orde
       sum += n;
     }
     if (lane == 0) cls[kMaxRanked] = sum;
-    for (int i = 0; i < tiles; i += 64) {
-      const int m = i + lane < tiles ? cls[i + lane] : 0;
+    for (int i = 0; i < row_units; i += 64) {
+      const int m = i + lane < row_units ? cls[i + lane] : 0;
 #pragma unroll
       for (int k = 1; k <= kClasses; ++k) {
         const uint64_t same = __ballot(m == k);
@@ -429,7 +438,7 @@ __device__ inline int rank_pairs(const qmoe_gemm::Tiles& t, int tiles, int* orde
   return units;
 }
 
-// row_units, unit_rows: of one matrix (unit_rows <= kPairRows); a table's units are its own.
+// row_units: of one matrix, or as many as a table has room for.
 template <class Forms>
 __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t row_units, int unit_rows, int NB) {
   constexpr int kCols = Forms::kCols;
@@ -441,9 +450,9 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
   const qmoe_gemm::Tiles table{a.offsets, a.tile_row, a.tile_exp, a.ntiles, a.n_rows, a.num_experts};
   bool ranked = false;
   if (a.offsets) {
-    row_units = min((int64_t)max(a.ntiles[0], 0), row_units);  // of as many as the caller says there is room for
+    row_units = min((int64_t)max(a.ntiles[0], 0) * (unit_rows < kTileRows ? 2 : 1), row_units);
     ranked = row_units <= kMaxRanked;
-    if (ranked) row_units = rank_pairs(table, (int)row_units, order, reinterpret_cast<int*>(smem));
+    if (ranked) row_units = rank_units(table, (int)row_units, unit_rows, order, reinterpret_cast<int*>(smem));
   }
   const qmoe_gemm::Snake snake(row_units * NB);
   constexpr int kBand = 8;  // column blocks of a band
@@ -462,8 +471,8 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
   const auto plan = [&](int64_t first) {
     const int64_t r = first + threadIdx.x % 64, at = r < rounds ? snake.unit(reversed ? rounds - 1 - r : r) : -1;
     if (at < 0) return Planned{0, 0, 0, 0};
-    const int64_t tile = at / NB;
-    const qmoe_gemm::TileRows t = pair_rows_of(table, ranked ? order[tile] : (int)tile);
+    const int64_t unit = at / NB;
+    const qmoe_gemm::TileRows t = unit_rows_of(table, ranked ? order[unit] : (int)unit, unit_rows);
     return Planned{t.e, t.valid, (int)t.row0, (int)(at % NB)};
   };
   Planned planned{0, 0, 0, 0};
@@ -510,7 +519,7 @@ __global__ __launch_bounds__(kThreads) void int8_gemm_kernel(Product a, int64_t 
 
 template <class Forms>
 int launch(const Product& a, int64_t max_tiles, int unit_rows, hipStream_t st) {
-  const int64_t NB = (a.N + Forms::kCols - 1) / Forms::kCols, rows = a.offsets ? max_tiles : (a.n_rows + unit_rows - 1) / unit_rows;
+  const int64_t NB = (a.N + Forms::kCols - 1) / Forms::kCols, rows = a.offsets ? max_tiles * (unit_rows < kTileRows ? 2 : 1) : (a.n_rows + unit_rows - 1) / unit_rows;
   const dim3 grid((unsigned)qmoe_gemm::grid_blocks(rows * NB, 1));
   int8_gemm_kernel<Forms><<<grid, dim3(kThreads), 0, st>>>(a, rows, unit_rows, (int)NB);
   return qmoe::launch_status("int8_gemm_kernel");
@@ -539,6 +548,24 @@ int dense(const Product& a, hipStream_t st) {
   return least == middle ? launch<Middle>(a, 0, kTileRows, st) : launch<Narrow>(a, 0, kNarrowRows, st);
 }
 
+// A table's rows.  The smallest units that one round of the chip takes, by the
+// units that n rows make on as many experts as they can reach, each with half a
+// unit to spare; where none are, the widest (64 x 128 / 128 x 128 / 128 x 256 / 256
+// x 256, us per call in a graph: 2300 rows on 6 experts, 2016 -> 520 13.3 / 15.8 /
+// 20.9 / 34.8; 1860 on 7, 1744 -> 912 19.8 / 16.2 / 21.1 / 34.3; 9500 on 17, 800 ->
+// 472 21.5 / 19.8 / 15.5 / 23.7; past a round 8200 on 32, 2048 -> 1024 55 / 45 / 44 /
+// 44; 41,000 on 256 - / - / 177 / 164).
+int grouped(const Product& a, int64_t max_tiles, hipStream_t st) {
+  const int64_t experts = std::min<int64_t>(a.num_experts, a.n_rows);
+  const auto fits = [&](int64_t rows, int64_t cols) {
+    const int64_t units = std::max(experts, (a.n_rows + rows * experts / 2 + rows - 1) / rows);
+    return units * ((a.N + cols - 1) / cols) <= kRoundUnits;
+  };
+  if (fits(kNarrowRows, 128)) return launch<Narrow>(a, max_tiles, kNarrowRows, st);
+  if (fits(kTileRows, 128)) return launch<Middle>(a, max_tiles, kTileRows, st);
+  return launch<Wide>(a, max_tiles, fits(kTileRows, 256) ? kTileRows : kPairRows, st);
+}
+
 }  // namespace
 
 extern "C" int qmoe_int8_gather_qqmm(const int8_t* x, const float* sx, int64_t n_x, const int32_t* x_rows, int64_t n_rows,
@@ -556,5 +583,5 @@ extern "C" int qmoe_int8_gather_qqmm(const int8_t* x, const float* sx, int64_t n
   if (any && max_tiles <= 0) return qmoe::fail(QMOE_ERR_INVALID, "an empty tile table");
   if (max_tiles > 0x7FFFFFFF) return qmoe::fail(QMOE_ERR_UNSUPPORTED, "sizes too large");
   hipStream_t st = qmoe::as_stream(stream);
-  return any ? launch<Wide>(a, max_tiles, kPairRows, st) : dense(a, st);
+  return any ? grouped(a, max_tiles, st) : dense(a, st);
 }
