@@ -527,14 +527,14 @@ int launch(const Product& a, int64_t max_tiles, int unit_rows, hipStream_t st) {
 
 // One matrix.  Up to kFewBlocks blocks of 32 x 32 outputs are the few-rows
 // kernel's, which splits the contraction (4096 x 2048 weights, 128 / 160 / 192 / 224
-// rows: 9.4 / 10.9 / 11.7 / 12.9 us, in 64 x 128 units 11.7 / 11.4 / 11.7 / 11.3; 8192
-// x 2048, 64 / 96 rows: 10.4 / 12.6 and 12.1 / 11.6; 2048 x 8192, 128 rows: 14.9 and
-// 31).  Beyond, the form whose rounds of 256 units cost least.
-// A round's cost, as measured with K = 2048: 64 x 128 units 9.5 us, 128 x 128 13,
-// 128 x 256 19, 256 x 256 33; a product of one round takes 3 more (N = 4096: 512
-// rows 12.4 / 14.4 / 19.7 / 35.5 us, 1024 rows 22.6 / 15.8 / 20.0 / 34.8, 4096 rows
-// 76 / 55 / 43 / 40).
-constexpr int64_t kFewBlocks = 768, kRoundUnits = 256;
+// rows: 9.4 / 10.9 / 11.7 / 12.9 us, in 64 x 128 units 11.7 / 11.4 / 11.7 / 11.3;
+// 1000 rows of 520 x 1600 9.2 and 10.1, of 520 x 4096 15.8 and 15.7; 3000 rows of
+// 215 x 4096 19.6 and 15.7; 100 rows of 2048 x 4096 8.3 and 15.4).  Beyond, the form
+// whose rounds of 256 units cost least.  A round's cost, as measured with K = 2048:
+// 64 x 128 units 9.5 us, 128 x 128 13, 128 x 256 19, 256 x 256 33; a product of one
+// round takes 3 more (N = 4096: 512 rows 12.1 / 13.7 / 18.9 / 29.1 us, 1024 rows 21.0 /
+// 15.3 / 18.1 / 29.2, 4096 rows 73 / 55 / 44.5 / 37.6).
+constexpr int64_t kFewBlocks = 544, kRoundUnits = 256;
 int dense(const Product& a, hipStream_t st) {
   const auto blocks = [&](int64_t rows, int64_t cols) { return (a.n_rows + rows - 1) / rows * ((a.N + cols - 1) / cols); };
   if (blocks(32, 32) <= kFewBlocks) return few_product(a, st);
