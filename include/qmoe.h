@@ -584,6 +584,15 @@ int qmoe_int8_quantize(const void* x, int dtype, int64_t rows, int64_t K,
 int qmoe_int8_dequantize(const int8_t* codes, const float* scales,
                          int64_t rows, int64_t K, int dtype, void* out,
                          void* stream);
+/* qmoe_int8_quantize, and in the same launch qmoe_build_tiles_clamped of the
+ * sorted ids that a product of those rows goes by. */
+int qmoe_int8_quantize_sorted(const void* x, int dtype, int64_t rows, int64_t K,
+                              int8_t* codes, float* scales,
+                              const int32_t* sorted_ids, int64_t n_rows,
+                              int32_t num_experts, int32_t tile_rows,
+                              int32_t* offsets, int32_t* tile_row,
+                              int32_t* tile_exp, int32_t* ntiles,
+                              int64_t max_tiles, void* stream);
 
 /* RMS norm into that form (an extension): h = x + residual, rounded to the
  * rows' type (residual NULL: h = x), v = h / sqrt(mean(h^2) + eps) * weight

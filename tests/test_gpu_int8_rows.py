@@ -239,3 +239,22 @@ def test_refusals_on_the_gpu(dev):
         ops.quantize(x.cpu(), mode="int8")
     with pytest.raises(ValueError):
         ops.rms_norm_quantize(x, None, float("nan"))
+
+
+@pytest.mark.parametrize("rows,K,dtype", [(1, 5, BF), (700, 2048, BF), (3000, 1000, HF), (40, 4096, F4), (5, 20000, F4), (9, 0, BF), (0, 64, BF)])
+@pytest.mark.parametrize("n,E", [(0, 3), (64, 1), (1000, 60), (5000, 256), (300, 700)])
+def test_quantize_with_the_table_of_sorted_ids(dev, rows, K, dtype, n, E):
+    """One launch for both: the bits of the two."""
+    from titan_amd import _lib
+
+    x = _rows((rows, K), dtype, 16).to(dev) if K else torch.zeros(rows, 0, dtype=dtype, device=dev)
+    ids = torch.randint(-1, E + 1, (n,), generator=torch.Generator().manual_seed(n)).sort().values.int().to(dev)
+    q, s = ops.quantize(x, mode="int8")
+    t = ops.build_tiles(ids, E)
+    codes, scales = torch.full_like(q, 99), torch.full_like(s, -1.0)
+    tables = [torch.full_like(i, -7) for i in (t.offsets, t.tile_row, t.tile_exp, t.ntiles)]
+    _lib.call("qmoe_int8_quantize_sorted", x.data_ptr(), ops._DTYPES[dtype], rows, K, codes.data_ptr(), scales.data_ptr(),
+              ids.data_ptr(), n, E, ops.tile_rows(), *(i.data_ptr() for i in tables), t.maxt,
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(codes, q) and torch.equal(scales, s)
+    assert all(torch.equal(a, b) for a, b in zip(tables, (t.offsets, t.tile_row, t.tile_exp, t.ntiles)))

@@ -200,6 +200,12 @@ def test_rows_entries():
                     ((P, 0, 2, 8, ODD, P, None), _lib.ERR_UNSUPPORTED), ((P, 0, 1 << 33, 8, P, P, None), _lib.ERR_UNSUPPORTED),
                     ((P, 0, 2, 1 << 31, P, P, None), _lib.ERR_UNSUPPORTED), ((None, 0, 0, 8, None, None, None), _lib.OK)):
         assert _rc("qmoe_int8_quantize", *bad) == rc, bad
+    both = dict(x=P, dt=0, rows=2, K=8, q=P, s=P, ids=P, n=4, E=2, tr=128, off=P, row=P, exp=P, nt=P, maxt=3)
+    for change, rc in (({"dt": 3}, _lib.ERR_UNSUPPORTED), ({"x": None}, _lib.ERR_INVALID), ({"q": ODD}, _lib.ERR_UNSUPPORTED),
+                       ({"n": -1}, _lib.ERR_INVALID), ({"E": 0}, _lib.ERR_INVALID), ({"tr": 0}, _lib.ERR_INVALID),
+                       ({"ids": None}, _lib.ERR_INVALID), ({"off": None}, _lib.ERR_INVALID), ({"nt": None}, _lib.ERR_INVALID),
+                       ({"n": 1 << 31}, _lib.ERR_UNSUPPORTED), ({"maxt": -1}, _lib.ERR_INVALID)):
+        assert _rc("qmoe_int8_quantize_sorted", *{**both, **change}.values(), None) == rc, change
     for bad, rc in (((P, P, 2, 8, 3, P, None), _lib.ERR_UNSUPPORTED), ((P, None, 2, 8, 0, P, None), _lib.ERR_INVALID),
                     ((P, P, 2, 8, 0, ODD, None), _lib.ERR_UNSUPPORTED), ((P, P, 2, 0, 0, P, None), _lib.OK)):
         assert _rc("qmoe_int8_dequantize", *bad) == rc, bad

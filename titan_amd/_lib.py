@@ -100,6 +100,7 @@ SIGNATURES: dict[str, tuple] = {
     "qmoe_unsort_sum": (INT, [P, I64, INT, P, P, P, I64, I64, I64, INT, P, P]),
     "qmoe_unsort_grad": (INT, [P, P, I64, INT, P, P, I64, I64, I64, P, P, P]),
     "qmoe_int8_quantize": (INT, [P, INT, I64, I64, P, P, P]),
+    "qmoe_int8_quantize_sorted": (INT, [P, INT, I64, I64, P, P, P, I64, I32, I32, P, P, P, P, I64, P]),
     "qmoe_int8_dequantize": (INT, [P, P, I64, I64, INT, P, P]),
     "qmoe_int8_rms_norm": (INT, [P, P, P, INT, INT, I64, I64, ctypes.c_double, P, P, P, P, P]),
     "qmoe_int8_gather_qqmv": (INT, [P, P, I64, P, I32, P, I64, P, P, I32, I64, I64, INT, P, P]),

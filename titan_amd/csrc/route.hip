@@ -22,12 +22,15 @@
 #include <mutex>
 
 #include "common.h"
+#include "tiles.h"
 
 namespace {
 
 constexpr int kChunk = 1024;    // rows per histogram chunk
 constexpr int kCountThreads = 256;
 constexpr int kScanThreads = 1024;
+using qmoe_tiles::block_exclusive_scan;
+using qmoe_tiles::emit_tiles;
 
 // What the MoE block's routing writes besides the tables (all off by default):
 // x_rows[sorted position] = the pair's token, pair / top_k, which the gate_up
@@ -77,71 +80,6 @@ __global__ __launch_bounds__(kCountThreads) void route_count_kernel(const int32_
   __syncthreads();
   for (int e = threadIdx.x; e <= E; e += blockDim.x)
     counts[chunk_major ? (int64_t)blockIdx.x * (E + 1) + e : (int64_t)e * nchunks + blockIdx.x] = hist[e];
-}
-
-// Exclusive scan of one value per thread over a block of T threads; also
-// returns the total.  Each wave scans its 64 values with shuffles, one wave
-// scans the wave totals, and every thread adds its wave's base: three
-// barriers.  lds holds at least T / 64 + 1 ints.
-template <int T = kScanThreads>
-__device__ int block_exclusive_scan(int v, int* lds, int* total) {
-  static_assert(T % 64 == 0 && T <= 4096, "whole waves, at most 64");
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  constexpr int kWavesPerBlock = T / 64;
-  int x = v;  // inclusive scan within the wave
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) lds[w] = x;
-  __syncthreads();
-  if (w == 0) {
-    const int t = lane < kWavesPerBlock ? lds[lane] : 0;
-    int u = t;
-#pragma unroll
-    for (int d = 1; d < kWavesPerBlock; d <<= 1) {
-      const int y = __shfl_up(u, d, 64);
-      if (lane >= d) u += y;
-    }
-    if (lane < kWavesPerBlock) lds[lane] = u - t;  // exclusive base of wave `lane`
-    if (lane == kWavesPerBlock - 1) lds[kWavesPerBlock] = u;
-  }
-  __syncthreads();
-  *total = lds[kWavesPerBlock];
-  const int res = lds[w] + x - v;
-  __syncthreads();  // lds is free for the caller's next use
-  return res;
-}
-
-// Tiles from offsets (offsets[0..E] visible to the block of T threads): one
-// (row_start, expert) per tile_rows rows, expert-major; zero-fills
-// [ntiles, max_tiles).
-template <int T = kScanThreads>
-__device__ void emit_tiles(const int32_t* offsets, int E, int tile_rows, int32_t* tile_row,
-                           int32_t* tile_exp, int32_t* ntiles, int64_t max_tiles, int* lds) {
-  const int tid = threadIdx.x;
-  const int seg = (E + T - 1) / T;
-  const int lo = min(tid * seg, E), hi = min(lo + seg, E);
-  int local = 0;
-  for (int e = lo; e < hi; ++e) local += (offsets[e + 1] - offsets[e] + tile_rows - 1) / tile_rows;
-  int total;
-  int64_t t = block_exclusive_scan<T>(local, lds, &total);
-  for (int e = lo; e < hi; ++e) {
-    const int s = offsets[e], q = offsets[e + 1];
-    for (int r = s; r < q; r += tile_rows, ++t) {
-      if (t < max_tiles) {
-        tile_row[t] = r;
-        tile_exp[t] = e;
-      }
-    }
-  }
-  const int64_t nt = min((int64_t)total, max_tiles);
-  if (tid == 0) ntiles[0] = (int32_t)nt;
-  for (int64_t j = nt + tid; j < max_tiles; j += T) {
-    tile_row[j] = 0;
-    tile_exp[j] = 0;
-  }
 }
 
 // counts is the [E + 1][nchunks] table of route_count_kernel (row E: ids out
@@ -450,43 +388,9 @@ __global__ __launch_bounds__(64 * kScanScatterWaves) void route_scan_scatter_ker
   }
 }
 
-__global__ __launch_bounds__(kScanThreads) void tiles_from_sorted_kernel(const int32_t* __restrict__ sorted_ids,
-                                                                         int64_t n, int E, int tile_rows,
-                                                                         int32_t* __restrict__ offsets,
-                                                                         int32_t* __restrict__ tile_row,
-                                                                         int32_t* __restrict__ tile_exp,
-                                                                         int32_t* __restrict__ ntiles,
-                                                                         int64_t max_tiles, bool all) {
-  // all: ids below 0 are expert 0's, ids from E on expert E - 1's, so that every row has a tile
-  // first row whose id >= e, in two levels: a search over every stride-th id,
-  // read by the block at once, then one inside a stride.  (Each step of a
-  // search in memory is a dependent read, 15 of them at 20,480 rows: 4.8 -> 4.5
-  // us per call in a graph, where the ids are in the caches.)
-  __shared__ int lds[kScanThreads];
-  const int64_t stride = (n + kScanThreads - 1) / kScanThreads;
-  const int ns = n > 0 ? (int)((n + stride - 1) / stride) : 0;  // samples
-  if ((int)threadIdx.x < ns) lds[threadIdx.x] = sorted_ids[threadIdx.x * stride];
-  __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += kScanThreads) {
-    int a = 0, b = ns;
-    while (a < b) {
-      const int mid = (a + b) >> 1;
-      if (lds[mid] < e) a = mid + 1;
-      else b = mid;
-    }
-    // sample a is the first with id >= e: the row lies past sample a - 1
-    int64_t lo = a > 0 ? (a - 1) * stride + 1 : 0, hi = min(a * stride, n);
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (sorted_ids[mid] < e) lo = mid + 1;
-      else hi = mid;
-    }
-    if (all && e == 0) lo = 0;
-    if (all && e == E) lo = n;
-    offsets[e] = (int32_t)lo;
-  }
-  __syncthreads();
-  emit_tiles(offsets, E, tile_rows, tile_row, tile_exp, ntiles, max_tiles, lds);
+__global__ __launch_bounds__(kScanThreads) void tiles_from_sorted_kernel(qmoe_tiles::Sorted t) {
+  __shared__ int lds[qmoe_tiles::kSamples];
+  qmoe_tiles::from_sorted<kScanThreads>(t, lds);
 }
 
 // The whole routing step in one block, for up to kFusedMaxN pairs and
@@ -718,7 +622,7 @@ static int build_tiles(const int32_t* sorted_ids, int64_t n_rows, int32_t num_ex
   if (!offsets || !tile_row || !tile_exp || !ntiles || (n_rows > 0 && !sorted_ids))
     return qmoe::fail(QMOE_ERR_INVALID, "null pointer");
   tiles_from_sorted_kernel<<<dim3(1), dim3(kScanThreads), 0, qmoe::as_stream(stream)>>>(
-      sorted_ids, n_rows, num_experts, tile_rows, offsets, tile_row, tile_exp, ntiles, max_tiles, all);
+      {sorted_ids, n_rows, num_experts, tile_rows, offsets, tile_row, tile_exp, ntiles, max_tiles, all});
   return qmoe::launch_status("tiles_from_sorted_kernel");
 }
 

@@ -432,7 +432,8 @@ py::object matmul(py::handle x_, py::handle w_, py::handle s_, bool transpose, b
   return give(y);
 }
 
-bool table(const Tensor& experts, int64_t E, Rows* r) {
+// Room for the table of r's rows.
+bool room(const Tensor& experts, int64_t E, Rows* r) {
   const int64_t tr = qmoe_gemm_tile_rows(), n = r->n;
   if (E <= 0 || E > INT32_MAX || n > INT32_MAX) return false;
   r->maxt = (n + tr - 1) / tr + E;
@@ -444,9 +445,13 @@ bool table(const Tensor& experts, int64_t E, Rows* r) {
   r->tile_row = all.narrow(0, a, r->maxt);
   r->tile_exp = all.narrow(0, a + b, r->maxt);
   r->ntiles = all.narrow(0, a + 2 * b, 1);
-  ok(qmoe_build_tiles_clamped(ptr<int32_t>(experts), n, (int32_t)E, (int32_t)tr, r->offsets.data_ptr<int32_t>(),
-                      r->tile_row.data_ptr<int32_t>(), r->tile_exp.data_ptr<int32_t>(), r->ntiles.data_ptr<int32_t>(),
-                      r->maxt, stream(experts)),
+  return true;
+}
+bool table(const Tensor& experts, int64_t E, Rows* r) {
+  if (!room(experts, E, r)) return false;
+  ok(qmoe_build_tiles_clamped(ptr<int32_t>(experts), r->n, (int32_t)E, (int32_t)qmoe_gemm_tile_rows(),
+                              r->offsets.data_ptr<int32_t>(), r->tile_row.data_ptr<int32_t>(),
+                              r->tile_exp.data_ptr<int32_t>(), r->ntiles.data_ptr<int32_t>(), r->maxt, stream(experts)),
      "qmoe_build_tiles_clamped");
   return true;
 }
@@ -550,9 +555,19 @@ bool scales32(const Tensor& t) {  // scales need no alignment past their own
   return t.scalar_type() == at::kFloat && t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() && !t.is_neg();
 }
 
-std::pair<Tensor, Tensor> int8_run(const Tensor& x) {
+// sorted: the table of its experts is made by the same launch.
+std::pair<Tensor, Tensor> int8_run(const Tensor& x, Rows* sorted = nullptr, int64_t E = 0) {
   Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar).requires_grad(false));
   Tensor s = at::empty(batch_of(x), x.options().dtype(at::kFloat).requires_grad(false));
+  if (sorted) {
+    ok(qmoe_int8_quantize_sorted(x.const_data_ptr(), type_of(x), row_count(x), x.size(-1), q.data_ptr<int8_t>(),
+                                 s.data_ptr<float>(), ptr<int32_t>(sorted->experts), sorted->n, (int32_t)E,
+                                 (int32_t)qmoe_gemm_tile_rows(), sorted->offsets.data_ptr<int32_t>(),
+                                 sorted->tile_row.data_ptr<int32_t>(), sorted->tile_exp.data_ptr<int32_t>(),
+                                 sorted->ntiles.data_ptr<int32_t>(), sorted->maxt, stream(x)),
+       "qmoe_int8_quantize_sorted");
+    return {q, s};
+  }
   ok(qmoe_int8_quantize(x.const_data_ptr(), type_of(x), row_count(x), x.size(-1), q.data_ptr<int8_t>(), s.data_ptr<float>(),
                         stream(x)),
      "qmoe_int8_quantize");
@@ -689,8 +704,11 @@ py::object int8_gather(py::handle x_, py::handle sx_, py::handle w_, py::handle 
       !arranged(a.x, g.E, lhs_, rhs_, is_sorted, false, &r, &rhs))
     return py::none();
   const c10::hip::HIPGuard guard(a.x.get_device());
-  if (r.n >= kSortedMinRows && !table(r.experts, g.E, &r)) return py::none();
   type = a.type(type);
+  if (r.n >= kSortedMinRows) {
+    if (a.s.defined() ? !table(r.experts, g.E, &r) : !room(r.experts, g.E, &r)) return py::none();
+    if (!a.s.defined()) std::tie(a.x, a.s) = int8_run(a.x, &r, g.E);
+  }
   auto sizes = rhs.sizes().vec();
   sizes.push_back(1);
   sizes.push_back(g.N);
