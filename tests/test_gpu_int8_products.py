@@ -424,3 +424,27 @@ def test_units_of_tables(dev, E, n, N, K):
         y = ops.gather_qqmm((x.to(dev).unsqueeze(1), sx.to(dev).unsqueeze(1)), w.to(dev), sw.to(dev), lhs_indices=rows.to(dev),
                             rhs_indices=ids.to(dev), mode="int8", sorted_indices=True, dtype=out)
         o.assert_rounded(y.squeeze(1), want, what=out)
+
+
+def test_tables_that_do_not_fit(dev):
+    """A table for other rows is made anew; one whose tensors are too short, of another type or of another device is refused."""
+    import dataclasses
+
+    x, sx = (t.to(dev) for t in _codes((100, 1, 64), 39))
+    w, sw = (t.to(dev) for t in _codes((4, 48, 64), 40))
+    ids = torch.randint(0, 4, (100,), generator=torch.Generator().manual_seed(3)).sort().values.int().to(dev)
+
+    def call(t, i=ids):
+        return ops.gather_qqmm((x[:i.numel()], sx[:i.numel()]), w, sw, rhs_indices=i, mode="int8", sorted_indices=True, tiles=t)
+
+    want, table = call(None), ops.build_tiles(ids, 4)
+    assert torch.equal(call(table), want) and torch.equal(call(table, ids[:70]), want[:70])
+    assert torch.equal(call(table, ids.long()), want) and torch.equal(call(table, ids[:9]), want[:9])
+    for change in ({"tile_row": table.tile_row[:1]}, {"tile_exp": table.tile_exp.long()}, {"offsets": table.offsets[:4]},
+                   {"ntiles": table.ntiles[:0]}, {"maxt": 0}, {"tile_row": table.tile_row.cpu()}):
+        with pytest.raises(RuntimeError, match="tile table"):
+            call(dataclasses.replace(table, **change))
+    with pytest.raises(ValueError, match="tile table"):
+        call(dataclasses.replace(table, num_experts=5))
+    with pytest.raises(ValueError, match="tile table"):
+        call(dataclasses.replace(table, tile_rows=64))

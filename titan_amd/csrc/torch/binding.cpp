@@ -693,8 +693,20 @@ py::object int8_matmul(py::handle x_, py::handle sx_, py::handle w_, py::handle 
   return give(int8_product_run(a, g, r, type).reshape(sizes));
 }
 
+// offsets, rows, experts and number of tiles, and how many there is room for; takes it if it is a table as the kernels
+// read it.
+using Table = std::tuple<Tensor, Tensor, Tensor, Tensor, int64_t>;
+bool take(const Table& t, int64_t E, const at::Device& device, Rows* r) {
+  std::tie(r->offsets, r->tile_row, r->tile_exp, r->ntiles, r->maxt) = t;
+  for (const Tensor* i : {&r->offsets, &r->tile_row, &r->tile_exp, &r->ntiles})
+    if (!i->defined() || i->scalar_type() != at::kInt || !i->is_contiguous() || i->device() != device) return false;
+  return r->offsets.numel() > E && r->maxt > 0 && r->tile_row.numel() >= r->maxt && r->tile_exp.numel() >= r->maxt &&
+         r->ntiles.numel() >= 1;
+}
+
+// tiles: the table of sorted rows, if there is one for this call.
 py::object int8_gather(py::handle x_, py::handle sx_, py::handle w_, py::handle s_, py::handle lhs_, py::handle rhs_,
-                       bool is_sorted, int type) {
+                       bool is_sorted, int type, const std::optional<Table>& tiles) {
   refuse_recorders();
   Acts a;
   Weights8 g;
@@ -705,7 +717,9 @@ py::object int8_gather(py::handle x_, py::handle sx_, py::handle w_, py::handle 
     return py::none();
   const c10::hip::HIPGuard guard(a.x.get_device());
   type = a.type(type);
-  if (r.n >= kSortedMinRows) {
+  if (r.n >= kSortedMinRows && tiles) {
+    if (!take(*tiles, g.E, a.x.device(), &r)) return py::none();
+  } else if (r.n >= kSortedMinRows) {
     if (a.s.defined() ? !table(r.experts, g.E, &r) : !room(r.experts, g.E, &r)) return py::none();
     if (!a.s.defined()) std::tie(a.x, a.s) = int8_run(a.x, &r, g.E);
   }
@@ -718,8 +732,7 @@ py::object int8_gather(py::handle x_, py::handle sx_, py::handle w_, py::handle 
 // Rows already arranged by the wrapper, as rows_product has them.
 py::object int8_rows_product(py::handle x_, py::handle sx_, py::handle w_, py::handle s_,
                              const std::optional<Tensor>& x_rows, int64_t div, const std::optional<Tensor>& experts,
-                             const std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, int64_t>>& tiles, int64_t n,
-                             int type) {
+                             const std::optional<Table>& tiles, int64_t n, int type) {
   refuse_recorders();
   Acts a;
   Weights8 g;
@@ -729,8 +742,8 @@ py::object int8_rows_product(py::handle x_, py::handle sx_, py::handle w_, py::h
   r.div = div;
   if (x_rows) r.x_rows = *x_rows;
   if (experts) r.experts = *experts;
-  if (tiles) std::tie(r.offsets, r.tile_row, r.tile_exp, r.ntiles, r.maxt) = *tiles;
-  for (const Tensor* t : {&r.x_rows, &r.experts, &r.offsets, &r.tile_row, &r.tile_exp, &r.ntiles})
+  TORCH_CHECK(!tiles || take(*tiles, g.E, a.x.device(), &r), "the tile table is not what the kernels read");
+  for (const Tensor* t : {&r.x_rows, &r.experts})
     TORCH_CHECK(!t->defined() || (t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == a.x.device()),
                 "the arguments are not what the kernels read");
   TORCH_CHECK((!x_rows || r.x_rows.numel() == n) && (!experts || r.experts.numel() == n), "the rows disagree");

@@ -220,8 +220,11 @@ def gather_qqmm(x, w: torch.Tensor, scales: torch.Tensor, lhs_indices=None, rhs_
     _format(group_size, bits)
     x, sx = _acts(x)
     t = _type(dtype)
-    if tiles is None:
-        y = _lib.binding().int8_gather(x, sx, w, scales, lhs_indices, rhs_indices, bool(sorted_indices), t)
+    table = None if tiles is None else (tiles.offsets, tiles.tile_row, tiles.tile_exp, tiles.ntiles, tiles.maxt)
+    if tiles is None or (isinstance(rhs_indices, torch.Tensor) and tiles.rows == rhs_indices.numel() and
+                         isinstance(w, torch.Tensor) and w.dim() == 3 and tiles.num_experts == w.shape[0] and
+                         tiles.tile_rows == ops.tile_rows()):
+        y = _lib.binding().int8_gather(x, sx, w, scales, lhs_indices, rhs_indices, bool(sorted_indices), t, table)
         if y is not None:
             return y
     own = x.dtype
