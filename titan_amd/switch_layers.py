@@ -15,7 +15,9 @@ sort, which also yields the tile table that affine projections share (mxfp4
 ones make their own), and the row gather, the default activation and the
 un-sort are one kernel each (at 512 tokens x top-10, hidden 2048, 13 torch
 launches of 75 us before); CPU tensors use torch's stable argsort and the stock
-gather.
+gather.  Projections in 8-bit integers (``mode="int8"``, an extension) quantise a
+token once and take its codes by index, without gathering them; they run on the
+GPU and have no gradient.
 """
 
 from __future__ import annotations
@@ -25,7 +27,7 @@ import math
 import torch
 from torch.autograd import forward_ad
 
-from . import core, kernels, ops
+from . import core, int8, kernels, ops
 from ._lib import QmoeLibraryMissing
 
 __all__ = ["QuantizedSwitchLinear", "SwitchGLU", "SwiGLU", "swiglu"]
@@ -101,6 +103,21 @@ def _gather_sort(x: torch.Tensor, indices: torch.Tensor, num_experts: int, learn
     return x.flatten(0, -3)[order // M], ids, inv, tiles
 
 
+def _quantised_sort(x: torch.Tensor, indices: torch.Tensor, num_experts: int):
+    """The pairs sorted by expert for projections in 8-bit integers: the tokens'
+    codes and scales, sorted ids, inverse permutation, tile table and the token of
+    each sorted pair."""
+    M = indices.shape[-1]
+    x = x.reshape(-1, x.shape[-1])
+    int8._no_grad(x, "x")
+    if indices.numel() > x.shape[0] * M:
+        raise IndexError(f"ids of {indices.numel() // M} rows of {M}, x has {x.shape[0]}")
+    q, s = ops.quantize(x, mode="int8")
+    r = ops.route(indices.reshape(-1), num_experts)
+    rows = torch.div(r.order, M, rounding_mode="floor")
+    return (q.unsqueeze(1), s.unsqueeze(1)), r.sorted_ids, r.inv_order, r.tiles, rows
+
+
 def _scatter_unsort(x: torch.Tensor, inv_order: torch.Tensor, shape=None) -> torch.Tensor:
     """switch_layers.py:21-25."""
     if isinstance(inv_order, tuple):
@@ -117,11 +134,16 @@ def _scatter_unsort(x: torch.Tensor, inv_order: torch.Tensor, shape=None) -> tor
 class QuantizedSwitchLinear:
     """Per-expert quantized linear layer: weight [E, N, K*bits/32] packed
     words, scales/biases [E, N, K/group_size] bf16, optional bias [E, N].
-    ``mode="mxfp4"``: 4-bit codes, scales uint8 [E, N, K/32], biases None."""
+    ``mode="mxfp4"``: 4-bit codes, scales uint8 [E, N, K/32], biases None.
+    ``mode="int8"``: codes int8 [E, N, K], scales float32 [E, N], biases None."""
 
     def __init__(self, weight, scales, biases=None, group_size: int | None = None, bits: int = 4, mode: str = "affine",
                  bias: torch.Tensor | None = None):
-        if group_size is None:
+        if mode == "int8":
+            if biases is not None or group_size is not None:
+                raise ValueError("8-bit integers have one scale per row, and no biases")
+            bits = 8
+        elif group_size is None:
             group_size = 32 if mode == "mxfp4" else 64
         self.weight, self.scales, self.biases = weight, scales, biases
         self.group_size, self.bits, self.mode = group_size, bits, mode
@@ -129,7 +151,7 @@ class QuantizedSwitchLinear:
 
     @property
     def input_dims(self) -> int:
-        return self.scales.shape[2] * self.group_size
+        return self.weight.shape[2] if self.mode == "int8" else self.scales.shape[2] * self.group_size
 
     @property
     def output_dims(self) -> int:
@@ -139,11 +161,16 @@ class QuantizedSwitchLinear:
     def num_experts(self) -> int:
         return self.weight.shape[0]
 
-    def __call__(self, x, indices, sorted_indices: bool = False, tiles=None):
+    def __call__(self, x, indices, sorted_indices: bool = False, tiles=None, rows=None, dtype=None):
         """switch_layers.py:76-127: registry ops first for sorted calls, the
-        namespace's gather otherwise or when both decline."""
+        namespace's gather otherwise or when both decline.  ``rows`` and ``dtype``
+        are of 8-bit integers, whose x may be codes and scales: the row of x that
+        each index takes, and the result's type."""
         gathered = None
-        if sorted_indices and self.mode == "affine" and self.bias is None:
+        if self.mode == "int8":
+            gathered = ops.gather_qqmm(x, self.weight, self.scales, lhs_indices=rows, rhs_indices=indices, mode="int8",
+                                       sorted_indices=sorted_indices, tiles=tiles, dtype=dtype)
+        elif sorted_indices and self.mode == "affine" and self.bias is None:
             for name in ("moe.gather_qmm_int8", "moe.gather_qmm_ws"):
                 op = kernels.get(name)
                 if op is None:
@@ -194,21 +221,25 @@ class SwitchGLU:
         """x [..., D], indices [..., k] -> [..., k, D] (switch_layers.py:213-245)."""
         x = x.unsqueeze(-2).unsqueeze(-2)
         do_sort = indices.numel() >= 64
-        idx, inv_order, tiles = indices, None, None
-        if do_sort:
+        idx, inv_order, tiles, once = indices, None, None, {}
+        first = (self.gate_proj, self.up_proj) if self.gate_up_proj is None else (self.gate_up_proj,)
+        if do_sort and all(getattr(p, "mode", None) == "int8" for p in first):
+            once["dtype"] = x.dtype
+            x, idx, inv_order, tiles, once["rows"] = _quantised_sort(x, indices, self.num_experts)
+        elif do_sort:
             # through mxfp4 experts a layer can be trained: rows and gradients by the token sort's kernels
             learns = self.down_proj.mode == "mxfp4" and _learns(x)
             x, idx, inv_order, tiles = _gather_sort(x, indices, self.num_experts, learns)
         if self.gate_up_proj is not None:
-            gu = self.gate_up_proj(x, idx, sorted_indices=do_sort, tiles=tiles)
+            gu = self.gate_up_proj(x, idx, sorted_indices=do_sort, tiles=tiles, **once)
             if _default(self.activation) and gu.shape[-1] % 2 == 0 and _plain(gu, gu.shape[-1] // 2):
                 h = ops.swiglu(gu)
             else:
                 x_gate, x_up = gu.chunk(2, dim=-1)
                 h = self.activation(x_up, x_gate)
         else:
-            x_up = self.up_proj(x, idx, sorted_indices=do_sort, tiles=tiles)
-            x_gate = self.gate_proj(x, idx, sorted_indices=do_sort, tiles=tiles)
+            x_up = self.up_proj(x, idx, sorted_indices=do_sort, tiles=tiles, **once)
+            x_gate = self.gate_proj(x, idx, sorted_indices=do_sort, tiles=tiles, **once)
             h = self.activation(x_up, x_gate)
         x = self.down_proj(h, idx, sorted_indices=do_sort, tiles=tiles)
         if do_sort:
