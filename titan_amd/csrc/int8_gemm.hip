@@ -6,7 +6,7 @@
 // by a block of eight waves, one block per CU.  Its form by its rows: WM x WN
 // waves of MSUB x NSUB subtiles of v_mfma_i32_32x32x32_i8 each.  Both operands
 // reach LDS by asynchronous copies, 128 bytes of a row at a time (a whole line;
-// with 64, twice the requests for the same bytes), into a ring of NS stages, and
+// with 64, twice the requests for the same bytes), into a ring of stages, and
 // are read from there as fragments, those of a step during the step before.  The
 // barrier that hands over a stage stands before a group's last step, whose
 // operands are in registers by then; the copies into the stage that it frees are
@@ -130,10 +130,10 @@ __device__ __forceinline__ void copy_x(const Ctx<COLS>& c, int g, uint32_t st, i
   qmoe_gemm::dma16(in ? p : reinterpret_cast<const char*>(zero_unit), st + (d * kWaves + c.wave) * 1024);
 }
 template <int COLS>
-__device__ __forceinline__ void copy_w(const Ctx<COLS>& c, int g, uint32_t st, int na, int d) {
+__device__ __forceinline__ void copy_w(const Ctx<COLS>& c, int g, uint32_t st, int d) {
   const bool in = g * kUnits + c.unit < c.units;
   qmoe_gemm::dma16s(c.w + (size_t)g * kGroup, c.woff[d] - (in ? 0u : (uint32_t)c.unit * 16),
-                    st + ((na + d) * kWaves + c.wave) * 1024);
+                    st + (d * kWaves + c.wave) * 1024);
 }
 
 // A unit's addresses, and the copies of its scales (into s: rows', then columns') and of its first group.
@@ -165,37 +165,39 @@ __device__ __forceinline__ Ctx<Forms::kCols> begin(const Product& a, const Unit&
   for (int d = 0; d < kMaxACopies; ++d)
     if (d < na) copy_x(c, 0, c.lds, d);
 #pragma unroll
-  for (int d = 0; d < kBCopies; ++d) copy_w(c, 0, c.lds, na, d);
+  for (int d = 0; d < kBCopies; ++d) copy_w(c, 0, c.lds + na * kWaves * 1024, d);
   return c;
 }
 
-template <int WM_, int WN_, int MSUB_, int NSUB_, int NS_>
+// NX stages of a group's x and w, and NW - NX more of w, which comes from further
+// away (192 rows on each of 256 experts, three of w beside two of x: 162 -> 152 us).
+template <int WM_, int WN_, int MSUB_, int NSUB_, int NX_, int NW_ = NX_>
 struct Form {
-  static constexpr int WM = WM_, WN = WN_, MSUB = MSUB_, NSUB = NSUB_, NS = NS_;
+  static constexpr int WM = WM_, WN = WN_, MSUB = MSUB_, NSUB = NSUB_, NX = NX_, NW = NW_;
   static constexpr int kRows = 32 * WM * MSUB, kCols = 32 * WN * NSUB;
   static constexpr int kBCopies = kCols / kRound, kACopies = (kRows + kRound - 1) / kRound, kCopies = kACopies + kBCopies;  // per wave and group
-  static constexpr int kA = kACopies * kWaves * 1024, kStage = kA + kCols * kGroup;
+  static constexpr int kA = kACopies * kWaves * 1024, kB = kCols * kGroup, kStage = kA + kB;
+  static constexpr int kAfter = (NX - 2) * kCopies + (NW - NX) * kBCopies;  // copies under way past the group that is waited for
   static_assert(WM * WN == kWaves, "eight waves");
-  static_assert(NS * kStage <= kRing && kStage <= kStaging, "the ring");
+  static_assert(NX * kStage + (NW - NX) * kB <= kRing && kStage <= kStaging && NW - NX <= 1, "the ring");
   typedef i32x16_t Acc[MSUB][NSUB];
   typedef ::Ctx<kCols> Ctx;
 
   struct Frag {
     i32x4_t a[MSUB], b[NSUB];
   };
-  static __device__ __forceinline__ void copy(const Ctx& c, int g, int stage, int d) {
-    const uint32_t st = c.lds + stage * kStage;
-    if (d < kACopies) copy_x(c, g, st, d);
-    else copy_w(c, g, st, kACopies, d - kACopies);
+  static __device__ __forceinline__ int x_at(int stage) { return stage * kStage; }
+  static __device__ __forceinline__ int w_at(int stage) {
+    return NW == NX || stage < NX ? stage * kStage + kA : NX * kStage + (stage - NX) * kB;
   }
-  static __device__ __forceinline__ void read(const Ctx& c, const char* st, int kk, int row0, int col0, Frag& f) {
+  static __device__ __forceinline__ void read(const Ctx& c, const char* sx, const char* sw, int kk, int row0, int col0, Frag& f) {
     const int l32 = c.lane % 32, unit = (2 * kk + c.lane / 32) ^ swz(l32);  // swz repeats every 16 rows
 #pragma unroll
     for (int i = 0; i < MSUB; ++i)
-      f.a[i] = *reinterpret_cast<const i32x4_t*>(st + (row0 + 32 * i + l32) * kGroup + unit * 16);
+      f.a[i] = *reinterpret_cast<const i32x4_t*>(sx + (row0 + 32 * i + l32) * kGroup + unit * 16);
 #pragma unroll
     for (int j = 0; j < NSUB; ++j)
-      f.b[j] = *reinterpret_cast<const i32x4_t*>(st + kA + (col0 + 32 * j + l32) * kGroup + unit * 16);
+      f.b[j] = *reinterpret_cast<const i32x4_t*>(sw + (col0 + 32 * j + l32) * kGroup + unit * 16);
   }
   // A step's products with PIECES calls of more(i) spread between them.
   template <int PIECES, class More>
@@ -223,34 +225,45 @@ struct Form {
     const int row0 = 32 * MSUB * (c.wave / WN), col0 = 32 * NSUB * (c.wave % WN);
     const int G = (c.units + kUnits - 1) / kUnits;
     Acc acc = {};
-    if (NS > 2) meet();  // the staging of the unit before, which other stages overlap, is read
+    if (NW > 2) meet();  // the staging of the unit before, which other stages overlap, is read
     // past the end: the last group again, into stages that nothing reads any more
 #pragma unroll
-    for (int i = 1; i < NS - 1; ++i)
+    for (int i = 1; i < NW - 1; ++i) {
+      if (i < NX - 1) {
 #pragma unroll
-      for (int d = 0; d < kCopies; ++d) copy(c, min(i, G - 1), i, d);
-    qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
+        for (int d = 0; d < kACopies; ++d) copy_x(c, min(i, G - 1), c.lds + x_at(i), d);
+      }
+#pragma unroll
+      for (int d = 0; d < kBCopies; ++d) copy_w(c, min(i, G - 1), c.lds + w_at(i), d);
+    }
+    qmoe_gemm::wait_vmem<kAfter>();
     meet();
     Frag f[2];
-    read(c, smem, 0, row0, col0, f[0]);
-    int at = 0;  // the stage of group g
+    read(c, smem + x_at(0), smem + w_at(0), 0, row0, col0, f[0]);
+    int ax = 0, aw = 0;  // the stages of group g
     for (int g = 0; g < G; ++g) {
       if (g + 1 == G) last();
-      const char* st = smem + at * kStage;
-      const int freed = at == 0 ? NS - 1 : at - 1, from = min(g + NS - 1, G - 1);
+      const char *sx = smem + x_at(ax), *sw = smem + w_at(aw);
+      const int fx = ax == 0 ? NX - 1 : ax - 1, fw = NW == NX ? fx : aw == 0 ? NW - 1 : aw - 1;  // freed
+      const int gx = min(g + NX - 1, G - 1), gw = min(g + NW - 1, G - 1);
 #pragma unroll
       for (int kk = 0; kk + 1 < kSteps; ++kk) {
-        read(c, st, kk + 1, row0, col0, f[(kk + 1) & 1]);
-        if (kk == 0) products<kCopies>(f[0], acc, [&](int p) { copy(c, from, freed, p); });
+        read(c, sx, sw, kk + 1, row0, col0, f[(kk + 1) & 1]);
+        if (kk == 0)
+          products<kCopies>(f[0], acc, [&](int p) {
+            if (p < kACopies) copy_x(c, gx, c.lds + x_at(fx), p);
+            else copy_w(c, gw, c.lds + w_at(fw), p - kACopies);
+          });
         else products<0>(f[kk & 1], acc, [](int) {});
         __builtin_amdgcn_sched_barrier(0);
       }
-      at = at + 1 == NS ? 0 : at + 1;
+      ax = ax + 1 == NX ? 0 : ax + 1;
+      aw = NW == NX ? ax : aw + 1 == NW ? 0 : aw + 1;
       if (g + 1 < G) {
-        // the next group landed (copies of NS - 2 groups after it may be in flight); this one's reads are done
-        qmoe_gemm::wait_vmem<(NS - 2) * kCopies>();
+        // the next group landed (copies of those after it may be in flight); this one's reads are done
+        qmoe_gemm::wait_vmem<kAfter>();
         meet();
-        read(c, smem + at * kStage, 0, row0, col0, f[kSteps & 1]);
+        read(c, smem + x_at(ax), smem + w_at(aw), 0, row0, col0, f[kSteps & 1]);
       }
       __builtin_amdgcn_sched_barrier(0);
       products<0>(f[(kSteps - 1) & 1], acc, [](int) {});
@@ -372,7 +385,7 @@ struct Pick<F, G, Rest...> {
     else Pick<G, Rest...>::run(a, u, rest...);
   }
 };
-typedef Pick<Form<2, 4, 4, 2, 2>, Form<2, 4, 3, 2, 2>, Form<2, 4, 2, 2, 3>, Form<1, 8, 3, 1, 3>, Form<1, 8, 2, 1, 3>,
+typedef Pick<Form<2, 4, 4, 2, 2>, Form<2, 4, 3, 2, 2, 3>, Form<2, 4, 2, 2, 3>, Form<1, 8, 3, 1, 3>, Form<1, 8, 2, 1, 3>,
              Form<1, 8, 1, 1, 3>> Wide;
 // 64 x 128 and 128 x 128 outputs, for products of few units: five and three
 // groups ahead, where it is the copies' way that takes the time.
