@@ -448,3 +448,16 @@ def test_tables_that_do_not_fit(dev):
         call(dataclasses.replace(table, num_experts=5))
     with pytest.raises(ValueError, match="tile table"):
         call(dataclasses.replace(table, tile_rows=64))
+
+
+@pytest.mark.parametrize("M", [2, 3, 5, 8, 16, 17])
+@pytest.mark.parametrize("N,K", [(301, 272), (4099, 2080), (9, 16384), (2000, 1040), (70, 16400)])
+def test_few_rows_of_values(dev, M, N, K):
+    """However few rows of values are taken, the bits of the product of the rows quantised before."""
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(dev, BF)
+    w, sw = (t.to(dev) for t in _codes((N, K), 41))
+    q, s = ops.quantize(x, mode="int8")
+    y = ops.qqmm(x, w, sw, mode="int8")
+    assert torch.equal(y, ops.qqmm((q, s), w, sw, mode="int8"))
+    i = torch.tensor([0, N // 2, N - 1])
+    o.assert_rounded(y[:, i.to(dev)], o.product(q.cpu(), s.cpu(), w[i.to(dev)].cpu(), sw[i.to(dev)].cpu()))

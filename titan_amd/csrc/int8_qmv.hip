@@ -117,22 +117,27 @@ __global__ __launch_bounds__(kThreads) void int8_qmv_kernel(Product a) {
 template <int DT, int LPR, int NR>
 int launch(const Product& a, hipStream_t st) {
   constexpr int kRows = (64 / LPR) * NR * kWaves;
-  const dim3 grid((unsigned)((a.N + kRows - 1) / kRows), (unsigned)a.n_rows);
+  // in eights, so that the rows of x that take the same weights run on the same XCD (block ids are dealt round-robin) and
+  // find them in its L2 (eight rows by 4099 of 2080: 15.4 -> 9.7 us); what is past the end works on the last weight row
+  const int64_t blocks = (a.N + kRows - 1) / kRows;
+  const dim3 grid((unsigned)(a.n_rows > 1 ? (blocks + 7) / 8 * 8 : blocks), (unsigned)a.n_rows);
   if (qmoe::too_many((int64_t)grid.x * grid.y, kThreads))
     return qmoe::fail(QMOE_ERR_UNSUPPORTED, "n_rows=%lld: too many for weights of this size", (long long)a.n_rows);
   int8_qmv_kernel<DT, LPR, NR><<<grid, dim3(kThreads), 0, st>>>(a);
   return qmoe::launch_status("int8_qmv_kernel");
 }
 // Lanes per weight row: as many as leave each two loads one after the other,
-// and where the rows are many four of them, in fewer and longer waves.  64 / 32 /
-// 16 lanes, codes (us per call in a graph): 4096 rows of 2048 4.6 / 5.1 / 7.2,
+// and where the rows are many about four of them, in fewer and longer waves.  64 /
+// 32 / 16 lanes, codes (us per call in a graph): 4096 rows of 2048 4.6 / 5.1 / 7.2,
 // 16384 6.1 / 5.7 / 7.5; 4096 rows of 1024 (8 experts) 3.3 / 2.9 / 3.8, 24576 5.9 /
-// 4.8 / 4.6; 20480 rows of 2048 (two tokens x top-10) 10.7 / 9.5 / 9.9.
+// 4.8 / 4.6; 20480 rows of 2048 (two tokens x top-10) 10.7 / 9.5 / 9.9.  Values, eight
+// rows by 4096: of 1040 6.1 / 6.1 / 5.3, of 2064 11.9 / 8.2 / 9.1, of 3008 12.7 / 9.5 / 11.2.
 template <int DT>
 int launch_lanes(const Product& a, hipStream_t st) {
-  const int64_t loads = a.n_rows * a.N >= 16384 ? 4 : 2, lanes = (a.K / 16 + loads - 1) / loads;
-  if (lanes > 32) return launch<DT, 64, 2>(a, st);
-  return lanes > 16 ? launch<DT, 32, 2>(a, st) : launch<DT, 16, 2>(a, st);
+  const bool many = a.n_rows * a.N >= 16384;
+  const int64_t loads = many ? 4 : 2, lanes = (a.K / 16 + loads - 1) / loads, spare = many ? 3 : 2;  // halves
+  if (lanes > 16 * spare) return launch<DT, 64, 2>(a, st);
+  return lanes > 8 * spare ? launch<DT, 32, 2>(a, st) : launch<DT, 16, 2>(a, st);
 }
 
 }  // namespace

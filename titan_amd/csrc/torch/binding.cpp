@@ -621,6 +621,12 @@ py::object rms_norm_quantize(py::handle x_, py::handle w_, double eps, py::handl
 }
 
 constexpr int64_t kMaxValues = 16384;  // longest row of values that the matrix-vector kernel quantises itself
+// Rows of values that it takes, and their products: a launch less, but the weights
+// are read once per row, mostly from the caches after the first (values / quantised
+// before, us per call in a graph: 4096 x 2048 weights, 5 rows 6.2 / 7.5, 8 rows 6.8 /
+// 7.6, 12 rows 10.0 / 7.7; 1024 x 1024, 16 rows 4.6 / 6.3; 8192 x 2048, 4 rows 7.6 /
+// 8.9, 5 rows 10.2 / 9.0; 32768 x 2048, 2 rows 22.8 / 18.1).
+constexpr int64_t kValuesMaxRows = 16, kValuesMaxWork = int64_t(1) << 26;
 // Activations: codes and scales, or (scales None) values to be quantised here.
 struct Acts {
   Tensor x, s;
@@ -651,10 +657,11 @@ Tensor int8_product_run(Acts& a, const Weights8& g, const Rows& r, int type) {
   if (out.numel() == 0) return out;
   if (g.K == 0) return out.zero_();
   const int64_t n_x = row_count(a.x);
-  // codes: two rows of 4096 x 2048 take 5.1 us here and 5.0 by the kernel for few rows, four 5.7 and 5.0; values are
-  // quantised on the way (four 6.5, a launch less)
-  const bool few = !r.offsets.defined() && (r.experts.defined() || r.n == 1 ||
-                                            (r.n <= kQmvMaxRows && (!a.s.defined() || r.n * g.N * g.K <= kQmvMaxWork)));
+  // codes: two rows of 4096 x 2048 take 5.1 us here and 5.0 by the kernel for few rows, four 5.0 and 5.0
+  const int64_t work = r.n * g.N * g.K;
+  const bool one = a.s.defined() ? r.n <= kQmvMaxRows && work <= kQmvMaxWork
+                                 : r.n <= kValuesMaxRows && work <= kValuesMaxWork && g.K <= kMaxValues;
+  const bool few = !r.offsets.defined() && (r.experts.defined() || r.n == 1 || one);
   if (few && !a.s.defined() && g.K <= kMaxValues) {
     ok(qmoe_int8_gather_qmv(a.x.const_data_ptr(), type_of(a.x), n_x, ptr<int32_t>(r.x_rows), (int32_t)r.div,
                             ptr<int32_t>(r.experts), r.n, ptr<int8_t>(g.w), ptr<float>(g.s), (int32_t)g.E, g.N, g.K, type,
