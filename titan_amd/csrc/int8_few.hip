@@ -103,7 +103,10 @@ __global__ __launch_bounds__(64 * kWaves) void int8_few_kernel(Product a) {
 
 template <int MT, int BK>
 int launch(const Product& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.n_rows + 16 * MT - 1) / (16 * MT)));
+  // blocks of the same weights on the same XCD, as in int8_qmv.hip (64 rows by 1000 of 4096: 6.4 -> 5.2 us); what is
+  // past the end works on the last weight row
+  const int64_t rows = (a.n_rows + 16 * MT - 1) / (16 * MT), cols = (a.N + 15) / 16;
+  const dim3 grid((unsigned)(rows > 1 ? (cols + 7) / 8 * 8 : cols), (unsigned)rows);
   if (qmoe::too_many((int64_t)grid.x * grid.y, 64 * kWaves))
     return qmoe::fail(QMOE_ERR_UNSUPPORTED, "N=%lld: too large", (long long)a.N);
   int8_few_kernel<MT, BK><<<grid, dim3(64 * kWaves), 0, st>>>(a);
