@@ -432,8 +432,7 @@ py::object matmul(py::handle x_, py::handle w_, py::handle s_, bool transpose, b
   return give(y);
 }
 
-// Room for the table of r's rows.
-bool room(const Tensor& experts, int64_t E, Rows* r) {
+bool table(const Tensor& experts, int64_t E, Rows* r) {
   const int64_t tr = qmoe_gemm_tile_rows(), n = r->n;
   if (E <= 0 || E > INT32_MAX || n > INT32_MAX) return false;
   r->maxt = (n + tr - 1) / tr + E;
@@ -445,13 +444,9 @@ bool room(const Tensor& experts, int64_t E, Rows* r) {
   r->tile_row = all.narrow(0, a, r->maxt);
   r->tile_exp = all.narrow(0, a + b, r->maxt);
   r->ntiles = all.narrow(0, a + 2 * b, 1);
-  return true;
-}
-bool table(const Tensor& experts, int64_t E, Rows* r) {
-  if (!room(experts, E, r)) return false;
-  ok(qmoe_build_tiles_clamped(ptr<int32_t>(experts), r->n, (int32_t)E, (int32_t)qmoe_gemm_tile_rows(),
-                              r->offsets.data_ptr<int32_t>(), r->tile_row.data_ptr<int32_t>(),
-                              r->tile_exp.data_ptr<int32_t>(), r->ntiles.data_ptr<int32_t>(), r->maxt, stream(experts)),
+  ok(qmoe_build_tiles_clamped(ptr<int32_t>(experts), n, (int32_t)E, (int32_t)tr, r->offsets.data_ptr<int32_t>(),
+                      r->tile_row.data_ptr<int32_t>(), r->tile_exp.data_ptr<int32_t>(), r->ntiles.data_ptr<int32_t>(),
+                      r->maxt, stream(experts)),
      "qmoe_build_tiles_clamped");
   return true;
 }
@@ -555,19 +550,9 @@ bool scales32(const Tensor& t) {  // scales need no alignment past their own
   return t.scalar_type() == at::kFloat && t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() && !t.is_neg();
 }
 
-// sorted: the table of its experts is made by the same launch.
-std::pair<Tensor, Tensor> int8_run(const Tensor& x, Rows* sorted = nullptr, int64_t E = 0) {
+std::pair<Tensor, Tensor> int8_run(const Tensor& x) {
   Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar).requires_grad(false));
   Tensor s = at::empty(batch_of(x), x.options().dtype(at::kFloat).requires_grad(false));
-  if (sorted) {
-    ok(qmoe_int8_quantize_sorted(x.const_data_ptr(), type_of(x), row_count(x), x.size(-1), q.data_ptr<int8_t>(),
-                                 s.data_ptr<float>(), ptr<int32_t>(sorted->experts), sorted->n, (int32_t)E,
-                                 (int32_t)qmoe_gemm_tile_rows(), sorted->offsets.data_ptr<int32_t>(),
-                                 sorted->tile_row.data_ptr<int32_t>(), sorted->tile_exp.data_ptr<int32_t>(),
-                                 sorted->ntiles.data_ptr<int32_t>(), sorted->maxt, stream(x)),
-       "qmoe_int8_quantize_sorted");
-    return {q, s};
-  }
   ok(qmoe_int8_quantize(x.const_data_ptr(), type_of(x), row_count(x), x.size(-1), q.data_ptr<int8_t>(), s.data_ptr<float>(),
                         stream(x)),
      "qmoe_int8_quantize");
@@ -652,35 +637,65 @@ struct Weights8 {
   }
 };
 
-Tensor int8_product_run(Acts& a, const Weights8& g, const Rows& r, int type) {
+// sorted: the rows' experts ascend, and a table of them is to be made.
+Tensor int8_product_run(const Acts& a, const Weights8& g, const Rows& r, int type, bool sorted = false) {
   Tensor out = at::empty({r.n, g.N}, a.x.options().dtype(kTypes[type]).requires_grad(false));
   if (out.numel() == 0) return out;
   if (g.K == 0) return out.zero_();
   const int64_t n_x = row_count(a.x);
+  const bool values = !a.s.defined(), tabled = sorted || r.offsets.defined();
   // codes: two rows of 4096 x 2048 take 5.1 us here and 5.0 by the kernel for few rows, four 5.0 and 5.0
   const int64_t work = r.n * g.N * g.K;
-  const bool one = a.s.defined() ? r.n <= kQmvMaxRows && work <= kQmvMaxWork
-                                 : r.n <= kValuesMaxRows && work <= kValuesMaxWork && g.K <= kMaxValues;
-  const bool few = !r.offsets.defined() && (r.experts.defined() || r.n == 1 || one);
-  if (few && !a.s.defined() && g.K <= kMaxValues) {
+  const bool one = values ? r.n <= kValuesMaxRows && work <= kValuesMaxWork && g.K <= kMaxValues
+                          : r.n <= kQmvMaxRows && work <= kQmvMaxWork;
+  const bool few = !tabled && (r.experts.defined() || r.n == 1 || one);
+  if (few && values && g.K <= kMaxValues) {
     ok(qmoe_int8_gather_qmv(a.x.const_data_ptr(), type_of(a.x), n_x, ptr<int32_t>(r.x_rows), (int32_t)r.div,
                             ptr<int32_t>(r.experts), r.n, ptr<int8_t>(g.w), ptr<float>(g.s), (int32_t)g.E, g.N, g.K, type,
                             out.data_ptr(), stream(a.x)),
        "qmoe_int8_gather_qmv");
     return out;
   }
-  if (!a.s.defined()) std::tie(a.x, a.s) = int8_run(a.x);
+  // codes, scales and table of this call in one allocation, each from a 256-byte boundary
+  const int8_t* q = values ? nullptr : ptr<int8_t>(a.x);
+  const float* sx = values ? nullptr : ptr<float>(a.s);
+  const int32_t *offsets = ptr<int32_t>(r.offsets), *tile_row = ptr<int32_t>(r.tile_row), *tile_exp = ptr<int32_t>(r.tile_exp),
+                *ntiles = ptr<int32_t>(r.ntiles);
+  int64_t maxt = r.maxt;
+  Tensor own;
+  if (values || sorted) {
+    const auto pad = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+    const int64_t tr = qmoe_gemm_tile_rows();
+    if (sorted) maxt = (r.n + tr - 1) / tr + g.E;
+    const int64_t codes = values ? pad(n_x * g.K) : 0, scales = values ? pad(4 * n_x) : 0, heads = sorted ? pad(4 * (g.E + 1)) : 0,
+                  tiles = sorted ? pad(4 * maxt) : 0;
+    own = at::empty({codes + scales + heads + 2 * tiles + 4}, a.x.options().dtype(at::kByte).requires_grad(false));
+    uint8_t* p = own.data_ptr<uint8_t>();
+    int8_t* new_q = reinterpret_cast<int8_t*>(p);
+    float* new_s = reinterpret_cast<float*>(p + codes);
+    const auto ints = [&](int64_t at) { return reinterpret_cast<int32_t*>(p + codes + scales + at); };
+    int32_t *o = ints(0), *row = ints(heads), *exp = ints(heads + tiles), *nt = ints(heads + 2 * tiles);
+    if (values && sorted)
+      ok(qmoe_int8_quantize_sorted(a.x.const_data_ptr(), type_of(a.x), n_x, g.K, new_q, new_s, ptr<int32_t>(r.experts), r.n,
+                                   (int32_t)g.E, (int32_t)tr, o, row, exp, nt, maxt, stream(a.x)),
+         "qmoe_int8_quantize_sorted");
+    else if (values)
+      ok(qmoe_int8_quantize(a.x.const_data_ptr(), type_of(a.x), n_x, g.K, new_q, new_s, stream(a.x)), "qmoe_int8_quantize");
+    else
+      ok(qmoe_build_tiles_clamped(ptr<int32_t>(r.experts), r.n, (int32_t)g.E, (int32_t)tr, o, row, exp, nt, maxt, stream(a.x)),
+         "qmoe_build_tiles_clamped");
+    if (values) q = new_q, sx = new_s;
+    if (sorted) offsets = o, tile_row = row, tile_exp = exp, ntiles = nt;
+  }
   if (few) {
-    ok(qmoe_int8_gather_qqmv(ptr<int8_t>(a.x), ptr<float>(a.s), n_x, ptr<int32_t>(r.x_rows), (int32_t)r.div,
-                             ptr<int32_t>(r.experts), r.n, ptr<int8_t>(g.w), ptr<float>(g.s), (int32_t)g.E, g.N, g.K, type,
-                             out.data_ptr(), stream(a.x)),
+    ok(qmoe_int8_gather_qqmv(q, sx, n_x, ptr<int32_t>(r.x_rows), (int32_t)r.div, ptr<int32_t>(r.experts), r.n,
+                             ptr<int8_t>(g.w), ptr<float>(g.s), (int32_t)g.E, g.N, g.K, type, out.data_ptr(), stream(a.x)),
        "qmoe_int8_gather_qqmv");
     return out;
   }
   const Tensor rows = gemm_rows(r, a.x);
-  ok(qmoe_int8_gather_qqmm(ptr<int8_t>(a.x), ptr<float>(a.s), n_x, ptr<int32_t>(rows), r.n, ptr<int8_t>(g.w), ptr<float>(g.s),
-                           (int32_t)g.E, g.N, g.K, ptr<int32_t>(r.offsets), ptr<int32_t>(r.tile_row),
-                           ptr<int32_t>(r.tile_exp), ptr<int32_t>(r.ntiles), r.maxt, type, out.data_ptr(), stream(a.x)),
+  ok(qmoe_int8_gather_qqmm(q, sx, n_x, ptr<int32_t>(rows), r.n, ptr<int8_t>(g.w), ptr<float>(g.s), (int32_t)g.E, g.N, g.K,
+                           offsets, tile_row, tile_exp, ntiles, maxt, type, out.data_ptr(), stream(a.x)),
      "qmoe_int8_gather_qqmm");
   return out;
 }
@@ -724,16 +739,12 @@ py::object int8_gather(py::handle x_, py::handle sx_, py::handle w_, py::handle 
     return py::none();
   const c10::hip::HIPGuard guard(a.x.get_device());
   type = a.type(type);
-  if (r.n >= kSortedMinRows && tiles) {
-    if (!take(*tiles, g.E, a.x.device(), &r)) return py::none();
-  } else if (r.n >= kSortedMinRows) {
-    if (a.s.defined() ? !table(r.experts, g.E, &r) : !room(r.experts, g.E, &r)) return py::none();
-    if (!a.s.defined()) std::tie(a.x, a.s) = int8_run(a.x, &r, g.E);
-  }
+  const bool table = r.n >= kSortedMinRows;
+  if (table && (g.E > INT32_MAX || r.n > INT32_MAX || (tiles && !take(*tiles, g.E, a.x.device(), &r)))) return py::none();
   auto sizes = rhs.sizes().vec();
   sizes.push_back(1);
   sizes.push_back(g.N);
-  return give(int8_product_run(a, g, r, type).reshape(sizes));
+  return give(int8_product_run(a, g, r, type, table && !tiles).reshape(sizes));
 }
 
 // Rows already arranged by the wrapper, as rows_product has them.
