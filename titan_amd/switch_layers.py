@@ -165,8 +165,10 @@ class QuantizedSwitchLinear:
         """switch_layers.py:76-127: registry ops first for sorted calls, the
         namespace's gather otherwise or when both decline.  ``rows`` and ``dtype``
         are of 8-bit integers, whose x may be codes and scales: the row of x that
-        each index takes, and the result's type."""
+        each index takes, and the result's type.  The other modes refuse them."""
         gathered = None
+        if self.mode != "int8" and (rows is not None or dtype is not None):
+            raise ValueError(f"rows and dtype are arguments of 8-bit integers, not of mode {self.mode!r}")
         if self.mode == "int8":
             gathered = ops.gather_qqmm(x, self.weight, self.scales, lhs_indices=rows, rhs_indices=indices, mode="int8",
                                        sorted_indices=sorted_indices, tiles=tiles, dtype=dtype)
