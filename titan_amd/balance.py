@@ -29,8 +29,9 @@ def router_balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: torch.Ten
 
     The gradient goes to the logits, the counts being constants; it is exactly 0
     for masked tokens, whatever they hold.  It is not differentiable again;
-    forward-mode tangents, torch.jit.trace and make_fx are refused.  Sums over
-    tokens go in a fixed order: results repeat bit for bit.  E is at most 1024.
+    forward-mode tangents, function transforms (vmap, torch.func), torch.jit.trace
+    and make_fx are refused.  Sums over tokens go in a fixed order: results repeat
+    bit for bit.  E is at most 1024.
     """
     got = _lib.binding().router_balance(logits, ids, mask, False)
     if got is not None:

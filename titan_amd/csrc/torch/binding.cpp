@@ -6,11 +6,11 @@
 // without it, it returns None for anything but tensors the entry points can
 // read as they are (GPU, contiguous, aligned, of the right types and sizes),
 // and the wrapper then checks, converts or refuses; with it, such a call is an
-// error.  Tracers, which would not see a launch, and tangents are refused.  A
-// call made this way costs the host about 5 us where ctypes cost 11, and the
-// token sort and the way back with their gradients 46 to 79 from run to run
-// where Python autograd nodes cost 136, which is what a small call's time is
-// made of.
+// error.  Tracers, which would not see a launch, tangents and tensors that a
+// function transform has wrapped are refused.  A call made this way costs the
+// host about 5 us where ctypes cost 11, and the token sort and the way back with
+// their gradients 46 to 79 from run to run where Python autograd nodes cost 136,
+// which is what a small call's time is made of.
 //
 // Launches go to the tensors' device and its current stream; nothing
 // synchronises; outputs and tables come from torch's allocator.
@@ -78,9 +78,12 @@ bool words(const Tensor& t) { return (t.scalar_type() == at::kInt || t.scalar_ty
 bool bytes(const Tensor& t) {
   return t.scalar_type() == at::kByte && t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous();
 }
+// What vmap and torch.func's transforms wrap has no memory of its own: refused.
 bool get(py::handle h, Tensor* t) {
   if (!THPVariable_Check(h.ptr())) return false;
   *t = THPVariable_Unpack(h.ptr());
+  if (t->key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper})))
+    throw Failure("vmap and torch.func's transforms are not supported here");
   return true;
 }
 template <class T>

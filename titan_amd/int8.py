@@ -11,7 +11,7 @@ is computed from it is NaN.  Products are summed exactly in 32-bit integers
 (K up to 131,056) and rounded once.
 
 Nothing here has a gradient: both operands are rounded.  Forward-mode tangents,
-torch.jit.trace and make_fx are refused.
+function transforms (vmap, torch.func), torch.jit.trace and make_fx are refused.
 
 The calls are csrc/torch/binding.cpp's.  It takes what the kernels can read as
 it is; the functions here check, convert, arrange or refuse the rest.
