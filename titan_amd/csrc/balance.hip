@@ -16,6 +16,10 @@
 // where V does not divide E it overlaps the one before, and what it has as well
 // is not its own: computed alike, stored twice, counted once.
 //
+// A sum in 32 bits is over at most 16 rows of a lane, the next ones go to another
+// and these are added in 64: equal probabilities all round to one side, and one
+// sum's error would grow with the tokens.
+//
 // Bound by HBM and by the exponentials' issue, then by the join's launch: 32768
 // tokens of 256 fp32 logits, per call in a graph, 10.3 us for the sums (3.3 TB/s),
 // 6.1 for the join, 12.0 for the gradient (5.6 TB/s); 61 tokens of 60 in one launch
@@ -29,6 +33,7 @@ using qmoe_lanes::over;
 
 constexpr int kMaxE = 1024;
 constexpr int kWaves = 16, kThreads = 64 * kWaves;
+constexpr int kTerms = 16;    // rows that a lane adds in 32 bits
 constexpr int kFinal = 1024;  // threads of the block that finishes
 
 struct Tokens {
@@ -151,14 +156,26 @@ __global__ __launch_bounds__(kThreads) void balance_sums_kernel(Tokens a, float*
   __syncthreads();
   count(a, counts, &tokens);
   float acc[R::P];
+  double wide[R::P];
 #pragma unroll
-  for (int i = 0; i < R::P; ++i) acc[i] = 0.f;
-  for (; t - sub < a.T; t += step) {
+  for (int i = 0; i < R::P; ++i) acc[i] = 0.f, wide[i] = 0.0;
+  const auto widen = [&] {
+#pragma unroll
+    for (int i = 0; i < R::P; ++i) wide[i] += acc[i], acc[i] = 0.f;
+  };
+  bool more = false;
+  for (int terms = 0; t - sub < a.T; t += step) {
+    if (terms++ == kTerms) widen(), more = true, terms = 1;
     then.load(a, t + step, lane);
     now.softmax(a, lane);
 #pragma unroll
     for (int i = 0; i < R::P; ++i) acc[i] += now.live ? now.p[i] : 0.f;
     now = then;
+  }
+  if (more) {
+    widen();
+#pragma unroll
+    for (int i = 0; i < R::P; ++i) acc[i] = (float)wide[i];
   }
   // the rows that a wave works on at a time, then the waves
 #pragma unroll
