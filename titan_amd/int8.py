@@ -148,8 +148,8 @@ def _acts(x):
     if isinstance(x, torch.Tensor):
         return x, None
     if isinstance(x, Normed):
-        return x.codes, x.scales
-    if isinstance(x, (tuple, list)) and len(x) == 2:
+        x = x[:2]
+    if isinstance(x, (tuple, list)) and len(x) == 2 and isinstance(x[0], torch.Tensor):
         return x
     raise TypeError("x must be a tensor, a pair of codes and scales, or what rms_norm_quantize returns")
 
