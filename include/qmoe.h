@@ -605,7 +605,7 @@ int qmoe_int8_rms_norm(const void* x, const void* residual, const void* weight,
                        void* norm, void* stream);
 
 /* Products: out[r, n] = sx[xr] sw[e, n] sum_k x[xr, k] w[e, n, k], summed
- * exactly in 32 bits, rounded once to out_dtype; codes [-128, 127].  K is a
+ * exactly in 32 bits, scaled in fp32, rounded once to out_dtype; codes [-128, 127].  K is a
  * multiple of 16, at most 131056.  Indices are clamped into range.
  *   qmoe_int8_gather_qqmv  few rows (at most 65535), xr = x_rows[r], or r /
  *                          x_div where x_rows is NULL; experts NULL: expert 0

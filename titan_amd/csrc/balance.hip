@@ -20,10 +20,12 @@
 // and these are added in 64: equal probabilities all round to one side, and one
 // sum's error would grow with the tokens.
 //
-// Bound by HBM and by the exponentials' issue, then by the join's launch: 32768
-// tokens of 256 fp32 logits, per call in a graph, 10.3 us for the sums (3.3 TB/s),
-// 6.1 for the join, 12.0 for the gradient (5.6 TB/s); 61 tokens of 60 in one launch
-// of 4.2, gradient 3.0.
+// 32768 tokens of 256 fp32 logits, per call in a graph: 10.3 us for the sums (3.3
+// TB/s, where a copy reaches 4.9: a block counts its pairs before its first row's
+// softmax, and then has eight rounds alone to hide the loads in), 6.1 for the join
+// (a launch, and chains of sixteen loads by a block per 64 experts), 12.0 for the
+// gradient (5.6 TB/s, bound by HBM); 61 tokens of 60 in one launch of 4.2,
+// gradient 3.0.
 #include "elem.h"
 #include "lanes.h"
 

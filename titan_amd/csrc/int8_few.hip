@@ -1,5 +1,6 @@
 // Products of one matrix of 8-bit integers with a few rows (int8_product.h),
-// every weight read once.
+// every weight read once for 16 or 32 of them: from HBM the first time, by more
+// rows from the caches.
 //
 // A block owns 16 outputs of 16 * MT rows, and its eight waves take batches of
 // BK of the contraction in turn; their partial sums meet in LDS at the end and

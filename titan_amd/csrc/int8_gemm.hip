@@ -21,16 +21,25 @@
 //
 // 256 x 256 by eight waves: a wave's 128 x 64 outputs read 6 KiB of fragments for
 // 8 matrix instructions (with four waves of 128 x 128 4 for 8, but one wave per
-// SIMD waits alone: 75 us at 4096^3, this 60), and a unit copies half the bytes
-// per product that 128 x 128 does (both operands pass L2 -> LDS at up to 33 TB/s
-// in 128-byte pieces, 17 in 64-byte ones).  Large products are bound by power: 60
-// us at 4096^3 (2.3 POP/s), 445 at 8192^3 (2.5), where a loop of the matrix
-// instructions alone reaches 3.45.  Experts are bound by their weights' way from
-// HBM and by the chains of units: 4096 tokens x top-10 of 256, 2048 -> 1024, take
-// 164 us (537 MB of weights and 84 of results: 130 at a copy's rate), 512 tokens 102 (5.4 TB/s).
+// SIMD waits alone: 75 us at 4096^3 where eight took 65), and a unit copies half the
+// bytes per product that 128 x 128 does (both operands pass L2 -> LDS at up to 33 TB/s
+// in 128-byte pieces, 17 in 64-byte ones).
+//
+// 4096^3 takes 61-66 us by the card (2.1-2.25 POP/s), 8192^3 444-462 (2.4-2.5), where
+// a loop of the matrix instructions alone reaches 3.42: 40 and 322 us.  Two things keep
+// them there: the board is at or near its power limit (1336-1400 of 1400 W; the clock
+// falls from 2.4 GHz to 1.69-1.81, the loop's own is 1.77), and at that clock the
+// matrix cores are busy in 59% and 66% of the cycles, the rest going to waits (for
+// copies and LDS and at barriers, 36-39% of the waves' cycles) and to what stands
+// beside the loop of a unit.  Experts: 4096 tokens x top-10 of 256, 2048 -> 1024,
+// take 157-165 us (537 MB of weights and 84 of results: 130 at a copy's rate) with the
+// matrix cores busy in 30% of the cycles and the waves waiting in 51%, 512 tokens
+// 102-111 (109 for the weights alone at a copy's rate, 87 at a stream read's); few rows
+// an expert, in tokens: 7 (61 experts) 27.5 us, 16 (101) 51, 32 (147) 74, 64 (201) 96,
+// 128 (226) 103, which is 4.2 to 4.7 TB/s of weights.
 // Three stages of 128-column units for experts, more in flight but more units:
 // 185 us instead of 164; results stored from the registers, with the ring filled
-// meanwhile, 170.
+// meanwhile, 170 instead of 165.
 #include <algorithm>
 
 #include "gemm_common.h"
@@ -564,7 +573,7 @@ int dense(const Product& a, hipStream_t st) {
 // A table's rows.  The smallest units that one round of the chip takes, by the
 // units that n rows make on as many experts as they can reach, each with half a
 // unit to spare; where none are, the widest (64 x 128 / 128 x 128 / 128 x 256 / 256
-// x 256, us per call in a graph: 2300 rows on 6 experts, 2016 -> 520 13.3 / 15.8 /
+// x 256, us per call in a graph: 2300 rows on 6 experts, 2016 -> 520 13.2 / 15.8 /
 // 20.9 / 34.8; 1860 on 7, 1744 -> 912 19.8 / 16.2 / 21.1 / 34.3; 9500 on 17, 800 ->
 // 472 21.5 / 19.8 / 15.5 / 23.7; past a round 8200 on 32, 2048 -> 1024 55 / 45 / 44 /
 // 44; 41,000 on 256 - / - / 177 / 164).

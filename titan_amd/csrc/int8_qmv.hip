@@ -118,7 +118,7 @@ template <int DT, int LPR, int NR>
 int launch(const Product& a, hipStream_t st) {
   constexpr int kRows = (64 / LPR) * NR * kWaves;
   // in eights, so that the rows of x that take the same weights run on the same XCD (block ids are dealt round-robin) and
-  // find them in its L2 (eight rows by 4099 of 2080: 15.4 -> 9.7 us); what is past the end works on the last weight row
+  // find them in its L2 (eight rows by 4099 of 2080: 15.4 -> 9.8 us); what is past the end works on the last weight row
   const int64_t blocks = (a.N + kRows - 1) / kRows;
   const dim3 grid((unsigned)(a.n_rows > 1 ? (blocks + 7) / 8 * 8 : blocks), (unsigned)a.n_rows);
   if (qmoe::too_many((int64_t)grid.x * grid.y, kThreads))

@@ -8,10 +8,13 @@ weights [N, K] or [E, N, K] by output channel.  scale = max|v| / 127, codes =
 rint(v / scale), as :func:`titan_amd.ops.quantize_act_int8` has them; a row of
 zeros has scale 0, a row with a NaN or an infinity scale NaN, so that all that
 is computed from it is NaN.  Products are summed exactly in 32-bit integers
-(K up to 131,056) and rounded once.
+(K up to 131,056), scaled in fp32 and rounded once to the result's type.
 
-Nothing here has a gradient: both operands are rounded.  Forward-mode tangents,
-function transforms (vmap, torch.func), torch.jit.trace and make_fx are refused.
+Nothing here has a gradient: both operands are rounded.  The norm, the products
+and dequantize refuse operands that ask for one; quantize takes them, and what it
+returns asks for none, as if its operand had been detached.  Forward-mode
+tangents, function transforms (vmap, torch.func), torch.jit.trace and make_fx are
+refused.
 
 The calls are csrc/torch/binding.cpp's.  It takes what the kernels can read as
 it is; the functions here check, convert, arrange or refuse the rest.
